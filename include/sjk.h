@@ -402,6 +402,128 @@ typedef struct sjk_hip_store_job {
 } sjk_hip_store_job;
 int sjk_hip_store_batch(const sjk_hip_store_job * jobs, int n_jobs, uint32_t n_pos, int rotate, void * stream);
 
+/* ---- rows between a layer's projections and its cache (no counterpart in the reference, whose API takes rows that are
+ * normed, turned and rotated already, sj_kvarn.h:1475-1492) ---- */
+
+/* element types of the rows an engine hands over */
+enum { SJK_F32 = 0, SJK_F16 = 1, SJK_BF16 = 2 };
+
+/* Frequencies of rotary positions: pair i of the n_rot / 2 turned pairs of channels has f_i = base^(-2 i / n_rot) radians
+ * per position, divided by divisors[i] where that list is given, then scaled for contexts longer than the trained one:
+ *   SJK_ROPE_PLAIN   as it is
+ *   SJK_ROPE_LINEAR  f_i / factor
+ *   SJK_ROPE_NTK     base * factor^(n_rot / (n_rot - 2)) in place of base (n_rot = 2: f_0 / factor)
+ *   SJK_ROPE_RAMP    between f_i / factor and f_i along i: f_i up to the pair that turns `high` times in n_orig positions,
+ *                    f_i / factor from the pair that turns `low` times on (pair indices floor and ceil of
+ *                    n_rot ln(n_orig / (2 pi turns)) / (2 ln base), cut to 0 and n_rot - 1); magnitude 0.1 ln(factor) + 1
+ *   SJK_ROPE_BANDS   between them by turns r = n_orig f_i / 2 pi: f_i from r = high on, f_i / factor up to r = low */
+enum { SJK_ROPE_PLAIN = 0, SJK_ROPE_LINEAR = 1, SJK_ROPE_NTK = 2, SJK_ROPE_RAMP = 3, SJK_ROPE_BANDS = 4 };
+typedef struct sjk_rope_config {
+    int            n_rot;       /* turned channels of a head, even */
+    int            scaling;     /* SJK_ROPE_* */
+    double         base;        /* > 1 */
+    double         factor;      /* > 0; for RAMP >= 1 */
+    double         n_orig;      /* RAMP, BANDS: the trained context, > 0 */
+    double         low, high;   /* RAMP, BANDS: turns in n_orig positions, 0 < low < high */
+    const double * divisors;    /* NULL, or n_rot / 2 values > 0 (host) */
+} sjk_rope_config;
+
+/* The table that the calls below read: turns[i] = f_i / 2 pi, n_rot / 2 doubles (host; a program copies it to the device
+ * once), and *mscale, the factor that the scaling puts on sines and cosines (1 but for RAMP). Host arithmetic, no GPU call.
+ * SJKVARN_ERR_ARG, writing nothing, for values outside the ranges above. */
+int sjk_rope_turns(const sjk_rope_config * c, double * turns, float * mscale);
+
+/* A turn of rotary positions. Channels behind n_rot pass through. With a pair (a, b) at position p, u = p turns[i]:
+ * (a, b) -> mscale (a cos 2 pi u - b sin 2 pi u, a sin 2 pi u + b cos 2 pi u); the angle is reduced in 64 bits, so far
+ * positions lose nothing. inverse: the sine's sign turned (the way back, and the gradient of the turn, for mscale = 1). */
+enum { SJK_ROPE_HALVES = 0 /* pairs (i, i + n_rot / 2) */, SJK_ROPE_PAIRS = 1 /* pairs (2 i, 2 i + 1) */ };
+typedef struct sjk_hip_rope {
+    int            layout;      /* SJK_ROPE_HALVES or SJK_ROPE_PAIRS */
+    int            n_rot;       /* even, 0 (no turn) to the head's width */
+    int            inverse;
+    float          mscale;
+    const double * d_turns;     /* device, n_rot / 2 */
+} sjk_hip_rope;
+
+/* One set of heads of sjk_hip_head_rows: rows x[pos][head][D] of x_type at d_x + pos * x_pos + head * x_head (strides in
+ * elements, any; the channels of a head adjacent) to rows of out_type at d_out. In order, each where asked for: the norm
+ * x / sqrt(mean(x^2) + eps) * w (d_norm: fp32 weights [D] of head h at d_norm + h * norm_head, 0 = shared), the turn
+ * (rope != 0), the orthonormal Hadamard (rotate != 0; D = 64, 128, 256 or 512), one rounding to out_type. */
+typedef struct sjk_hip_head_job {
+    const void  * d_x;
+    void        * d_out;        /* may be d_x, with the same type and strides; no other overlap */
+    int64_t       x_pos, x_head, out_pos, out_head;
+    int           x_type, out_type, n_heads, rope, rotate;
+    float         eps;          /* > 0 where d_norm is given */
+    const float * d_norm;       /* NULL: no norm */
+    int64_t       norm_head;
+} sjk_hip_head_job;
+
+/* n_pos positions of every job's heads (the queries and the keys of a layer, say) in one launch for up to three jobs of one
+ * x_type. Head widths 1 to 512. Position i is d_pos[i] (device, int32) or, with d_pos NULL, pos0 + i. rope may be NULL if
+ * no job turns. Sums, angles and products in 32 bits or more. */
+int sjk_hip_head_rows(const sjk_hip_head_job * jobs, int n_jobs, uint32_t n_pos, int D, const sjk_hip_rope * rope,
+                      uint32_t pos0, const int32_t * d_pos, void * stream);
+
+/* What a layer's projection rows are, the same for each of its calls: q [n_pos][n_head][D], k and v [n_pos][n_head_kv][D]
+ * of one type with strides in elements (views of one fused output, or three tensors). */
+typedef struct sjk_hip_qkv {
+    int           type;         /* SJK_F32, _F16, _BF16 */
+    int           n_head;       /* query heads; 0: no queries, keys and values only */
+    int           rotate_qk;    /* the Hadamard on queries and keys: 1 unless the caller has rotated them */
+    int           rotate_v;     /* the Hadamard on values: 0 where it is folded into W_v (a turn or a norm lies between W_q,
+                                   W_k and the cache, so there it cannot be folded) */
+    float         eps;
+    int64_t       q_pos, q_head, k_pos, k_head, v_pos, v_head;
+    const float * d_q_norm;     /* NULL or fp32 weights, as sjk_hip_head_job.d_norm */
+    const float * d_k_norm;
+    int64_t       norm_head;
+    sjk_hip_rope  rope;         /* n_rot = 0: no turn */
+} sjk_hip_qkv;
+
+/* Queries, keys and values of positions pos0 .. pos0 + n_pos - 1 from a layer's projections in one launch: queries normed,
+ * turned and rotated to d_q_out [n_pos][n_head][D] fp32, as sjk_hip_attend takes them; keys the same, values rotated,
+ * both staged into the view's sink and ring at the positions' slots. The bytes are those of sjk_hip_head_rows to fp32
+ * followed by sjk_hip_layer_store. d_pos (device, int32): positions of the turn other than pos0 + i; the slots stay those of
+ * pos0 + i. d_q_out may be d_q (fp32 rows [n_pos][n_head][D]); no other overlap. n_pos beyond what sink and ring hold at
+ * once is SJKVARN_ERR_CAPACITY (positions would share a slot). D = 128 or 256, as layers have. */
+int sjk_hip_store_qkv(const sjk_hip_view * v, uint32_t pos0, uint32_t n_pos, const sjk_hip_qkv * m, const int32_t * d_pos,
+                      const void * d_q, const void * d_k, const void * d_v, float * d_q_out, void * stream);
+
+/* The same with pos0 = d_desc[SJK_DESC_QPOS0] read on the device when the kernel runs (sjk_hip_layer_store_dyn): one
+ * captured graph takes every step. A negative entry writes nothing, d_q_out included. */
+int sjk_hip_store_qkv_dyn(const sjk_hip_view * v, const int32_t * d_desc, uint32_t n_pos, const sjk_hip_qkv * m,
+                          const int32_t * d_pos, const void * d_q, const void * d_k, const void * d_v, float * d_q_out,
+                          void * stream);
+
+/* n_jobs independent sjk_hip_store_qkv calls of n_pos positions each, 32 a launch where the views agree in KV heads, staging
+ * and sink type. Two jobs on one ring are refused (SJKVARN_ERR_ARG). */
+typedef struct sjk_hip_qkv_job {
+    sjk_hip_view    v;
+    uint32_t        pos0;
+    const int32_t * d_pos;
+    const void    * d_q;
+    const void    * d_k;
+    const void    * d_v;
+    float         * d_q_out;
+} sjk_hip_qkv_job;
+int sjk_hip_store_qkv_batch(const sjk_hip_qkv_job * jobs, int n_jobs, uint32_t n_pos, const sjk_hip_qkv * m, void * stream);
+
+/* The same for layer il of several sequences (a decode batch), as sjk_hip_seq_store_batch: each sequence's position count
+ * is extended. SJKVARN_ERR_ARG for a bad layer index or a gap before pos0, SJKVARN_ERR_CAPACITY where the staged positions
+ * (from the sealed end on) would not fit the ring. */
+typedef struct sjk_hip_seq_qkv_job {
+    sj_kvarn_seq  * seq;
+    uint32_t        pos0;
+    const int32_t * d_pos;
+    const void    * d_q;
+    const void    * d_k;
+    const void    * d_v;
+    float         * d_q_out;
+} sjk_hip_seq_qkv_job;
+int sjk_hip_seq_store_qkv_batch(const sjk_hip_seq_qkv_job * jobs, int n_jobs, int il, uint32_t n_pos, const sjk_hip_qkv * m,
+                                void * stream);
+
 /* K and V rows (fp32, rotated) of positions pos0 .. pos0+n_pos-1 of KV head h with sealed end B:
  * d_k, d_v [n_pos][D] (the region resolver of sj_kvarn_layer_kv_row, sj_kvarn.h:1516-1533, and of
  * sj_kvarn_cuda_kv_row, sj_kvarn_cuda.cuh:82-100) */
@@ -469,6 +591,51 @@ int sjk_hip_seq_state_poll(const sj_kvarn_seq * s);
 int sjk_hip_seq_state_finish(sj_kvarn_seq * s, size_t * written);
 int sjk_hip_seq_attend_batch(const sjk_hip_seq_job * jobs, int n_jobs, int il, int n_q, int n_head, float scale,
                              void * stream);
+
+/* ---- pages: from one sequence to another, and from place to place in a pool (no counterpart in the reference, whose
+ * sequences own their blocks alone) ----
+ *
+ * A sealed record never changes, so sequences of one pool can hold the same block: a pool of sj_kvarn_pool_init counts the
+ * holders of its blocks. sj_kvarn_pool_release takes one holder off and frees the block with the last one; seq_truncate,
+ * seq_reset, seq_free and a state restore release the blocks they drop in that way and clear only those that no one else holds
+ * (sj_kvarn_layer_truncate on a pool sequence's layer knows no holders and clears every dropped record: use seq_truncate).
+ * These calls change the pool on the host: the caller orders them with each other and with commits on that pool. */
+
+/* The sink entries [0, min(N, S)) and the staged rows of positions [B, N) of n_layers layers copied from src's buffers to dst's
+ * slots of the same positions, in one launch for up to 64 layers; nothing else in dst is written. Records are not copied: dst's
+ * view brings its own body or block table. The views agree in layout, KV heads, staging, sink type and S (capacities may
+ * differ), buffers 4-byte aligned, dst's not src's. SJKVARN_ERR_ARG otherwise and for B < S, B inside a group or N < B with
+ * B > S; SJKVARN_ERR_CAPACITY where [B, N) does not fit a ring. */
+int sjk_hip_fork(const sjk_hip_view * dst, const sjk_hip_view * src, int n_layers, uint32_t B, uint32_t N, void * stream);
+
+/* Blocks src_ids[i] of one pool's slab to blocks dst_ids[i] of another's (or the same) in every layer: block id of layer il lies
+ * at base + il * layer_bytes + id * block_bytes. Ids are host arrays, read before the call returns; 448 pairs a launch. One
+ * source may go to several destinations. SJKVARN_ERR_ARG for an id outside its slab, a destination twice, a destination that is
+ * also a source of the same slab, slabs that overlap without being one, or addresses and sizes that are no multiples of 4. */
+int sjk_hip_copy_blocks(uint8_t * d_dst, size_t dst_layer_bytes, uint32_t dst_blocks, const uint8_t * d_src, size_t src_layer_bytes,
+                        uint32_t src_blocks, int n_layers, size_t block_bytes, const uint32_t * src_ids,
+                        const uint32_t * dst_ids, uint32_t n, void * stream);
+
+/* child goes on from parent's first pos positions (parallel samples, beams, a shared prompt). On one pool the child holds the
+ * parent's sealed blocks with it; otherwise (another pool, or no pool on either side) their records are copied. Sink and staged
+ * rows are copied. Everything is enqueued on `stream` after what the caller enqueued there, with no host wait; the caller orders
+ * other streams. Where pos lies inside the sealed part the child starts at the group boundary below it, as
+ * sj_kvarn_seq_truncate does; *kept (may be NULL) is the child's position count. The child is a new or reset sequence with the
+ * parent's configuration (the status codes of sj_kvarn_seq_state_read otherwise; n_ctx and n_ubatch may differ:
+ * SJKVARN_ERR_CAPACITY where the positions do not fit). SJKVARN_ERR_ARG for a child that is not empty or is the parent, or pos past the
+ * parent's positions; SJKVARN_ERR_PENDING while a seal or a state restore of the parent, or any transfer of the child, is
+ * pending; SJKVARN_ERR_POOL_FULL. A refused call changes nothing. */
+int sjk_hip_seq_fork(sj_kvarn_seq * child, sj_kvarn_seq * parent, uint32_t pos, uint32_t * kept, void * stream);
+
+/* Holders of a block of a pool of sj_kvarn_pool_init (0: free or no block of it) */
+uint32_t sjk_hip_pool_refs(const sj_kvarn_pool * pool, uint32_t id);
+
+/* Move the pool's live blocks to its lowest ids: afterwards ids [0, n_blocks - n_free) are held and the rest are free, lowest
+ * first. seqs: every sequence that holds blocks of the pool, each once. Records are moved and the sequences' device block
+ * tables rewritten on `stream`; the caller orders other streams that use these sequences. What the vacated blocks hold stays in
+ * them. *moved (may be NULL): the blocks moved. SJKVARN_ERR_ARG, changing nothing, where a live block is not held by the
+ * sequences given alone; SJKVARN_ERR_PENDING while a restore of one of them is in flight. */
+int sjk_hip_pool_compact(sj_kvarn_pool * pool, sj_kvarn_seq * const * seqs, int n_seqs, uint32_t * moved, void * stream);
 
 /* The log-domain scale update of the seal's variance balance, element-wise over device arrays: with
  * s = clamp(d_sd[i], 1e-3, 1e3), d_acc[i] = clamp(d_acc[i] + log((double) s), -0.3, 10) and d_scale[i] =

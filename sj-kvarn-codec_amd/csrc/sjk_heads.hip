@@ -1,0 +1,602 @@
+// sjk_heads.hip - rows between a layer's projections and its cache: head norms, rotary positions, the rotation into the
+// cache's basis, and the append, in one pass over the rows (sjk_hip_head_rows, sjk_hip_store_qkv).
+//
+// A row (one head at one position) lies 8 consecutive channels a lane in LPR lanes, so a wavefront holds 64 / LPR rows and
+// reads and writes 16 or 32 bytes a lane. It takes `iters` groups of 64 / LPR consecutive rows of one set of heads (head
+// index fastest), the next group's loads issued before the current one's arithmetic.
+//   * norm: the sum of squares is a fixed tree (pairs in the lane, then lanes 1, 2, 4, ... apart), so a row's bits do not
+//     depend on the rows beside it.
+//   * turn: u = position * turns per position in double, reduced to (-1/2, 1/2] turns and then to an eighth of one either
+//     side of a quarter before it becomes a float: nothing is lost at far positions, and the sine and cosine are short
+//     polynomials. They are made per lane and kept while the lane's position stays (the heads of one position follow one
+//     another); no table of positions is read.
+//   * the Hadamard and the staging are those of the row kernel (sjk_rows.hip): the same bytes.
+#include "sjk_dev.h"
+#include "sjk_row.h"
+
+namespace sjk {
+
+constexpr int HW = 4;                  // wavefronts a workgroup
+constexpr int HEAD_PARTS = 3;          // sets of heads a launch: q, k, v
+constexpr int HEAD_SEQS = 32;          // sequences a launch
+constexpr int HEAD_ITERS = 8;          // row groups a wavefront at most
+enum { HP_ROWS = 0, HP_K = 1, HP_V = 2 };                               // where a part's rows go
+enum { HF_XVEC = 1, HF_OVEC = 2, HF_ROPE = 4, HF_ROT = 8 };
+enum { HM_ROWS = 0, HM_F16 = 1, HM_TQ6 = 2 };                           // a launch: plain rows only, or a cache's staging
+
+struct HeadPart {
+    int64_t x_pos, x_head, o_pos, o_head, w_head;
+    const float * w;
+    float eps;
+    int n_heads, n_units, flags, kind, o_type;
+};
+
+struct HeadSeq {
+    const void * x[HEAD_PARTS];
+    void * o[HEAD_PARTS];              // HP_ROWS: the part's rows; of a cache also [1] sink, [2] ring
+    const int32_t * pos;
+    uint32_t pos0, S, cap;
+};
+
+struct HeadBatch {
+    HeadPart part[HEAD_PARTS];
+    HeadSeq seq[HEAD_SEQS];
+    const double * turns;
+    const int32_t * desc;
+    size_t stage_bytes;
+    int n_parts, n_seqs, n_pos, D, iters, units;       // units: wavefronts of one sequence
+    int layout, n_rot, H, sink_type;
+    float mscale, sine, rot_scale, inv_D;              // sine: the sign of sines (inverse)
+};
+
+static_assert(sizeof(HeadBatch) <= 4096, "the table travels in the kernel arguments");
+
+// sine and cosine of u turns, times m (sines also times sg)
+SJK_DEV void turn(double u, float m, float sg, float & s, float & c) {
+    u -= __builtin_rint(u);
+    const float q = __builtin_rintf(4.0f * (float) u);
+    const float r = (float) __builtin_fma((double) q, -0.25, u);        // |r| <= 1/8 (and an ulp)
+    const float z = r * r;
+    // Taylor series in r, coefficients (2 pi)^k / k!: the first term left out is below 3e-9 of the
+    // sine, 2e-10 of the cosine
+    float p = __builtin_fmaf(z, 42.058693944897654f, -76.70585975306138f);
+    p = __builtin_fmaf(z, p, 81.60524927607504f);
+    p = __builtin_fmaf(z, p, -41.341702240399755f);
+    const float sn = __builtin_fmaf(r * z, p, r * 6.283185307179586f);
+    p = __builtin_fmaf(z, -26.426256783374398f, 60.24464137187666f);
+    p = __builtin_fmaf(z, p, -85.45681720669373f);
+    p = __builtin_fmaf(z, p, 64.93939402266829f);
+    p = __builtin_fmaf(z, p, -19.739208802178716f);
+    const float cs = __builtin_fmaf(z, p, 1.0f);
+    const int k = (int) q;                                              // quarter turns, -2 .. 2
+    const float a = k & 1 ? cs : sn, b = k & 1 ? sn : cs;
+    s = (k & 2 ? -a : a) * m * sg;
+    c = ((k + 1) & 2 ? -b : b) * m;
+}
+
+// 8 channels of a row from its element e0 on, as raw words; elements behind D are zero
+template <typename T> struct Raw { uint32_t w[2 * sizeof(T)]; };
+template <typename T> SJK_DEV void load_row(Raw<T> & r, const T * p, int e0, int D, bool vec) {
+    constexpr int NW = 2 * (int) sizeof(T);
+#pragma unroll
+    for (int i = 0; i < NW; ++i) r.w[i] = 0;
+    if (vec) {
+        if (e0 < D) {
+#pragma unroll
+            for (int i = 0; i < NW; i += 4) {
+                const uint4 v = *(const uint4 *) ((const uint32_t *) (p + e0) + i);
+                r.w[i] = v.x; r.w[i + 1] = v.y; r.w[i + 2] = v.z; r.w[i + 3] = v.w;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int m = 0; m < 8; ++m)
+            if (e0 + m < D) {
+                if constexpr (sizeof(T) == 4) r.w[m] = __builtin_bit_cast(uint32_t, p[e0 + m]);
+                else r.w[m >> 1] |= (uint32_t) __builtin_bit_cast(uint16_t, p[e0 + m]) << (16 * (m & 1));
+            }
+    }
+}
+template <typename T> SJK_DEV float raw_at(const Raw<T> & r, int m) {
+    if constexpr (sizeof(T) == 4) return bits_f(r.w[m]);
+    else return (float) __builtin_bit_cast(T, (uint16_t) (r.w[m >> 1] >> (16 * (m & 1))));
+}
+
+SJK_DEV uint32_t pack16(uint16_t a, uint16_t b) { return (uint32_t) a | (uint32_t) b << 16; }
+
+// 8 channels of a row of `type`, one rounding (to nearest even)
+SJK_DEV void store_row(void * p, int type, const float (&x)[8], int e0, int D, bool vec) {
+    if (type == SJK_F32) {
+        float * o = (float *) p + e0;
+        if (vec) {
+            if (e0 < D) {
+                ((float4 *) o)[0] = float4{x[0], x[1], x[2], x[3]};
+                ((float4 *) o)[1] = float4{x[4], x[5], x[6], x[7]};
+            }
+        } else {
+#pragma unroll
+            for (int m = 0; m < 8; ++m) if (e0 + m < D) o[m] = x[m];
+        }
+        return;
+    }
+    uint16_t h[8];
+#pragma unroll
+    for (int m = 0; m < 8; ++m)
+        h[m] = type == SJK_F16 ? __builtin_bit_cast(uint16_t, (_Float16) x[m]) : __builtin_bit_cast(uint16_t, (__bf16) x[m]);
+    uint16_t * o = (uint16_t *) p + e0;
+    if (vec) {
+        if (e0 < D) *(uint4 *) o = uint4{pack16(h[0], h[1]), pack16(h[2], h[3]), pack16(h[4], h[5]), pack16(h[6], h[7])};
+    } else {
+#pragma unroll
+        for (int m = 0; m < 8; ++m) if (e0 + m < D) o[m] = h[m];
+    }
+}
+
+template <typename T, int LPR, int MODE>
+__global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
+    constexpr int RPW = 64 / LPR;                          // rows a wavefront holds
+    constexpr int BS = 132;                                // floats from a 128-value block to the next (walks: other banks)
+    constexpr int WS = MODE == HM_TQ6 ? 4 * BS : 512;      // floats of a wavefront's LDS
+    __shared__ alignas(16) float s_buf[HW * WS];
+    __shared__ float s_mid[MODE == HM_TQ6 ? 64 : 1], s_cent[MODE == HM_TQ6 ? 64 : 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane % LPR, sub = lane / LPR, e0 = 8 * l;
+    if (MODE == HM_TQ6) {
+        if (threadIdx.x < 64) {
+            s_mid[threadIdx.x] = threadIdx.x < 63 ? tq6_mid(threadIdx.x) : __builtin_inff();
+            s_cent[threadIdx.x] = tq6_cent(threadIdx.x);
+        }
+        __syncthreads();
+    }
+    // this wavefront's sequence, part and rows (wave-uniform)
+    int u = __builtin_amdgcn_readfirstlane((int) blockIdx.x * HW + wave);
+    const int si = u / bt.units;
+    if (si >= bt.n_seqs) return;
+    u -= si * bt.units;
+    int pi = 0;
+    while (pi + 1 < bt.n_parts && u >= bt.part[pi].n_units) u -= bt.part[pi++].n_units;
+    const HeadPart & P = bt.part[pi];
+    const HeadSeq & Q = bt.seq[si];
+    if (bt.desc && bt.desc[SJK_DESC_QPOS0] < 0) return;
+    const uint32_t pos0 = bt.desc ? (uint32_t) bt.desc[SJK_DESC_QPOS0] : Q.pos0;
+    const int D = bt.D, n_heads = P.n_heads, n_rows = bt.n_pos * n_heads;
+    const T * x_in = (const T *) Q.x[pi];
+    const bool xvec = P.flags & HF_XVEC, ovec = P.flags & HF_OVEC, rope = P.flags & HF_ROPE, rot = P.flags & HF_ROT;
+    float * buf = s_buf + wave * WS;
+
+    int row = u * bt.iters * RPW + sub;
+    int ip = row / n_heads, hh = row - ip * n_heads;
+    int at = -1;                                           // position whose sines and cosines the lane holds
+    float cs[8], sn[8], w[8];
+    const int n_rot = bt.n_rot, half = n_rot / 2;
+    auto load_w = [&](int h) {
+        const float * p = P.w + (int64_t) h * P.w_head;
+#pragma unroll
+        for (int m = 0; m < 8; ++m) w[m] = e0 + m < D ? p[e0 + m] : 0.0f;
+    };
+    if (P.w && !P.w_head) load_w(0);
+    Raw<T> raw;
+    if (row < n_rows) load_row<T>(raw, x_in + (int64_t) ip * P.x_pos + (int64_t) hh * P.x_head, e0, D, xvec);
+
+    for (int it = 0; it < bt.iters; ++it) {
+        const bool live = row < n_rows;
+        if (!__any(live)) break;
+        float x[8];
+#pragma unroll
+        for (int m = 0; m < 8; ++m) x[m] = live ? raw_at<T>(raw, m) : 0.0f;
+        const int cp = ip, ch = hh;
+        row += RPW;
+        for (hh += RPW; hh >= n_heads; hh -= n_heads) ++ip;
+        if (it + 1 < bt.iters && row < n_rows)
+            load_row<T>(raw, x_in + (int64_t) ip * P.x_pos + (int64_t) hh * P.x_head, e0, D, xvec);
+
+        if (P.w) {
+            if (P.w_head && live) load_w(ch);
+            float ss = ((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])) +
+                       ((x[4] * x[4] + x[5] * x[5]) + (x[6] * x[6] + x[7] * x[7]));
+            ss += lane_xor<1>(ss, lane);
+            ss += lane_xor<2>(ss, lane);
+            ss += lane_xor<4>(ss, lane);
+            if constexpr (LPR > 8) ss += lane_xor<8>(ss, lane);
+            if constexpr (LPR > 16) ss += lane_xor<16>(ss, lane);
+            if constexpr (LPR > 32) ss += lane_xor<32>(ss, lane);
+            const float r = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, bt.inv_D, P.eps));
+#pragma unroll
+            for (int m = 0; m < 8; ++m) x[m] = x[m] * r * w[m];
+        }
+
+        if (rope) {
+            if (live && cp != at) {
+                at = cp;
+                const double p = Q.pos ? (double) Q.pos[cp] : (double) (pos0 + (uint32_t) cp);
+                if (bt.layout == SJK_ROPE_PAIRS) {
+#pragma unroll
+                    for (int m = 0; m < 8; m += 2) {
+                        if (e0 + m < n_rot) turn(p * bt.turns[(e0 + m) >> 1], bt.mscale, bt.sine, sn[m], cs[m]);
+                        cs[m + 1] = cs[m];
+                        sn[m + 1] = sn[m];
+                        sn[m] = -sn[m];
+                    }
+                } else {
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) {
+                        const int e = e0 + m;
+                        if (e < n_rot) {
+                            turn(p * bt.turns[e < half ? e : e - half], bt.mscale, bt.sine, sn[m], cs[m]);
+                            if (e < half) sn[m] = -sn[m];
+                        }
+                    }
+                }
+            }
+            float y[8];                                    // the other channel of each pair
+            if (bt.layout == SJK_ROPE_PAIRS) {
+#pragma unroll
+                for (int m = 0; m < 8; ++m) y[m] = x[m ^ 1];
+            } else if (n_rot == 8 * LPR) {
+#pragma unroll
+                for (int m = 0; m < 8; ++m) y[m] = lane_xor<LPR / 2>(x[m], lane);
+            } else {
+                // channel e in slot (e % 8) * 64 + sub * LPR + e / 8: both sides touch neighbouring words
+                wave_sync();
+#pragma unroll
+                for (int m = 0; m < 8; ++m) buf[m * 64 + lane] = x[m];
+                wave_sync();
+#pragma unroll
+                for (int m = 0; m < 8; ++m) {
+                    const int e = e0 + m, pe = e < half ? e + half : e < n_rot ? e - half : e;
+                    y[m] = buf[(pe & 7) * 64 + sub * LPR + (pe >> 3)];
+                }
+                wave_sync();
+            }
+#pragma unroll
+            for (int m = 0; m < 8; ++m)
+                if (e0 + m < n_rot) x[m] = __builtin_fmaf(x[m], cs[m], y[m] * sn[m]);
+        }
+
+        // a row holding an infinity or a NaN takes the rotation and the tq6_0 sums with the host's NaN rule
+        bool xn = false;
+        uint64_t nf_rows = 0;
+        if (rot || MODE == HM_TQ6) {
+            bool nf = false;
+#pragma unroll
+            for (int m = 0; m < 8; ++m) nf |= (f_bits(x[m]) & 0x7F800000u) == 0x7F800000u;
+            nf_rows = __ballot(nf);
+            xn = ((LPR == 64 ? nf_rows : nf_rows >> (sub * LPR)) & ((LPR == 64 ? 0 : 1ull << (LPR % 64)) - 1ull)) != 0;
+        }
+        if (rot) {
+            if (nf_rows) hadamard_row<8, LPR, true>(x, lane, bt.rot_scale, xn);
+            else hadamard_row<8, LPR, false>(x, lane, bt.rot_scale);
+        }
+
+        if (MODE == HM_ROWS || P.kind == HP_ROWS) {
+            if (live) {
+                const size_t size = P.o_type == SJK_F32 ? 4 : 2;
+                store_row((uint8_t *) Q.o[pi] + size * (size_t) ((int64_t) cp * P.o_pos + (int64_t) ch * P.o_head), P.o_type, x, e0, D, ovec);
+            }
+            continue;
+        }
+        if constexpr (MODE != HM_ROWS) {
+            // the cache's entry of this position and head: sink, or the ring's slot
+            const uint32_t pos = pos0 + (uint32_t) cp;
+            const bool in_sink = pos < Q.S, sink_f16 = in_sink && bt.sink_type == SJKVARN_SINK_F16;
+            const int side = P.kind == HP_V;
+            uint8_t * dst = sink_f16 ? (uint8_t *) Q.o[1] + ((size_t) pos * bt.H + ch) * 4 * D + (size_t) side * 2 * D
+                            : (in_sink ? (uint8_t *) Q.o[1] + ((size_t) pos * bt.H + ch) * 2 * bt.stage_bytes
+                                       : (uint8_t *) Q.o[2] + ((size_t) ((pos - Q.S) % Q.cap) * bt.H + ch) * 2 * bt.stage_bytes) +
+                                  (size_t) side * bt.stage_bytes;
+            if (live && (MODE == HM_F16 || sink_f16)) {
+                uint16_t h[8];
+#pragma unroll
+                for (int m = 0; m < 8; ++m) h[m] = f32_to_f16(x[m]);
+                uint16_t * o = (uint16_t *) dst + e0;
+                if (ovec) *(uint4 *) o = uint4{pack16(h[0], h[1]), pack16(h[2], h[3]), pack16(h[4], h[5]), pack16(h[6], h[7])};
+                else {
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) o[m] = h[m];
+                }
+            }
+            if constexpr (MODE == HM_TQ6) {
+                const bool tq = live && !sink_f16;
+                if (!__any(tq)) continue;
+                // sj_kvarn.h:1221-1247: two sums of 128 values in index order, walked by every lane of the block (16 lanes)
+                float * blk = buf + (lane >> 4) * BS, * sq = blk + 8 * (lane & 15);
+                wave_sync();
+#pragma unroll
+                for (int m = 0; m < 8; ++m) sq[m] = xn ? xmul(x[m], x[m]) : x[m] * x[m];
+                wave_sync();
+                const float nsq = nf_rows ? walk<true>(blk, xn) : walk<false>(blk);
+                const float norm = nsq != nsq ? nan_of(nsq) : __builtin_sqrtf(nsq);
+                const bool big = norm > 1e-10f;
+                const float inv = big ? 1.0f / norm : 0.0f;
+                int code[8];
+#pragma unroll
+                for (int m = 0; m < 8; ++m) code[m] = tq6_level(big ? x[m] * inv : 0.0f, s_mid);
+                wave_sync();
+#pragma unroll
+                for (int m = 0; m < 8; ++m) { const float c = s_cent[code[m]]; sq[m] = c * c; }
+                wave_sync();
+                const float rn = __builtin_sqrtf(walk<false>(blk));
+                wave_sync();
+                if (tq) {
+                    uint8_t * o = dst + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES;
+                    const int i0 = 8 * (l & 15);
+                    if (!(l & 15)) *(uint16_t *) o = f32_to_f16(rn > 1e-10f ? xdiv(norm, rn) : norm);
+                    uint32_t qs = 0, qh = 0;               // low nibbles; high pairs
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) {
+                        qs |= (uint32_t) (code[m] & 15) << (4 * m);
+                        qh |= (uint32_t) ((code[m] >> 4) & 3) << (2 * m);
+                    }
+                    *(uint16_t *) (o + 2 + i0 / 2) = (uint16_t) qs;
+                    *(uint16_t *) (o + 4 + i0 / 2) = (uint16_t) (qs >> 16);
+                    *(uint16_t *) (o + 66 + i0 / 4) = (uint16_t) qh;
+                }
+            }
+        }
+    }
+}
+
+static int refuse(const char * what) {
+    set_error(what);
+    return SJKVARN_ERR_ARG;
+}
+
+static size_t elem_size(int type) { return type == SJK_F32 ? 4 : 2; }
+static bool type_ok(int type) { return type == SJK_F32 || type == SJK_F16 || type == SJK_BF16; }
+// rows at p with strides in elements of `size` bytes can be read and written 16 bytes at a time
+static bool wide(const void * p, int64_t pos, int64_t head, size_t size, int D) {
+    return D % 8 == 0 && !((uintptr_t) p & 15u) && !((uint64_t) pos * size & 15u) && !((uint64_t) head * size & 15u);
+}
+
+static int rope_ok(const sjk_hip_rope & r, int D) {
+    if (r.n_rot == 0) return 0;
+    if ((r.layout != SJK_ROPE_HALVES && r.layout != SJK_ROPE_PAIRS) || r.n_rot < 0 || r.n_rot > D || r.n_rot % 2)
+        return refuse("rotary positions: a layout of SJK_ROPE_HALVES or _PAIRS and an even n_rot up to the head's width");
+    if (!r.d_turns || (uintptr_t) r.d_turns % 8 || !__builtin_isfinite(r.mscale))
+        return refuse("rotary positions: a table of turns (device, 8-byte aligned) and a finite mscale");
+    return 0;
+}
+
+static int norm_ok(const float * w, float eps) {
+    if (!w) return 0;
+    if ((uintptr_t) w % 4 || !(eps > 0.0f) || !__builtin_isfinite(eps)) return refuse("head norms: fp32 weights and a finite eps > 0");
+    return 0;
+}
+
+static void set_rope(HeadBatch & bt, const sjk_hip_rope & r) {
+    bt.layout = r.layout;
+    bt.n_rot = r.n_rot;
+    bt.turns = r.d_turns;
+    bt.mscale = r.mscale;
+    bt.sine = r.inverse ? -1.0f : 1.0f;
+}
+
+template <typename T>
+static int launch_typed(const HeadBatch & bt, int lpr, int mode, unsigned grid, hipStream_t st) {
+    const dim3 g(grid), b(64 * HW);
+#define SJK_HEADS(L, M) hipLaunchKernelGGL((heads_kernel<T, L, M>), g, b, 0, st, bt)
+    if (mode == HM_ROWS) {
+        if (lpr == 8) SJK_HEADS(8, HM_ROWS);
+        else if (lpr == 16) SJK_HEADS(16, HM_ROWS);
+        else if (lpr == 32) SJK_HEADS(32, HM_ROWS);
+        else SJK_HEADS(64, HM_ROWS);
+    } else if (mode == HM_F16) {
+        if (lpr == 16) SJK_HEADS(16, HM_F16);
+        else SJK_HEADS(32, HM_F16);
+    } else {
+        if (lpr == 16) SJK_HEADS(16, HM_TQ6);
+        else SJK_HEADS(32, HM_TQ6);
+    }
+#undef SJK_HEADS
+    return SJK_CHECK_LAUNCH();
+}
+
+// The launch's shape: a wavefront takes `iters` groups of rows, so that the sines and cosines of a position serve
+// several of its heads, once there are more wavefronts than the device holds resident
+static int launch_heads(HeadBatch & bt, int type, int mode, hipStream_t st) {
+    const int lpr = bt.D <= 64 ? 8 : bt.D <= 128 ? 16 : bt.D <= 256 ? 32 : 64, rpw = 64 / lpr;
+    int64_t groups = 0;
+    for (int p = 0; p < bt.n_parts; ++p) groups += ((int64_t) bt.n_pos * bt.part[p].n_heads + rpw - 1) / rpw;
+    groups *= bt.n_seqs;
+    if (!groups) return 0;
+    const int64_t it = groups / ((int64_t) n_cus() * 4 * HW);
+    bt.iters = it < 1 ? 1 : it > HEAD_ITERS ? HEAD_ITERS : (int) it;
+    bt.units = 0;
+    for (int p = 0; p < bt.n_parts; ++p) {
+        const int64_t per = (int64_t) rpw * bt.iters;
+        bt.part[p].n_units = (int) (((int64_t) bt.n_pos * bt.part[p].n_heads + per - 1) / per);
+        bt.units += bt.part[p].n_units;
+    }
+    bt.inv_D = 1.0f / (float) bt.D;
+    bt.rot_scale = rot_scale(bt.D);
+    const unsigned grid = (unsigned) (((int64_t) bt.units * bt.n_seqs + HW - 1) / HW);
+    if (type == SJK_F32) return launch_typed<float>(bt, lpr, mode, grid, st);
+    if (type == SJK_F16) return launch_typed<_Float16>(bt, lpr, mode, grid, st);
+    return launch_typed<__bf16>(bt, lpr, mode, grid, st);
+}
+
+// rows of a launch are counted in 32 bits
+static bool rows_fit(uint64_t n_pos, uint64_t heads, uint64_t seqs) { return n_pos <= 0x7fffffffu && n_pos * heads * seqs <= 0x7fffffffu; }
+
+}  // namespace sjk
+
+using namespace sjk;
+
+extern "C" int sjk_hip_head_rows(const sjk_hip_head_job * jobs, int n_jobs, uint32_t n_pos, int D, const sjk_hip_rope * rope,
+                                 uint32_t pos0, const int32_t * d_pos, void * stream) {
+    if (n_jobs < 0 || (n_jobs > 0 && !jobs)) return SJKVARN_ERR_ARG;
+    if (D < 1 || D > 512) return refuse("sjk_hip_head_rows: head widths 1 to 512");
+    if (d_pos && (uintptr_t) d_pos % 4) return SJKVARN_ERR_ARG;
+    uint64_t heads = 0;
+    for (int k = 0; k < n_jobs; ++k) {
+        const sjk_hip_head_job & J = jobs[k];
+        if (!J.d_x || !J.d_out || J.n_heads < 0 || !type_ok(J.x_type) || !type_ok(J.out_type)) return SJKVARN_ERR_ARG;
+        if ((uintptr_t) J.d_x % elem_size(J.x_type) || (uintptr_t) J.d_out % elem_size(J.out_type)) return SJKVARN_ERR_ARG;
+        int rc = norm_ok(J.d_norm, J.eps);
+        if (!rc && J.rope) rc = rope ? rope_ok(*rope, D) : refuse("sjk_hip_head_rows: a job turns its rows and rope is NULL");
+        if (rc) return rc;
+        if (J.rotate && D != 64 && D != 128 && D != 256 && D != 512) {
+            set_error("sjk_hip_head_rows: the rotation needs a head width of 64, 128, 256 or 512");
+            return SJK_ERR_UNSUPPORTED;
+        }
+        heads += (uint64_t) J.n_heads;
+    }
+    if (!rows_fit(n_pos, heads, 1)) return refuse("sjk_hip_head_rows: more than 2^31 - 1 rows");
+    for (int k0 = 0; k0 < n_jobs;) {
+        HeadBatch bt = {};
+        bt.n_pos = (int) n_pos;
+        bt.D = D;
+        bt.n_seqs = 1;
+        bt.seq[0].pos = d_pos;
+        bt.seq[0].pos0 = pos0;
+        if (rope) set_rope(bt, *rope);
+        int k = k0;
+        for (; k < n_jobs && k - k0 < HEAD_PARTS && jobs[k].x_type == jobs[k0].x_type; ++k) {
+            const sjk_hip_head_job & J = jobs[k];
+            HeadPart & P = bt.part[bt.n_parts];
+            P.x_pos = J.x_pos; P.x_head = J.x_head; P.o_pos = J.out_pos; P.o_head = J.out_head;
+            P.w = J.d_norm; P.w_head = J.norm_head; P.eps = J.eps;
+            P.n_heads = J.n_heads; P.kind = HP_ROWS; P.o_type = J.out_type;
+            P.flags = (wide(J.d_x, J.x_pos, J.x_head, elem_size(J.x_type), D) ? HF_XVEC : 0) |
+                      (wide(J.d_out, J.out_pos, J.out_head, elem_size(J.out_type), D) ? HF_OVEC : 0) |
+                      (J.rope && rope->n_rot ? HF_ROPE : 0) | (J.rotate ? HF_ROT : 0);
+            bt.seq[0].x[bt.n_parts] = J.d_x;
+            bt.seq[0].o[bt.n_parts] = J.d_out;
+            if (J.n_heads) ++bt.n_parts;
+        }
+        const int rc = n_pos && bt.n_parts ? launch_heads(bt, jobs[k0].x_type, HM_ROWS, (hipStream_t) stream) : 0;
+        if (rc) return rc;
+        k0 = k;
+    }
+    return 0;
+}
+
+namespace sjk {
+
+// the checks of one store_qkv call that need no device
+static int qkv_ok(const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t pos0, uint32_t n_pos, const int32_t * d_pos, const void * d_q,
+                  const void * d_k, const void * d_v, const float * d_q_out) {
+    const int D = v.lay.D, H = v.n_head_kv;
+    if (!d_k || !d_v || !v.sink || !v.ring || v.cap == 0 || H <= 0 || m.n_head < 0 || !type_ok(m.type)) return SJKVARN_ERR_ARG;
+    if (m.n_head && (!d_q || !d_q_out)) return SJKVARN_ERR_ARG;
+    if (D != 128 && D != 256) {
+        set_error("sjk_hip_store_qkv: head_dim 128 or 256");
+        return SJK_ERR_UNSUPPORTED;
+    }
+    if ((v.staging != SJKVARN_STAGING_TQ6_0 && v.staging != SJKVARN_STAGING_F16) || v.stage_bytes != sj_kvarn_stage_row_bytes(v.staging, D) ||
+        (v.sink_type != SJKVARN_SINK_F16 && v.sink_type != SJKVARN_SINK_INHERIT))
+        return SJKVARN_ERR_ARG;
+    const size_t size = elem_size(m.type);
+    if (((uintptr_t) d_k | (uintptr_t) d_v | (m.n_head ? (uintptr_t) d_q : 0)) % size || (uintptr_t) d_q_out % 4 || (uintptr_t) d_pos % 4 ||
+        (((uintptr_t) v.sink | (uintptr_t) v.ring) & 1u))
+        return SJKVARN_ERR_ARG;
+    if ((uint64_t) pos0 + n_pos > 0xffffffffull) return refuse("sjk_hip_store_qkv: positions past 2^32 - 1");
+    const uint64_t room = (uint64_t) v.cap + (pos0 < v.S ? v.S - pos0 : 0);
+    if (n_pos > room) {
+        set_error("sjk_hip_store_qkv: more positions than sink and ring hold at once");
+        return SJKVARN_ERR_CAPACITY;
+    }
+    if (!rows_fit(n_pos, (uint64_t) m.n_head + 2u * (uint64_t) H, HEAD_SEQS)) return refuse("sjk_hip_store_qkv: more than 2^31 - 1 rows");
+    int rc = norm_ok(m.n_head ? m.d_q_norm : nullptr, m.eps);
+    if (!rc) rc = norm_ok(m.d_k_norm, m.eps);
+    if (!rc) rc = rope_ok(m.rope, D);
+    return rc;
+}
+
+// the launch's table without its sequences; vec: every sequence's rows of the part can be read / written wide
+static void qkv_table(HeadBatch & bt, const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t n_pos) {
+    const int D = v.lay.D;
+    bt.n_pos = (int) n_pos;
+    bt.D = D;
+    bt.n_parts = HEAD_PARTS;
+    bt.H = v.n_head_kv;
+    bt.sink_type = v.sink_type;
+    bt.stage_bytes = v.stage_bytes;
+    set_rope(bt, m.rope);
+    const int qk = (m.rope.n_rot ? HF_ROPE : 0) | (m.rotate_qk ? HF_ROT : 0);
+    const int64_t pos[3] = {m.q_pos, m.k_pos, m.v_pos}, head[3] = {m.q_head, m.k_head, m.v_head};
+    const float * w[3] = {m.d_q_norm, m.d_k_norm, nullptr};
+    for (int p = 0; p < HEAD_PARTS; ++p) {
+        HeadPart & P = bt.part[p];
+        P.x_pos = pos[p]; P.x_head = head[p];
+        P.o_pos = (int64_t) m.n_head * D; P.o_head = D;
+        P.w = w[p]; P.w_head = m.norm_head; P.eps = m.eps;
+        P.n_heads = p ? v.n_head_kv : m.n_head;
+        P.kind = p; P.o_type = SJK_F32;
+        P.flags = (p < 2 ? qk : m.rotate_v ? HF_ROT : 0) | HF_XVEC | HF_OVEC;
+    }
+}
+
+static void qkv_seq(HeadBatch & bt, const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t pos0, const int32_t * d_pos, const void * d_q,
+                    const void * d_k, const void * d_v, float * d_q_out) {
+    HeadSeq & Q = bt.seq[bt.n_seqs++];
+    const void * x[3] = {d_q, d_k, d_v};
+    const size_t size = elem_size(m.type);
+    const bool cache = !(((uintptr_t) v.sink | (uintptr_t) v.ring) & 15u);
+    for (int p = 0; p < HEAD_PARTS; ++p) {
+        HeadPart & P = bt.part[p];
+        Q.x[p] = x[p];
+        if (!wide(x[p], P.x_pos, P.x_head, size, bt.D)) P.flags &= ~HF_XVEC;
+        if (!(p ? cache : wide(d_q_out, P.o_pos, P.o_head, 4, bt.D))) P.flags &= ~HF_OVEC;
+    }
+    Q.o[0] = d_q_out; Q.o[1] = v.sink; Q.o[2] = v.ring;
+    Q.pos = d_pos; Q.pos0 = pos0; Q.S = v.S; Q.cap = v.cap;
+}
+
+static int qkv_launch(HeadBatch & bt, const sjk_hip_view & v, int type, hipStream_t st) {
+    if (!bt.n_pos) return 0;
+    return launch_heads(bt, type, v.staging == SJKVARN_STAGING_F16 ? HM_F16 : HM_TQ6, st);
+}
+
+}  // namespace sjk
+
+extern "C" int sjk_hip_store_qkv(const sjk_hip_view * v, uint32_t pos0, uint32_t n_pos, const sjk_hip_qkv * m, const int32_t * d_pos,
+                                 const void * d_q, const void * d_k, const void * d_v, float * d_q_out, void * stream) {
+    if (!v || !m) return SJKVARN_ERR_ARG;
+    const int rc = qkv_ok(*v, *m, pos0, n_pos, d_pos, d_q, d_k, d_v, d_q_out);
+    if (rc) return rc;
+    HeadBatch bt = {};
+    qkv_table(bt, *v, *m, n_pos);
+    qkv_seq(bt, *v, *m, pos0, d_pos, d_q, d_k, d_v, d_q_out);
+    return qkv_launch(bt, *v, m->type, (hipStream_t) stream);
+}
+
+extern "C" int sjk_hip_store_qkv_dyn(const sjk_hip_view * v, const int32_t * d_desc, uint32_t n_pos, const sjk_hip_qkv * m,
+                                     const int32_t * d_pos, const void * d_q, const void * d_k, const void * d_v, float * d_q_out,
+                                     void * stream) {
+    if (!v || !m || !d_desc) return SJKVARN_ERR_ARG;
+    // the positions are not known here: as for one that starts behind the sink
+    const int rc = qkv_ok(*v, *m, v->S, n_pos, d_pos, d_q, d_k, d_v, d_q_out);
+    if (rc) return rc;
+    HeadBatch bt = {};
+    qkv_table(bt, *v, *m, n_pos);
+    qkv_seq(bt, *v, *m, 0, d_pos, d_q, d_k, d_v, d_q_out);
+    bt.desc = d_desc;
+    return qkv_launch(bt, *v, m->type, (hipStream_t) stream);
+}
+
+extern "C" int sjk_hip_store_qkv_batch(const sjk_hip_qkv_job * jobs, int n_jobs, uint32_t n_pos, const sjk_hip_qkv * m, void * stream) {
+    if (n_jobs < 0 || (n_jobs > 0 && !jobs) || !m) return SJKVARN_ERR_ARG;
+    for (int k = 0; k < n_jobs; ++k) {
+        const sjk_hip_qkv_job & J = jobs[k];
+        const int rc = J.v.lay.D != jobs[0].v.lay.D ? SJKVARN_ERR_ARG
+                                                    : qkv_ok(J.v, *m, J.pos0, n_pos, J.d_pos, J.d_q, J.d_k, J.d_v, J.d_q_out);
+        if (rc) return rc;
+    }
+    // two jobs on one ring could write one slot
+    for (int k = 1; k < n_jobs; ++k)
+        for (int i = 0; i < k; ++i)
+            if (jobs[i].v.ring == jobs[k].v.ring) return refuse("sjk_hip_store_qkv_batch: two jobs on one ring");
+    for (int k = 0; k < n_jobs;) {
+        const sjk_hip_view & v = jobs[k].v;
+        HeadBatch bt = {};
+        qkv_table(bt, v, *m, n_pos);
+        for (; k < n_jobs && bt.n_seqs < HEAD_SEQS; ++k) {
+            const sjk_hip_qkv_job & J = jobs[k];
+            if (J.v.n_head_kv != v.n_head_kv || J.v.staging != v.staging || J.v.sink_type != v.sink_type) break;
+            qkv_seq(bt, J.v, *m, J.pos0, J.d_pos, J.d_q, J.d_k, J.d_v, J.d_q_out);
+        }
+        const int rc = qkv_launch(bt, v, m->type, (hipStream_t) stream);
+        if (rc) return rc;
+    }
+    return 0;
+}

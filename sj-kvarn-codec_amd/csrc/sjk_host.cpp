@@ -309,6 +309,43 @@ size_t sj_kvarn_stage_row_bytes(int staging, int D) {
 }
 
 // ---------------------------------------------------------------------------------------------------
+// rotary frequencies: host arithmetic in double, as a program makes its tables once
+// ---------------------------------------------------------------------------------------------------
+
+int sjk_rope_turns(const sjk_rope_config * c, double * turns, float * mscale) {
+    const auto pos = [](double v) { return v > 0 && std::isfinite(v); };
+    if (!c || !turns || c->n_rot < 0 || c->n_rot % 2 || c->scaling < SJK_ROPE_PLAIN || c->scaling > SJK_ROPE_BANDS || !pos(c->base) ||
+        c->base <= 1)
+        return SJKVARN_ERR_ARG;
+    const bool ramp = c->scaling == SJK_ROPE_RAMP, bands = c->scaling == SJK_ROPE_BANDS;
+    if (c->scaling != SJK_ROPE_PLAIN && (!pos(c->factor) || (ramp && c->factor < 1))) return SJKVARN_ERR_ARG;
+    if ((ramp || bands) && (!pos(c->n_orig) || !pos(c->low) || !pos(c->high) || c->low >= c->high)) return SJKVARN_ERR_ARG;
+    const int n = c->n_rot;
+    for (int i = 0; c->divisors && i < n / 2; ++i) if (!pos(c->divisors[i])) return SJKVARN_ERR_ARG;
+    const double two_pi = 6.283185307179586476925, f = c->factor;
+    const bool ntk = c->scaling == SJK_ROPE_NTK && n > 2;
+    const double base = ntk ? c->base * std::pow(f, (double) n / (n - 2)) : c->base;
+    double a = 0, b = 0;                                  // ramp: from pair a to pair b
+    if (ramp) {
+        a = std::floor(n * std::log(c->n_orig / (c->high * two_pi)) / (2 * std::log(base)));
+        b = std::ceil(n * std::log(c->n_orig / (c->low * two_pi)) / (2 * std::log(base)));
+        if (a < 0) a = 0;
+        if (b > n - 1) b = n - 1;
+    }
+    for (int i = 0; i < n / 2; ++i) {
+        double w = std::pow(base, -2.0 * i / n), x = 1;   // x: the share of the unscaled frequency
+        if (c->divisors) w /= c->divisors[i];
+        if (c->scaling == SJK_ROPE_LINEAR || (c->scaling == SJK_ROPE_NTK && !ntk)) x = 0;
+        if (ramp) x = 1 - (i - a) / (b - a > 0.001 ? b - a : 0.001);
+        if (bands) x = (c->n_orig * w / two_pi - c->low) / (c->high - c->low);
+        x = x < 0 ? 0 : x > 1 ? 1 : x;
+        turns[i] = (x == 1 ? w : w / f * (1 - x) + w * x) / two_pi;
+    }
+    if (mscale) *mscale = ramp ? (float) (0.1 * std::log(f) + 1) : 1.0f;
+    return 0;
+}
+
+// ---------------------------------------------------------------------------------------------------
 // codec calls on host arrays (device round trip)
 // ---------------------------------------------------------------------------------------------------
 
@@ -686,11 +723,12 @@ void sj_kvarn_layer_attend_row(const sj_kvarn_layer * L, uint32_t B, uint32_t N,
 }
 
 // The byte ranges a truncation clears in one layer (sj_kvarn.h:1581-1603): the records of groups [B_new, B_old)
-// (in pool mode only the blocks the sequence holds), the sink entries of positions [resume, min(n_old, S)) and
+// (in pool mode only the blocks the sequence holds, and with `pool` only those it holds alone), the sink entries of positions [resume, min(n_old, S)) and
 // the ring rows of positions [max(resume, S), n_old) that can still be resident (the last cap of them), as
 // contiguous runs.
+static bool pool_shared(const sj_kvarn_pool * pool, uint32_t id);
 static void truncate_runs(const sj_kvarn_layer * L, uint32_t B_old, uint32_t B_new, uint32_t n_old, uint32_t resume,
-                          std::vector<sjk::CopyRun> & runs) {
+                          std::vector<sjk::CopyRun> & runs, const sj_kvarn_pool * pool = nullptr) {
     const uint32_t S = L->cfg.sink, G = (uint32_t) L->cfg.group;
     const size_t H = (size_t) L->cfg.n_head_kv;
     auto add = [&](const uint8_t * p, size_t n) {
@@ -702,6 +740,7 @@ static void truncate_runs(const sj_kvarn_layer * L, uint32_t B_old, uint32_t B_n
     if (B_new < B_old)
         for (uint32_t g = (B_new - S) / G; g < (B_old - S) / G; ++g) {
             if (L->blocks && L->blocks[g] == SJKVARN_NO_BLOCK) continue;
+            if (L->blocks && pool && pool_shared(pool, L->blocks[g])) continue;
             add(sj_kvarn_layer_record(L, g, 0), H * L->lay.bytes);
         }
     const uint32_t se = n_old < S ? n_old : S;
@@ -795,13 +834,16 @@ int sj_kvarn_pool_init(sj_kvarn_pool * pool, const sj_kvarn_config * cfg, int n_
     pool->n_layers = n_layers;
     pool->n_blocks = n_blocks;
     const size_t body_b = (size_t) n_layers * n_blocks * (size_t) cfg->n_head_kv * pool->lay.bytes;
-    pool->free_ids = (uint32_t *) malloc((size_t) n_blocks * sizeof(uint32_t));
+    pool->free_ids = (uint32_t *) malloc(2 * (size_t) n_blocks * sizeof(uint32_t));   // and the shared counts behind them
     if (!pool->free_ids || hipMalloc((void **) &pool->body, body_b) != hipSuccess ||
         hipMemset(pool->body, 0, body_b) != hipSuccess) {
         sj_kvarn_pool_free(pool);
         return SJKVARN_ERR_NOMEM;
     }
-    for (uint32_t i = 0; i < n_blocks; ++i) pool->free_ids[i] = n_blocks - 1u - i;  // LIFO: block 0 first
+    for (uint32_t i = 0; i < n_blocks; ++i) {
+        pool->free_ids[i] = n_blocks - 1u - i;      // LIFO: block 0 first
+        pool->free_ids[n_blocks + i] = 0;
+    }
     pool->n_free = n_blocks;
     return 0;
 }
@@ -816,8 +858,20 @@ void sj_kvarn_pool_free(sj_kvarn_pool * pool) {
 
 uint32_t sj_kvarn_pool_alloc(sj_kvarn_pool * pool) { return pool->n_free ? pool->free_ids[--pool->n_free] : SJKVARN_NO_BLOCK; }
 
+// Holders of a block beyond its first (sequences forked from the one that sealed it): kept behind the free list, so that
+// the reference's struct stays as it is
+static uint32_t * pool_extra(const sj_kvarn_pool * pool) { return pool->free_ids + pool->n_blocks; }
+static bool pool_shared(const sj_kvarn_pool * pool, uint32_t id) { return id < pool->n_blocks && pool_extra(pool)[id] != 0; }
+
 void sj_kvarn_pool_release(sj_kvarn_pool * pool, uint32_t id) {
+    if (pool_shared(pool, id)) { --pool_extra(pool)[id]; return; }
     if (id != SJKVARN_NO_BLOCK && pool->n_free < pool->n_blocks) pool->free_ids[pool->n_free++] = id;
+}
+
+uint32_t sjk_hip_pool_refs(const sj_kvarn_pool * pool, uint32_t id) {
+    if (!pool || !pool->free_ids || id >= pool->n_blocks) return 0;
+    for (uint32_t i = 0; i < pool->n_free; ++i) if (pool->free_ids[i] == id) return 0;
+    return pool_extra(pool)[id] + 1u;
 }
 
 // the device copy of a sequence's block table lives in layers[0].work (shared by every layer): entries [g0, g1)
@@ -884,6 +938,14 @@ static int seq_release(sj_kvarn_seq * s, uint32_t g0, uint32_t g1) {
     return seq_sync_blocks(s, g0, g1);
 }
 
+// the blocks that releasing everything the sequence holds would free
+static uint32_t seq_held_alone(const sj_kvarn_seq * s) {
+    uint32_t held = 0;
+    for (uint32_t g = 0; g < s->layers[0].n_groups; ++g)
+        held += s->blocks[g] != SJKVARN_NO_BLOCK && !pool_shared(s->pool, s->blocks[g]);
+    return held;
+}
+
 // take pool blocks for groups [g0, g1) on the host; the caller copies the table's range to the device
 static int seq_reserve(sj_kvarn_seq * s, uint32_t g0, uint32_t g1) {
     if (!s->pool) return 0;
@@ -920,7 +982,7 @@ void sj_kvarn_seq_free(sj_kvarn_seq * s) {
 // the truncation scrub of every layer of a sequence in one launch
 static int seq_scrub(sj_kvarn_seq * s, uint32_t B_old, uint32_t B_new, uint32_t n_old, uint32_t resume) {
     std::vector<sjk::CopyRun> runs;
-    for (int il = 0; il < s->n_layers; ++il) truncate_runs(&s->layers[il], B_old, B_new, n_old, resume, runs);
+    for (int il = 0; il < s->n_layers; ++il) truncate_runs(&s->layers[il], B_old, B_new, n_old, resume, runs, s->pool);
     return zero_runs(rt_of(s), runs);
 }
 
@@ -1075,6 +1137,44 @@ int sjk_hip_seq_attend_batch(const sjk_hip_seq_job * jobs, int n_jobs, int il, i
         }
         const int rc = sjk_hip_attend_batch(aj, n, n_q, n_head, scale, stream);
         if (rc) return rc;
+    }
+    return 0;
+}
+
+int sjk_hip_seq_store_qkv_batch(const sjk_hip_seq_qkv_job * jobs, int n_jobs, int il, uint32_t n_pos, const sjk_hip_qkv * m,
+                                void * stream) {
+    if (n_jobs < 0 || (n_jobs > 0 && !jobs) || !m) return SJKVARN_ERR_ARG;
+    for (int k = 0; k < n_jobs; ++k) {
+        const sj_kvarn_seq * s = jobs[k].seq;
+        if (!s || il < 0 || il >= s->n_layers || jobs[k].pos0 > s->n) return SJKVARN_ERR_ARG;
+        const uint64_t end = (uint64_t) jobs[k].pos0 + n_pos;
+        if (end > s->pol.B && end - s->pol.B > s->layers[il].cap) {
+            sjk::set_error("sjk_hip_seq_store_qkv_batch: more staged positions than the ring holds");
+            return SJKVARN_ERR_CAPACITY;
+        }
+        for (int i = 0; i < k; ++i)
+            if (jobs[i].seq == s) {
+                sjk::set_error("sjk_hip_seq_store_qkv_batch: a sequence twice");
+                return SJKVARN_ERR_ARG;
+            }
+    }
+    constexpr int CHUNK = 32;
+    sjk_hip_qkv_job qj[CHUNK];
+    for (int k0 = 0; k0 < n_jobs; k0 += CHUNK) {
+        const int n = n_jobs - k0 < CHUNK ? n_jobs - k0 : CHUNK;
+        for (int k = 0; k < n; ++k) {
+            const sjk_hip_seq_qkv_job & J = jobs[k0 + k];
+            qj[k].v = sjk_layer_view(&J.seq->layers[il]);
+            qj[k].pos0 = J.pos0; qj[k].d_pos = J.d_pos;
+            qj[k].d_q = J.d_q; qj[k].d_k = J.d_k; qj[k].d_v = J.d_v; qj[k].d_q_out = J.d_q_out;
+        }
+        const int rc = sjk_hip_store_qkv_batch(qj, n, n_pos, m, stream);
+        if (rc) return rc;
+        for (int k = 0; k < n; ++k) {
+            sj_kvarn_seq * s = jobs[k0 + k].seq;
+            if (jobs[k0 + k].pos0 + n_pos > s->n) s->n = jobs[k0 + k].pos0 + n_pos;
+            rt_note_store(rt_of(s), (hipStream_t) stream);
+        }
     }
     return 0;
 }
@@ -1536,9 +1636,7 @@ static int state_read_checks(sj_kvarn_seq * s, const void * src, size_t size, sj
     if (t.n > c->n_ctx || n_rec > s->layers[0].n_groups || (t.n > t.B && t.n - t.B > s->layers[0].cap))
         return SJKVARN_ERR_CAPACITY;
     if (s->pool) {
-        uint32_t held = 0;
-        for (uint32_t g = 0; g < s->layers[0].n_groups; ++g) held += s->blocks[g] != SJKVARN_NO_BLOCK;
-        if (s->pool->n_free + held < n_rec) return SJKVARN_ERR_POOL_FULL;
+        if (s->pool->n_free + seq_held_alone(s) < n_rec) return SJKVARN_ERR_POOL_FULL;
     }
     *out = t;
     return 0;
@@ -1622,9 +1720,7 @@ static int state_job_wait(sj_kvarn_seq * s, size_t * written) {
     // the restore: the pool may have changed since _begin
     const uint32_t n_rec = (t.B - s->cfg.sink) / (uint32_t) s->cfg.group;
     if (s->pool) {
-        uint32_t held = 0;
-        for (uint32_t g = 0; g < s->layers[0].n_groups; ++g) held += s->blocks[g] != SJKVARN_NO_BLOCK;
-        if (s->pool->n_free + held < n_rec) return SJKVARN_ERR_POOL_FULL;
+        if (s->pool->n_free + seq_held_alone(s) < n_rec) return SJKVARN_ERR_POOL_FULL;
     }
     rc = state_read_prepare(s, t);
     if (!rc) rc = run_copy(r, image_runs(s, t.n, t.B, r->snap, false));
@@ -1634,5 +1730,182 @@ static int state_job_wait(sj_kvarn_seq * s, size_t * written) {
 }
 
 int sjk_hip_seq_state_finish(sj_kvarn_seq * s, size_t * written) { return state_job_wait(s, written); }
+
+// ---------------------------------------------------------------------------------------------------
+// forks and pool compaction (sjk_pages.hip moves the bytes)
+// ---------------------------------------------------------------------------------------------------
+
+// the first field of a configuration in which two sequences differ (the codes of a state read)
+static int same_config(const sj_kvarn_seq * a, const sj_kvarn_seq * b) {
+    const sj_kvarn_config * c = &a->cfg, * t = &b->cfg;
+    if (t->head_dim != c->head_dim) return SJKVARN_ERR_HEAD_DIM;
+    if (t->n_head_kv != c->n_head_kv) return SJKVARN_ERR_N_HEAD_KV;
+    if (t->group != c->group) return SJKVARN_ERR_GROUP;
+    if (t->sink != c->sink || t->sink_type != c->sink_type) return SJKVARN_ERR_SINK;
+    if (t->bits_k != c->bits_k || t->bits_v != c->bits_v) return SJKVARN_ERR_BITS;
+    if (t->body != c->body) return SJKVARN_ERR_BODY;
+    if (t->iters != c->iters) return SJKVARN_ERR_ITERS;
+    if (t->staging != c->staging) return SJKVARN_ERR_STAGING;
+    if (t->tail != c->tail || t->tail_max != c->tail_max || t->flush_chunk != c->flush_chunk) return SJKVARN_ERR_TAIL;
+    if (a->n_layers != b->n_layers) return SJKVARN_ERR_N_LAYERS;
+    return 0;
+}
+
+int sjk_hip_seq_fork(sj_kvarn_seq * child, sj_kvarn_seq * parent, uint32_t pos, uint32_t * kept, void * stream) {
+    if (!child || !parent || child == parent || !child->layers || !parent->layers || pos > parent->n) return SJKVARN_ERR_ARG;
+    Rt * rc = rt_of(child), * rp = rt_of(parent);
+    if (!rc || !rp) return SJKVARN_ERR_ARG;
+    if (rc->job || (rp->job && !rp->job->out)) {
+        sjk::set_error("sjk_hip_seq_fork: a state transfer of the child, or a restore of the parent, is in flight");
+        return SJKVARN_ERR_PENDING;
+    }
+    if (parent->pol.B_pending != parent->pol.B) return SJKVARN_ERR_PENDING;
+    int st = same_config(child, parent);
+    if (st) return st;
+    const uint32_t S = parent->cfg.sink, G = (uint32_t) parent->cfg.group;
+    bool empty = child->n == 0 && child->pol.B == S && child->pol.B_pending == S;
+    for (uint32_t g = 0; empty && child->pool && g < child->layers[0].n_groups; ++g) empty = child->blocks[g] == SJKVARN_NO_BLOCK;
+    if (!empty) {
+        sjk::set_error("sjk_hip_seq_fork: the child is not empty");
+        return SJKVARN_ERR_ARG;
+    }
+    // the child's policy: the parent's, cut at pos as a truncation cuts it
+    sj_kvarn_policy pol = parent->pol;
+    const uint32_t n = sj_kvarn_policy_truncate(&pol, pos, nullptr), n_rec = (pol.B - S) / G;
+    if (n > child->cfg.n_ctx || n_rec > child->layers[0].n_groups || (n > pol.B && n - pol.B > child->layers[0].cap))
+        return SJKVARN_ERR_CAPACITY;
+    const bool share = child->pool && child->pool == parent->pool;
+    if (child->pool && !share && child->pool->n_free < n_rec) return SJKVARN_ERR_POOL_FULL;
+    for (uint32_t g = 0; parent->pool && g < n_rec; ++g)
+        if (parent->blocks[g] >= parent->pool->n_blocks) return SJKVARN_ERR_ARG;
+
+    // the child's blocks, then the copies
+    uint32_t * ids = nullptr;
+    if (!share && n_rec && (!child->pool || !parent->pool)) {              // a body of its own per layer: block g at place g
+        ids = (uint32_t *) malloc((size_t) n_rec * 4);
+        if (!ids) return SJKVARN_ERR_NOMEM;
+        for (uint32_t g = 0; g < n_rec; ++g) ids[g] = g;
+    }
+    if (share) {
+        for (uint32_t g = 0; g < n_rec; ++g) {
+            child->blocks[g] = parent->blocks[g];
+            ++pool_extra(child->pool)[child->blocks[g]];
+        }
+    } else {
+        st = seq_reserve(child, 0, n_rec);
+        if (st) { free(ids); return st; }
+    }
+    const hipStream_t hs = (hipStream_t) stream;
+    constexpr int CHUNK = 64;
+    sjk_hip_view to[CHUNK], from[CHUNK];
+    for (int i0 = 0; i0 < child->n_layers && !st; i0 += CHUNK) {
+        const int nl = child->n_layers - i0 < CHUNK ? child->n_layers - i0 : CHUNK;
+        for (int k = 0; k < nl; ++k) { to[k] = sjk_layer_view(&child->layers[i0 + k]); from[k] = sjk_layer_view(&parent->layers[i0 + k]); }
+        st = sjk_hip_fork(to, from, nl, pol.B, n, stream);
+    }
+    if (!share && n_rec && !st) {
+        const uint32_t * src = parent->pool ? parent->blocks : ids, * dst = child->pool ? child->blocks : ids;
+        const size_t gb = (size_t) parent->cfg.n_head_kv * parent->layers[0].lay.bytes;
+        const uint32_t ns = parent->pool ? parent->pool->n_blocks : parent->layers[0].n_groups;
+        const uint32_t nd = child->pool ? child->pool->n_blocks : child->layers[0].n_groups;
+        if (child->pool && parent->pool) {
+            st = sjk_hip_copy_blocks(child->layers[0].body, nd * gb, nd, parent->layers[0].body, ns * gb, ns, child->n_layers, gb, src, dst,
+                                     n_rec, stream);
+        } else {
+            for (int il = 0; il < child->n_layers && !st; ++il)
+                st = sjk_hip_copy_blocks(child->layers[il].body, 0, nd, parent->layers[il].body, 0, ns, 1, gb, src, dst, n_rec, stream);
+        }
+    }
+    free(ids);
+    if (!st) st = seq_sync_blocks(child, 0, n_rec, hs, false);
+    rt_note_store(rc, hs);                                // the sequences' later scrubs, transfers and commits wait for the copies
+    rt_note_store(rp, hs);
+    if (st) {
+        for (uint32_t g = 0; child->pool && g < n_rec; ++g) {
+            sj_kvarn_pool_release(child->pool, child->blocks[g]);
+            child->blocks[g] = SJKVARN_NO_BLOCK;
+        }
+        return st;
+    }
+    child->pol = pol;
+    child->n = n;
+    if (kept) *kept = n;
+    return 0;
+}
+
+int sjk_hip_pool_compact(sj_kvarn_pool * pool, sj_kvarn_seq * const * seqs, int n_seqs, uint32_t * moved, void * stream) {
+    if (!pool || !pool->free_ids || !pool->body || n_seqs < 0 || (n_seqs > 0 && !seqs)) return SJKVARN_ERR_ARG;
+    const uint32_t nb = pool->n_blocks, n_live = nb - pool->n_free;
+    for (int k = 0; k < n_seqs; ++k) {
+        if (!seqs[k] || !seqs[k]->layers || seqs[k]->pool != pool || !rt_of(seqs[k])) return SJKVARN_ERR_ARG;
+        for (int i = 0; i < k; ++i)
+            if (seqs[i] == seqs[k]) return SJKVARN_ERR_ARG;
+        const Rt * r = rt_of(seqs[k]);
+        if (r->job && !r->job->out) {
+            sjk::set_error("sjk_hip_pool_compact: a state restore of a sequence is in flight");
+            return SJKVARN_ERR_PENDING;
+        }
+    }
+    // holders among the given sequences against the pool's counts; where[id]: the block's new place
+    struct Buf {
+        uint32_t * p;
+        explicit Buf(size_t n) : p((uint32_t *) calloc(n ? n : 1, 4)) {}
+        ~Buf() { free(p); }
+    } held(nb), where(nb), pairs(2 * (size_t) nb);
+    if (!held.p || !where.p || !pairs.p) return SJKVARN_ERR_NOMEM;
+    for (int k = 0; k < n_seqs; ++k)
+        for (uint32_t g = 0; g < seqs[k]->layers[0].n_groups; ++g) {
+            const uint32_t id = seqs[k]->blocks[g];
+            if (id == SJKVARN_NO_BLOCK) continue;
+            if (id >= nb) return SJKVARN_ERR_ARG;
+            ++held.p[id];
+        }
+    bool ok = pool->n_free <= nb;
+    for (uint32_t i = 0; ok && i < pool->n_free; ++i) {
+        const uint32_t id = pool->free_ids[i];
+        ok = id < nb && held.p[id] == 0 && where.p[id] == 0;
+        if (ok) where.p[id] = SJKVARN_NO_BLOCK;                            // free
+    }
+    for (uint32_t id = 0; ok && id < nb; ++id) ok = where.p[id] == SJKVARN_NO_BLOCK || held.p[id] == pool_extra(pool)[id] + 1u;
+    if (!ok) {
+        sjk::set_error("sjk_hip_pool_compact: a live block is not held by the given sequences alone");
+        return SJKVARN_ERR_ARG;
+    }
+    uint32_t * src = pairs.p, * dst = pairs.p + nb, n = 0, hole = 0;
+    for (uint32_t id = 0; id < nb; ++id) {
+        if (where.p[id] == SJKVARN_NO_BLOCK) continue;
+        where.p[id] = id;
+        if (id < n_live) continue;
+        while (where.p[hole] != SJKVARN_NO_BLOCK) ++hole;                  // a free block below n_live for each live one above
+        src[n] = id;
+        dst[n++] = hole;
+        where.p[id] = hole++;
+    }
+    const size_t gb = (size_t) pool->cfg.n_head_kv * pool->lay.bytes;
+    int st = sjk_hip_copy_blocks(pool->body, nb * gb, nb, pool->body, nb * gb, nb, pool->n_layers, gb, src, dst, n, stream);
+    if (st) return st;
+    for (int k = 0; k < n_seqs; ++k) {
+        sj_kvarn_seq * s = seqs[k];
+        const uint32_t ng = s->layers[0].n_groups;
+        uint32_t g0 = ng, g1 = 0;
+        for (uint32_t g = 0; g < ng; ++g) {
+            const uint32_t id = s->blocks[g];
+            if (id == SJKVARN_NO_BLOCK || where.p[id] == id) continue;
+            s->blocks[g] = where.p[id];
+            if (g < g0) g0 = g;
+            g1 = g + 1;
+        }
+        const int rc = seq_sync_blocks(s, g0, g1, (hipStream_t) stream, false);
+        if (rc && !st) st = rc;
+        rt_note_store(rt_of(s), (hipStream_t) stream);
+    }
+    for (uint32_t i = 0; i < n; ++i) {
+        pool_extra(pool)[dst[i]] = pool_extra(pool)[src[i]];
+        pool_extra(pool)[src[i]] = 0;
+    }
+    for (uint32_t i = 0; i < pool->n_free; ++i) pool->free_ids[i] = nb - 1u - i;
+    if (moved) *moved = n;
+    return st;
+}
 
 }  // extern "C"

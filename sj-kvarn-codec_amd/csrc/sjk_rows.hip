@@ -11,6 +11,7 @@
 //     large one by one lane per block, the workgroup's blocks side by side in one wavefront. The level
 //     search, packing and stores are parallel over lanes.
 #include "sjk_dev.h"
+#include "sjk_row.h"
 
 namespace sjk {
 
@@ -78,82 +79,6 @@ struct RowBatch {
 
 static_assert(sizeof(RowBatch) <= 4096, "the job table travels in the kernel arguments");
 
-// Hadamard of one row held V values per lane (sj_kvarn.h:735-752): stages h < V inside the lane, stages h >= V
-// between lanes l and l ^ (h / V) (the lower partner keeps a + b, the upper a - b, a = the lower value), then one
-// multiply by 1/sqrt(D). XN: the host's NaN rule (a row holding an infinity or a NaN).
-template <int V, bool XN>
-SJK_DEV void hadamard_row(float (&x)[V], int lane, float scale) {
-#pragma unroll
-    for (int h = 1; h < V; h *= 2)
-#pragma unroll
-        for (int m = 0; m < V; ++m)
-            if (!(m & h)) {
-                const float a = x[m], b = x[m + h];
-                x[m] = XN ? xadd(a, b) : a + b;
-                x[m + h] = XN ? xsub(a, b) : a - b;
-            }
-    if (XN) {
-#pragma unroll
-        for (int lm = 1; lm < 64; lm *= 2) {
-            const bool upper = (lane & lm) != 0;
-#pragma unroll
-            for (int m = 0; m < V; ++m) {
-                const float o = __shfl_xor(x[m], lm, 64);
-                x[m] = upper ? xsub(o, x[m]) : xadd(x[m], o);
-            }
-        }
-    } else {
-        // the partners' values by DPP inside a 16-lane row, then by row swaps: none of a lane shuffle's LDS round trips
-        // (six one after the other; appends of 8 rows at D = 256 4.5 -> 4.3 us, of 8,192 9.2 -> 8.7, fp16 rows 2.85 -> 2.63
-        // and 5.1 -> 4.95)
-        auto stage = [&](int lm, auto && partner) {
-            const bool upper = (lane & lm) != 0;
-#pragma unroll
-            for (int m = 0; m < V; ++m) {
-                const float o = partner(x[m]);
-                x[m] = upper ? o - x[m] : x[m] + o;
-            }
-        };
-        stage(1, [](float v) { return dpp<0xB1>(v); });                 // quad_perm 1 0 3 2
-        stage(2, [](float v) { return dpp<0x4E>(v); });                 // quad_perm 2 3 0 1
-        stage(4, [](float v) { return dpp<0x1B>(dpp<0x141>(v)); });     // 7 - l (row_half_mirror), then quad_perm 3 2 1 0
-        stage(8, [](float v) { return dpp<0x128>(v); });                // row_ror 8
-#pragma unroll
-        for (int lm = 16; lm < 64; lm *= 2) {
-            const bool upper = (lane & lm) != 0;
-#pragma unroll
-            for (int m = 0; m < V; ++m) {
-                uint32_t lo = f_bits(x[m]), hi = lo;                    // the lower and the upper partner's value
-                if (lm == 16) swap16(lo, hi);
-                else swap32(lo, hi);
-                const float p = __builtin_bit_cast(float, lo), q = __builtin_bit_cast(float, hi);
-                x[m] = upper ? p - q : p + q;
-            }
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < V; ++m) x[m] = XN ? xmul(x[m], scale) : x[m] * scale;
-}
-
-// the sum of 128 values in index order; XN: the host's NaN rule
-template <bool XN> SJK_DEV float walk(const float * sq) {
-    const float4 * p = (const float4 *) sq;
-    float s = 0.0f;
-    if (XN) {
-        for (int i = 0; i < 32; ++i) {
-            const float4 q = p[i];
-            s = xadd(s, q.x); s = xadd(s, q.y); s = xadd(s, q.z); s = xadd(s, q.w);
-        }
-    } else {
-#pragma unroll 8
-        for (int i = 0; i < 32; ++i) {
-            const float4 q = p[i];
-            s = s + q.x; s = s + q.y; s = s + q.z; s = s + q.w;
-        }
-    }
-    return s;
-}
-
 template <int V, int NW>
 __global__ __launch_bounds__(64 * NW) void rows_kernel(const RowBatch bt) {
     constexpr bool BIG = NW > ROW_WAVES;   // one wavefront walks the blocks of all rows
@@ -192,8 +117,8 @@ __global__ __launch_bounds__(64 * NW) void rows_kernel(const RowBatch bt) {
     for (int m = 0; m < V; ++m) nf |= (f_bits(x[m]) & 0x7F800000u) == 0x7F800000u;
     const bool xn = __any(nf);
     if (live && j.rotate) {
-        if (xn) hadamard_row<V, true>(x, lane, j.rot_scale);
-        else hadamard_row<V, false>(x, lane, j.rot_scale);
+        if (xn) hadamard_row<V, 64, true>(x, lane, j.rot_scale);
+        else hadamard_row<V, 64, false>(x, lane, j.rot_scale);
     }
     const bool tq = live && mode == OUT_TQ6;
     bool any_tq = tq;
@@ -310,8 +235,6 @@ static int launch_rows(const RowJob & j, hipStream_t st) {
     bt.n_jobs = 1;
     return launch_batch(bt, st);
 }
-
-static float rot_scale(int D) { return 1.0f / __builtin_sqrtf((float) D); }
 
 // ---- unstage: one thread per value (sj_kvarn.h:1249-1260, 1276-1284) ----
 __global__ void unstage_kernel(int staging, const uint8_t * src, size_t src_row_bytes, float * x, int D, int n_rows) {

@@ -21,6 +21,9 @@ vp = C.c_void_p
 
 BODY_SCALAR, BODY_TRELLIS, BODY_AUTO = 0, 1, 2
 STAGING_TQ6, STAGING_F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2                                  # element types of projection rows
+ROPE_HALVES, ROPE_PAIRS = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_RAMP, ROPE_BANDS = 0, 1, 2, 3, 4
 SINK_F16, SINK_INHERIT = 0, 1
 NO_POS = NO_BLOCK = 0xFFFFFFFF
 OK, ERR_ARG, ERR_PENDING, ERR_CORRUPT, ERR_POOL_FULL = 0, -100, -108, -107, -110
@@ -85,6 +88,37 @@ class StoreJob(C.Structure):
 
 class SeqJob(C.Structure):
     _fields_ = [("seq", C.POINTER(Seq)), ("pos0", C.c_uint32), ("d_k", vp), ("d_v", vp), ("d_q", vp), ("d_out", vp)]
+
+
+class RopeConfig(C.Structure):
+    _fields_ = [("n_rot", C.c_int), ("scaling", C.c_int), ("base", C.c_double), ("factor", C.c_double),
+                ("n_orig", C.c_double), ("low", C.c_double), ("high", C.c_double), ("divisors", C.POINTER(C.c_double))]
+
+
+class Rope(C.Structure):
+    _fields_ = [("layout", C.c_int), ("n_rot", C.c_int), ("inverse", C.c_int), ("mscale", C.c_float), ("d_turns", vp)]
+
+
+class HeadJob(C.Structure):
+    _fields_ = [("d_x", vp), ("d_out", vp), ("x_pos", C.c_int64), ("x_head", C.c_int64), ("out_pos", C.c_int64),
+                ("out_head", C.c_int64), ("x_type", C.c_int), ("out_type", C.c_int), ("n_heads", C.c_int),
+                ("rope", C.c_int), ("rotate", C.c_int), ("eps", C.c_float), ("d_norm", vp), ("norm_head", C.c_int64)]
+
+
+class Qkv(C.Structure):
+    _fields_ = [("type", C.c_int), ("n_head", C.c_int), ("rotate_qk", C.c_int), ("rotate_v", C.c_int), ("eps", C.c_float),
+                ("q_pos", C.c_int64), ("q_head", C.c_int64), ("k_pos", C.c_int64), ("k_head", C.c_int64),
+                ("v_pos", C.c_int64), ("v_head", C.c_int64), ("d_q_norm", vp), ("d_k_norm", vp),
+                ("norm_head", C.c_int64), ("rope", Rope)]
+
+
+class QkvJob(C.Structure):
+    _fields_ = [("v", View), ("pos0", C.c_uint32), ("d_pos", vp), ("d_q", vp), ("d_k", vp), ("d_v", vp), ("d_q_out", vp)]
+
+
+class SeqQkvJob(C.Structure):
+    _fields_ = [("seq", C.POINTER(Seq)), ("pos0", C.c_uint32), ("d_pos", vp), ("d_q", vp), ("d_k", vp), ("d_v", vp),
+                ("d_q_out", vp)]
 
 
 LP, CP, PP, LYP, PLP, SQP = (C.POINTER(Layout), C.POINTER(Config), C.POINTER(Policy), C.POINTER(Layer),
@@ -185,6 +219,18 @@ SIGNATURES = {
     "sjk_hip_seq_state_finish": (C.c_int, [SQP, C.POINTER(C.c_size_t)]),
     "sjk_hip_seq_attend_batch": (C.c_int, [C.POINTER(SeqJob), C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, vp]),
     "sjk_hip_balance_step": (C.c_int, [vp, vp, vp, C.c_int, vp]),
+    "sjk_rope_turns": (C.c_int, [C.POINTER(RopeConfig), C.POINTER(C.c_double), C.POINTER(C.c_float)]),
+    "sjk_hip_head_rows": (C.c_int, [C.POINTER(HeadJob), C.c_int, C.c_uint32, C.c_int, C.POINTER(Rope), C.c_uint32, vp, vp]),
+    "sjk_hip_store_qkv": (C.c_int, [C.POINTER(View), C.c_uint32, C.c_uint32, C.POINTER(Qkv), vp, vp, vp, vp, vp, vp]),
+    "sjk_hip_store_qkv_dyn": (C.c_int, [C.POINTER(View), vp, C.c_uint32, C.POINTER(Qkv), vp, vp, vp, vp, vp, vp]),
+    "sjk_hip_store_qkv_batch": (C.c_int, [C.POINTER(QkvJob), C.c_int, C.c_uint32, C.POINTER(Qkv), vp]),
+    "sjk_hip_seq_store_qkv_batch": (C.c_int, [C.POINTER(SeqQkvJob), C.c_int, C.c_int, C.c_uint32, C.POINTER(Qkv), vp]),
+    "sjk_hip_fork": (C.c_int, [C.POINTER(View), C.POINTER(View), C.c_int, C.c_uint32, C.c_uint32, vp]),
+    "sjk_hip_copy_blocks": (C.c_int, [vp, C.c_size_t, C.c_uint32, vp, C.c_size_t, C.c_uint32, C.c_int, C.c_size_t, u32p, u32p,
+                                      C.c_uint32, vp]),
+    "sjk_hip_seq_fork": (C.c_int, [SQP, SQP, C.c_uint32, u32p, vp]),
+    "sjk_hip_pool_refs": (C.c_uint32, [PLP, C.c_uint32]),
+    "sjk_hip_pool_compact": (C.c_int, [PLP, C.POINTER(SQP), C.c_int, u32p, vp]),
     "sjk_layer_view": (View, [LYP]),
     "sjk_last_error": (C.c_char_p, []),
 }
