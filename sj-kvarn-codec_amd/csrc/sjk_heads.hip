@@ -2,14 +2,16 @@
 // cache's basis, and the append, in one pass over the rows (sjk_hip_head_rows, sjk_hip_store_qkv).
 //
 // A row (one head at one position) lies 8 consecutive channels a lane in LPR lanes, so a wavefront holds 64 / LPR rows and
-// reads and writes 16 or 32 bytes a lane. It takes `iters` groups of 64 / LPR consecutive rows of one set of heads (head
-// index fastest), the next group's loads issued before the current one's arithmetic.
+// reads and writes 16 or 32 bytes a lane. The rows are the same head at adjacent positions, and the wavefront goes through a
+// run of heads of one set, the next head's loads issued before the current one's arithmetic: a lane keeps its position, whose
+// sines, cosines and cache slot it works out once. A call with fewer positions than the wavefront has rows takes adjacent
+// heads of one position instead.
 //   * norm: the sum of squares is a fixed tree (pairs in the lane, then lanes 1, 2, 4, ... apart), so a row's bits do not
 //     depend on the rows beside it.
 //   * turn: u = position * turns per position in double, reduced to (-1/2, 1/2] turns and then to an eighth of one either
 //     side of a quarter before it becomes a float: nothing is lost at far positions, and the sine and cosine are short
-//     polynomials. They are made per lane and kept while the lane's position stays (the heads of one position follow one
-//     another); no table of positions is read.
+//     polynomials; no table of positions is read. Where the halves of a whole head are paired, the two lanes of a pair make
+//     half of their sines and cosines each and exchange them.
 //   * the Hadamard and the staging are those of the row kernel (sjk_rows.hip): the same bytes.
 #include "sjk_dev.h"
 #include "sjk_row.h"
@@ -19,7 +21,7 @@ namespace sjk {
 constexpr int HW = 4;                  // wavefronts a workgroup
 constexpr int HEAD_PARTS = 3;          // sets of heads a launch: q, k, v
 constexpr int HEAD_SEQS = 32;          // sequences a launch
-constexpr int HEAD_ITERS = 8;          // row groups a wavefront at most
+constexpr int HEAD_ITERS = 8;          // heads a wavefront goes through at most
 enum { HP_ROWS = 0, HP_K = 1, HP_V = 2 };                               // where a part's rows go
 enum { HF_XVEC = 1, HF_OVEC = 2, HF_ROPE = 4, HF_ROT = 8 };
 enum { HM_ROWS = 0, HM_F16 = 1, HM_TQ6 = 2 };                           // a launch: plain rows only, or a cache's staging
@@ -28,7 +30,7 @@ struct HeadPart {
     int64_t x_pos, x_head, o_pos, o_head, w_head;
     const float * w;
     float eps;
-    int n_heads, n_units, flags, kind, o_type;
+    int n_heads, n_iters, n_chunks, n_units, flags, kind, o_type;      // iterations of a wavefront, runs of heads, wavefronts
 };
 
 struct HeadSeq {
@@ -44,7 +46,7 @@ struct HeadBatch {
     const double * turns;
     const int32_t * desc;
     size_t stage_bytes;
-    int n_parts, n_seqs, n_pos, D, iters, units;       // units: wavefronts of one sequence
+    int n_parts, n_seqs, n_pos, D, by_head, units;     // by_head: rows are adjacent heads; units: wavefronts of one sequence
     int layout, n_rot, H, sink_type;
     float mscale, sine, rot_scale, inv_D;              // sine: the sign of sines (inverse)
 };
@@ -132,6 +134,9 @@ SJK_DEV void store_row(void * p, int type, const float (&x)[8], int e0, int D, b
     }
 }
 
+// whether v is an infinity or a NaN
+SJK_DEV bool nonfinite(float v) { return __builtin_amdgcn_classf(v, 0x207); }
+
 template <typename T, int LPR, int MODE>
 __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     constexpr int RPW = 64 / LPR;                          // rows a wavefront holds
@@ -147,7 +152,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
         }
         __syncthreads();
     }
-    // this wavefront's sequence, part and rows (wave-uniform)
+    // this wavefront's sequence, part, positions and heads (wave-uniform)
     int u = __builtin_amdgcn_readfirstlane((int) blockIdx.x * HW + wave);
     const int si = u / bt.units;
     if (si >= bt.n_seqs) return;
@@ -158,36 +163,89 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     const HeadSeq & Q = bt.seq[si];
     if (bt.desc && bt.desc[SJK_DESC_QPOS0] < 0) return;
     const uint32_t pos0 = bt.desc ? (uint32_t) bt.desc[SJK_DESC_QPOS0] : Q.pos0;
-    const int D = bt.D, n_heads = P.n_heads, n_rows = bt.n_pos * n_heads;
-    const T * x_in = (const T *) Q.x[pi];
+    const int D = bt.D, n_heads = P.n_heads, n_iters = P.n_iters, step = bt.by_head ? RPW : 1;
     const bool xvec = P.flags & HF_XVEC, ovec = P.flags & HF_OVEC, rope = P.flags & HF_ROPE, rot = P.flags & HF_ROT;
     float * buf = s_buf + wave * WS;
 
-    int row = u * bt.iters * RPW + sub;
-    int ip = row / n_heads, hh = row - ip * n_heads;
-    int at = -1;                                           // position whose sines and cosines the lane holds
+    // the lane's row: position cp, heads ch, ch + step, ...
+    const int block = u / P.n_chunks, run = u - block * P.n_chunks;
+    const int cp = bt.by_head ? block : block * RPW + sub;
+    int ch = run * n_iters * step + (bt.by_head ? sub : 0);
+    const bool here = cp < bt.n_pos;
+    const T * x_row = (const T *) Q.x[pi] + ((int64_t) cp * P.x_pos + (int64_t) ch * P.x_head);
+    const int64_t x_step = step * P.x_head;
+    Raw<T> raw;
+    if (here && ch < n_heads) load_row<T>(raw, x_row, e0, D, xvec);
+
     float cs[8], sn[8], w[8];
-    const int n_rot = bt.n_rot, half = n_rot / 2;
     auto load_w = [&](int h) {
         const float * p = P.w + (int64_t) h * P.w_head;
 #pragma unroll
         for (int m = 0; m < 8; ++m) w[m] = e0 + m < D ? p[e0 + m] : 0.0f;
     };
     if (P.w && !P.w_head) load_w(0);
-    Raw<T> raw;
-    if (row < n_rows) load_row<T>(raw, x_in + (int64_t) ip * P.x_pos + (int64_t) hh * P.x_head, e0, D, xvec);
+    const int n_rot = bt.n_rot, half = n_rot / 2;
+    const bool pairs = bt.layout == SJK_ROPE_PAIRS, whole = n_rot == 8 * LPR;
+    if (rope && here) {
+        const double p = Q.pos ? (double) Q.pos[cp] : (double) (pos0 + (uint32_t) cp);
+        if (pairs) {
+#pragma unroll
+            for (int m = 0; m < 8; m += 2) {
+                if (e0 + m < n_rot) turn(p * bt.turns[(e0 + m) >> 1], bt.mscale, bt.sine, sn[m + 1], cs[m + 1]);
+                cs[m] = cs[m + 1];
+                sn[m] = -sn[m + 1];
+            }
+        } else if (whole) {
+            const bool up = l >= LPR / 2;                  // the pairs' second channels
+            const double * t = bt.turns + (up ? e0 - half + 4 : e0);
+            float s[4], c[4];
+#pragma unroll
+            for (int m = 0; m < 4; ++m) turn(p * t[m], bt.mscale, bt.sine, s[m], c[m]);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const float so = lane_xor<LPR / 2>(s[m], lane), co = lane_xor<LPR / 2>(c[m], lane);
+                cs[m] = up ? co : c[m];
+                cs[m + 4] = up ? c[m] : co;
+                sn[m] = up ? so : -s[m];
+                sn[m + 4] = up ? s[m] : -so;
+            }
+        } else {
+#pragma unroll
+            for (int m = 0; m < 8; ++m) {
+                const int e = e0 + m;
+                if (e < n_rot) {
+                    turn(p * bt.turns[e < half ? e : e - half], bt.mscale, bt.sine, sn[m], cs[m]);
+                    if (e < half) sn[m] = -sn[m];
+                }
+            }
+        }
+    }
 
-    for (int it = 0; it < bt.iters; ++it) {
-        const bool live = row < n_rows;
+    // where the rows go: d_row and d_step in bytes. A cache's entry of the position: sink, or the ring's slot.
+    uint8_t * d_row;
+    int64_t d_step;
+    bool f16_row = MODE == HM_F16;
+    if (MODE == HM_ROWS || P.kind == HP_ROWS) {
+        const int64_t size = P.o_type == SJK_F32 ? 4 : 2;
+        d_row = (uint8_t *) Q.o[pi] + size * ((int64_t) cp * P.o_pos + (int64_t) ch * P.o_head);
+        d_step = size * step * P.o_head;
+    } else {
+        const uint32_t pos = pos0 + (uint32_t) cp;
+        const bool in_sink = pos < Q.S, sink_f16 = in_sink && bt.sink_type == SJKVARN_SINK_F16;
+        const size_t side = sink_f16 ? 2 * (size_t) D : bt.stage_bytes, at = in_sink ? pos : (pos - Q.S) % Q.cap;
+        d_row = (uint8_t *) (in_sink ? Q.o[1] : Q.o[2]) + (at * bt.H + ch) * 2 * side + (P.kind == HP_V ? side : 0);
+        d_step = (int64_t) (2 * side * step);
+        f16_row |= sink_f16;
+    }
+
+    for (int it = 0; it < n_iters; ++it, ch += step, d_row += d_step) {
+        const bool live = here && ch < n_heads;
         if (!__any(live)) break;
         float x[8];
 #pragma unroll
         for (int m = 0; m < 8; ++m) x[m] = live ? raw_at<T>(raw, m) : 0.0f;
-        const int cp = ip, ch = hh;
-        row += RPW;
-        for (hh += RPW; hh >= n_heads; hh -= n_heads) ++ip;
-        if (it + 1 < bt.iters && row < n_rows)
-            load_row<T>(raw, x_in + (int64_t) ip * P.x_pos + (int64_t) hh * P.x_head, e0, D, xvec);
+        x_row += x_step;
+        if (it + 1 < n_iters && here && ch + step < n_heads) load_row<T>(raw, x_row, e0, D, xvec);
 
         if (P.w) {
             if (P.w_head && live) load_w(ch);
@@ -205,33 +263,11 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
         }
 
         if (rope) {
-            if (live && cp != at) {
-                at = cp;
-                const double p = Q.pos ? (double) Q.pos[cp] : (double) (pos0 + (uint32_t) cp);
-                if (bt.layout == SJK_ROPE_PAIRS) {
-#pragma unroll
-                    for (int m = 0; m < 8; m += 2) {
-                        if (e0 + m < n_rot) turn(p * bt.turns[(e0 + m) >> 1], bt.mscale, bt.sine, sn[m], cs[m]);
-                        cs[m + 1] = cs[m];
-                        sn[m + 1] = sn[m];
-                        sn[m] = -sn[m];
-                    }
-                } else {
-#pragma unroll
-                    for (int m = 0; m < 8; ++m) {
-                        const int e = e0 + m;
-                        if (e < n_rot) {
-                            turn(p * bt.turns[e < half ? e : e - half], bt.mscale, bt.sine, sn[m], cs[m]);
-                            if (e < half) sn[m] = -sn[m];
-                        }
-                    }
-                }
-            }
             float y[8];                                    // the other channel of each pair
-            if (bt.layout == SJK_ROPE_PAIRS) {
+            if (pairs) {
 #pragma unroll
                 for (int m = 0; m < 8; ++m) y[m] = x[m ^ 1];
-            } else if (n_rot == 8 * LPR) {
+            } else if (whole) {
 #pragma unroll
                 for (int m = 0; m < 8; ++m) y[m] = lane_xor<LPR / 2>(x[m], lane);
             } else {
@@ -247,9 +283,14 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
                 }
                 wave_sync();
             }
+            if (whole) {
 #pragma unroll
-            for (int m = 0; m < 8; ++m)
-                if (e0 + m < n_rot) x[m] = __builtin_fmaf(x[m], cs[m], y[m] * sn[m]);
+                for (int m = 0; m < 8; ++m) x[m] = __builtin_fmaf(x[m], cs[m], y[m] * sn[m]);
+            } else {
+#pragma unroll
+                for (int m = 0; m < 8; ++m)
+                    if (e0 + m < n_rot) x[m] = __builtin_fmaf(x[m], cs[m], y[m] * sn[m]);
+            }
         }
 
         // a row holding an infinity or a NaN takes the rotation and the tq6_0 sums with the host's NaN rule
@@ -258,7 +299,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
         if (rot || MODE == HM_TQ6) {
             bool nf = false;
 #pragma unroll
-            for (int m = 0; m < 8; ++m) nf |= (f_bits(x[m]) & 0x7F800000u) == 0x7F800000u;
+            for (int m = 0; m < 8; ++m) nf |= nonfinite(x[m]);
             nf_rows = __ballot(nf);
             xn = ((LPR == 64 ? nf_rows : nf_rows >> (sub * LPR)) & ((LPR == 64 ? 0 : 1ull << (LPR % 64)) - 1ull)) != 0;
         }
@@ -268,26 +309,15 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
         }
 
         if (MODE == HM_ROWS || P.kind == HP_ROWS) {
-            if (live) {
-                const size_t size = P.o_type == SJK_F32 ? 4 : 2;
-                store_row((uint8_t *) Q.o[pi] + size * (size_t) ((int64_t) cp * P.o_pos + (int64_t) ch * P.o_head), P.o_type, x, e0, D, ovec);
-            }
+            if (live) store_row(d_row, P.o_type, x, e0, D, ovec);
             continue;
         }
         if constexpr (MODE != HM_ROWS) {
-            // the cache's entry of this position and head: sink, or the ring's slot
-            const uint32_t pos = pos0 + (uint32_t) cp;
-            const bool in_sink = pos < Q.S, sink_f16 = in_sink && bt.sink_type == SJKVARN_SINK_F16;
-            const int side = P.kind == HP_V;
-            uint8_t * dst = sink_f16 ? (uint8_t *) Q.o[1] + ((size_t) pos * bt.H + ch) * 4 * D + (size_t) side * 2 * D
-                            : (in_sink ? (uint8_t *) Q.o[1] + ((size_t) pos * bt.H + ch) * 2 * bt.stage_bytes
-                                       : (uint8_t *) Q.o[2] + ((size_t) ((pos - Q.S) % Q.cap) * bt.H + ch) * 2 * bt.stage_bytes) +
-                                  (size_t) side * bt.stage_bytes;
-            if (live && (MODE == HM_F16 || sink_f16)) {
+            if (live && f16_row) {
                 uint16_t h[8];
 #pragma unroll
                 for (int m = 0; m < 8; ++m) h[m] = f32_to_f16(x[m]);
-                uint16_t * o = (uint16_t *) dst + e0;
+                uint16_t * o = (uint16_t *) d_row + e0;
                 if (ovec) *(uint4 *) o = uint4{pack16(h[0], h[1]), pack16(h[2], h[3]), pack16(h[4], h[5]), pack16(h[6], h[7])};
                 else {
 #pragma unroll
@@ -295,7 +325,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
                 }
             }
             if constexpr (MODE == HM_TQ6) {
-                const bool tq = live && !sink_f16;
+                const bool tq = live && !f16_row;
                 if (!__any(tq)) continue;
                 // sj_kvarn.h:1221-1247: two sums of 128 values in index order, walked by every lane of the block (16 lanes)
                 float * blk = buf + (lane >> 4) * BS, * sq = blk + 8 * (lane & 15);
@@ -317,7 +347,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
                 const float rn = __builtin_sqrtf(walk<false>(blk));
                 wave_sync();
                 if (tq) {
-                    uint8_t * o = dst + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES;
+                    uint8_t * o = d_row + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES;
                     const int i0 = 8 * (l & 15);
                     if (!(l & 15)) *(uint16_t *) o = f32_to_f16(rn > 1e-10f ? xdiv(norm, rn) : norm);
                     uint32_t qs = 0, qh = 0;               // low nibbles; high pairs
@@ -390,21 +420,27 @@ static int launch_typed(const HeadBatch & bt, int lpr, int mode, unsigned grid, 
     return SJK_CHECK_LAUNCH();
 }
 
-// The launch's shape: a wavefront takes `iters` groups of rows, so that the sines and cosines of a position serve
-// several of its heads, once there are more wavefronts than the device holds resident
+// The launch's shape. With as many positions as a wavefront has rows, a wavefront goes through up to HEAD_ITERS heads once
+// there are more wavefronts than the device holds resident (the sines and cosines of a position serve them all).
 static int launch_heads(HeadBatch & bt, int type, int mode, hipStream_t st) {
     const int lpr = bt.D <= 64 ? 8 : bt.D <= 128 ? 16 : bt.D <= 256 ? 32 : 64, rpw = 64 / lpr;
+    bt.by_head = bt.n_pos < rpw;
+    const int step = bt.by_head ? rpw : 1;                                 // heads an iteration takes on
+    const int64_t blocks = bt.by_head ? bt.n_pos : (bt.n_pos + rpw - 1) / rpw;
     int64_t groups = 0;
-    for (int p = 0; p < bt.n_parts; ++p) groups += ((int64_t) bt.n_pos * bt.part[p].n_heads + rpw - 1) / rpw;
+    for (int p = 0; p < bt.n_parts; ++p) groups += blocks * ((bt.part[p].n_heads + step - 1) / step);
     groups *= bt.n_seqs;
     if (!groups) return 0;
     const int64_t it = groups / ((int64_t) n_cus() * 4 * HW);
-    bt.iters = it < 1 ? 1 : it > HEAD_ITERS ? HEAD_ITERS : (int) it;
+    const int most = it < 1 ? 1 : it > HEAD_ITERS ? HEAD_ITERS : (int) it;
     bt.units = 0;
     for (int p = 0; p < bt.n_parts; ++p) {
-        const int64_t per = (int64_t) rpw * bt.iters;
-        bt.part[p].n_units = (int) (((int64_t) bt.n_pos * bt.part[p].n_heads + per - 1) / per);
-        bt.units += bt.part[p].n_units;
+        HeadPart & P = bt.part[p];
+        const int steps = (P.n_heads + step - 1) / step;
+        P.n_chunks = (steps + most - 1) / most;
+        P.n_iters = P.n_chunks ? (steps + P.n_chunks - 1) / P.n_chunks : 0;
+        P.n_units = (int) (blocks * P.n_chunks);
+        bt.units += P.n_units;
     }
     bt.inv_D = 1.0f / (float) bt.D;
     bt.rot_scale = rot_scale(bt.D);

@@ -5,12 +5,18 @@
 
 namespace sjk {
 
+// v of the lane that the DPP control names, in an arithmetic instruction's own operand where the compiler can put it there
+// (every lane of these controls has a source, so nothing stands in for a missing one)
+template <int CTRL> SJK_DEV float dpp_in(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+
 // v of lane l ^ LM. Inside a 16-lane row by DPP, across rows by row swaps: none of a lane shuffle's LDS round trips.
 template <int LM> SJK_DEV float lane_xor(float v, int lane) {
-    if constexpr (LM == 1) return dpp<0xB1>(v);                       // quad_perm 1 0 3 2
-    else if constexpr (LM == 2) return dpp<0x4E>(v);                  // quad_perm 2 3 0 1
-    else if constexpr (LM == 4) return dpp<0x1B>(dpp<0x141>(v));      // 7 - l (row_half_mirror), then quad_perm 3 2 1 0
-    else if constexpr (LM == 8) return dpp<0x128>(v);                 // row_ror 8
+    if constexpr (LM == 1) return dpp_in<0xB1>(v);                    // quad_perm 1 0 3 2
+    else if constexpr (LM == 2) return dpp_in<0x4E>(v);               // quad_perm 2 3 0 1
+    else if constexpr (LM == 4) return dpp_in<0x1B>(dpp_in<0x141>(v));// 7 - l (row_half_mirror), then quad_perm 3 2 1 0
+    else if constexpr (LM == 8) return dpp_in<0x128>(v);              // row_ror 8
     else {
         uint32_t lo = f_bits(v), hi = lo;                             // the lower and the upper partner's value
         if constexpr (LM == 16) swap16(lo, hi);
@@ -46,15 +52,13 @@ SJK_DEV void hadamard_row(float (&x)[V], int lane, float scale, bool xn = true) 
             }
         }
     } else {
-        // appends of 8 rows at D = 256 4.5 -> 4.3 us, of 8,192 9.2 -> 8.7, fp16 rows 2.85 -> 2.63 and 5.1 -> 4.95, against
-        // lane shuffles (six LDS round trips one after the other)
+        // the partner's value plus or minus the lane's own: a sign flip and one addition, whose DPP operand is the partner
+        // (against lane shuffles, six LDS round trips one after the other: appends of 8 rows at D = 256 4.5 -> 4.3 us, of
+        // 8,192 9.2 -> 8.7, fp16 rows 2.85 -> 2.63 and 5.1 -> 4.95)
         auto stage = [&](int lm, auto && partner) {
-            const bool upper = (lane & lm) != 0;
+            const uint32_t flip = lane & lm ? 0x80000000u : 0u;
 #pragma unroll
-            for (int m = 0; m < V; ++m) {
-                const float o = partner(x[m]);
-                x[m] = upper ? o - x[m] : x[m] + o;
-            }
+            for (int m = 0; m < V; ++m) x[m] = partner(x[m]) + bits_f(f_bits(x[m]) ^ flip);
         };
         if constexpr (LPR > 1) stage(1, [&](float v) { return lane_xor<1>(v, lane); });
         if constexpr (LPR > 2) stage(2, [&](float v) { return lane_xor<2>(v, lane); });
@@ -62,14 +66,13 @@ SJK_DEV void hadamard_row(float (&x)[V], int lane, float scale, bool xn = true) 
         if constexpr (LPR > 8) stage(8, [&](float v) { return lane_xor<8>(v, lane); });
 #pragma unroll
         for (int lm = 16; lm < LPR; lm *= 2) {
-            const bool upper = (lane & lm) != 0;
+            const uint32_t flip = lane & lm ? 0x80000000u : 0u;
 #pragma unroll
             for (int m = 0; m < V; ++m) {
                 uint32_t lo = f_bits(x[m]), hi = lo;                    // the lower and the upper partner's value
                 if (lm == 16) swap16(lo, hi);
                 else swap32(lo, hi);
-                const float p = bits_f(lo), q = bits_f(hi);
-                x[m] = upper ? p - q : p + q;
+                x[m] = bits_f(lo) + bits_f(hi ^ flip);
             }
         }
     }
