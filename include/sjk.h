@@ -454,7 +454,7 @@ typedef struct sjk_hip_head_job {
     void        * d_out;        /* may be d_x, with the same type and strides; no other overlap */
     int64_t       x_pos, x_head, out_pos, out_head;
     int           x_type, out_type, n_heads, rope, rotate;
-    float         eps;          /* > 0 where d_norm is given */
+    float         eps;          /* where d_norm is given: normal, finite, > 0 */
     const float * d_norm;       /* NULL: no norm */
     int64_t       norm_head;
 } sjk_hip_head_job;

@@ -23,7 +23,7 @@ constexpr int HEAD_PARTS = 3;          // sets of heads a launch: q, k, v
 constexpr int HEAD_SEQS = 32;          // sequences a launch
 constexpr int HEAD_ITERS = 8;          // heads a wavefront goes through at most
 enum { HP_ROWS = 0, HP_K = 1, HP_V = 2 };                               // where a part's rows go
-enum { HF_XVEC = 1, HF_OVEC = 2, HF_ROPE = 4, HF_ROT = 8 };
+enum { HF_ROPE = 1, HF_ROT = 2 };
 enum { HM_ROWS = 0, HM_F16 = 1, HM_TQ6 = 2 };                           // a launch: plain rows only, or a cache's staging
 
 struct HeadPart {
@@ -74,15 +74,14 @@ SJK_DEV void turn(double u, float m, float sg, float & s, float & c) {
     const float a = k & 1 ? cs : sn, b = k & 1 ? sn : cs;
     s = (k & 2 ? -a : a) * m * sg;
     c = ((k + 1) & 2 ? -b : b) * m;
+    __builtin_amdgcn_sched_barrier(0);       // one after the other: interleaved, their temporaries set the kernel's registers
 }
 
-// 8 channels of a row from its element e0 on, as raw words; elements behind D are zero
+// 8 channels of a row from its element e0 on, as raw words. WIDE: 16 bytes at a time, else element by element up to D.
 template <typename T> struct Raw { uint32_t w[2 * sizeof(T)]; };
-template <typename T> SJK_DEV void load_row(Raw<T> & r, const T * p, int e0, int D, bool vec) {
+template <typename T, bool WIDE> SJK_DEV void load_row(Raw<T> & r, const T * p, int e0, int D) {
     constexpr int NW = 2 * (int) sizeof(T);
-#pragma unroll
-    for (int i = 0; i < NW; ++i) r.w[i] = 0;
-    if (vec) {
+    if constexpr (WIDE) {
         if (e0 < D) {
 #pragma unroll
             for (int i = 0; i < NW; i += 4) {
@@ -91,6 +90,8 @@ template <typename T> SJK_DEV void load_row(Raw<T> & r, const T * p, int e0, int
             }
         }
     } else {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) r.w[i] = 0;
 #pragma unroll
         for (int m = 0; m < 8; ++m)
             if (e0 + m < D) {
@@ -101,16 +102,31 @@ template <typename T> SJK_DEV void load_row(Raw<T> & r, const T * p, int e0, int
 }
 template <typename T> SJK_DEV float raw_at(const Raw<T> & r, int m) {
     if constexpr (sizeof(T) == 4) return bits_f(r.w[m]);
+    else if constexpr (__is_same(T, __bf16)) return bits_f(m & 1 ? r.w[m >> 1] & 0xFFFF0000u : r.w[m >> 1] << 16);
     else return (float) __builtin_bit_cast(T, (uint16_t) (r.w[m >> 1] >> (16 * (m & 1))));
 }
 
-SJK_DEV uint32_t pack16(uint16_t a, uint16_t b) { return (uint32_t) a | (uint32_t) b << 16; }
+typedef float float2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+SJK_DEV uint32_t pack_f16(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{a, b}), f16x2_t)); }
+SJK_DEV uint32_t pack_bf16(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{a, b}), bf16x2_t)); }
+
+template <bool WIDE> SJK_DEV void store_halves(uint16_t * o, const uint32_t (&h)[4], int e0, int D) {
+    if constexpr (WIDE) {
+        if (e0 < D) *(uint4 *) o = uint4{h[0], h[1], h[2], h[3]};
+    } else {
+#pragma unroll
+        for (int m = 0; m < 8; ++m) if (e0 + m < D) o[m] = (uint16_t) (h[m >> 1] >> (16 * (m & 1)));
+    }
+}
 
 // 8 channels of a row of `type`, one rounding (to nearest even)
-SJK_DEV void store_row(void * p, int type, const float (&x)[8], int e0, int D, bool vec) {
+template <bool WIDE> SJK_DEV void store_row(void * p, int type, const float (&x)[8], int e0, int D) {
     if (type == SJK_F32) {
         float * o = (float *) p + e0;
-        if (vec) {
+        if constexpr (WIDE) {
             if (e0 < D) {
                 ((float4 *) o)[0] = float4{x[0], x[1], x[2], x[3]};
                 ((float4 *) o)[1] = float4{x[4], x[5], x[6], x[7]};
@@ -121,24 +137,51 @@ SJK_DEV void store_row(void * p, int type, const float (&x)[8], int e0, int D, b
         }
         return;
     }
-    uint16_t h[8];
+    uint32_t h[4];
 #pragma unroll
-    for (int m = 0; m < 8; ++m)
-        h[m] = type == SJK_F16 ? __builtin_bit_cast(uint16_t, (_Float16) x[m]) : __builtin_bit_cast(uint16_t, (__bf16) x[m]);
-    uint16_t * o = (uint16_t *) p + e0;
-    if (vec) {
-        if (e0 < D) *(uint4 *) o = uint4{pack16(h[0], h[1]), pack16(h[2], h[3]), pack16(h[4], h[5]), pack16(h[6], h[7])};
-    } else {
-#pragma unroll
-        for (int m = 0; m < 8; ++m) if (e0 + m < D) o[m] = h[m];
-    }
+    for (int m = 0; m < 4; ++m) h[m] = type == SJK_F16 ? pack_f16(x[2 * m], x[2 * m + 1]) : pack_bf16(x[2 * m], x[2 * m + 1]);
+    store_halves<WIDE>((uint16_t *) p + e0, h, e0, D);
 }
 
 // whether v is an infinity or a NaN
 SJK_DEV bool nonfinite(float v) { return __builtin_amdgcn_classf(v, 0x207); }
 
-template <typename T, int LPR, int MODE>
+// The rotation with the host's NaN rule in the rows where xn is set, through the wavefront's LDS (512 floats), a lane four pairs
+// of every stage: such rows are rare, so this is short rather than fast. The values of the other rows are hadamard_row's.
+template <int LPR> SJK_DEV void hadamard_rows_x(float (&x)[8], float * buf, int lane, float scale, bool xn) {
+    const int l = lane % LPR;
+    float * row = buf + lane / LPR * (8 * LPR);
+    wave_sync();
+#pragma unroll
+    for (int m = 0; m < 8; ++m) row[8 * l + m] = x[m];
+    wave_sync();
+#pragma unroll 1
+    for (int h = 1; h < 8 * LPR; h *= 2) {
+#pragma unroll 1
+        for (int k = 4 * l; k < 4 * l + 4; ++k) {
+            const int j = 2 * (k & -h) + (k & (h - 1));
+            const float a = row[j], b = row[j + h];
+            row[j] = xn ? xadd(a, b) : a + b;
+            row[j + h] = xn ? xsub(a, b) : a - b;
+        }
+        wave_sync();
+    }
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+        const float v = row[8 * l + m];
+        x[m] = xn ? xmul(v, scale) : v * scale;
+    }
+    wave_sync();
+}
+
+// KIND: which calls the kernel is for. The first has no masks and no addresses for what it does not do (92 registers for one
+// kernel of all calls, two wavefronts a SIMD less).
+enum { HK_WHOLE = 0,        // rows whose addresses and strides take 16-byte accesses, turned over all 8 * LPR channels or not at all
+       HK_PART = 1,         // such rows, turned over a part of those channels
+       HK_ANY = 2 };        // rows of any width, address and stride
+template <typename T, int LPR, int MODE, int KIND>
 __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
+    constexpr bool WIDE = KIND != HK_ANY;
     constexpr int RPW = 64 / LPR;                          // rows a wavefront holds
     constexpr int BS = 132;                                // floats from a 128-value block to the next (walks: other banks)
     constexpr int WS = MODE == HM_TQ6 ? 4 * BS : 512;      // floats of a wavefront's LDS
@@ -164,7 +207,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     if (bt.desc && bt.desc[SJK_DESC_QPOS0] < 0) return;
     const uint32_t pos0 = bt.desc ? (uint32_t) bt.desc[SJK_DESC_QPOS0] : Q.pos0;
     const int D = bt.D, n_heads = P.n_heads, n_iters = P.n_iters, step = bt.by_head ? RPW : 1;
-    const bool xvec = P.flags & HF_XVEC, ovec = P.flags & HF_OVEC, rope = P.flags & HF_ROPE, rot = P.flags & HF_ROT;
+    const bool rope = P.flags & HF_ROPE, rot = P.flags & HF_ROT;
     float * buf = s_buf + wave * WS;
 
     // the lane's row: position cp, heads ch, ch + step, ...
@@ -174,24 +217,26 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     const bool here = cp < bt.n_pos;
     const T * x_row = (const T *) Q.x[pi] + ((int64_t) cp * P.x_pos + (int64_t) ch * P.x_head);
     const int64_t x_step = step * P.x_head;
-    Raw<T> raw;
-    if (here && ch < n_heads) load_row<T>(raw, x_row, e0, D, xvec);
+    Raw<T> raw = {};
+    if (here && ch < n_heads) load_row<T, WIDE>(raw, x_row, e0, D);
 
-    float cs[8], sn[8], w[8];
+    const float * norm = P.w;
+    const int64_t norm_head = P.w_head;
+    float cs[8] = {}, sn[8] = {}, w[8];
     auto load_w = [&](int h) {
-        const float * p = P.w + (int64_t) h * P.w_head;
+        const float * p = norm + h * norm_head;
 #pragma unroll
         for (int m = 0; m < 8; ++m) w[m] = e0 + m < D ? p[e0 + m] : 0.0f;
     };
-    if (P.w && !P.w_head) load_w(0);
+    if (norm) load_w(norm_head ? (ch < n_heads ? ch : 0) : 0);
     const int n_rot = bt.n_rot, half = n_rot / 2;
-    const bool pairs = bt.layout == SJK_ROPE_PAIRS, whole = n_rot == 8 * LPR;
+    const bool pairs = bt.layout == SJK_ROPE_PAIRS, whole = KIND == HK_WHOLE || n_rot == 8 * LPR;
     if (rope && here) {
         const double p = Q.pos ? (double) Q.pos[cp] : (double) (pos0 + (uint32_t) cp);
         if (pairs) {
 #pragma unroll
             for (int m = 0; m < 8; m += 2) {
-                if (e0 + m < n_rot) turn(p * bt.turns[(e0 + m) >> 1], bt.mscale, bt.sine, sn[m + 1], cs[m + 1]);
+                if (whole || e0 + m < n_rot) turn(p * bt.turns[(e0 + m) >> 1], bt.mscale, bt.sine, sn[m + 1], cs[m + 1]);
                 cs[m] = cs[m + 1];
                 sn[m] = -sn[m + 1];
             }
@@ -225,8 +270,10 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     uint8_t * d_row;
     int64_t d_step;
     bool f16_row = MODE == HM_F16;
-    if (MODE == HM_ROWS || P.kind == HP_ROWS) {
-        const int64_t size = P.o_type == SJK_F32 ? 4 : 2;
+    const bool rows_out = MODE == HM_ROWS || P.kind == HP_ROWS;
+    const int o_type = P.o_type;
+    if (rows_out) {
+        const int64_t size = o_type == SJK_F32 ? 4 : 2;
         d_row = (uint8_t *) Q.o[pi] + size * ((int64_t) cp * P.o_pos + (int64_t) ch * P.o_head);
         d_step = size * step * P.o_head;
     } else {
@@ -238,26 +285,26 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
         f16_row |= sink_f16;
     }
 
+    const float inv_D = bt.inv_D, eps = P.eps, rot_scale = bt.rot_scale;
     for (int it = 0; it < n_iters; ++it, ch += step, d_row += d_step) {
         const bool live = here && ch < n_heads;
-        if (!__any(live)) break;
         float x[8];
 #pragma unroll
-        for (int m = 0; m < 8; ++m) x[m] = live ? raw_at<T>(raw, m) : 0.0f;
+        for (int m = 0; m < 8; ++m) x[m] = raw_at<T>(raw, m);
         x_row += x_step;
-        if (it + 1 < n_iters && here && ch + step < n_heads) load_row<T>(raw, x_row, e0, D, xvec);
+        if (it + 1 < n_iters && here && ch + step < n_heads) load_row<T, WIDE>(raw, x_row, e0, D);
 
-        if (P.w) {
-            if (P.w_head && live) load_w(ch);
-            float ss = ((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])) +
-                       ((x[4] * x[4] + x[5] * x[5]) + (x[6] * x[6] + x[7] * x[7]));
+        if (norm) {
+            if (norm_head && it && live) load_w(ch);
+            float ss = (__builtin_fmaf(x[1], x[1], x[0] * x[0]) + __builtin_fmaf(x[3], x[3], x[2] * x[2])) +
+                       (__builtin_fmaf(x[5], x[5], x[4] * x[4]) + __builtin_fmaf(x[7], x[7], x[6] * x[6]));
             ss += lane_xor<1>(ss, lane);
             ss += lane_xor<2>(ss, lane);
             ss += lane_xor<4>(ss, lane);
             if constexpr (LPR > 8) ss += lane_xor<8>(ss, lane);
             if constexpr (LPR > 16) ss += lane_xor<16>(ss, lane);
             if constexpr (LPR > 32) ss += lane_xor<32>(ss, lane);
-            const float r = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, bt.inv_D, P.eps));
+            const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(ss, inv_D, eps));      // within an ulp; eps keeps it normal
 #pragma unroll
             for (int m = 0; m < 8; ++m) x[m] = x[m] * r * w[m];
         }
@@ -293,36 +340,52 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
             }
         }
 
-        // a row holding an infinity or a NaN takes the rotation and the tq6_0 sums with the host's NaN rule
-        bool xn = false;
+        // A row holding an infinity or a NaN takes the rotation and the tq6_0 sums with the host's NaN rule. Every value of its
+        // rotation is an infinity or a NaN then, so a look at one of each lane's finds it. A row that overflows on the way keeps
+        // the plain rotation, but where that makes NaNs their signs are hadamard_row's.
         uint64_t nf_rows = 0;
-        if (rot || MODE == HM_TQ6) {
+        bool xn = false;
+        auto look = [&](const float (&v)[8]) {
             bool nf = false;
 #pragma unroll
-            for (int m = 0; m < 8; ++m) nf |= nonfinite(x[m]);
-            nf_rows = __ballot(nf);
+            for (int m = 0; m < 8; ++m) nf |= nonfinite(v[m]);
+            nf_rows = __ballot(nf && live);
             xn = ((LPR == 64 ? nf_rows : nf_rows >> (sub * LPR)) & ((LPR == 64 ? 0 : 1ull << (LPR % 64)) - 1ull)) != 0;
-        }
+        };
+        bool nan = true;                                   // whether the rows may hold NaNs (wave-uniform)
         if (rot) {
-            if (nf_rows) hadamard_row<8, LPR, true>(x, lane, bt.rot_scale, xn);
-            else hadamard_row<8, LPR, false>(x, lane, bt.rot_scale);
+            float y[8];
+#pragma unroll
+            for (int m = 0; m < 8; ++m) y[m] = x[m];
+            hadamard_finite<8, LPR>(y, lane, rot_scale);
+            nan = __any(live && (nonfinite(y[0]) || __builtin_isunordered(y[0], y[1]) || __builtin_isunordered(y[2], y[3]) ||
+                                 __builtin_isunordered(y[4], y[5]) || __builtin_isunordered(y[6], y[7])));
+            if (nan) {
+                look(x);
+                hadamard_rows_x<LPR>(x, buf, lane, rot_scale, xn);
+            } else {
+#pragma unroll
+                for (int m = 0; m < 8; ++m) x[m] = y[m];
+            }
+        } else if (MODE == HM_TQ6 && !rows_out) {
+            look(x);
         }
 
-        if (MODE == HM_ROWS || P.kind == HP_ROWS) {
-            if (live) store_row(d_row, P.o_type, x, e0, D, ovec);
+        if (rows_out) {
+            if (live) store_row<WIDE>(d_row, o_type, x, e0, D);
             continue;
         }
         if constexpr (MODE != HM_ROWS) {
             if (live && f16_row) {
-                uint16_t h[8];
+                uint32_t h[4];
 #pragma unroll
-                for (int m = 0; m < 8; ++m) h[m] = f32_to_f16(x[m]);
-                uint16_t * o = (uint16_t *) d_row + e0;
-                if (ovec) *(uint4 *) o = uint4{pack16(h[0], h[1]), pack16(h[2], h[3]), pack16(h[4], h[5]), pack16(h[6], h[7])};
-                else {
+                for (int m = 0; m < 4; ++m) h[m] = pack_f16(x[2 * m], x[2 * m + 1]);
+                // a NaN is stored as its sign | 0x7E00 (f32_to_f16)
+                if (nan) {
 #pragma unroll
-                    for (int m = 0; m < 8; ++m) o[m] = h[m];
+                    for (int m = 0; m < 4; ++m) h[m] = (uint32_t) f32_to_f16(x[2 * m]) | (uint32_t) f32_to_f16(x[2 * m + 1]) << 16;
                 }
+                store_halves<WIDE>((uint16_t *) d_row + e0, h, e0, D);
             }
             if constexpr (MODE == HM_TQ6) {
                 const bool tq = live && !f16_row;
@@ -373,7 +436,7 @@ static int refuse(const char * what) {
 static size_t elem_size(int type) { return type == SJK_F32 ? 4 : 2; }
 static bool type_ok(int type) { return type == SJK_F32 || type == SJK_F16 || type == SJK_BF16; }
 // rows at p with strides in elements of `size` bytes can be read and written 16 bytes at a time
-static bool wide(const void * p, int64_t pos, int64_t head, size_t size, int D) {
+static bool wide_rows(const void * p, int64_t pos, int64_t head, size_t size, int D) {
     return D % 8 == 0 && !((uintptr_t) p & 15u) && !((uint64_t) pos * size & 15u) && !((uint64_t) head * size & 15u);
 }
 
@@ -388,7 +451,7 @@ static int rope_ok(const sjk_hip_rope & r, int D) {
 
 static int norm_ok(const float * w, float eps) {
     if (!w) return 0;
-    if ((uintptr_t) w % 4 || !(eps > 0.0f) || !__builtin_isfinite(eps)) return refuse("head norms: fp32 weights and a finite eps > 0");
+    if ((uintptr_t) w % 4 || !(eps >= 1.17549435e-38f) || !__builtin_isfinite(eps)) return refuse("head norms: fp32 weights and a finite, normal eps > 0");
     return 0;
 }
 
@@ -400,10 +463,10 @@ static void set_rope(HeadBatch & bt, const sjk_hip_rope & r) {
     bt.sine = r.inverse ? -1.0f : 1.0f;
 }
 
-template <typename T>
-static int launch_typed(const HeadBatch & bt, int lpr, int mode, unsigned grid, hipStream_t st) {
+template <typename T, int KIND>
+static int launch_kind(const HeadBatch & bt, int lpr, int mode, unsigned grid, hipStream_t st) {
     const dim3 g(grid), b(64 * HW);
-#define SJK_HEADS(L, M) hipLaunchKernelGGL((heads_kernel<T, L, M>), g, b, 0, st, bt)
+#define SJK_HEADS(L, M) hipLaunchKernelGGL((heads_kernel<T, L, M, KIND>), g, b, 0, st, bt)
     if (mode == HM_ROWS) {
         if (lpr == 8) SJK_HEADS(8, HM_ROWS);
         else if (lpr == 16) SJK_HEADS(16, HM_ROWS);
@@ -420,9 +483,18 @@ static int launch_typed(const HeadBatch & bt, int lpr, int mode, unsigned grid, 
     return SJK_CHECK_LAUNCH();
 }
 
+template <typename T>
+static int launch_typed(const HeadBatch & bt, int lpr, int mode, bool wide, unsigned grid, hipStream_t st) {
+    bool turned = false;
+    for (int p = 0; p < bt.n_parts; ++p) turned |= (bt.part[p].flags & HF_ROPE) != 0;
+    if (!wide) return launch_kind<T, HK_ANY>(bt, lpr, mode, grid, st);
+    if (turned && bt.n_rot != 8 * lpr) return launch_kind<T, HK_PART>(bt, lpr, mode, grid, st);
+    return launch_kind<T, HK_WHOLE>(bt, lpr, mode, grid, st);
+}
+
 // The launch's shape. With as many positions as a wavefront has rows, a wavefront goes through up to HEAD_ITERS heads once
 // there are more wavefronts than the device holds resident (the sines and cosines of a position serve them all).
-static int launch_heads(HeadBatch & bt, int type, int mode, hipStream_t st) {
+static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream_t st) {
     const int lpr = bt.D <= 64 ? 8 : bt.D <= 128 ? 16 : bt.D <= 256 ? 32 : 64, rpw = 64 / lpr;
     bt.by_head = bt.n_pos < rpw;
     const int step = bt.by_head ? rpw : 1;                                 // heads an iteration takes on
@@ -445,9 +517,9 @@ static int launch_heads(HeadBatch & bt, int type, int mode, hipStream_t st) {
     bt.inv_D = 1.0f / (float) bt.D;
     bt.rot_scale = rot_scale(bt.D);
     const unsigned grid = (unsigned) (((int64_t) bt.units * bt.n_seqs + HW - 1) / HW);
-    if (type == SJK_F32) return launch_typed<float>(bt, lpr, mode, grid, st);
-    if (type == SJK_F16) return launch_typed<_Float16>(bt, lpr, mode, grid, st);
-    return launch_typed<__bf16>(bt, lpr, mode, grid, st);
+    if (type == SJK_F32) return launch_typed<float>(bt, lpr, mode, wide, grid, st);
+    if (type == SJK_F16) return launch_typed<_Float16>(bt, lpr, mode, wide, grid, st);
+    return launch_typed<__bf16>(bt, lpr, mode, wide, grid, st);
 }
 
 // rows of a launch are counted in 32 bits
@@ -486,20 +558,22 @@ extern "C" int sjk_hip_head_rows(const sjk_hip_head_job * jobs, int n_jobs, uint
         bt.seq[0].pos0 = pos0;
         if (rope) set_rope(bt, *rope);
         int k = k0;
+        bool wide = true;
         for (; k < n_jobs && k - k0 < HEAD_PARTS && jobs[k].x_type == jobs[k0].x_type; ++k) {
             const sjk_hip_head_job & J = jobs[k];
             HeadPart & P = bt.part[bt.n_parts];
             P.x_pos = J.x_pos; P.x_head = J.x_head; P.o_pos = J.out_pos; P.o_head = J.out_head;
             P.w = J.d_norm; P.w_head = J.norm_head; P.eps = J.eps;
             P.n_heads = J.n_heads; P.kind = HP_ROWS; P.o_type = J.out_type;
-            P.flags = (wide(J.d_x, J.x_pos, J.x_head, elem_size(J.x_type), D) ? HF_XVEC : 0) |
-                      (wide(J.d_out, J.out_pos, J.out_head, elem_size(J.out_type), D) ? HF_OVEC : 0) |
-                      (J.rope && rope->n_rot ? HF_ROPE : 0) | (J.rotate ? HF_ROT : 0);
+            P.flags = (J.rope && rope->n_rot ? HF_ROPE : 0) | (J.rotate ? HF_ROT : 0);
+            if (J.n_heads)
+                wide = wide && wide_rows(J.d_x, J.x_pos, J.x_head, elem_size(J.x_type), D) &&
+                       wide_rows(J.d_out, J.out_pos, J.out_head, elem_size(J.out_type), D);
             bt.seq[0].x[bt.n_parts] = J.d_x;
             bt.seq[0].o[bt.n_parts] = J.d_out;
             if (J.n_heads) ++bt.n_parts;
         }
-        const int rc = n_pos && bt.n_parts ? launch_heads(bt, jobs[k0].x_type, HM_ROWS, (hipStream_t) stream) : 0;
+        const int rc = n_pos && bt.n_parts ? launch_heads(bt, jobs[k0].x_type, HM_ROWS, wide, (hipStream_t) stream) : 0;
         if (rc) return rc;
         k0 = k;
     }
@@ -538,7 +612,7 @@ static int qkv_ok(const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t pos0, 
     return rc;
 }
 
-// the launch's table without its sequences; vec: every sequence's rows of the part can be read / written wide
+// the launch's table without its sequences
 static void qkv_table(HeadBatch & bt, const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t n_pos) {
     const int D = v.lay.D;
     bt.n_pos = (int) n_pos;
@@ -558,29 +632,29 @@ static void qkv_table(HeadBatch & bt, const sjk_hip_view & v, const sjk_hip_qkv 
         P.w = w[p]; P.w_head = m.norm_head; P.eps = m.eps;
         P.n_heads = p ? v.n_head_kv : m.n_head;
         P.kind = p; P.o_type = SJK_F32;
-        P.flags = (p < 2 ? qk : m.rotate_v ? HF_ROT : 0) | HF_XVEC | HF_OVEC;
+        P.flags = p < 2 ? qk : m.rotate_v ? HF_ROT : 0;
     }
 }
 
-static void qkv_seq(HeadBatch & bt, const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t pos0, const int32_t * d_pos, const void * d_q,
+// one more sequence; whether its rows and its cache take 16-byte accesses
+static bool qkv_seq(HeadBatch & bt, const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t pos0, const int32_t * d_pos, const void * d_q,
                     const void * d_k, const void * d_v, float * d_q_out) {
     HeadSeq & Q = bt.seq[bt.n_seqs++];
     const void * x[3] = {d_q, d_k, d_v};
-    const size_t size = elem_size(m.type);
-    const bool cache = !(((uintptr_t) v.sink | (uintptr_t) v.ring) & 15u);
+    bool wide = !(((uintptr_t) v.sink | (uintptr_t) v.ring) & 15u) && wide_rows(d_q_out, 0, 0, 4, bt.D);
     for (int p = 0; p < HEAD_PARTS; ++p) {
-        HeadPart & P = bt.part[p];
+        const HeadPart & P = bt.part[p];
         Q.x[p] = x[p];
-        if (!wide(x[p], P.x_pos, P.x_head, size, bt.D)) P.flags &= ~HF_XVEC;
-        if (!(p ? cache : wide(d_q_out, P.o_pos, P.o_head, 4, bt.D))) P.flags &= ~HF_OVEC;
+        wide = wide && (P.n_heads == 0 || wide_rows(x[p], P.x_pos, P.x_head, elem_size(m.type), bt.D));
     }
     Q.o[0] = d_q_out; Q.o[1] = v.sink; Q.o[2] = v.ring;
     Q.pos = d_pos; Q.pos0 = pos0; Q.S = v.S; Q.cap = v.cap;
+    return wide;
 }
 
-static int qkv_launch(HeadBatch & bt, const sjk_hip_view & v, int type, hipStream_t st) {
+static int qkv_launch(HeadBatch & bt, const sjk_hip_view & v, int type, bool wide, hipStream_t st) {
     if (!bt.n_pos) return 0;
-    return launch_heads(bt, type, v.staging == SJKVARN_STAGING_F16 ? HM_F16 : HM_TQ6, st);
+    return launch_heads(bt, type, v.staging == SJKVARN_STAGING_F16 ? HM_F16 : HM_TQ6, wide, st);
 }
 
 }  // namespace sjk
@@ -592,8 +666,8 @@ extern "C" int sjk_hip_store_qkv(const sjk_hip_view * v, uint32_t pos0, uint32_t
     if (rc) return rc;
     HeadBatch bt = {};
     qkv_table(bt, *v, *m, n_pos);
-    qkv_seq(bt, *v, *m, pos0, d_pos, d_q, d_k, d_v, d_q_out);
-    return qkv_launch(bt, *v, m->type, (hipStream_t) stream);
+    const bool wide = qkv_seq(bt, *v, *m, pos0, d_pos, d_q, d_k, d_v, d_q_out);
+    return qkv_launch(bt, *v, m->type, wide, (hipStream_t) stream);
 }
 
 extern "C" int sjk_hip_store_qkv_dyn(const sjk_hip_view * v, const int32_t * d_desc, uint32_t n_pos, const sjk_hip_qkv * m,
@@ -605,9 +679,9 @@ extern "C" int sjk_hip_store_qkv_dyn(const sjk_hip_view * v, const int32_t * d_d
     if (rc) return rc;
     HeadBatch bt = {};
     qkv_table(bt, *v, *m, n_pos);
-    qkv_seq(bt, *v, *m, 0, d_pos, d_q, d_k, d_v, d_q_out);
+    const bool wide = qkv_seq(bt, *v, *m, 0, d_pos, d_q, d_k, d_v, d_q_out);
     bt.desc = d_desc;
-    return qkv_launch(bt, *v, m->type, (hipStream_t) stream);
+    return qkv_launch(bt, *v, m->type, wide, (hipStream_t) stream);
 }
 
 extern "C" int sjk_hip_store_qkv_batch(const sjk_hip_qkv_job * jobs, int n_jobs, uint32_t n_pos, const sjk_hip_qkv * m, void * stream) {
@@ -625,13 +699,14 @@ extern "C" int sjk_hip_store_qkv_batch(const sjk_hip_qkv_job * jobs, int n_jobs,
     for (int k = 0; k < n_jobs;) {
         const sjk_hip_view & v = jobs[k].v;
         HeadBatch bt = {};
+        bool wide = true;
         qkv_table(bt, v, *m, n_pos);
         for (; k < n_jobs && bt.n_seqs < HEAD_SEQS; ++k) {
             const sjk_hip_qkv_job & J = jobs[k];
             if (J.v.n_head_kv != v.n_head_kv || J.v.staging != v.staging || J.v.sink_type != v.sink_type) break;
-            qkv_seq(bt, J.v, *m, J.pos0, J.d_pos, J.d_q, J.d_k, J.d_v, J.d_q_out);
+            wide = qkv_seq(bt, J.v, *m, J.pos0, J.d_pos, J.d_q, J.d_k, J.d_v, J.d_q_out) && wide;
         }
-        const int rc = qkv_launch(bt, v, m->type, (hipStream_t) stream);
+        const int rc = qkv_launch(bt, v, m->type, wide, (hipStream_t) stream);
         if (rc) return rc;
     }
     return 0;

@@ -27,11 +27,11 @@ template <int LM> SJK_DEV float lane_xor(float v, int lane) {
 
 // Hadamard of one row (sj_kvarn.h:735-752): stages h < V inside the lane, stages h >= V between lanes l and l ^ (h / V)
 // (the lower partner keeps a + b, the upper a - b, a = the lower value), then one multiply by 1/sqrt(V * LPR). XN: the
-// host's NaN rule for a row holding an infinity or a NaN; with several rows in the wavefront, in the lanes where xn is set.
+// host's NaN rule (a row holding an infinity or a NaN).
 template <int V, int LPR, bool XN>
-SJK_DEV void hadamard_row(float (&x)[V], int lane, float scale, bool xn = true) {
-    auto add = [&](float a, float b) { return XN && xn ? xadd(a, b) : a + b; };
-    auto sub = [&](float a, float b) { return XN && xn ? xsub(a, b) : a - b; };
+SJK_DEV void hadamard_row(float (&x)[V], int lane, float scale) {
+    auto add = [&](float a, float b) { return XN ? xadd(a, b) : a + b; };
+    auto sub = [&](float a, float b) { return XN ? xsub(a, b) : a - b; };
 #pragma unroll
     for (int h = 1; h < V; h *= 2)
 #pragma unroll
@@ -52,13 +52,15 @@ SJK_DEV void hadamard_row(float (&x)[V], int lane, float scale, bool xn = true) 
             }
         }
     } else {
-        // the partner's value plus or minus the lane's own: a sign flip and one addition, whose DPP operand is the partner
-        // (against lane shuffles, six LDS round trips one after the other: appends of 8 rows at D = 256 4.5 -> 4.3 us, of
-        // 8,192 9.2 -> 8.7, fp16 rows 2.85 -> 2.63 and 5.1 -> 4.95)
+        // appends of 8 rows at D = 256 4.5 -> 4.3 us, of 8,192 9.2 -> 8.7, fp16 rows 2.85 -> 2.63 and 5.1 -> 4.95, against
+        // lane shuffles (six LDS round trips one after the other)
         auto stage = [&](int lm, auto && partner) {
-            const uint32_t flip = lane & lm ? 0x80000000u : 0u;
+            const bool upper = (lane & lm) != 0;
 #pragma unroll
-            for (int m = 0; m < V; ++m) x[m] = partner(x[m]) + bits_f(f_bits(x[m]) ^ flip);
+            for (int m = 0; m < V; ++m) {
+                const float o = partner(x[m]);
+                x[m] = upper ? o - x[m] : x[m] + o;
+            }
         };
         if constexpr (LPR > 1) stage(1, [&](float v) { return lane_xor<1>(v, lane); });
         if constexpr (LPR > 2) stage(2, [&](float v) { return lane_xor<2>(v, lane); });
@@ -66,18 +68,56 @@ SJK_DEV void hadamard_row(float (&x)[V], int lane, float scale, bool xn = true) 
         if constexpr (LPR > 8) stage(8, [&](float v) { return lane_xor<8>(v, lane); });
 #pragma unroll
         for (int lm = 16; lm < LPR; lm *= 2) {
-            const uint32_t flip = lane & lm ? 0x80000000u : 0u;
+            const bool upper = (lane & lm) != 0;
 #pragma unroll
             for (int m = 0; m < V; ++m) {
                 uint32_t lo = f_bits(x[m]), hi = lo;                    // the lower and the upper partner's value
                 if (lm == 16) swap16(lo, hi);
                 else swap32(lo, hi);
-                x[m] = bits_f(lo) + bits_f(hi ^ flip);
+                const float p = bits_f(lo), q = bits_f(hi);
+                x[m] = upper ? p - q : p + q;
             }
         }
     }
 #pragma unroll
-    for (int m = 0; m < V; ++m) x[m] = XN && xn ? xmul(x[m], scale) : x[m] * scale;
+    for (int m = 0; m < V; ++m) x[m] = XN ? xmul(x[m], scale) : x[m] * scale;
+}
+
+// hadamard_row<V, LPR, false> for rows whose result is finite: a stage across lanes is the lane's own value with its sign
+// turned in the upper partner, added to the partner's value as the addition's DPP operand (two instructions a value for four).
+// A NaN on the way may come out with another sign.
+template <int V, int LPR> SJK_DEV void hadamard_finite(float (&x)[V], int lane, float scale) {
+#pragma unroll
+    for (int h = 1; h < V; h *= 2)
+#pragma unroll
+        for (int m = 0; m < V; ++m)
+            if (!(m & h)) {
+                const float a = x[m], b = x[m + h];
+                x[m] = a + b;
+                x[m + h] = a - b;
+            }
+    auto stage = [&](int lm, auto && partner) {
+        const uint32_t flip = lane & lm ? 0x80000000u : 0u;
+#pragma unroll
+        for (int m = 0; m < V; ++m) x[m] = partner(x[m]) + bits_f(f_bits(x[m]) ^ flip);
+    };
+    if constexpr (LPR > 1) stage(1, [&](float v) { return lane_xor<1>(v, lane); });
+    if constexpr (LPR > 2) stage(2, [&](float v) { return lane_xor<2>(v, lane); });
+    if constexpr (LPR > 4) stage(4, [&](float v) { return lane_xor<4>(v, lane); });
+    if constexpr (LPR > 8) stage(8, [&](float v) { return lane_xor<8>(v, lane); });
+#pragma unroll
+    for (int lm = 16; lm < LPR; lm *= 2) {
+        const uint32_t flip = lane & lm ? 0x80000000u : 0u;
+#pragma unroll
+        for (int m = 0; m < V; ++m) {
+            uint32_t lo = f_bits(x[m]), hi = lo;                        // the lower and the upper partner's value
+            if (lm == 16) swap16(lo, hi);
+            else swap32(lo, hi);
+            x[m] = bits_f(lo) + bits_f(hi ^ flip);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < V; ++m) x[m] = x[m] * scale;
 }
 
 // the sum of 128 values in index order; XN: the host's NaN rule where xn is set

@@ -109,7 +109,7 @@ def test_head_rows_refusals(lib):
         assert call(job(**bad)) == ARG, bad
     for D in (0, -1, 513):
         assert call(job(), D=D) == ARG
-    for eps in (0.0, -1e-6, np.nan, np.inf):
+    for eps in (0.0, -1e-6, 1e-40, np.nan, np.inf):
         assert call(job(d_norm=FAKE, eps=eps)) == ARG
     assert call(job(d_norm=FAKE + 2, eps=1e-6)) == ARG
     assert call(job(rope=1)) == ARG                                   # no rope given
