@@ -25,6 +25,8 @@ constexpr int HEAD_ITERS = 8;          // heads a wavefront goes through at most
 enum { HP_ROWS = 0, HP_K = 1, HP_V = 2 };                               // where a part's rows go
 enum { HF_ROPE = 1, HF_ROT = 2 };
 enum { HM_ROWS = 0, HM_F16 = 1, HM_TQ6 = 2 };                           // a launch: plain rows only, or a cache's staging
+enum { HO_F32 = 0, HO_HALF = 1, HO_CACHE = 2 };                         // a wavefront's rows
+template <int N> struct Int { static constexpr int value = N; };
 
 struct HeadPart {
     int64_t x_pos, x_head, o_pos, o_head, w_head;
@@ -79,10 +81,10 @@ SJK_DEV void turn(double u, float m, float sg, float & s, float & c) {
 
 // 8 channels of a row from its element e0 on, as raw words. WIDE: 16 bytes at a time, else element by element up to D.
 template <typename T> struct Raw { uint32_t w[2 * sizeof(T)]; };
-template <typename T, bool WIDE> SJK_DEV void load_row(Raw<T> & r, const T * p, int e0, int D) {
+template <typename T, bool WIDE, bool ALL> SJK_DEV void load_row(Raw<T> & r, const T * p, int e0, int D) {
     constexpr int NW = 2 * (int) sizeof(T);
     if constexpr (WIDE) {
-        if (e0 < D) {
+        if (ALL || e0 < D) {
 #pragma unroll
             for (int i = 0; i < NW; i += 4) {
                 const uint4 v = *(const uint4 *) ((const uint32_t *) (p + e0) + i);
@@ -113,34 +115,25 @@ typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 SJK_DEV uint32_t pack_f16(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{a, b}), f16x2_t)); }
 SJK_DEV uint32_t pack_bf16(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{a, b}), bf16x2_t)); }
 
-template <bool WIDE> SJK_DEV void store_halves(uint16_t * o, const uint32_t (&h)[4], int e0, int D) {
+template <bool WIDE, bool ALL> SJK_DEV void store_halves(uint16_t * o, const uint32_t (&h)[4], int e0, int D) {
     if constexpr (WIDE) {
-        if (e0 < D) *(uint4 *) o = uint4{h[0], h[1], h[2], h[3]};
+        if (ALL || e0 < D) *(uint4 *) o = uint4{h[0], h[1], h[2], h[3]};
     } else {
 #pragma unroll
         for (int m = 0; m < 8; ++m) if (e0 + m < D) o[m] = (uint16_t) (h[m >> 1] >> (16 * (m & 1)));
     }
 }
 
-// 8 channels of a row of `type`, one rounding (to nearest even)
-template <bool WIDE> SJK_DEV void store_row(void * p, int type, const float (&x)[8], int e0, int D) {
-    if (type == SJK_F32) {
-        float * o = (float *) p + e0;
-        if constexpr (WIDE) {
-            if (e0 < D) {
-                ((float4 *) o)[0] = float4{x[0], x[1], x[2], x[3]};
-                ((float4 *) o)[1] = float4{x[4], x[5], x[6], x[7]};
-            }
-        } else {
-#pragma unroll
-            for (int m = 0; m < 8; ++m) if (e0 + m < D) o[m] = x[m];
+template <bool WIDE, bool ALL> SJK_DEV void store_row(float * o, const float (&x)[8], int e0, int D) {
+    if constexpr (WIDE) {
+        if (ALL || e0 < D) {
+            ((float4 *) o)[0] = float4{x[0], x[1], x[2], x[3]};
+            ((float4 *) o)[1] = float4{x[4], x[5], x[6], x[7]};
         }
-        return;
-    }
-    uint32_t h[4];
+    } else {
 #pragma unroll
-    for (int m = 0; m < 4; ++m) h[m] = type == SJK_F16 ? pack_f16(x[2 * m], x[2 * m + 1]) : pack_bf16(x[2 * m], x[2 * m + 1]);
-    store_halves<WIDE>((uint16_t *) p + e0, h, e0, D);
+        for (int m = 0; m < 8; ++m) if (e0 + m < D) o[m] = x[m];
+    }
 }
 
 // whether v is an infinity or a NaN
@@ -176,12 +169,19 @@ template <int LPR> SJK_DEV void hadamard_rows_x(float (&x)[8], float * buf, int 
 
 // KIND: which calls the kernel is for. The first has no masks and no addresses for what it does not do (92 registers for one
 // kernel of all calls, two wavefronts a SIMD less).
-enum { HK_WHOLE = 0,        // rows whose addresses and strides take 16-byte accesses, turned over all 8 * LPR channels or not at all
-       HK_PART = 1,         // such rows, turned over a part of those channels
+enum { HK_WHOLE = 0,        // rows of 8 * LPR channels whose addresses and strides take 16-byte accesses, turned whole or not at all, and one set of
+                            // norm weights for all heads of a job
+       HK_PART = 1,         // such accesses otherwise
        HK_ANY = 2 };        // rows of any width, address and stride
 template <typename T, int LPR, int MODE, int KIND>
 __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     constexpr bool WIDE = KIND != HK_ANY;
+    // Where every lane has a row's channels, lanes behind the last row take the last row again and write the same values once
+    // more (both read it in one instruction, so also where rows are written over themselves): loads and stores without a
+    // branch around them, so that a wait for the next row's loads does not wait for this row's stores (on gfx9 one counter
+    // holds both, and the compiler can count past the stores only where they are certain: 8,192 positions x 40 heads of
+    // 128 turned in 39.5 us with branches).
+    constexpr bool ALL = KIND == HK_WHOLE;
     constexpr int RPW = 64 / LPR;                          // rows a wavefront holds
     constexpr int BS = 132;                                // floats from a 128-value block to the next (walks: other banks)
     constexpr int WS = MODE == HM_TQ6 ? 4 * BS : 512;      // floats of a wavefront's LDS
@@ -206,19 +206,21 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     const HeadSeq & Q = bt.seq[si];
     if (bt.desc && bt.desc[SJK_DESC_QPOS0] < 0) return;
     const uint32_t pos0 = bt.desc ? (uint32_t) bt.desc[SJK_DESC_QPOS0] : Q.pos0;
-    const int D = bt.D, n_heads = P.n_heads, n_iters = P.n_iters, step = bt.by_head ? RPW : 1;
+    const int D = bt.D, n_heads = P.n_heads, step = bt.by_head ? RPW : 1;
     const bool rope = P.flags & HF_ROPE, rot = P.flags & HF_ROT;
     float * buf = s_buf + wave * WS;
 
     // the lane's row: position cp, heads ch, ch + step, ...
-    const int block = u / P.n_chunks, run = u - block * P.n_chunks;
-    const int cp = bt.by_head ? block : block * RPW + sub;
-    int ch = run * n_iters * step + (bt.by_head ? sub : 0);
-    const bool here = cp < bt.n_pos;
-    const T * x_row = (const T *) Q.x[pi] + ((int64_t) cp * P.x_pos + (int64_t) ch * P.x_head);
-    const int64_t x_step = step * P.x_head;
+    const int block = u / P.n_chunks, run = u - block * P.n_chunks, h0 = run * P.n_iters * step;
+    const int iters = min(P.n_iters, (n_heads - h0 + step - 1) / step);
+    int cp = bt.by_head ? block : block * RPW + sub, ch = h0 + (bt.by_head ? sub : 0);
+    if (ALL) cp = min(cp, bt.n_pos - 1);
+    const bool here = ALL || cp < bt.n_pos;
+    auto head_of = [&](int h) { return ALL && bt.by_head ? min(h, n_heads - 1) : h; };
+    const T * x_base = (const T *) Q.x[pi] + (int64_t) cp * P.x_pos, * x_row = x_base + head_of(ch) * P.x_head;
+    const int64_t x_head = P.x_head;
     Raw<T> raw = {};
-    if (here && ch < n_heads) load_row<T, WIDE>(raw, x_row, e0, D);
+    if (ALL || (here && ch < n_heads)) load_row<T, WIDE, ALL>(raw, x_row, e0, D);
 
     const float * norm = P.w;
     const int64_t norm_head = P.w_head;
@@ -226,24 +228,28 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     auto load_w = [&](int h) {
         const float * p = norm + h * norm_head;
 #pragma unroll
-        for (int m = 0; m < 8; ++m) w[m] = e0 + m < D ? p[e0 + m] : 0.0f;
+        for (int m = 0; m < 8; ++m) w[m] = ALL || e0 + m < D ? p[e0 + m] : 0.0f;
     };
-    if (norm) load_w(norm_head ? (ch < n_heads ? ch : 0) : 0);
+    if (norm) load_w(norm_head && ch < n_heads ? ch : 0);
     const int n_rot = bt.n_rot, half = n_rot / 2;
     const bool pairs = bt.layout == SJK_ROPE_PAIRS, whole = KIND == HK_WHOLE || n_rot == 8 * LPR;
     if (rope && here) {
         const double p = Q.pos ? (double) Q.pos[cp] : (double) (pos0 + (uint32_t) cp);
+        double t[8];                                       // all of the table's loads before the first turn
         if (pairs) {
 #pragma unroll
-            for (int m = 0; m < 8; m += 2) {
-                if (whole || e0 + m < n_rot) turn(p * bt.turns[(e0 + m) >> 1], bt.mscale, bt.sine, sn[m + 1], cs[m + 1]);
-                cs[m] = cs[m + 1];
-                sn[m] = -sn[m + 1];
+            for (int m = 0; m < 4; ++m) t[m] = whole || e0 + 2 * m < n_rot ? bt.turns[(e0 >> 1) + m] : 0.0;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                turn(p * t[m], bt.mscale, bt.sine, sn[2 * m + 1], cs[2 * m]);
+                cs[2 * m + 1] = cs[2 * m];
+                sn[2 * m] = -sn[2 * m + 1];
             }
         } else if (whole) {
             const bool up = l >= LPR / 2;                  // the pairs' second channels
-            const double * t = bt.turns + (up ? e0 - half + 4 : e0);
             float s[4], c[4];
+#pragma unroll
+            for (int m = 0; m < 4; ++m) t[m] = bt.turns[(up ? e0 - half + 4 : e0) + m];
 #pragma unroll
             for (int m = 0; m < 4; ++m) turn(p * t[m], bt.mscale, bt.sine, s[m], c[m]);
 #pragma unroll
@@ -258,44 +264,60 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
 #pragma unroll
             for (int m = 0; m < 8; ++m) {
                 const int e = e0 + m;
-                if (e < n_rot) {
-                    turn(p * bt.turns[e < half ? e : e - half], bt.mscale, bt.sine, sn[m], cs[m]);
-                    if (e < half) sn[m] = -sn[m];
-                }
+                t[m] = e < n_rot ? bt.turns[e < half ? e : e - half] : 0.0;
+            }
+#pragma unroll
+            for (int m = 0; m < 8; ++m) {
+                turn(p * t[m], bt.mscale, bt.sine, sn[m], cs[m]);
+                if (e0 + m < half) sn[m] = -sn[m];
             }
         }
     }
 
-    // where the rows go: d_row and d_step in bytes. A cache's entry of the position: sink, or the ring's slot.
+    // where the rows go: d_row and from head to head d_head, in bytes. A cache's entry of the position: sink, or the ring's slot.
     uint8_t * d_row;
-    int64_t d_step;
+    int64_t d_head;
     bool f16_row = MODE == HM_F16;
     const bool rows_out = MODE == HM_ROWS || P.kind == HP_ROWS;
     const int o_type = P.o_type;
     if (rows_out) {
         const int64_t size = o_type == SJK_F32 ? 4 : 2;
-        d_row = (uint8_t *) Q.o[pi] + size * ((int64_t) cp * P.o_pos + (int64_t) ch * P.o_head);
-        d_step = size * step * P.o_head;
+        d_row = (uint8_t *) Q.o[pi] + size * ((int64_t) cp * P.o_pos);
+        d_head = size * P.o_head;
     } else {
         const uint32_t pos = pos0 + (uint32_t) cp;
         const bool in_sink = pos < Q.S, sink_f16 = in_sink && bt.sink_type == SJKVARN_SINK_F16;
         const size_t side = sink_f16 ? 2 * (size_t) D : bt.stage_bytes, at = in_sink ? pos : (pos - Q.S) % Q.cap;
-        d_row = (uint8_t *) (in_sink ? Q.o[1] : Q.o[2]) + (at * bt.H + ch) * 2 * side + (P.kind == HP_V ? side : 0);
-        d_step = (int64_t) (2 * side * step);
+        d_row = (uint8_t *) (in_sink ? Q.o[1] : Q.o[2]) + at * bt.H * 2 * side + (P.kind == HP_V ? side : 0);
+        d_head = (int64_t) (2 * side);
         f16_row |= sink_f16;
     }
 
     const float inv_D = bt.inv_D, eps = P.eps, rot_scale = bt.rot_scale;
-    for (int it = 0; it < n_iters; ++it, ch += step, d_row += d_step) {
-        const bool live = here && ch < n_heads;
+    d_row += head_of(ch) * d_head;
+    // what the rows become: fp32, halves, or the cache's entries (stores of one kind only, for the same reason as ALL)
+    auto heads = [&](auto out) {
+    constexpr int OUT = decltype(out)::value;
+    for (int it = 0; it < iters; ++it) {
+        const bool live = ALL || (here && ch < n_heads);
         float x[8];
 #pragma unroll
         for (int m = 0; m < 8; ++m) x[m] = raw_at<T>(raw, m);
-        x_row += x_step;
-        if (it + 1 < n_iters && here && ch + step < n_heads) load_row<T, WIDE>(raw, x_row, e0, D);
+        uint8_t * const d_this = d_row;
+        const int c_this = ch;
+        ch += step;
+        if (bt.by_head) {
+            const int64_t d = head_of(ch) - head_of(c_this);
+            if (it + 1 < iters) x_row += d * x_head;
+            d_row += d * d_head;
+        } else {
+            if (it + 1 < iters) x_row += x_head;           // (the last iteration of ALL loads its own row again)
+            d_row += d_head;
+        }
+        if (ALL || (it + 1 < iters && here && ch < n_heads)) load_row<T, WIDE, ALL>(raw, x_row, e0, D);
 
         if (norm) {
-            if (norm_head && it && live) load_w(ch);
+            if (!ALL && norm_head && it && live) load_w(c_this);
             float ss = (__builtin_fmaf(x[1], x[1], x[0] * x[0]) + __builtin_fmaf(x[3], x[3], x[2] * x[2])) +
                        (__builtin_fmaf(x[5], x[5], x[4] * x[4]) + __builtin_fmaf(x[7], x[7], x[6] * x[6]));
             ss += lane_xor<1>(ss, lane);
@@ -358,8 +380,11 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
 #pragma unroll
             for (int m = 0; m < 8; ++m) y[m] = x[m];
             hadamard_finite<8, LPR>(y, lane, rot_scale);
-            nan = __any(live && (nonfinite(y[0]) || __builtin_isunordered(y[0], y[1]) || __builtin_isunordered(y[2], y[3]) ||
-                                 __builtin_isunordered(y[4], y[5]) || __builtin_isunordered(y[6], y[7])));
+            nan = ((__builtin_amdgcn_ballot_w64(nonfinite(y[0])) | __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[0], y[1])) |
+                    __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[2], y[3])) |
+                    __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[4], y[5])) |
+                    __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[6], y[7]))) &
+                   (ALL ? ~0ull : __builtin_amdgcn_ballot_w64(live))) != 0;
             if (nan) {
                 look(x);
                 hadamard_rows_x<LPR>(x, buf, lane, rot_scale, xn);
@@ -367,27 +392,27 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
 #pragma unroll
                 for (int m = 0; m < 8; ++m) x[m] = y[m];
             }
-        } else if (MODE == HM_TQ6 && !rows_out) {
+        } else if (OUT == HO_CACHE && MODE == HM_TQ6) {
             look(x);
         }
 
-        if (rows_out) {
-            if (live) store_row<WIDE>(d_row, o_type, x, e0, D);
-            continue;
-        }
-        if constexpr (MODE != HM_ROWS) {
-            if (live && f16_row) {
-                uint32_t h[4];
+        if constexpr (OUT == HO_F32) {
+            if (live) store_row<WIDE, ALL>((float *) d_this + e0, x, e0, D);
+        } else {
+            uint32_t h[4];
+            if (OUT == HO_CACHE || o_type == SJK_F16) {
 #pragma unroll
                 for (int m = 0; m < 4; ++m) h[m] = pack_f16(x[2 * m], x[2 * m + 1]);
-                // a NaN is stored as its sign | 0x7E00 (f32_to_f16)
-                if (nan) {
+            } else {
 #pragma unroll
-                    for (int m = 0; m < 4; ++m) h[m] = (uint32_t) f32_to_f16(x[2 * m]) | (uint32_t) f32_to_f16(x[2 * m + 1]) << 16;
-                }
-                store_halves<WIDE>((uint16_t *) d_row + e0, h, e0, D);
+                for (int m = 0; m < 4; ++m) h[m] = pack_bf16(x[2 * m], x[2 * m + 1]);
             }
-            if constexpr (MODE == HM_TQ6) {
+            if (OUT == HO_CACHE && nan) {                  // a NaN is stored as its sign | 0x7E00 (f32_to_f16)
+#pragma unroll
+                for (int m = 0; m < 4; ++m) h[m] = (uint32_t) f32_to_f16(x[2 * m]) | (uint32_t) f32_to_f16(x[2 * m + 1]) << 16;
+            }
+            if (live && (OUT == HO_HALF || f16_row)) store_halves<WIDE, ALL>((uint16_t *) d_this + e0, h, e0, D);
+            if constexpr (OUT == HO_CACHE && MODE == HM_TQ6) {
                 const bool tq = live && !f16_row;
                 if (!__any(tq)) continue;
                 // sj_kvarn.h:1221-1247: two sums of 128 values in index order, walked by every lane of the block (16 lanes)
@@ -410,7 +435,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
                 const float rn = __builtin_sqrtf(walk<false>(blk));
                 wave_sync();
                 if (tq) {
-                    uint8_t * o = d_row + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES;
+                    uint8_t * o = d_this + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES;
                     const int i0 = 8 * (l & 15);
                     if (!(l & 15)) *(uint16_t *) o = f32_to_f16(rn > 1e-10f ? xdiv(norm, rn) : norm);
                     uint32_t qs = 0, qh = 0;               // low nibbles; high pairs
@@ -426,6 +451,10 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
             }
         }
     }
+    };
+    if (!rows_out) heads(Int<MODE == HM_ROWS ? HO_F32 : HO_CACHE>());
+    else if (MODE != HM_ROWS || o_type == SJK_F32) heads(Int<HO_F32>());
+    else heads(Int<HO_HALF>());
 }
 
 static int refuse(const char * what) {
@@ -485,10 +514,13 @@ static int launch_kind(const HeadBatch & bt, int lpr, int mode, unsigned grid, h
 
 template <typename T>
 static int launch_typed(const HeadBatch & bt, int lpr, int mode, bool wide, unsigned grid, hipStream_t st) {
-    bool turned = false;
-    for (int p = 0; p < bt.n_parts; ++p) turned |= (bt.part[p].flags & HF_ROPE) != 0;
+    bool turned = false, weights = false;
+    for (int p = 0; p < bt.n_parts; ++p) {
+        turned |= (bt.part[p].flags & HF_ROPE) != 0;
+        weights |= bt.part[p].w && bt.part[p].w_head;
+    }
     if (!wide) return launch_kind<T, HK_ANY>(bt, lpr, mode, grid, st);
-    if (turned && bt.n_rot != 8 * lpr) return launch_kind<T, HK_PART>(bt, lpr, mode, grid, st);
+    if (bt.D != 8 * lpr || weights || (turned && bt.n_rot != 8 * lpr)) return launch_kind<T, HK_PART>(bt, lpr, mode, grid, st);
     return launch_kind<T, HK_WHOLE>(bt, lpr, mode, grid, st);
 }
 
