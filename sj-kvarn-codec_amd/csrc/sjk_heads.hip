@@ -124,9 +124,9 @@ template <bool WIDE, bool ALL> SJK_DEV void store_halves(uint16_t * o, const uin
     }
 }
 
-template <bool WIDE, bool ALL> SJK_DEV void store_row(float * o, const float (&x)[8], int e0, int D) {
+template <bool WIDE> SJK_DEV void store_row(float * o, const float (&x)[8], int e0, int D) {
     if constexpr (WIDE) {
-        if (ALL || e0 < D) {
+        if (e0 < D) {
             ((float4 *) o)[0] = float4{x[0], x[1], x[2], x[3]};
             ((float4 *) o)[1] = float4{x[4], x[5], x[6], x[7]};
         }
@@ -210,17 +210,24 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     const bool rope = P.flags & HF_ROPE, rot = P.flags & HF_ROT;
     float * buf = s_buf + wave * WS;
 
-    // the lane's row: position cp, heads ch, ch + step, ...
+    // the lane's rows: position cp, heads head_at(it, sub) of iterations it (ALL: of adjacent heads not past the last)
     const int block = u / P.n_chunks, run = u - block * P.n_chunks, h0 = run * P.n_iters * step;
     const int iters = min(P.n_iters, (n_heads - h0 + step - 1) / step);
-    int cp = bt.by_head ? block : block * RPW + sub, ch = h0 + (bt.by_head ? sub : 0);
-    if (ALL) cp = min(cp, bt.n_pos - 1);
-    const bool here = ALL || cp < bt.n_pos;
-    auto head_of = [&](int h) { return ALL && bt.by_head ? min(h, n_heads - 1) : h; };
-    const T * x_base = (const T *) Q.x[pi] + (int64_t) cp * P.x_pos, * x_row = x_base + head_of(ch) * P.x_head;
+    const bool by_head = bt.by_head;
+    auto pos_at = [&](int r) {
+        const int c = by_head ? block : block * RPW + r;
+        return ALL ? min(c, bt.n_pos - 1) : c;
+    };
+    auto head_at = [&](int it, int r) {
+        const int h = h0 + it * step + (by_head ? r : 0);
+        return ALL && by_head ? min(h, n_heads - 1) : h;
+    };
+    const int cp = pos_at(sub);
+    const bool here = cp < bt.n_pos;
     const int64_t x_head = P.x_head;
+    const T * const x_base = (const T *) Q.x[pi] + (int64_t) cp * P.x_pos, * x_row = x_base + head_at(0, sub) * x_head;
     Raw<T> raw = {};
-    if (ALL || (here && ch < n_heads)) load_row<T, WIDE, ALL>(raw, x_row, e0, D);
+    if (ALL || (here && head_at(0, sub) < n_heads)) load_row<T, WIDE, ALL>(raw, x_row, e0, D);
 
     const float * norm = P.w;
     const int64_t norm_head = P.w_head;
@@ -230,7 +237,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
 #pragma unroll
         for (int m = 0; m < 8; ++m) w[m] = ALL || e0 + m < D ? p[e0 + m] : 0.0f;
     };
-    if (norm) load_w(norm_head && ch < n_heads ? ch : 0);
+    if (norm) load_w(norm_head && head_at(0, sub) < n_heads ? head_at(0, sub) : 0);
     const int n_rot = bt.n_rot, half = n_rot / 2;
     const bool pairs = bt.layout == SJK_ROPE_PAIRS, whole = KIND == HK_WHOLE || n_rot == 8 * LPR;
     if (rope && here) {
@@ -274,16 +281,26 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
         }
     }
 
-    // where the rows go: d_row and from head to head d_head, in bytes. A cache's entry of the position: sink, or the ring's slot.
-    uint8_t * d_row;
+    // Where the rows go, d_head bytes from head to head. A cache's entry of the position: sink, or the ring's slot. Rows of fp32
+    // with ALL: a lane's 32 bytes go through LDS, so that a store takes 1 KB on end (16 bytes a lane 32 apart reach 3.7 TB/s);
+    // d_row and d_row2 are of the first and the second KB's rows then.
+    uint8_t * d_row, * d_row2 = nullptr;
     int64_t d_head;
     bool f16_row = MODE == HM_F16;
     const bool rows_out = MODE == HM_ROWS || P.kind == HP_ROWS;
     const int o_type = P.o_type;
+    const bool swapped = ALL && rows_out && (MODE != HM_ROWS || o_type == SJK_F32);
+    constexpr int CPR = 2 * LPR;                           // 16-byte pieces of a row of fp32
+    const int r1 = swapped ? lane / CPR : sub, r2 = (64 + lane) / CPR;
     if (rows_out) {
         const int64_t size = o_type == SJK_F32 ? 4 : 2;
-        d_row = (uint8_t *) Q.o[pi] + size * ((int64_t) cp * P.o_pos);
+        uint8_t * o = (uint8_t *) Q.o[pi];
+        d_row = o + size * (int64_t) pos_at(r1) * P.o_pos;
         d_head = size * P.o_head;
+        if (swapped) {
+            d_row += 16 * (lane % CPR);
+            d_row2 = o + size * (int64_t) pos_at(r2) * P.o_pos + 16 * ((64 + lane) % CPR);
+        }
     } else {
         const uint32_t pos = pos0 + (uint32_t) cp;
         const bool in_sink = pos < Q.S, sink_f16 = in_sink && bt.sink_type == SJKVARN_SINK_F16;
@@ -292,32 +309,34 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
         d_head = (int64_t) (2 * side);
         f16_row |= sink_f16;
     }
+    if (!by_head) {
+        d_row += h0 * d_head;
+        d_row2 += h0 * d_head;
+    }
 
     const float inv_D = bt.inv_D, eps = P.eps, rot_scale = bt.rot_scale;
-    d_row += head_of(ch) * d_head;
     // what the rows become: fp32, halves, or the cache's entries (stores of one kind only, for the same reason as ALL)
     auto heads = [&](auto out) {
     constexpr int OUT = decltype(out)::value;
     for (int it = 0; it < iters; ++it) {
-        const bool live = ALL || (here && ch < n_heads);
+        const bool live = ALL || (here && head_at(it, sub) < n_heads);
         float x[8];
 #pragma unroll
         for (int m = 0; m < 8; ++m) x[m] = raw_at<T>(raw, m);
-        uint8_t * const d_this = d_row;
-        const int c_this = ch;
-        ch += step;
-        if (bt.by_head) {
-            const int64_t d = head_of(ch) - head_of(c_this);
-            if (it + 1 < iters) x_row += d * x_head;
-            d_row += d * d_head;
+        uint8_t * d1 = d_row, * d2 = d_row2;
+        if (by_head) {
+            x_row = x_base + head_at(min(it + 1, iters - 1), sub) * x_head;
+            d1 += head_at(it, r1) * d_head;
+            d2 += head_at(it, r2) * d_head;
         } else {
             if (it + 1 < iters) x_row += x_head;           // (the last iteration of ALL loads its own row again)
             d_row += d_head;
+            d_row2 += d_head;
         }
-        if (ALL || (it + 1 < iters && here && ch < n_heads)) load_row<T, WIDE, ALL>(raw, x_row, e0, D);
+        if (ALL || (it + 1 < iters && here && head_at(it + 1, sub) < n_heads)) load_row<T, WIDE, ALL>(raw, x_row, e0, D);
 
         if (norm) {
-            if (!ALL && norm_head && it && live) load_w(c_this);
+            if (!ALL && norm_head && it && live) load_w(head_at(it, sub));
             float ss = (__builtin_fmaf(x[1], x[1], x[0] * x[0]) + __builtin_fmaf(x[3], x[3], x[2] * x[2])) +
                        (__builtin_fmaf(x[5], x[5], x[4] * x[4]) + __builtin_fmaf(x[7], x[7], x[6] * x[6]));
             ss += lane_xor<1>(ss, lane);
@@ -397,7 +416,17 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
         }
 
         if constexpr (OUT == HO_F32) {
-            if (live) store_row<WIDE, ALL>((float *) d_this + e0, x, e0, D);
+            if constexpr (ALL) {
+                float4 * t = (float4 *) buf;
+                wave_sync();
+                t[2 * lane] = float4{x[0], x[1], x[2], x[3]};
+                t[2 * lane + 1] = float4{x[4], x[5], x[6], x[7]};
+                wave_sync();
+                *(float4 *) d1 = t[lane];
+                *(float4 *) d2 = t[64 + lane];
+            } else if (live) {
+                store_row<WIDE>((float *) d1 + e0, x, e0, D);
+            }
         } else {
             uint32_t h[4];
             if (OUT == HO_CACHE || o_type == SJK_F16) {
@@ -411,7 +440,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
 #pragma unroll
                 for (int m = 0; m < 4; ++m) h[m] = (uint32_t) f32_to_f16(x[2 * m]) | (uint32_t) f32_to_f16(x[2 * m + 1]) << 16;
             }
-            if (live && (OUT == HO_HALF || f16_row)) store_halves<WIDE, ALL>((uint16_t *) d_this + e0, h, e0, D);
+            if (live && (OUT == HO_HALF || f16_row)) store_halves<WIDE, ALL>((uint16_t *) d1 + e0, h, e0, D);
             if constexpr (OUT == HO_CACHE && MODE == HM_TQ6) {
                 const bool tq = live && !f16_row;
                 if (!__any(tq)) continue;
@@ -435,7 +464,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
                 const float rn = __builtin_sqrtf(walk<false>(blk));
                 wave_sync();
                 if (tq) {
-                    uint8_t * o = d_this + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES;
+                    uint8_t * o = d1 + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES;
                     const int i0 = 8 * (l & 15);
                     if (!(l & 15)) *(uint16_t *) o = f32_to_f16(rn > 1e-10f ? xdiv(norm, rn) : norm);
                     uint32_t qs = 0, qh = 0;               // low nibbles; high pairs
