@@ -2,10 +2,9 @@
 // cache's basis, and the append, in one pass over the rows (sjk_hip_head_rows, sjk_hip_store_qkv).
 //
 // A row (one head at one position) lies 8 consecutive channels a lane in LPR lanes, so a wavefront holds 64 / LPR rows and
-// reads and writes 16 or 32 bytes a lane. The rows are the same head at adjacent positions, and the wavefront goes through a
-// run of heads of one set, the next head's loads issued before the current one's arithmetic: a lane keeps its position, whose
-// sines, cosines and cache slot it works out once. A call with fewer positions than the wavefront has rows takes adjacent
-// heads of one position instead.
+// reads and writes 16 or 32 bytes a lane. The rows are the same head at adjacent positions, or adjacent heads of one position
+// (HF_BY_HEAD), and the wavefront goes through a run of heads of one set, the next loads issued before the current rows'
+// arithmetic: a lane keeps its position, whose sines, cosines and cache slot it works out once.
 //   * norm: the sum of squares is a fixed tree (pairs in the lane, then lanes 1, 2, 4, ... apart), so a row's bits do not
 //     depend on the rows beside it.
 //   * turn: u = position * turns per position in double, reduced to (-1/2, 1/2] turns and then to an eighth of one either
@@ -23,7 +22,7 @@ constexpr int HEAD_PARTS = 3;          // sets of heads a launch: q, k, v
 constexpr int HEAD_SEQS = 32;          // sequences a launch
 constexpr int HEAD_ITERS = 8;          // heads a wavefront goes through at most
 enum { HP_ROWS = 0, HP_K = 1, HP_V = 2 };                               // where a part's rows go
-enum { HF_ROPE = 1, HF_ROT = 2 };
+enum { HF_ROPE = 1, HF_ROT = 2, HF_BY_HEAD = 4 };
 enum { HM_ROWS = 0, HM_F16 = 1, HM_TQ6 = 2 };                           // a launch: plain rows only, or a cache's staging
 enum { HO_F32 = 0, HO_HALF = 1, HO_CACHE = 2 };                         // a wavefront's rows
 template <int N> struct Int { static constexpr int value = N; };
@@ -48,7 +47,7 @@ struct HeadBatch {
     const double * turns;
     const int32_t * desc;
     size_t stage_bytes;
-    int n_parts, n_seqs, n_pos, D, by_head, units;     // by_head: rows are adjacent heads; units: wavefronts of one sequence
+    int n_parts, n_seqs, n_pos, D, units;              // units: wavefronts of one sequence
     int layout, n_rot, H, sink_type;
     float mscale, sine, rot_scale, inv_D;              // sine: the sign of sines (inverse)
 };
@@ -206,14 +205,14 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     const HeadSeq & Q = bt.seq[si];
     if (bt.desc && bt.desc[SJK_DESC_QPOS0] < 0) return;
     const uint32_t pos0 = bt.desc ? (uint32_t) bt.desc[SJK_DESC_QPOS0] : Q.pos0;
-    const int D = bt.D, n_heads = P.n_heads, step = bt.by_head ? RPW : 1;
+    const int D = bt.D, n_heads = P.n_heads, step = P.flags & HF_BY_HEAD ? RPW : 1;
     const bool rope = P.flags & HF_ROPE, rot = P.flags & HF_ROT;
     float * buf = s_buf + wave * WS;
 
     // the lane's rows: position cp, heads head_at(it, sub) of iterations it (ALL: of adjacent heads not past the last)
     const int block = u / P.n_chunks, run = u - block * P.n_chunks, h0 = run * P.n_iters * step;
     const int iters = min(P.n_iters, (n_heads - h0 + step - 1) / step);
-    const bool by_head = bt.by_head;
+    const bool by_head = P.flags & HF_BY_HEAD, uneven = ALL && by_head && n_heads % RPW;
     auto pos_at = [&](int r) {
         const int c = by_head ? block : block * RPW + r;
         return ALL ? min(c, bt.n_pos - 1) : c;
@@ -224,7 +223,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     };
     const int cp = pos_at(sub);
     const bool here = cp < bt.n_pos;
-    const int64_t x_head = P.x_head;
+    const int64_t x_head = P.x_head, x_step = step * x_head;
     const T * const x_base = (const T *) Q.x[pi] + (int64_t) cp * P.x_pos, * x_row = x_base + head_at(0, sub) * x_head;
     Raw<T> raw = {};
     if (ALL || (here && head_at(0, sub) < n_heads)) load_row<T, WIDE, ALL>(raw, x_row, e0, D);
@@ -309,10 +308,10 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
         d_head = (int64_t) (2 * side);
         f16_row |= sink_f16;
     }
-    if (!by_head) {
-        d_row += h0 * d_head;
-        d_row2 += h0 * d_head;
-    }
+    uint8_t * const d_base = d_row, * const d_base2 = d_row2;
+    d_row += head_at(0, r1) * d_head;
+    d_row2 += head_at(0, r2) * d_head;
+    const int64_t d_step = step * d_head;
 
     const float inv_D = bt.inv_D, eps = P.eps, rot_scale = bt.rot_scale;
     // what the rows become: fp32, halves, or the cache's entries (stores of one kind only, for the same reason as ALL)
@@ -324,14 +323,14 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
 #pragma unroll
         for (int m = 0; m < 8; ++m) x[m] = raw_at<T>(raw, m);
         uint8_t * d1 = d_row, * d2 = d_row2;
-        if (by_head) {
+        if (uneven) {                                      // (a last iteration with fewer heads than rows)
             x_row = x_base + head_at(min(it + 1, iters - 1), sub) * x_head;
-            d1 += head_at(it, r1) * d_head;
-            d2 += head_at(it, r2) * d_head;
+            d_row = d_base + head_at(it + 1, r1) * d_head;
+            d_row2 = d_base2 + head_at(it + 1, r2) * d_head;
         } else {
-            if (it + 1 < iters) x_row += x_head;           // (the last iteration of ALL loads its own row again)
-            d_row += d_head;
-            d_row2 += d_head;
+            if (it + 1 < iters) x_row += x_step;           // (the last iteration of ALL loads its own rows again)
+            d_row += d_step;
+            d_row2 += d_step;
         }
         if (ALL || (it + 1 < iters && here && head_at(it + 1, sub) < n_heads)) load_row<T, WIDE, ALL>(raw, x_row, e0, D);
 
@@ -553,15 +552,22 @@ static int launch_typed(const HeadBatch & bt, int lpr, int mode, bool wide, unsi
     return launch_kind<T, HK_WHOLE>(bt, lpr, mode, grid, st);
 }
 
-// The launch's shape. With as many positions as a wavefront has rows, a wavefront goes through up to HEAD_ITERS heads once
-// there are more wavefronts than the device holds resident (the sines and cosines of a position serve them all).
+// The launch's shape. A wavefront goes through up to HEAD_ITERS heads once there are more wavefronts than the device holds
+// resident (the sines and cosines of a position serve them all). Its rows are adjacent positions, except in calls of fewer
+// positions than that, and where rows of fp32 go out: those of one position lie on end, and stores of 2 KB reach 5.0 TB/s where
+// four of 512 bytes reach 4.6. (Rows of 16 bits: 4.5 by head, 4.9 by position, whose sines also serve more heads.)
 static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream_t st) {
     const int lpr = bt.D <= 64 ? 8 : bt.D <= 128 ? 16 : bt.D <= 256 ? 32 : 64, rpw = 64 / lpr;
-    bt.by_head = bt.n_pos < rpw;
-    const int step = bt.by_head ? rpw : 1;                                 // heads an iteration takes on
-    const int64_t blocks = bt.by_head ? bt.n_pos : (bt.n_pos + rpw - 1) / rpw;
-    int64_t groups = 0;
-    for (int p = 0; p < bt.n_parts; ++p) groups += blocks * ((bt.part[p].n_heads + step - 1) / step);
+    int64_t groups = 0, blocks[HEAD_PARTS];
+    int step[HEAD_PARTS];
+    for (int p = 0; p < bt.n_parts; ++p) {
+        HeadPart & P = bt.part[p];
+        const bool by_head = bt.n_pos < rpw || (P.kind == HP_ROWS && P.o_type == SJK_F32 && P.n_heads % rpw == 0);
+        if (by_head) P.flags |= HF_BY_HEAD;
+        step[p] = by_head ? rpw : 1;                                       // heads an iteration takes on
+        blocks[p] = by_head ? bt.n_pos : (bt.n_pos + rpw - 1) / rpw;
+        groups += blocks[p] * ((P.n_heads + step[p] - 1) / step[p]);
+    }
     groups *= bt.n_seqs;
     if (!groups) return 0;
     const int64_t it = groups / ((int64_t) n_cus() * 4 * HW);
@@ -569,10 +575,10 @@ static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream
     bt.units = 0;
     for (int p = 0; p < bt.n_parts; ++p) {
         HeadPart & P = bt.part[p];
-        const int steps = (P.n_heads + step - 1) / step;
+        const int steps = (P.n_heads + step[p] - 1) / step[p];
         P.n_chunks = (steps + most - 1) / most;
         P.n_iters = P.n_chunks ? (steps + P.n_chunks - 1) / P.n_chunks : 0;
-        P.n_units = (int) (blocks * P.n_chunks);
+        P.n_units = (int) (blocks[p] * P.n_chunks);
         bt.units += P.n_units;
     }
     bt.inv_D = 1.0f / (float) bt.D;
