@@ -166,27 +166,28 @@ template <int LPR> SJK_DEV void hadamard_rows_x(float (&x)[8], float * buf, int 
     wave_sync();
 }
 
-// KIND: which calls the kernel is for. The first has no masks and no addresses for what it does not do (92 registers for one
-// kernel of all calls, two wavefronts a SIMD less).
-enum { HK_WHOLE = 0,        // rows of 8 * LPR channels whose addresses and strides take 16-byte accesses, turned whole or not at all, and one set of
-                            // norm weights for all heads of a job
-       HK_PART = 1,         // such accesses otherwise
-       HK_ANY = 2 };        // rows of any width, address and stride
+// KIND: which calls the kernel is for. The first has no masks and no addresses for what it does not do.
+enum { HK_WHOLE = 0,        // rows of 8 * LPR channels whose addresses and strides take 16-byte accesses, turned whole or not at
+                            // all, and one set of norm weights for all heads of a job
+       HK_PART = 1,         // such accesses otherwise, a turn of halves over a multiple of 16 channels
+       HK_ANY = 2 };        // rows of any width, address and stride, any turn
 template <typename T, int LPR, int MODE, int KIND>
 __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     constexpr bool WIDE = KIND != HK_ANY;
-    // Where every lane has a row's channels, lanes behind the last row take the last row again and write the same values once
-    // more (both read it in one instruction, so also where rows are written over themselves): loads and stores without a
-    // branch around them, so that a wait for the next row's loads does not wait for this row's stores (on gfx9 one counter
+    // Lanes behind the last row take the last row again, and lanes behind a row's channels its first ones, and write the same
+    // values once more (both read in one instruction, so also where rows are written over themselves): loads and stores without
+    // a branch around them, so that a wait for the next row's loads does not wait for this row's stores (on gfx9 one counter
     // holds both, and the compiler can count past the stores only where they are certain: 8,192 positions x 40 heads of
-    // 128 turned in 39.5 us with branches).
-    constexpr bool ALL = KIND == HK_WHOLE;
+    // 128 turned in 39.5 us with branches, 36.1 without).
+    constexpr bool ALL = WIDE;
     constexpr int RPW = 64 / LPR;                          // rows a wavefront holds
     constexpr int BS = 132;                                // floats from a 128-value block to the next (walks: other banks)
     constexpr int WS = MODE == HM_TQ6 ? 4 * BS : 512;      // floats of a wavefront's LDS
     __shared__ alignas(16) float s_buf[HW * WS];
     __shared__ float s_mid[MODE == HM_TQ6 ? 64 : 1], s_cent[MODE == HM_TQ6 ? 64 : 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane % LPR, sub = lane / LPR, e0 = 8 * l;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPR, D = KIND == HK_WHOLE ? 8 * LPR : bt.D;
+    const bool again = KIND == HK_PART && lane % LPR >= D / 8;             // a lane behind the row's channels
+    const int l = lane % LPR - (again ? D / 8 : 0), e0 = 8 * l;
     if (MODE == HM_TQ6) {
         if (threadIdx.x < 64) {
             s_mid[threadIdx.x] = threadIdx.x < 63 ? tq6_mid(threadIdx.x) : __builtin_inff();
@@ -205,7 +206,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     const HeadSeq & Q = bt.seq[si];
     if (bt.desc && bt.desc[SJK_DESC_QPOS0] < 0) return;
     const uint32_t pos0 = bt.desc ? (uint32_t) bt.desc[SJK_DESC_QPOS0] : Q.pos0;
-    const int D = bt.D, n_heads = P.n_heads, step = P.flags & HF_BY_HEAD ? RPW : 1;
+    const int n_heads = P.n_heads, step = P.flags & HF_BY_HEAD ? RPW : 1;
     const bool rope = P.flags & HF_ROPE, rot = P.flags & HF_ROT;
     float * buf = s_buf + wave * WS;
 
@@ -235,10 +236,14 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
         const float * p = norm + h * norm_head;
 #pragma unroll
         for (int m = 0; m < 8; ++m) w[m] = ALL || e0 + m < D ? p[e0 + m] : 0.0f;
+#pragma unroll
+        for (int m = 0; m < 8; ++m) asm volatile("" : "+v"(w[m]));         // waited for here, not where they are used
     };
     if (norm) load_w(norm_head && head_at(0, sub) < n_heads ? head_at(0, sub) : 0);
     const int n_rot = bt.n_rot, half = n_rot / 2;
     const bool pairs = bt.layout == SJK_ROPE_PAIRS, whole = KIND == HK_WHOLE || n_rot == 8 * LPR;
+    // HK_PART: the lane of the other halves' channels; behind n_rot the lane itself
+    const int pair_lane = sub * LPR + (e0 < half ? l + half / 8 : e0 < n_rot ? l - half / 8 : l);
     if (rope && here) {
         const double p = Q.pos ? (double) Q.pos[cp] : (double) (pos0 + (uint32_t) cp);
         double t[8];                                       // all of the table's loads before the first turn
@@ -261,6 +266,21 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 const float so = lane_xor<LPR / 2>(s[m], lane), co = lane_xor<LPR / 2>(c[m], lane);
+                cs[m] = up ? co : c[m];
+                cs[m + 4] = up ? c[m] : co;
+                sn[m] = up ? so : -s[m];
+                sn[m + 4] = up ? s[m] : -so;
+            }
+        } else if (KIND == HK_PART) {                      // the same with the pair's lane half / 8 away
+            const bool up = e0 >= half, in = e0 < n_rot;
+            float s[4], c[4];
+#pragma unroll
+            for (int m = 0; m < 4; ++m) t[m] = in ? bt.turns[(up ? e0 - half + 4 : e0) + m] : 0.0;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) turn(p * t[m], bt.mscale, bt.sine, s[m], c[m]);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const float so = __shfl(s[m], pair_lane, 64), co = __shfl(c[m], pair_lane, 64);
                 cs[m] = up ? co : c[m];
                 cs[m + 4] = up ? c[m] : co;
                 sn[m] = up ? so : -s[m];
@@ -289,16 +309,17 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     const bool rows_out = MODE == HM_ROWS || P.kind == HP_ROWS;
     const int o_type = P.o_type;
     const bool swapped = ALL && rows_out && (MODE != HM_ROWS || o_type == SJK_F32);
-    constexpr int CPR = 2 * LPR;                           // 16-byte pieces of a row of fp32
-    const int r1 = swapped ? lane / CPR : sub, r2 = (64 + lane) / CPR;
+    const int cpr = D / 4;                                 // 16-byte pieces of a row of fp32
+    const int g1 = min(lane, RPW * cpr - 1), g2 = min(64 + lane, RPW * cpr - 1);
+    const int r1 = swapped ? g1 / cpr : sub, r2 = swapped ? g2 / cpr : sub;
     if (rows_out) {
         const int64_t size = o_type == SJK_F32 ? 4 : 2;
         uint8_t * o = (uint8_t *) Q.o[pi];
         d_row = o + size * (int64_t) pos_at(r1) * P.o_pos;
         d_head = size * P.o_head;
         if (swapped) {
-            d_row += 16 * (lane % CPR);
-            d_row2 = o + size * (int64_t) pos_at(r2) * P.o_pos + 16 * ((64 + lane) % CPR);
+            d_row += 16 * (g1 - r1 * cpr);
+            d_row2 = o + size * (int64_t) pos_at(r2) * P.o_pos + 16 * (g2 - r2 * cpr);
         }
     } else {
         const uint32_t pos = pos0 + (uint32_t) cp;
@@ -338,6 +359,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
             if (!ALL && norm_head && it && live) load_w(head_at(it, sub));
             float ss = (__builtin_fmaf(x[1], x[1], x[0] * x[0]) + __builtin_fmaf(x[3], x[3], x[2] * x[2])) +
                        (__builtin_fmaf(x[5], x[5], x[4] * x[4]) + __builtin_fmaf(x[7], x[7], x[6] * x[6]));
+            if (again) ss = 0.0f;
             ss += lane_xor<1>(ss, lane);
             ss += lane_xor<2>(ss, lane);
             ss += lane_xor<4>(ss, lane);
@@ -357,6 +379,9 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
             } else if (whole) {
 #pragma unroll
                 for (int m = 0; m < 8; ++m) y[m] = lane_xor<LPR / 2>(x[m], lane);
+            } else if (KIND == HK_PART) {
+#pragma unroll
+                for (int m = 0; m < 8; ++m) y[m] = __shfl(x[m], pair_lane, 64);
             } else {
                 // channel e in slot (e % 8) * 64 + sub * LPR + e / 8: both sides touch neighbouring words
                 wave_sync();
@@ -418,11 +443,11 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
             if constexpr (ALL) {
                 float4 * t = (float4 *) buf;
                 wave_sync();
-                t[2 * lane] = float4{x[0], x[1], x[2], x[3]};
-                t[2 * lane + 1] = float4{x[4], x[5], x[6], x[7]};
+                t[sub * cpr + 2 * l] = float4{x[0], x[1], x[2], x[3]};
+                t[sub * cpr + 2 * l + 1] = float4{x[4], x[5], x[6], x[7]};
                 wave_sync();
-                *(float4 *) d1 = t[lane];
-                *(float4 *) d2 = t[64 + lane];
+                *(float4 *) d1 = t[g1];
+                *(float4 *) d2 = t[g2];
             } else if (live) {
                 store_row<WIDE>((float *) d1 + e0, x, e0, D);
             }
@@ -547,7 +572,7 @@ static int launch_typed(const HeadBatch & bt, int lpr, int mode, bool wide, unsi
         turned |= (bt.part[p].flags & HF_ROPE) != 0;
         weights |= bt.part[p].w && bt.part[p].w_head;
     }
-    if (!wide) return launch_kind<T, HK_ANY>(bt, lpr, mode, grid, st);
+    if (!wide || (turned && bt.layout == SJK_ROPE_HALVES && bt.n_rot % 16)) return launch_kind<T, HK_ANY>(bt, lpr, mode, grid, st);
     if (bt.D != 8 * lpr || weights || (turned && bt.n_rot != 8 * lpr)) return launch_kind<T, HK_PART>(bt, lpr, mode, grid, st);
     return launch_kind<T, HK_WHOLE>(bt, lpr, mode, grid, st);
 }
