@@ -577,13 +577,14 @@ static int launch_typed(const HeadBatch & bt, int lpr, int mode, bool wide, unsi
     return launch_kind<T, HK_WHOLE>(bt, lpr, mode, grid, st);
 }
 
-// The launch's shape. A wavefront goes through up to HEAD_ITERS heads once there are more wavefronts than the device holds
-// resident (the sines and cosines of a position serve them all). Its rows are adjacent positions, except in calls of fewer
+// The launch's shape. A wavefront goes through as many heads, up to HEAD_ITERS, as it takes for all wavefronts to be on the
+// device at once (16 a CU; the sines and cosines of a position serve its heads): a second, partly filled round of them costs a
+// 512-position append 7.1 -> 8.5 us, 1,237 positions x 64 heads of 80 10.8 -> 12.1. Its rows are adjacent positions, except in calls of fewer
 // positions than that, and where rows of fp32 go out: those of one position lie on end, and stores of 2 KB reach 5.0 TB/s where
 // four of 512 bytes reach 4.6. (Rows of 16 bits: 4.5 by head, 4.9 by position, whose sines also serve more heads.)
 static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream_t st) {
     const int lpr = bt.D <= 64 ? 8 : bt.D <= 128 ? 16 : bt.D <= 256 ? 32 : 64, rpw = 64 / lpr;
-    int64_t groups = 0, blocks[HEAD_PARTS];
+    int64_t blocks[HEAD_PARTS];
     int step[HEAD_PARTS];
     for (int p = 0; p < bt.n_parts; ++p) {
         HeadPart & P = bt.part[p];
@@ -591,24 +592,25 @@ static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream
         if (by_head) P.flags |= HF_BY_HEAD;
         step[p] = by_head ? rpw : 1;                                       // heads an iteration takes on
         blocks[p] = by_head ? bt.n_pos : (bt.n_pos + rpw - 1) / rpw;
-        groups += blocks[p] * ((P.n_heads + step[p] - 1) / step[p]);
     }
-    groups *= bt.n_seqs;
-    if (!groups) return 0;
-    const int64_t it = groups / ((int64_t) n_cus() * 4 * HW);
-    const int most = it < 1 ? 1 : it > HEAD_ITERS ? HEAD_ITERS : (int) it;
-    bt.units = 0;
-    for (int p = 0; p < bt.n_parts; ++p) {
-        HeadPart & P = bt.part[p];
-        const int steps = (P.n_heads + step[p] - 1) / step[p];
-        P.n_chunks = (steps + most - 1) / most;
-        P.n_iters = P.n_chunks ? (steps + P.n_chunks - 1) / P.n_chunks : 0;
-        P.n_units = (int) (blocks[p] * P.n_chunks);
-        bt.units += P.n_units;
+    int64_t waves = 0;
+    for (int most = 1; most <= HEAD_ITERS; ++most) {
+        bt.units = 0;
+        for (int p = 0; p < bt.n_parts; ++p) {
+            HeadPart & P = bt.part[p];
+            const int steps = (P.n_heads + step[p] - 1) / step[p];
+            P.n_chunks = (steps + most - 1) / most;
+            P.n_iters = P.n_chunks ? (steps + P.n_chunks - 1) / P.n_chunks : 0;
+            P.n_units = (int) (blocks[p] * P.n_chunks);
+            bt.units += P.n_units;
+        }
+        waves = (int64_t) bt.units * bt.n_seqs;
+        if (waves <= (int64_t) n_cus() * 4 * HW) break;
     }
+    if (!waves) return 0;
     bt.inv_D = 1.0f / (float) bt.D;
     bt.rot_scale = rot_scale(bt.D);
-    const unsigned grid = (unsigned) (((int64_t) bt.units * bt.n_seqs + HW - 1) / HW);
+    const unsigned grid = (unsigned) ((waves + HW - 1) / HW);
     if (type == SJK_F32) return launch_typed<float>(bt, lpr, mode, wide, grid, st);
     if (type == SJK_F16) return launch_typed<_Float16>(bt, lpr, mode, wide, grid, st);
     return launch_typed<__bf16>(bt, lpr, mode, wide, grid, st);
