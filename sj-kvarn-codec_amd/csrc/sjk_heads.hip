@@ -78,6 +78,43 @@ SJK_DEV void turn(double u, float m, float sg, float & s, float & c) {
     __builtin_amdgcn_sched_barrier(0);       // one after the other: interleaved, their temporaries set the kernel's registers
 }
 
+// tq6_level by one look into a table: the line is cut into LV_CELLS cells so narrow that each holds at most one midpoint, which a
+// comparison then decides exactly. The cell of a value is a monotone function of it, the same for midpoints and values, so every
+// midpoint of a lower cell is below the value and every one of a higher cell above. (Six dependent reads of the search before:
+// 4,096 positions of 32 + 8 heads of 128 to tq6_0 LV_MEASURED us.) Not for NaNs.
+constexpr int LV_CELLS = 128;
+constexpr float LV_SCALE = 200.0f;
+struct LevelCell { float mid; int base; };                 // the cell's midpoint (or infinity), the midpoints of lower cells
+struct LevelTable { LevelCell cell[LV_CELLS]; };
+constexpr float level_at(float v) { return v * LV_SCALE + 64.0f; }
+constexpr int level_cell(float v) { const float t = level_at(v); return t < 0.0f ? 0 : t > 127.0f ? 127 : (int) t; }
+constexpr LevelTable level_table() {
+    constexpr uint32_t bits[63] = SJK_TQ6_MIDPOINT_BITS_INIT;
+    LevelTable t = {};
+    for (int c = 0; c < LV_CELLS; ++c) {
+        t.cell[c].mid = __builtin_inff();
+        for (int i = 0; i < 63; ++i) {
+            const float m = __builtin_bit_cast(float, bits[i]);
+            if (level_cell(m) < c) ++t.cell[c].base;
+            if (level_cell(m) == c) t.cell[c].mid = m;
+        }
+    }
+    return t;
+}
+constexpr bool level_table_ok() {                          // no cell with two midpoints, midpoints in ascending order
+    constexpr uint32_t bits[63] = SJK_TQ6_MIDPOINT_BITS_INIT;
+    for (int i = 1; i < 63; ++i)
+        if (level_cell(__builtin_bit_cast(float, bits[i])) <= level_cell(__builtin_bit_cast(float, bits[i - 1]))) return false;
+    return true;
+}
+static_assert(level_table_ok(), "one midpoint a cell");
+static __constant__ LevelTable c_levels = level_table();
+
+SJK_DEV int level_of(float v, const LevelCell * cells) {
+    const LevelCell c = cells[(int) __builtin_amdgcn_fmed3f(level_at(v), 0.0f, 127.0f)];
+    return c.base + (v < c.mid ? 0 : 1);
+}
+
 // 8 channels of a row from its element e0 on, as raw words. WIDE: 16 bytes at a time, else element by element up to D.
 template <typename T> struct Raw { uint32_t w[2 * sizeof(T)]; };
 template <typename T, bool WIDE, bool ALL> SJK_DEV void load_row(Raw<T> & r, const T * p, int e0, int D) {
@@ -184,15 +221,14 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     constexpr int BS = 132;                                // floats from a 128-value block to the next (walks: other banks)
     constexpr int WS = MODE == HM_TQ6 ? 4 * BS : 512;      // floats of a wavefront's LDS
     __shared__ alignas(16) float s_buf[HW * WS];
-    __shared__ float s_mid[MODE == HM_TQ6 ? 64 : 1], s_cent[MODE == HM_TQ6 ? 64 : 1];
+    __shared__ LevelCell s_cell[MODE == HM_TQ6 ? LV_CELLS : 1];
+    __shared__ float s_cent[MODE == HM_TQ6 ? 64 : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPR, D = KIND == HK_WHOLE ? 8 * LPR : bt.D;
     const bool again = KIND == HK_PART && lane % LPR >= D / 8;             // a lane behind the row's channels
     const int l = lane % LPR - (again ? D / 8 : 0), e0 = 8 * l;
     if (MODE == HM_TQ6) {
-        if (threadIdx.x < 64) {
-            s_mid[threadIdx.x] = threadIdx.x < 63 ? tq6_mid(threadIdx.x) : __builtin_inff();
-            s_cent[threadIdx.x] = tq6_cent(threadIdx.x);
-        }
+        if (threadIdx.x < LV_CELLS) s_cell[threadIdx.x] = c_levels.cell[threadIdx.x];
+        if (threadIdx.x < 64) s_cent[threadIdx.x] = tq6_cent(threadIdx.x);
         __syncthreads();
     }
     // this wavefront's sequence, part, positions and heads (wave-uniform)
@@ -480,7 +516,11 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
                 const float inv = big ? 1.0f / norm : 0.0f;
                 int code[8];
 #pragma unroll
-                for (int m = 0; m < 8; ++m) code[m] = tq6_level(big ? x[m] * inv : 0.0f, s_mid);
+                for (int m = 0; m < 8; ++m) {
+                    const float v = big ? x[m] * inv : 0.0f;
+                    code[m] = level_of(v, s_cell);
+                    if (nf_rows && v != v) code[m] = 63;
+                }
                 wave_sync();
 #pragma unroll
                 for (int m = 0; m < 8; ++m) { const float c = s_cent[code[m]]; sq[m] = c * c; }
