@@ -80,8 +80,8 @@ SJK_DEV void turn(double u, float m, float sg, float & s, float & c) {
 
 // tq6_level by one look into a table: the line is cut into LV_CELLS cells so narrow that each holds at most one midpoint, which a
 // comparison then decides exactly. The cell of a value is a monotone function of it, the same for midpoints and values, so every
-// midpoint of a lower cell is below the value and every one of a higher cell above. (Six dependent reads of the search before:
-// 4,096 positions of 32 + 8 heads of 128 to tq6_0 LV_MEASURED us.) Not for NaNs.
+// midpoint of a lower cell is below the value and every one of a higher cell above. (With the search's six dependent
+// reads 4,096 positions of 32 + 8 heads of 128 to tq6_0 take 6 us more.) Not for NaNs.
 constexpr int LV_CELLS = 128;
 constexpr float LV_SCALE = 200.0f;
 struct LevelCell { float mid; int base; };                 // the cell's midpoint (or infinity), the midpoints of lower cells
@@ -236,8 +236,9 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     const int si = u / bt.units;
     if (si >= bt.n_seqs) return;
     u -= si * bt.units;
-    int pi = 0;
-    while (pi + 1 < bt.n_parts && u >= bt.part[pi].n_units) u -= bt.part[pi++].n_units;
+    int pi = bt.n_parts - 1;                               // keys and values first: staging them takes longest (last, 4,096
+                                                           // positions to tq6_0 take 49 us for 39)
+    while (pi > 0 && u >= bt.part[pi].n_units) u -= bt.part[pi--].n_units;
     const HeadPart & P = bt.part[pi];
     const HeadSeq & Q = bt.seq[si];
     if (bt.desc && bt.desc[SJK_DESC_QPOS0] < 0) return;
@@ -638,8 +639,11 @@ static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream
         bt.units = 0;
         for (int p = 0; p < bt.n_parts; ++p) {
             HeadPart & P = bt.part[p];
+            // staging tq6_0 rows takes twice a query's time: half as many of them a wavefront, where all are on the device at once
+            // (512 positions of 32 + 8 heads 10.6 -> 9.2 us, 2,048 26.8 -> 20.1; 4,096, in several rounds, 38.6 -> 42.3)
             const int steps = (P.n_heads + step[p] - 1) / step[p];
-            P.n_chunks = (steps + most - 1) / most;
+            const int run = mode == HM_TQ6 && P.kind != HP_ROWS && most < HEAD_ITERS ? (most + 1) / 2 : most;
+            P.n_chunks = (steps + run - 1) / run;
             P.n_iters = P.n_chunks ? (steps + P.n_chunks - 1) / P.n_chunks : 0;
             P.n_units = (int) (blocks[p] * P.n_chunks);
             bt.units += P.n_units;
