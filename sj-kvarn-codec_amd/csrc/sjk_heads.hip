@@ -634,23 +634,25 @@ static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream
         step[p] = by_head ? rpw : 1;                                       // heads an iteration takes on
         blocks[p] = by_head ? bt.n_pos : (bt.n_pos + rpw - 1) / rpw;
     }
+    // staging tq6_0 rows takes twice a query's time: half as many of them a wavefront, where all are on the device at once (512
+    // positions of 32 + 8 heads 10.6 -> 9.2 us, 2,048 26.8 -> 20.1; 4,096, in several rounds, 38.6 -> 42.3)
     int64_t waves = 0;
-    for (int most = 1; most <= HEAD_ITERS; ++most) {
+    auto shape = [&](int most, int most_tq) {
         bt.units = 0;
         for (int p = 0; p < bt.n_parts; ++p) {
             HeadPart & P = bt.part[p];
-            // staging tq6_0 rows takes twice a query's time: half as many of them a wavefront, where all are on the device at once
-            // (512 positions of 32 + 8 heads 10.6 -> 9.2 us, 2,048 26.8 -> 20.1; 4,096, in several rounds, 38.6 -> 42.3)
-            const int steps = (P.n_heads + step[p] - 1) / step[p];
-            const int run = mode == HM_TQ6 && P.kind != HP_ROWS && most < HEAD_ITERS ? (most + 1) / 2 : most;
+            const int steps = (P.n_heads + step[p] - 1) / step[p], run = mode == HM_TQ6 && P.kind != HP_ROWS ? most_tq : most;
             P.n_chunks = (steps + run - 1) / run;
             P.n_iters = P.n_chunks ? (steps + P.n_chunks - 1) / P.n_chunks : 0;
             P.n_units = (int) (blocks[p] * P.n_chunks);
             bt.units += P.n_units;
         }
         waves = (int64_t) bt.units * bt.n_seqs;
-        if (waves <= (int64_t) n_cus() * 4 * HW) break;
-    }
+        return waves <= (int64_t) n_cus() * 4 * HW;
+    };
+    int most = 1;
+    while (most <= HEAD_ITERS && !shape(most, (most + 1) / 2)) ++most;
+    if (most > HEAD_ITERS) shape(HEAD_ITERS, HEAD_ITERS);
     if (!waves) return 0;
     bt.inv_D = 1.0f / (float) bt.D;
     bt.rot_scale = rot_scale(bt.D);
