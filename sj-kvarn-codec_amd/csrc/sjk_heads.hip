@@ -117,15 +117,13 @@ SJK_DEV int level_of(float v, const LevelCell * cells) {
 
 // 8 channels of a row from its element e0 on, as raw words. WIDE: 16 bytes at a time, else element by element up to D.
 template <typename T> struct Raw { uint32_t w[2 * sizeof(T)]; };
-template <typename T, bool WIDE, bool ALL> SJK_DEV void load_row(Raw<T> & r, const T * p, int e0, int D) {
+template <typename T, bool WIDE> SJK_DEV void load_row(Raw<T> & r, const T * p, int e0, int D) {
     constexpr int NW = 2 * (int) sizeof(T);
     if constexpr (WIDE) {
-        if (ALL || e0 < D) {
 #pragma unroll
-            for (int i = 0; i < NW; i += 4) {
-                const uint4 v = *(const uint4 *) ((const uint32_t *) (p + e0) + i);
-                r.w[i] = v.x; r.w[i + 1] = v.y; r.w[i + 2] = v.z; r.w[i + 3] = v.w;
-            }
+        for (int i = 0; i < NW; i += 4) {
+            const uint4 v = *(const uint4 *) ((const uint32_t *) (p + e0) + i);
+            r.w[i] = v.x; r.w[i + 1] = v.y; r.w[i + 2] = v.z; r.w[i + 3] = v.w;
         }
     } else {
 #pragma unroll
@@ -151,24 +149,12 @@ typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 SJK_DEV uint32_t pack_f16(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{a, b}), f16x2_t)); }
 SJK_DEV uint32_t pack_bf16(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{a, b}), bf16x2_t)); }
 
-template <bool WIDE, bool ALL> SJK_DEV void store_halves(uint16_t * o, const uint32_t (&h)[4], int e0, int D) {
+template <bool WIDE> SJK_DEV void store_halves(uint16_t * o, const uint32_t (&h)[4], int e0, int D) {
     if constexpr (WIDE) {
-        if (ALL || e0 < D) *(uint4 *) o = uint4{h[0], h[1], h[2], h[3]};
+        *(uint4 *) o = uint4{h[0], h[1], h[2], h[3]};
     } else {
 #pragma unroll
         for (int m = 0; m < 8; ++m) if (e0 + m < D) o[m] = (uint16_t) (h[m >> 1] >> (16 * (m & 1)));
-    }
-}
-
-template <bool WIDE> SJK_DEV void store_row(float * o, const float (&x)[8], int e0, int D) {
-    if constexpr (WIDE) {
-        if (e0 < D) {
-            ((float4 *) o)[0] = float4{x[0], x[1], x[2], x[3]};
-            ((float4 *) o)[1] = float4{x[4], x[5], x[6], x[7]};
-        }
-    } else {
-#pragma unroll
-        for (int m = 0; m < 8; ++m) if (e0 + m < D) o[m] = x[m];
     }
 }
 
@@ -207,16 +193,17 @@ template <int LPR> SJK_DEV void hadamard_rows_x(float (&x)[8], float * buf, int 
 enum { HK_WHOLE = 0,        // rows of 8 * LPR channels whose addresses and strides take 16-byte accesses, turned whole or not at
                             // all, and one set of norm weights for all heads of a job
        HK_PART = 1,         // such accesses otherwise, a turn of halves over a multiple of 16 channels
-       HK_ANY = 2 };        // rows of any width, address and stride, any turn
+       HK_ODD = 2,          // such accesses, a turn of halves over another number: pairs through LDS
+       HK_ANY = 3 };        // rows of any width, address and stride, any turn, element by element (3,226 positions x 6 heads of 256
+                            // turned over 232 channels: 25.7 us, 14.0 by HK_ODD)
 template <typename T, int LPR, int MODE, int KIND>
 __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
-    constexpr bool WIDE = KIND != HK_ANY;
     // Lanes behind the last row take the last row again, and lanes behind a row's channels its first ones, and write the same
     // values once more (both read in one instruction, so also where rows are written over themselves): loads and stores without
     // a branch around them, so that a wait for the next row's loads does not wait for this row's stores (on gfx9 one counter
     // holds both, and the compiler can count past the stores only where they are certain: 8,192 positions x 40 heads of
     // 128 turned in 39.5 us with branches, 36.1 without).
-    constexpr bool ALL = WIDE;
+    constexpr bool ALL = KIND != HK_ANY;
     constexpr int RPW = 64 / LPR;                          // rows a wavefront holds
     constexpr int BS = 132;                                // floats from a 128-value block to the next (walks: other banks)
     constexpr int WS = MODE == HM_TQ6 ? 4 * BS : 512;      // floats of a wavefront's LDS
@@ -224,7 +211,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     __shared__ LevelCell s_cell[MODE == HM_TQ6 ? LV_CELLS : 1];
     __shared__ float s_cent[MODE == HM_TQ6 ? 64 : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPR, D = KIND == HK_WHOLE ? 8 * LPR : bt.D;
-    const bool again = KIND == HK_PART && lane % LPR >= D / 8;             // a lane behind the row's channels
+    const bool again = ALL && KIND != HK_WHOLE && lane % LPR >= D / 8;    // a lane behind the row's channels
     const int l = lane % LPR - (again ? D / 8 : 0), e0 = 8 * l;
     if (MODE == HM_TQ6) {
         if (threadIdx.x < LV_CELLS) s_cell[threadIdx.x] = c_levels.cell[threadIdx.x];
@@ -264,7 +251,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     const int64_t x_head = P.x_head, x_step = step * x_head;
     const T * const x_base = (const T *) Q.x[pi] + (int64_t) cp * P.x_pos, * x_row = x_base + head_at(0, sub) * x_head;
     Raw<T> raw = {};
-    if (ALL || (here && head_at(0, sub) < n_heads)) load_row<T, WIDE, ALL>(raw, x_row, e0, D);
+    if (ALL || (here && head_at(0, sub) < n_heads)) load_row<T, ALL>(raw, x_row, e0, D);
 
     const float * norm = P.w;
     const int64_t norm_head = P.w_head;
@@ -374,177 +361,178 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     const float inv_D = bt.inv_D, eps = P.eps, rot_scale = bt.rot_scale;
     // what the rows become: fp32, halves, or the cache's entries (stores of one kind only, for the same reason as ALL)
     auto heads = [&](auto out) {
-    constexpr int OUT = decltype(out)::value;
-    for (int it = 0; it < iters; ++it) {
-        const bool live = ALL || (here && head_at(it, sub) < n_heads);
-        float x[8];
+        constexpr int OUT = decltype(out)::value;
+        for (int it = 0; it < iters; ++it) {
+            const bool live = ALL || (here && head_at(it, sub) < n_heads);
+            float x[8];
 #pragma unroll
-        for (int m = 0; m < 8; ++m) x[m] = raw_at<T>(raw, m);
-        uint8_t * d1 = d_row, * d2 = d_row2;
-        if (uneven) {                                      // (a last iteration with fewer heads than rows)
-            x_row = x_base + head_at(min(it + 1, iters - 1), sub) * x_head;
-            d_row = d_base + head_at(it + 1, r1) * d_head;
-            d_row2 = d_base2 + head_at(it + 1, r2) * d_head;
-        } else {
-            if (it + 1 < iters) x_row += x_step;           // (the last iteration of ALL loads its own rows again)
-            d_row += d_step;
-            d_row2 += d_step;
-        }
-        if (ALL || (it + 1 < iters && here && head_at(it + 1, sub) < n_heads)) load_row<T, WIDE, ALL>(raw, x_row, e0, D);
-
-        if (norm) {
-            if (!ALL && norm_head && it && live) load_w(head_at(it, sub));
-            float ss = (__builtin_fmaf(x[1], x[1], x[0] * x[0]) + __builtin_fmaf(x[3], x[3], x[2] * x[2])) +
-                       (__builtin_fmaf(x[5], x[5], x[4] * x[4]) + __builtin_fmaf(x[7], x[7], x[6] * x[6]));
-            if (again) ss = 0.0f;
-            ss += lane_xor<1>(ss, lane);
-            ss += lane_xor<2>(ss, lane);
-            ss += lane_xor<4>(ss, lane);
-            if constexpr (LPR > 8) ss += lane_xor<8>(ss, lane);
-            if constexpr (LPR > 16) ss += lane_xor<16>(ss, lane);
-            if constexpr (LPR > 32) ss += lane_xor<32>(ss, lane);
-            const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(ss, inv_D, eps));      // within an ulp; eps keeps it normal
-#pragma unroll
-            for (int m = 0; m < 8; ++m) x[m] = x[m] * r * w[m];
-        }
-
-        if (rope) {
-            float y[8];                                    // the other channel of each pair
-            if (pairs) {
-#pragma unroll
-                for (int m = 0; m < 8; ++m) y[m] = x[m ^ 1];
-            } else if (whole) {
-#pragma unroll
-                for (int m = 0; m < 8; ++m) y[m] = lane_xor<LPR / 2>(x[m], lane);
-            } else if (KIND == HK_PART) {
-#pragma unroll
-                for (int m = 0; m < 8; ++m) y[m] = __shfl(x[m], pair_lane, 64);
+            for (int m = 0; m < 8; ++m) x[m] = raw_at<T>(raw, m);
+            uint8_t * d1 = d_row, * d2 = d_row2;
+            if (uneven) {                                      // (a last iteration with fewer heads than rows)
+                x_row = x_base + head_at(min(it + 1, iters - 1), sub) * x_head;
+                d_row = d_base + head_at(it + 1, r1) * d_head;
+                d_row2 = d_base2 + head_at(it + 1, r2) * d_head;
             } else {
-                // channel e in slot (e % 8) * 64 + sub * LPR + e / 8: both sides touch neighbouring words
-                wave_sync();
-#pragma unroll
-                for (int m = 0; m < 8; ++m) buf[m * 64 + lane] = x[m];
-                wave_sync();
-#pragma unroll
-                for (int m = 0; m < 8; ++m) {
-                    const int e = e0 + m, pe = e < half ? e + half : e < n_rot ? e - half : e;
-                    y[m] = buf[(pe & 7) * 64 + sub * LPR + (pe >> 3)];
-                }
-                wave_sync();
+                if (it + 1 < iters) x_row += x_step;           // (the last iteration of ALL loads its own rows again)
+                d_row += d_step;
+                d_row2 += d_step;
             }
-            if (whole) {
-#pragma unroll
-                for (int m = 0; m < 8; ++m) x[m] = __builtin_fmaf(x[m], cs[m], y[m] * sn[m]);
-            } else {
-#pragma unroll
-                for (int m = 0; m < 8; ++m)
-                    if (e0 + m < n_rot) x[m] = __builtin_fmaf(x[m], cs[m], y[m] * sn[m]);
-            }
-        }
+            if (ALL || (it + 1 < iters && here && head_at(it + 1, sub) < n_heads)) load_row<T, ALL>(raw, x_row, e0, D);
 
-        // A row holding an infinity or a NaN takes the rotation and the tq6_0 sums with the host's NaN rule. Every value of its
-        // rotation is an infinity or a NaN then, so a look at one of each lane's finds it. A row that overflows on the way keeps
-        // the plain rotation, but where that makes NaNs their signs are hadamard_row's.
-        uint64_t nf_rows = 0;
-        bool xn = false;
-        auto look = [&](const float (&v)[8]) {
-            bool nf = false;
+            if (norm) {
+                if (KIND != HK_WHOLE && norm_head && it && live) load_w(head_at(it, sub));
+                float ss = (__builtin_fmaf(x[1], x[1], x[0] * x[0]) + __builtin_fmaf(x[3], x[3], x[2] * x[2])) +
+                           (__builtin_fmaf(x[5], x[5], x[4] * x[4]) + __builtin_fmaf(x[7], x[7], x[6] * x[6]));
+                if (again) ss = 0.0f;
+                ss += lane_xor<1>(ss, lane);
+                ss += lane_xor<2>(ss, lane);
+                ss += lane_xor<4>(ss, lane);
+                if constexpr (LPR > 8) ss += lane_xor<8>(ss, lane);
+                if constexpr (LPR > 16) ss += lane_xor<16>(ss, lane);
+                if constexpr (LPR > 32) ss += lane_xor<32>(ss, lane);
+                const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(ss, inv_D, eps));      // within an ulp; eps keeps it normal
 #pragma unroll
-            for (int m = 0; m < 8; ++m) nf |= nonfinite(v[m]);
-            nf_rows = __ballot(nf && live);
-            xn = ((LPR == 64 ? nf_rows : nf_rows >> (sub * LPR)) & ((LPR == 64 ? 0 : 1ull << (LPR % 64)) - 1ull)) != 0;
-        };
-        bool nan = true;                                   // whether the rows may hold NaNs (wave-uniform)
-        if (rot) {
-            float y[8];
-#pragma unroll
-            for (int m = 0; m < 8; ++m) y[m] = x[m];
-            hadamard_finite<8, LPR>(y, lane, rot_scale);
-            nan = ((__builtin_amdgcn_ballot_w64(nonfinite(y[0])) | __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[0], y[1])) |
-                    __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[2], y[3])) |
-                    __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[4], y[5])) |
-                    __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[6], y[7]))) &
-                   (ALL ? ~0ull : __builtin_amdgcn_ballot_w64(live))) != 0;
-            if (nan) {
-                look(x);
-                hadamard_rows_x<LPR>(x, buf, lane, rot_scale, xn);
-            } else {
-#pragma unroll
-                for (int m = 0; m < 8; ++m) x[m] = y[m];
+                for (int m = 0; m < 8; ++m) x[m] = x[m] * r * w[m];
             }
-        } else if (OUT == HO_CACHE && MODE == HM_TQ6) {
-            look(x);
-        }
 
-        if constexpr (OUT == HO_F32) {
-            if constexpr (ALL) {
-                float4 * t = (float4 *) buf;
-                wave_sync();
-                t[sub * cpr + 2 * l] = float4{x[0], x[1], x[2], x[3]};
-                t[sub * cpr + 2 * l + 1] = float4{x[4], x[5], x[6], x[7]};
-                wave_sync();
-                *(float4 *) d1 = t[g1];
-                *(float4 *) d2 = t[g2];
-            } else if (live) {
-                store_row<WIDE>((float *) d1 + e0, x, e0, D);
-            }
-        } else {
-            uint32_t h[4];
-            if (OUT == HO_CACHE || o_type == SJK_F16) {
+            if (rope) {
+                float y[8];                                    // the other channel of each pair
+                if (pairs) {
 #pragma unroll
-                for (int m = 0; m < 4; ++m) h[m] = pack_f16(x[2 * m], x[2 * m + 1]);
-            } else {
+                    for (int m = 0; m < 8; ++m) y[m] = x[m ^ 1];
+                } else if (whole) {
 #pragma unroll
-                for (int m = 0; m < 4; ++m) h[m] = pack_bf16(x[2 * m], x[2 * m + 1]);
-            }
-            if (OUT == HO_CACHE && nan) {                  // a NaN is stored as its sign | 0x7E00 (f32_to_f16)
+                    for (int m = 0; m < 8; ++m) y[m] = lane_xor<LPR / 2>(x[m], lane);
+                } else if (KIND == HK_PART) {
 #pragma unroll
-                for (int m = 0; m < 4; ++m) h[m] = (uint32_t) f32_to_f16(x[2 * m]) | (uint32_t) f32_to_f16(x[2 * m + 1]) << 16;
-            }
-            if (live && (OUT == HO_HALF || f16_row)) store_halves<WIDE, ALL>((uint16_t *) d1 + e0, h, e0, D);
-            if constexpr (OUT == HO_CACHE && MODE == HM_TQ6) {
-                const bool tq = live && !f16_row;
-                if (!__any(tq)) continue;
-                // sj_kvarn.h:1221-1247: two sums of 128 values in index order, walked by every lane of the block (16 lanes)
-                float * blk = buf + (lane >> 4) * BS, * sq = blk + 8 * (lane & 15);
-                wave_sync();
+                    for (int m = 0; m < 8; ++m) y[m] = __shfl(x[m], pair_lane, 64);
+                } else {
+                    // channel e in slot (e % 8) * 64 + sub * LPR + e / 8: both sides touch neighbouring words
+                    wave_sync();
 #pragma unroll
-                for (int m = 0; m < 8; ++m) sq[m] = xn ? xmul(x[m], x[m]) : x[m] * x[m];
-                wave_sync();
-                const float nsq = nf_rows ? walk<true>(blk, xn) : walk<false>(blk);
-                const float norm = nsq != nsq ? nan_of(nsq) : __builtin_sqrtf(nsq);
-                const bool big = norm > 1e-10f;
-                const float inv = big ? 1.0f / norm : 0.0f;
-                int code[8];
-#pragma unroll
-                for (int m = 0; m < 8; ++m) {
-                    const float v = big ? x[m] * inv : 0.0f;
-                    code[m] = level_of(v, s_cell);
-                    if (nf_rows && v != v) code[m] = 63;
-                }
-                wave_sync();
-#pragma unroll
-                for (int m = 0; m < 8; ++m) { const float c = s_cent[code[m]]; sq[m] = c * c; }
-                wave_sync();
-                const float rn = __builtin_sqrtf(walk<false>(blk));
-                wave_sync();
-                if (tq) {
-                    uint8_t * o = d1 + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES;
-                    const int i0 = 8 * (l & 15);
-                    if (!(l & 15)) *(uint16_t *) o = f32_to_f16(rn > 1e-10f ? xdiv(norm, rn) : norm);
-                    uint32_t qs = 0, qh = 0;               // low nibbles; high pairs
+                    for (int m = 0; m < 8; ++m) buf[m * 64 + lane] = x[m];
+                    wave_sync();
 #pragma unroll
                     for (int m = 0; m < 8; ++m) {
-                        qs |= (uint32_t) (code[m] & 15) << (4 * m);
-                        qh |= (uint32_t) ((code[m] >> 4) & 3) << (2 * m);
+                        const int e = e0 + m, pe = e < half ? e + half : e < n_rot ? e - half : e;
+                        y[m] = buf[(pe & 7) * 64 + sub * LPR + (pe >> 3)];
                     }
-                    *(uint16_t *) (o + 2 + i0 / 2) = (uint16_t) qs;
-                    *(uint16_t *) (o + 4 + i0 / 2) = (uint16_t) (qs >> 16);
-                    *(uint16_t *) (o + 66 + i0 / 4) = (uint16_t) qh;
+                    wave_sync();
+                }
+                if (whole) {
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) x[m] = __builtin_fmaf(x[m], cs[m], y[m] * sn[m]);
+                } else {
+#pragma unroll
+                    for (int m = 0; m < 8; ++m)
+                        if (e0 + m < n_rot) x[m] = __builtin_fmaf(x[m], cs[m], y[m] * sn[m]);
+                }
+            }
+
+            // A row holding an infinity or a NaN takes the rotation and the tq6_0 sums with the host's NaN rule. Every value of its
+            // rotation is an infinity or a NaN then, so a look at one of each lane's finds it. A row that overflows on the way keeps
+            // the plain rotation, but where that makes NaNs their signs are hadamard_row's.
+            uint64_t nf_rows = 0;
+            bool xn = false;
+            auto look = [&](const float (&v)[8]) {
+                bool nf = false;
+#pragma unroll
+                for (int m = 0; m < 8; ++m) nf |= nonfinite(v[m]);
+                nf_rows = __ballot(nf && live);
+                xn = ((LPR == 64 ? nf_rows : nf_rows >> (sub * LPR)) & ((LPR == 64 ? 0 : 1ull << (LPR % 64)) - 1ull)) != 0;
+            };
+            bool nan = true;                                   // whether the rows may hold NaNs (wave-uniform)
+            if (rot) {
+                float y[8];
+#pragma unroll
+                for (int m = 0; m < 8; ++m) y[m] = x[m];
+                hadamard_finite<8, LPR>(y, lane, rot_scale);
+                nan = ((__builtin_amdgcn_ballot_w64(nonfinite(y[0])) | __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[0], y[1])) |
+                        __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[2], y[3])) |
+                        __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[4], y[5])) |
+                        __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[6], y[7]))) &
+                       (ALL ? ~0ull : __builtin_amdgcn_ballot_w64(live))) != 0;
+                if (nan) {
+                    look(x);
+                    hadamard_rows_x<LPR>(x, buf, lane, rot_scale, xn);
+                } else {
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) x[m] = y[m];
+                }
+            } else if (OUT == HO_CACHE && MODE == HM_TQ6) {
+                look(x);
+            }
+
+            if constexpr (OUT == HO_F32) {
+                if constexpr (ALL) {
+                    float4 * t = (float4 *) buf;
+                    wave_sync();
+                    t[sub * cpr + 2 * l] = float4{x[0], x[1], x[2], x[3]};
+                    t[sub * cpr + 2 * l + 1] = float4{x[4], x[5], x[6], x[7]};
+                    wave_sync();
+                    *(float4 *) d1 = t[g1];
+                    *(float4 *) d2 = t[g2];
+                } else if (live) {
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) if (e0 + m < D) ((float *) d1)[e0 + m] = x[m];
+                }
+            } else {
+                uint32_t h[4];
+                if (OUT == HO_CACHE || o_type == SJK_F16) {
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) h[m] = pack_f16(x[2 * m], x[2 * m + 1]);
+                } else {
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) h[m] = pack_bf16(x[2 * m], x[2 * m + 1]);
+                }
+                if (OUT == HO_CACHE && nan) {                  // a NaN is stored as its sign | 0x7E00 (f32_to_f16)
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) h[m] = (uint32_t) f32_to_f16(x[2 * m]) | (uint32_t) f32_to_f16(x[2 * m + 1]) << 16;
+                }
+                if (live && (OUT == HO_HALF || f16_row)) store_halves<ALL>((uint16_t *) d1 + e0, h, e0, D);
+                if constexpr (OUT == HO_CACHE && MODE == HM_TQ6) {
+                    const bool tq = live && !f16_row;
+                    if (!__any(tq)) continue;
+                    // sj_kvarn.h:1221-1247: two sums of 128 values in index order, walked by every lane of the block (16 lanes)
+                    float * blk = buf + (lane >> 4) * BS, * sq = blk + 8 * (lane & 15);
+                    wave_sync();
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) sq[m] = xn ? xmul(x[m], x[m]) : x[m] * x[m];
+                    wave_sync();
+                    const float nsq = nf_rows ? walk<true>(blk, xn) : walk<false>(blk);
+                    const float norm = nsq != nsq ? nan_of(nsq) : __builtin_sqrtf(nsq);
+                    const bool big = norm > 1e-10f;
+                    const float inv = big ? 1.0f / norm : 0.0f;
+                    int code[8];
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) {
+                        const float v = big ? x[m] * inv : 0.0f;
+                        code[m] = level_of(v, s_cell);
+                        if (nf_rows && v != v) code[m] = 63;
+                    }
+                    wave_sync();
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) { const float c = s_cent[code[m]]; sq[m] = c * c; }
+                    wave_sync();
+                    const float rn = __builtin_sqrtf(walk<false>(blk));
+                    wave_sync();
+                    if (tq) {
+                        uint8_t * o = d1 + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES;
+                        const int i0 = 8 * (l & 15);
+                        if (!(l & 15)) *(uint16_t *) o = f32_to_f16(rn > 1e-10f ? xdiv(norm, rn) : norm);
+                        uint32_t qs = 0, qh = 0;               // low nibbles; high pairs
+#pragma unroll
+                        for (int m = 0; m < 8; ++m) {
+                            qs |= (uint32_t) (code[m] & 15) << (4 * m);
+                            qh |= (uint32_t) ((code[m] >> 4) & 3) << (2 * m);
+                        }
+                        *(uint16_t *) (o + 2 + i0 / 2) = (uint16_t) qs;
+                        *(uint16_t *) (o + 4 + i0 / 2) = (uint16_t) (qs >> 16);
+                        *(uint16_t *) (o + 66 + i0 / 4) = (uint16_t) qh;
+                    }
                 }
             }
         }
-    }
     };
     if (!rows_out) heads(Int<MODE == HM_ROWS ? HO_F32 : HO_CACHE>());
     else if (MODE != HM_ROWS || o_type == SJK_F32) heads(Int<HO_F32>());
@@ -613,7 +601,8 @@ static int launch_typed(const HeadBatch & bt, int lpr, int mode, bool wide, unsi
         turned |= (bt.part[p].flags & HF_ROPE) != 0;
         weights |= bt.part[p].w && bt.part[p].w_head;
     }
-    if (!wide || (turned && bt.layout == SJK_ROPE_HALVES && bt.n_rot % 16)) return launch_kind<T, HK_ANY>(bt, lpr, mode, grid, st);
+    if (!wide) return launch_kind<T, HK_ANY>(bt, lpr, mode, grid, st);
+    if (turned && bt.layout == SJK_ROPE_HALVES && bt.n_rot % 16) return launch_kind<T, HK_ODD>(bt, lpr, mode, grid, st);
     if (bt.D != 8 * lpr || weights || (turned && bt.n_rot != 8 * lpr)) return launch_kind<T, HK_PART>(bt, lpr, mode, grid, st);
     return launch_kind<T, HK_WHOLE>(bt, lpr, mode, grid, st);
 }
@@ -663,7 +652,7 @@ static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream
 }
 
 // rows of a launch are counted in 32 bits
-static bool rows_fit(uint64_t n_pos, uint64_t heads, uint64_t seqs) { return n_pos <= 0x7fffffffu && n_pos * heads * seqs <= 0x7fffffffu; }
+static bool rows_fit(uint64_t n_pos, uint64_t heads, uint64_t seqs) { return n_pos <= 0x7fffffffu && n_pos * heads * seqs < 0x7fffff00u; }
 
 }  // namespace sjk
 
@@ -688,7 +677,7 @@ extern "C" int sjk_hip_head_rows(const sjk_hip_head_job * jobs, int n_jobs, uint
         }
         heads += (uint64_t) J.n_heads;
     }
-    if (!rows_fit(n_pos, heads, 1)) return refuse("sjk_hip_head_rows: more than 2^31 - 1 rows");
+    if (!rows_fit(n_pos, heads, 1)) return refuse("sjk_hip_head_rows: 2^31 rows or more");
     for (int k0 = 0; k0 < n_jobs;) {
         HeadBatch bt = {};
         bt.n_pos = (int) n_pos;
@@ -745,7 +734,7 @@ static int qkv_ok(const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t pos0, 
         set_error("sjk_hip_store_qkv: more positions than sink and ring hold at once");
         return SJKVARN_ERR_CAPACITY;
     }
-    if (!rows_fit(n_pos, (uint64_t) m.n_head + 2u * (uint64_t) H, HEAD_SEQS)) return refuse("sjk_hip_store_qkv: more than 2^31 - 1 rows");
+    if (!rows_fit(n_pos, (uint64_t) m.n_head + 2u * (uint64_t) H, HEAD_SEQS)) return refuse("sjk_hip_store_qkv: 2^31 rows or more");
     int rc = norm_ok(m.n_head ? m.d_q_norm : nullptr, m.eps);
     if (!rc) rc = norm_ok(m.d_k_norm, m.eps);
     if (!rc) rc = rope_ok(m.rope, D);

@@ -287,6 +287,32 @@ def test_rows_do_not_depend_on_their_neighbours(lib, dev):
     assert np.array_equal(again, full)
 
 
+@pytest.mark.parametrize("D,t,t_out,heads", [(128, 2, 2, 40), (128, 2, 0, 40), (80, 1, 1, 13), (256, 0, 0, 6), (64, 2, 0, 9), (96, 1, 2, 33)])
+@pytest.mark.parametrize("n_rot", ["whole", "part", "odd"])
+def test_rows_of_a_large_call_are_those_of_small_ones(lib, dev, D, t, t_out, heads, n_rot):
+    """many positions of many heads, each head with weights of its own: wavefronts that go through runs of heads, and last
+    rows and runs that are not full, against the same rows one position at a time"""
+    rng = np.random.default_rng(D + heads)
+    n = 1501
+    n_rot = {"whole": D, "part": D // 32 * 16, "odd": D // 2 - 2}[n_rot]
+    rope = {"n_rot": n_rot, "layout": 0, "turns": turn_table(n_rot)}
+    dr, dw = make_rope(dev, rope), dev.put((1 + 0.3 * rng.standard_normal(heads * D)).astype(np.float32))
+    x, o = Set(dev, rng, n, heads, D, t, pos_stride=heads * D + 16), Set(dev, rng, n, heads, D, t_out)
+    run_rows(lib, dev, [head_job(x, o, rope=1, d_norm=dw, norm_head=D)], n, D, dr, pos0=9000)
+    got = untouched(o)
+    for p in (0, 1, 750, 1499, 1500):
+        a, b = Set(dev, rng, 1, heads, D, t), Set(dev, rng, 1, heads, D, t_out)
+        a.host[a.index()] = x.host[x.index()[p:p + 1]]
+        dev.upload(a.d, a.host)
+        run_rows(lib, dev, [head_job(a, b, rope=1, d_norm=dw, norm_head=D)], 1, D, dr, pos0=9000 + p)
+        assert np.array_equal(untouched(b)[0], got[p]), p
+        ref, err = reference(a.values(), np.array([9000 + p]), w=from_bits(dev.get(dw, heads * D * 4, np.uint32), 0).reshape(1, heads, D), rope=rope)
+        check_rows(got[p:p + 1], t_out, ref, err, p)
+    if t == t_out:                               # over themselves
+        run_rows(lib, dev, [head_job(x, x, rope=1, d_norm=dw, norm_head=D)], n, D, dr, pos0=9000)
+        assert np.array_equal(untouched(x), got)
+
+
 def test_inverse_turns_back(lib, dev):
     rng = np.random.default_rng(8)
     rope = {"n_rot": 96, "layout": 0, "turns": turn_table(96)}
