@@ -511,7 +511,7 @@ int sjk_hip_store_qkv_batch(const sjk_hip_qkv_job * jobs, int n_jobs, uint32_t n
 
 /* The same for layer il of several sequences (a decode batch), as sjk_hip_seq_store_batch: each sequence's position count
  * is extended. SJKVARN_ERR_ARG for a bad layer index or a gap before pos0, SJKVARN_ERR_CAPACITY where the staged positions
- * (from the sealed end on) would not fit the ring. */
+ * (from the sealed end on) would not fit the ring, SJKVARN_ERR_ARG for a sequence given twice; a refused call stores nothing. */
 typedef struct sjk_hip_seq_qkv_job {
     sj_kvarn_seq  * seq;
     uint32_t        pos0;
@@ -604,7 +604,7 @@ int sjk_hip_seq_attend_batch(const sjk_hip_seq_job * jobs, int n_jobs, int il, i
 /* The sink entries [0, min(N, S)) and the staged rows of positions [B, N) of n_layers layers copied from src's buffers to dst's
  * slots of the same positions, in one launch for up to 64 layers; nothing else in dst is written. Records are not copied: dst's
  * view brings its own body or block table. The views agree in layout, KV heads, staging, sink type and S (capacities may
- * differ), buffers 4-byte aligned, dst's not src's. SJKVARN_ERR_ARG otherwise and for B < S, B inside a group or N < B with
+ * differ), buffers 4-byte aligned, each of dst's its own and none of src's. SJKVARN_ERR_ARG otherwise and for B < S, B inside a group or N < B with
  * B > S; SJKVARN_ERR_CAPACITY where [B, N) does not fit a ring. */
 int sjk_hip_fork(const sjk_hip_view * dst, const sjk_hip_view * src, int n_layers, uint32_t B, uint32_t N, void * stream);
 

@@ -235,6 +235,10 @@ inline size_t ws_part_slots(const sjk_hip_view & v) {
     if (!v.work || v.work_bytes <= head || v.lay.D <= 0) return 0;
     return (v.work_bytes - head) / (ws_slot_floats(v.lay.D) * sizeof(float));
 }
+// the checks of one sjk_hip_store_qkv call, without a device (sjk_heads.hip)
+int qkv_ok(const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t pos0, uint32_t n_pos, const int32_t * d_pos, const void * d_q,
+           const void * d_k, const void * d_v, const float * d_q_out);
+
 // the text sjk_last_error() returns on the calling thread (sjk_host.cpp)
 void set_error(const char * what);
 

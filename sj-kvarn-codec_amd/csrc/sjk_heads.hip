@@ -84,7 +84,8 @@ SJK_DEV void turn(double u, float m, float sg, float & s, float & c) {
 // reads 4,096 positions of 32 + 8 heads of 128 to tq6_0 take 6 us more.) Not for NaNs.
 constexpr int LV_CELLS = 128;
 constexpr float LV_SCALE = 200.0f;
-struct LevelCell { float mid; int base; };                 // the cell's midpoint (or infinity), the midpoints of lower cells
+struct LevelCell { float mid; int base; };                 // the cell's midpoint, the midpoints of lower cells (a cell without one:
+                                                           // -infinity, and one fewer)
 struct LevelTable { LevelCell cell[LV_CELLS]; };
 constexpr float level_at(float v) { return v * LV_SCALE + 64.0f; }
 constexpr int level_cell(float v) { const float t = level_at(v); return t < 0.0f ? 0 : t > 127.0f ? 127 : (int) t; }
@@ -92,10 +93,11 @@ constexpr LevelTable level_table() {
     constexpr uint32_t bits[63] = SJK_TQ6_MIDPOINT_BITS_INIT;
     LevelTable t = {};
     for (int c = 0; c < LV_CELLS; ++c) {
-        t.cell[c].mid = __builtin_inff();
+        t.cell[c].mid = -__builtin_inff();
+        t.cell[c].base = -1;
         for (int i = 0; i < 63; ++i) {
             const float m = __builtin_bit_cast(float, bits[i]);
-            if (level_cell(m) < c) ++t.cell[c].base;
+            if (level_cell(m) <= c) ++t.cell[c].base;
             if (level_cell(m) == c) t.cell[c].mid = m;
         }
     }
@@ -146,8 +148,12 @@ typedef float float2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
-SJK_DEV uint32_t pack_f16(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{a, b}), f16x2_t)); }
-SJK_DEV uint32_t pack_bf16(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{a, b}), bf16x2_t)); }
+SJK_DEV uint32_t pack_f16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{a, b}), f16x2_t));
+}
+SJK_DEV uint32_t pack_bf16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2_t{a, b}), bf16x2_t));
+}
 
 template <bool WIDE> SJK_DEV void store_halves(uint16_t * o, const uint32_t (&h)[4], int e0, int D) {
     if constexpr (WIDE) {
@@ -429,9 +435,9 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
                 }
             }
 
-            // A row holding an infinity or a NaN takes the rotation and the tq6_0 sums with the host's NaN rule. Every value of its
-            // rotation is an infinity or a NaN then, so a look at one of each lane's finds it. A row that overflows on the way keeps
-            // the plain rotation, but where that makes NaNs their signs are hadamard_row's.
+            // A row holding an infinity or a NaN takes the rotation and the tq6_0 sums with the host's NaN rule. Every value of
+            // its rotation is an infinity or a NaN then, so a look at one of each lane's finds it. A row that overflows on the
+            // way keeps the plain rotation, but where that makes NaNs their signs are hadamard_row's.
             uint64_t nf_rows = 0;
             bool xn = false;
             auto look = [&](const float (&v)[8]) {
@@ -447,11 +453,10 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
 #pragma unroll
                 for (int m = 0; m < 8; ++m) y[m] = x[m];
                 hadamard_finite<8, LPR>(y, lane, rot_scale);
-                nan = ((__builtin_amdgcn_ballot_w64(nonfinite(y[0])) | __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[0], y[1])) |
-                        __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[2], y[3])) |
-                        __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[4], y[5])) |
-                        __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[6], y[7]))) &
-                       (ALL ? ~0ull : __builtin_amdgcn_ballot_w64(live))) != 0;
+                uint64_t bad = __builtin_amdgcn_ballot_w64(nonfinite(y[0]));
+#pragma unroll
+                for (int m = 0; m < 8; m += 2) bad |= __builtin_amdgcn_ballot_w64(__builtin_isunordered(y[m], y[m + 1]));
+                nan = (bad & (ALL ? ~0ull : __builtin_amdgcn_ballot_w64(live))) != 0;
                 if (nan) {
                     look(x);
                     hadamard_rows_x<LPR>(x, buf, lane, rot_scale, xn);
@@ -562,7 +567,8 @@ static int rope_ok(const sjk_hip_rope & r, int D) {
 
 static int norm_ok(const float * w, float eps) {
     if (!w) return 0;
-    if ((uintptr_t) w % 4 || !(eps >= 1.17549435e-38f) || !__builtin_isfinite(eps)) return refuse("head norms: fp32 weights and a finite, normal eps > 0");
+    if ((uintptr_t) w % 4 || !(eps >= 1.17549435e-38f) || !__builtin_isfinite(eps))
+        return refuse("head norms: fp32 weights and a finite, normal eps > 0");
     return 0;
 }
 
@@ -609,8 +615,8 @@ static int launch_typed(const HeadBatch & bt, int lpr, int mode, bool wide, unsi
 
 // The launch's shape. A wavefront goes through as many heads, up to HEAD_ITERS, as it takes for all wavefronts to be on the
 // device at once (16 a CU; the sines and cosines of a position serve its heads): a second, partly filled round of them costs a
-// 512-position append 7.1 -> 8.5 us, 1,237 positions x 64 heads of 80 10.8 -> 12.1. Its rows are adjacent positions, except in calls of fewer
-// positions than that, and where rows of fp32 go out: those of one position lie on end, and stores of 2 KB reach 5.0 TB/s where
+// 512-position append 7.1 -> 8.5 us, 1,237 positions x 64 heads of 80 10.8 -> 12.1. Its rows are adjacent positions, except in
+// calls of fewer positions than that, and where rows of fp32 go out: those of one position lie on end, and stores of 2 KB reach 5.0 TB/s where
 // four of 512 bytes reach 4.6. (Rows of 16 bits: 4.5 by head, 4.9 by position, whose sines also serve more heads.)
 static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream_t st) {
     const int lpr = bt.D <= 64 ? 8 : bt.D <= 128 ? 16 : bt.D <= 256 ? 32 : 64, rpw = 64 / lpr;
@@ -652,7 +658,9 @@ static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream
 }
 
 // rows of a launch are counted in 32 bits
-static bool rows_fit(uint64_t n_pos, uint64_t heads, uint64_t seqs) { return n_pos <= 0x7fffffffu && n_pos * heads * seqs < 0x7fffff00u; }
+static bool rows_fit(uint64_t n_pos, uint64_t heads, uint64_t seqs) {
+    return n_pos <= 0x7fffffffu && n_pos * heads * seqs < 0x7fffff00u;
+}
 
 }  // namespace sjk
 
@@ -711,9 +719,8 @@ extern "C" int sjk_hip_head_rows(const sjk_hip_head_job * jobs, int n_jobs, uint
 
 namespace sjk {
 
-// the checks of one store_qkv call that need no device
-static int qkv_ok(const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t pos0, uint32_t n_pos, const int32_t * d_pos, const void * d_q,
-                  const void * d_k, const void * d_v, const float * d_q_out) {
+int qkv_ok(const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t pos0, uint32_t n_pos, const int32_t * d_pos, const void * d_q,
+           const void * d_k, const void * d_v, const float * d_q_out) {
     const int D = v.lay.D, H = v.n_head_kv;
     if (!d_k || !d_v || !v.sink || !v.ring || v.cap == 0 || H <= 0 || m.n_head < 0 || !type_ok(m.type)) return SJKVARN_ERR_ARG;
     if (m.n_head && (!d_q || !d_q_out)) return SJKVARN_ERR_ARG;
@@ -721,12 +728,12 @@ static int qkv_ok(const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t pos0, 
         set_error("sjk_hip_store_qkv: head_dim 128 or 256");
         return SJK_ERR_UNSUPPORTED;
     }
-    if ((v.staging != SJKVARN_STAGING_TQ6_0 && v.staging != SJKVARN_STAGING_F16) || v.stage_bytes != sj_kvarn_stage_row_bytes(v.staging, D) ||
-        (v.sink_type != SJKVARN_SINK_F16 && v.sink_type != SJKVARN_SINK_INHERIT))
+    if ((v.staging != SJKVARN_STAGING_TQ6_0 && v.staging != SJKVARN_STAGING_F16) ||
+        v.stage_bytes != sj_kvarn_stage_row_bytes(v.staging, D) || (v.sink_type != SJKVARN_SINK_F16 && v.sink_type != SJKVARN_SINK_INHERIT))
         return SJKVARN_ERR_ARG;
     const size_t size = elem_size(m.type);
-    if (((uintptr_t) d_k | (uintptr_t) d_v | (m.n_head ? (uintptr_t) d_q : 0)) % size || (uintptr_t) d_q_out % 4 || (uintptr_t) d_pos % 4 ||
-        (((uintptr_t) v.sink | (uintptr_t) v.ring) & 1u))
+    if (((uintptr_t) d_k | (uintptr_t) d_v | (m.n_head ? (uintptr_t) d_q : 0)) % size || (uintptr_t) d_q_out % 4 ||
+        (uintptr_t) d_pos % 4 || (((uintptr_t) v.sink | (uintptr_t) v.ring) & 1u))
         return SJKVARN_ERR_ARG;
     if ((uint64_t) pos0 + n_pos > 0xffffffffull) return refuse("sjk_hip_store_qkv: positions past 2^32 - 1");
     const uint64_t room = (uint64_t) v.cap + (pos0 < v.S ? v.S - pos0 : 0);

@@ -1157,6 +1157,11 @@ int sjk_hip_seq_store_qkv_batch(const sjk_hip_seq_qkv_job * jobs, int n_jobs, in
                 sjk::set_error("sjk_hip_seq_store_qkv_batch: a sequence twice");
                 return SJKVARN_ERR_ARG;
             }
+        const sjk_hip_seq_qkv_job & J = jobs[k];             // before the first launch: a refused call stores nothing
+        const int rc = J.seq->layers[il].lay.D != jobs[0].seq->layers[il].lay.D
+                           ? SJKVARN_ERR_ARG
+                           : sjk::qkv_ok(sjk_layer_view(&s->layers[il]), *m, J.pos0, n_pos, J.d_pos, J.d_q, J.d_k, J.d_v, J.d_q_out);
+        if (rc) return rc;
     }
     constexpr int CHUNK = 32;
     sjk_hip_qkv_job qj[CHUNK];

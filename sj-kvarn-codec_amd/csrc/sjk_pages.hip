@@ -94,8 +94,8 @@ extern "C" int sjk_hip_fork(const sjk_hip_view * dst, const sjk_hip_view * src, 
     if (!n_layers) return 0;
     const sjk_hip_view & s0 = src[0], & d0 = dst[0];
     if (s0.n_head_kv <= 0 || s0.lay.D <= 0 || s0.lay.G <= 0 || s0.cap == 0 || d0.cap == 0) return SJKVARN_ERR_ARG;
-    if ((s0.staging != SJKVARN_STAGING_TQ6_0 && s0.staging != SJKVARN_STAGING_F16) || s0.stage_bytes != sj_kvarn_stage_row_bytes(s0.staging, s0.lay.D) ||
-        (s0.sink_type != SJKVARN_SINK_F16 && s0.sink_type != SJKVARN_SINK_INHERIT) || s0.stage_bytes == 0)
+    if ((s0.staging != SJKVARN_STAGING_TQ6_0 && s0.staging != SJKVARN_STAGING_F16) ||
+        s0.stage_bytes != sj_kvarn_stage_row_bytes(s0.staging, s0.lay.D) || (s0.sink_type != SJKVARN_SINK_F16 && s0.sink_type != SJKVARN_SINK_INHERIT) || s0.stage_bytes == 0)
         return SJKVARN_ERR_ARG;
     if (B < s0.S || (B - s0.S) % (uint32_t) s0.lay.G || (N < B && B > s0.S)) return refuse("sjk_hip_fork: B below S, inside a group or past N");
     for (int il = 0; il < n_layers; ++il)
@@ -105,8 +105,12 @@ extern "C" int sjk_hip_fork(const sjk_hip_view * dst, const sjk_hip_view * src, 
             if (v->lay.D != s0.lay.D || v->lay.G != s0.lay.G || v->n_head_kv != s0.n_head_kv || v->staging != s0.staging ||
                 v->sink_type != s0.sink_type || v->stage_bytes != s0.stage_bytes || v->S != s0.S || v->cap != w.cap)
                 return refuse("sjk_hip_fork: the views differ in layout, heads, staging, sink or (on one side) capacity");
-            if (dst[il].sink == src[il].sink || dst[il].ring == src[il].ring) return refuse("sjk_hip_fork: a layer onto itself");
         }
+    for (int i = 0; i < n_layers; ++i)                     // a layer's buffers written twice, or written and read
+        for (int k = 0; k < n_layers; ++k)
+            if (dst[i].sink == src[k].sink || dst[i].ring == src[k].ring ||
+                (k < i && (dst[i].sink == dst[k].sink || dst[i].ring == dst[k].ring)))
+                return refuse("sjk_hip_fork: a buffer of dst is another layer's, or src's");
     const uint32_t n = N > B ? N - B : 0;
     if (n > s0.cap || n > d0.cap) {
         set_error("sjk_hip_fork: the staged positions do not fit the ring");

@@ -227,6 +227,38 @@ def test_fork_equals_a_truncated_build(lib, dev, bk, bv, body, parent_pool, chil
         lib.sj_kvarn_pool_free(C.byref(p))
 
 
+def test_fork_into_a_ring_of_another_size(lib, dev):
+    """n_ubatch, and with it the ring, may differ: slots are those of the child's ring; a child too small is refused"""
+    cfg = config(lib)
+    rows, more = Rows(dev, 3000, seed=23), Rows(dev, 3000, seed=24)
+    pool = new_pool(lib, cfg)
+    parent = new_seq(lib, cfg, pool)
+    grow(lib, dev, parent, rows, 1500, 5, None, True)
+    for n_ubatch in (1, 64, 700):
+        other = sjk.Config.from_buffer_copy(bytes(cfg))
+        other.n_ubatch = n_ubatch
+        child, ref = new_seq(lib, other, pool), new_seq(lib, other)
+        assert child.layers[0].cap != parent.layers[0].cap
+        fork(lib, child, parent, parent.n - 3)
+        for p0 in range(0, 1500, 256):               # the reference's ubatches, in pieces that the smaller ring takes
+            sjk.check(lib.sjk_hip_seq_begin_ubatch(C.byref(ref), p0, min(256, 1500 - p0), None), "begin")
+            for il in range(NL):
+                sjk.check(lib.sjk_hip_seq_store(C.byref(ref), il, p0, min(256, 1500 - p0), rows.k(p0), rows.v(p0), 1, None), "store")
+        for _ in range(5):
+            step(lib, ref, rows, ref.n, W, None, True)
+        assert lib.sj_kvarn_seq_truncate(C.byref(ref), parent.n - 3) == parent.n - 3
+        same(lib, dev, child, ref, rows)
+        for s in (child, ref):
+            for _ in range(200):
+                step(lib, s, more, s.n, W, None, True)
+        same(lib, dev, child, ref, more)
+        lib.sj_kvarn_seq_free(C.byref(child))
+        lib.sj_kvarn_seq_free(C.byref(ref))
+    lib.sj_kvarn_seq_free(C.byref(parent))
+    assert pool.n_free == pool.n_blocks
+    lib.sj_kvarn_pool_free(C.byref(pool))
+
+
 def test_blocks_outlive_the_sequences_that_shared_them(lib, dev):
     """parent, child and grandchild: truncations, resets and frees of the others leave a sequence's records alone, a dropped
     block is cleared and freed with its last holder, and restores count only the blocks that a reset gives back"""

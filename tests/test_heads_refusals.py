@@ -206,6 +206,11 @@ def test_fork_refusals(lib):
     ds = (sjk.View * 2)(view(lib, **far), view(lib, cap=384, **far))
     ss = (sjk.View * 2)(s, s)
     assert lib.sjk_hip_fork(ds, ss, 2, 128, 200, None) == ARG          # capacities differ from layer to layer
+    ss[1] = view(lib, sink=FAKE * 64, ring=FAKE * 80)
+    for bad in (dict(sink=FAKE * 16, ring=FAKE * 48), dict(sink=FAKE * 48, ring=FAKE * 32), dict(sink=FAKE, ring=FAKE * 48),
+                dict(sink=FAKE * 48, ring=FAKE * 2)):                  # one buffer twice, or another layer's source
+        ds[1] = view(lib, **bad)
+        assert lib.sjk_hip_fork(ds, ss, 2, 128, 200, None) == ARG, bad
 
 
 def test_copy_blocks_refusals(lib):
