@@ -218,7 +218,8 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     __shared__ float s_cent[MODE == HM_TQ6 ? 64 : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPR, D = KIND == HK_WHOLE ? 8 * LPR : bt.D;
     const bool again = ALL && KIND != HK_WHOLE && lane % LPR >= D / 8;    // a lane behind the row's channels
-    const int l = lane % LPR - (again ? D / 8 : 0), e0 = 8 * l;
+    // (rows of 32 channels and more take at least half of their lanes, narrower ones a quarter or an eighth)
+    const int l = lane % LPR - (again ? LPR == 8 && D < 32 ? lane % LPR / (D / 8) * (D / 8) : D / 8 : 0), e0 = 8 * l;
     if (MODE == HM_TQ6) {
         if (threadIdx.x < LV_CELLS) s_cell[threadIdx.x] = c_levels.cell[threadIdx.x];
         if (threadIdx.x < 64) s_cent[threadIdx.x] = tq6_cent(threadIdx.x);

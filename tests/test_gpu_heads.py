@@ -192,6 +192,25 @@ def test_turn_against_64_bits(lib, dev, D, n_rot, layout, t, t_out):
             assert np.array_equal(o.read()[o.index()][..., n_rot:], to_bits(x.values()[..., n_rot:], t_out))
 
 
+@pytest.mark.parametrize("D", [8, 16, 24, 32, 40, 48, 56])
+@pytest.mark.parametrize("t,t_out", [(0, 0), (1, 1), (2, 2), (2, 0)], ids=["f32", "f16", "bf16", "bf16-f32"])
+@pytest.mark.parametrize("n_rot", ["whole", "part", "odd", "none"])
+def test_narrow_heads_against_64_bits(lib, dev, D, t, t_out, n_rot):
+    """heads narrower than the lanes they are given, down to an eighth of them, with norm and turn, beside each other and apart:
+    nothing but their own channels is read into them or written"""
+    rng = np.random.default_rng(100 * D + 10 * t + t_out)
+    n, c = 11, {"whole": D, "part": D // 16 * 16, "odd": D // 2 * 2 - (2 if D > 8 else 4), "none": 0}[n_rot]
+    rope = {"n_rot": c, "layout": sjk.ROPE_HALVES, "turns": turn_table(c)}
+    w = (1 + rng.standard_normal(D) / 4).astype(np.float32)
+    pos = 500 + np.arange(n)
+    for apart in (0, 16):
+        x = Set(dev, rng, n, 3, D, t, head_stride=D + apart)
+        o = Set(dev, rng, n, 3, D, t_out, head_stride=D + apart)
+        run_rows(lib, dev, [head_job(x, o, rope=1, d_norm=dev.put(w).value)], n, D, make_rope(dev, rope), pos0=500)
+        ref, err = reference(x.values(), pos, w=w, rope=rope)
+        check_rows(untouched(o), t_out, ref, err, "narrow heads")
+
+
 @pytest.mark.parametrize("D,rotate", [(128, 1), (256, 1), (64, 1), (512, 1), (128, 0), (80, 0), (1, 0), (7, 0), (200, 0)])
 @pytest.mark.parametrize("t", [0, 1, 2], ids=["f32", "f16", "bf16"])
 def test_norm_turn_rotation_against_64_bits(lib, dev, D, rotate, t):
