@@ -435,7 +435,7 @@ int sjk_rope_turns(const sjk_rope_config * c, double * turns, float * mscale);
 
 /* A turn of rotary positions. Channels behind n_rot pass through. With a pair (a, b) at position p, u = p turns[i]:
  * (a, b) -> mscale (a cos 2 pi u - b sin 2 pi u, a sin 2 pi u + b cos 2 pi u); the angle is reduced in 64 bits, so far
- * positions lose nothing. inverse: the sine's sign turned (the way back, and the gradient of the turn, for mscale = 1). */
+ * positions lose nothing. inverse: the sine's sign turned, which is the turn's gradient (for mscale = 1 also the way back). */
 enum { SJK_ROPE_HALVES = 0 /* pairs (i, i + n_rot / 2) */, SJK_ROPE_PAIRS = 1 /* pairs (2 i, 2 i + 1) */ };
 typedef struct sjk_hip_rope {
     int            layout;      /* SJK_ROPE_HALVES or SJK_ROPE_PAIRS */

@@ -211,6 +211,28 @@ def test_narrow_heads_against_64_bits(lib, dev, D, t, t_out, n_rot):
         check_rows(untouched(o), t_out, ref, err, "narrow heads")
 
 
+@pytest.mark.parametrize("D,n_rot,layout", [(128, 128, 0), (128, 96, 1), (80, 40, 0), (33, 20, 1)])
+def test_inverse_turn_is_the_gradient(lib, dev, D, n_rot, layout):
+    """sum(g (f(x + d) - f(x))) = sum(inverse(g) d): the turn is linear, so differences of any length show its gradient. Each
+    side's error: the kernel's bound and the last rounding of each row, against the other factor"""
+    rng = np.random.default_rng(D + n_rot)
+    n, heads = 4, 3
+    rope = {"n_rot": n_rot, "layout": layout, "turns": turn_table(n_rot), "mscale": 1.25}
+    back = dict(rope, inverse=True)
+    pos = 3000 + np.arange(n)
+    x, x2, g = (Set(dev, rng, n, heads, D, sjk.F32) for _ in range(3))
+    outs = []
+    for r, s in ((rope, x), (rope, x2), (back, g)):
+        o = Set(dev, rng, n, heads, D, sjk.F32)
+        run_rows(lib, dev, [head_job(s, o, rope=1)], n, D, make_rope(dev, r), pos0=3000)
+        ref, err = reference(s.values(), pos, rope=r)
+        outs.append((untouched(o).view(np.float32).astype(L), err + U * (np.abs(ref) + err)))
+    (f, ef), (f2, ef2), (dx, edx) = outs
+    d, gv = x2.values().astype(L) - x.values().astype(L), g.values().astype(L)
+    bound = (np.abs(gv) * (ef + ef2)).sum() + (np.abs(d) * edx).sum()
+    assert abs((gv * (f2 - f)).sum() - (dx * d).sum()) <= bound
+
+
 @pytest.mark.parametrize("D,rotate", [(128, 1), (256, 1), (64, 1), (512, 1), (128, 0), (80, 0), (1, 0), (7, 0), (200, 0)])
 @pytest.mark.parametrize("t", [0, 1, 2], ids=["f32", "f16", "bf16"])
 def test_norm_turn_rotation_against_64_bits(lib, dev, D, rotate, t):
