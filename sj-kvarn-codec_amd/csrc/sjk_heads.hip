@@ -21,6 +21,7 @@ constexpr int HW = 4;                  // wavefronts a workgroup
 constexpr int HEAD_PARTS = 3;          // sets of heads a launch: q, k, v
 constexpr int HEAD_SEQS = 32;          // sequences a launch
 constexpr int HEAD_ITERS = 8;          // heads a wavefront goes through at most
+constexpr int TQ_BATCH = 4;            // of them staged as tq6_0 together
 enum { HP_ROWS = 0, HP_K = 1, HP_V = 2 };                               // where a part's rows go
 enum { HF_ROPE = 1, HF_ROT = 2, HF_BY_HEAD = 4 };
 enum { HM_ROWS = 0, HM_F16 = 1, HM_TQ6 = 2 };                           // a launch: plain rows only, or a cache's staging
@@ -202,8 +203,9 @@ enum { HK_WHOLE = 0,        // rows of 8 * LPR channels whose addresses and stri
        HK_ODD = 2,          // such accesses, a turn of halves over another number: pairs through LDS
        HK_ANY = 3 };        // rows of any width, address and stride, any turn, element by element (3,226 positions x 6 heads of 256
                             // turned over 232 channels: 25.7 us, 14.0 by HK_ODD)
+// (HK_WHOLE: 16 wavefronts a CU, as launch_heads counts on; tq6_0 takes the 128 registers that leaves, 130 without the bound)
 template <typename T, int LPR, int MODE, int KIND>
-__global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
+__global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kernel(const HeadBatch bt) {
     // Lanes behind the last row take the last row again, and lanes behind a row's channels its first ones, and write the same
     // values once more (both read in one instruction, so also where rows are written over themselves): loads and stores without
     // a branch around them, so that a wait for the next row's loads does not wait for this row's stores (on gfx9 one counter
@@ -212,7 +214,8 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     constexpr bool ALL = KIND != HK_ANY;
     constexpr int RPW = 64 / LPR;                          // rows a wavefront holds
     constexpr int BS = 132;                                // floats from a 128-value block to the next (walks: other banks)
-    constexpr int WS = MODE == HM_TQ6 ? 4 * BS : 512;      // floats of a wavefront's LDS
+    constexpr int TB = MODE == HM_TQ6 ? TQ_BATCH : 1;      // heads staged together
+    constexpr int WS = MODE == HM_TQ6 ? TB * 4 * BS : 512; // floats of a wavefront's LDS
     __shared__ alignas(16) float s_buf[HW * WS];
     __shared__ LevelCell s_cell[MODE == HM_TQ6 ? LV_CELLS : 1];
     __shared__ float s_cent[MODE == HM_TQ6 ? 64 : 1];
@@ -231,7 +234,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     if (si >= bt.n_seqs) return;
     u -= si * bt.units;
     int pi = bt.n_parts - 1;                               // keys and values first: staging them takes longest (last, 4,096
-                                                           // positions to tq6_0 take 49 us for 39)
+                                                           // positions to tq6_0 took 49 us for 39)
     while (pi > 0 && u >= bt.part[pi].n_units) u -= bt.part[pi--].n_units;
     const HeadPart & P = bt.part[pi];
     const HeadSeq & Q = bt.seq[si];
@@ -369,7 +372,11 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
     // what the rows become: fp32, halves, or the cache's entries (stores of one kind only, for the same reason as ALL)
     auto heads = [&](auto out) {
         constexpr int OUT = decltype(out)::value;
+        constexpr bool TQ = OUT == HO_CACHE && MODE == HM_TQ6;
+        uint64_t nf_batch = 0;                                 // tq6_0: the heads collected for a walk
+        int xn_batch = 0;
         for (int it = 0; it < iters; ++it) {
+            float * const tmp = TQ ? buf + it % TB * (4 * BS) : buf;
             const bool live = ALL || (here && head_at(it, sub) < n_heads);
             float x[8];
 #pragma unroll
@@ -417,12 +424,12 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
                     // channel e in slot (e % 8) * 64 + sub * LPR + e / 8: both sides touch neighbouring words
                     wave_sync();
 #pragma unroll
-                    for (int m = 0; m < 8; ++m) buf[m * 64 + lane] = x[m];
+                    for (int m = 0; m < 8; ++m) tmp[m * 64 + lane] = x[m];
                     wave_sync();
 #pragma unroll
                     for (int m = 0; m < 8; ++m) {
                         const int e = e0 + m, pe = e < half ? e + half : e < n_rot ? e - half : e;
-                        y[m] = buf[(pe & 7) * 64 + sub * LPR + (pe >> 3)];
+                        y[m] = tmp[(pe & 7) * 64 + sub * LPR + (pe >> 3)];
                     }
                     wave_sync();
                 }
@@ -460,7 +467,7 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
                 nan = (bad & (ALL ? ~0ull : __builtin_amdgcn_ballot_w64(live))) != 0;
                 if (nan) {
                     look(x);
-                    hadamard_rows_x<LPR>(x, buf, lane, rot_scale, xn);
+                    hadamard_rows_x<LPR>(x, tmp, lane, rot_scale, xn);
                 } else {
 #pragma unroll
                     for (int m = 0; m < 8; ++m) x[m] = y[m];
@@ -496,46 +503,66 @@ __global__ __launch_bounds__(64 * HW) void heads_kernel(const HeadBatch bt) {
                     for (int m = 0; m < 4; ++m) h[m] = (uint32_t) f32_to_f16(x[2 * m]) | (uint32_t) f32_to_f16(x[2 * m + 1]) << 16;
                 }
                 if (live && (OUT == HO_HALF || f16_row)) store_halves<ALL>((uint16_t *) d1 + e0, h, e0, D);
-                if constexpr (OUT == HO_CACHE && MODE == HM_TQ6) {
-                    const bool tq = live && !f16_row;
-                    if (!__any(tq)) continue;
-                    // sj_kvarn.h:1221-1247: two sums of 128 values in index order, walked by every lane of the block (16 lanes)
-                    float * blk = buf + (lane >> 4) * BS, * sq = blk + 8 * (lane & 15);
+                if constexpr (TQ) {
+                    // sj_kvarn.h:1221-1247: two sums of 128 values in index order. The blocks of up to TQ_BATCH heads are
+                    // collected in LDS and walked at once, 4 of a block's 16 lanes a head (4,096 positions of 32 + 8 heads of
+                    // 128 take 36.9 us, 39.4 with a walk a head, whose 16 lanes did the same; 16 + 4 heads of 256 39.8 for 45.8).
+                    if (!__any(!f16_row)) continue;
+                    const int j = it % TB;
+                    float * const blk = buf + (lane >> 4) * BS, * const own = blk + 8 * (lane & 15);
                     wave_sync();
-#pragma unroll
-                    for (int m = 0; m < 8; ++m) sq[m] = xn ? xmul(x[m], x[m]) : x[m] * x[m];
+                    *(float4 *) (own + j * (4 * BS)) = float4{x[0], x[1], x[2], x[3]};
+                    *(float4 *) (own + j * (4 * BS) + 4) = float4{x[4], x[5], x[6], x[7]};
+                    nf_batch |= nf_rows;
+                    xn_batch |= (int) xn << j;
+                    if (j < TB - 1 && it < iters - 1) continue;
                     wave_sync();
-                    const float nsq = nf_rows ? walk<true>(blk, xn) : walk<false>(blk);
+                    const int jw = min((lane & 15) / (16 / TB), j);            // the head this lane walks
+                    const float * const row = blk + jw * (4 * BS);
+                    const bool xnw = xn_batch >> jw & 1;
+                    const float nsq = nf_batch ? walk<true, true>(row, xnw) : walk<false, true>(row);
                     const float norm = nsq != nsq ? nan_of(nsq) : __builtin_sqrtf(nsq);
-                    const bool big = norm > 1e-10f;
-                    const float inv = big ? 1.0f / norm : 0.0f;
-                    int code[8];
-#pragma unroll
-                    for (int m = 0; m < 8; ++m) {
-                        const float v = big ? x[m] * inv : 0.0f;
-                        code[m] = level_of(v, s_cell);
-                        if (nf_rows && v != v) code[m] = 63;
-                    }
+                    const float inv = norm > 1e-10f ? 1.0f / norm : 0.0f;
                     wave_sync();
-#pragma unroll
-                    for (int m = 0; m < 8; ++m) { const float c = s_cent[code[m]]; sq[m] = c * c; }
-                    wave_sync();
-                    const float rn = __builtin_sqrtf(walk<false>(blk));
-                    wave_sync();
-                    if (tq) {
-                        uint8_t * o = d1 + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES;
-                        const int i0 = 8 * (l & 15);
-                        if (!(l & 15)) *(uint16_t *) o = f32_to_f16(rn > 1e-10f ? xdiv(norm, rn) : norm);
+#pragma unroll 1
+                    for (int i = 0; i <= j; ++i) {
+                        float * const o4 = own + i * (4 * BS);
+                        const float4 a = *(const float4 *) o4, b = *(const float4 *) (o4 + 4);
+                        const float z[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                        const int from = (lane & 48) + i * (16 / TB);
+                        const float inv_i = __shfl(inv, from, 64);
+                        const bool big = __shfl(norm, from, 64) > 1e-10f;
                         uint32_t qs = 0, qh = 0;               // low nibbles; high pairs
+                        float c2[8];
 #pragma unroll
                         for (int m = 0; m < 8; ++m) {
-                            qs |= (uint32_t) (code[m] & 15) << (4 * m);
-                            qh |= (uint32_t) ((code[m] >> 4) & 3) << (2 * m);
+                            const float v = big ? z[m] * inv_i : 0.0f;
+                            int code = level_of(v, s_cell);
+                            if (nf_batch && v != v) code = 63;
+                            const float c = s_cent[code];
+                            c2[m] = c * c;
+                            qs |= (uint32_t) (code & 15) << (4 * m);
+                            qh |= (uint32_t) ((code >> 4) & 3) << (2 * m);
                         }
-                        *(uint16_t *) (o + 2 + i0 / 2) = (uint16_t) qs;
-                        *(uint16_t *) (o + 4 + i0 / 2) = (uint16_t) (qs >> 16);
-                        *(uint16_t *) (o + 66 + i0 / 4) = (uint16_t) qh;
+                        *(float4 *) o4 = float4{c2[0], c2[1], c2[2], c2[3]};
+                        *(float4 *) (o4 + 4) = float4{c2[4], c2[5], c2[6], c2[7]};
+                        const int h = head_at(it - j + i, sub);
+                        if (!f16_row && (ALL || (here && h < n_heads))) {
+                            uint8_t * o = d_base + h * d_head + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES;
+                            const int i0 = 8 * (l & 15);
+                            *(uint16_t *) (o + 2 + i0 / 2) = (uint16_t) qs;
+                            *(uint16_t *) (o + 4 + i0 / 2) = (uint16_t) (qs >> 16);
+                            *(uint16_t *) (o + 66 + i0 / 4) = (uint16_t) qh;
+                        }
                     }
+                    wave_sync();
+                    const float rn = __builtin_sqrtf(walk<false>(row));
+                    const int h = head_at(it - j + jw, sub);
+                    if (!f16_row && (lane & 15) % (16 / TB) == 0 && (ALL || (here && h < n_heads)))
+                        *(uint16_t *) (d_base + h * d_head + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES) =
+                            f32_to_f16(rn > 1e-10f ? xdiv(norm, rn) : norm);
+                    nf_batch = 0;
+                    xn_batch = 0;
                 }
             }
         }
@@ -630,8 +657,8 @@ static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream
         step[p] = by_head ? rpw : 1;                                       // heads an iteration takes on
         blocks[p] = by_head ? bt.n_pos : (bt.n_pos + rpw - 1) / rpw;
     }
-    // staging tq6_0 rows takes twice a query's time: half as many of them a wavefront, where all are on the device at once (512
-    // positions of 32 + 8 heads 10.6 -> 9.2 us, 2,048 26.8 -> 20.1; 4,096, in several rounds, 38.6 -> 42.3)
+    // staging tq6_0 rows takes longer than a query: half as many of them a wavefront, where all are on the device at once
+    // (512 positions of 32 + 8 heads 9.7 -> 9.3 us, 2,048 21.0 -> 18.8; 4,096, in several rounds, 37.4 -> 37.9)
     int64_t waves = 0;
     auto shape = [&](int most, int most_tq) {
         bt.units = 0;

@@ -120,21 +120,25 @@ template <int V, int LPR> SJK_DEV void hadamard_finite(float (&x)[V], int lane, 
     for (int m = 0; m < V; ++m) x[m] = x[m] * scale;
 }
 
-// the sum of 128 values in index order; XN: the host's NaN rule where xn is set
-template <bool XN> SJK_DEV float walk(const float * sq, bool xn = true) {
+// the sum of 128 values (SQUARED: of their squares) in index order; XN: the host's NaN rule where xn is set
+template <bool XN, bool SQUARED = false> SJK_DEV float walk(const float * sq, bool xn = true) {
     const float4 * p = (const float4 *) sq;
     float s = 0.0f;
     if (XN) {
-        auto add = [&](float a, float b) { return xn ? xadd(a, b) : a + b; };
+        auto add = [&](float a, float v) {
+            const float b = SQUARED ? xn ? xmul(v, v) : v * v : v;
+            return xn ? xadd(a, b) : a + b;
+        };
         for (int i = 0; i < 32; ++i) {
             const float4 q = p[i];
             s = add(s, q.x); s = add(s, q.y); s = add(s, q.z); s = add(s, q.w);
         }
     } else {
+        auto sq1 = [](float v) { return SQUARED ? v * v : v; };
 #pragma unroll 8
         for (int i = 0; i < 32; ++i) {
             const float4 q = p[i];
-            s = s + q.x; s = s + q.y; s = s + q.z; s = s + q.w;
+            s = s + sq1(q.x); s = s + sq1(q.y); s = s + sq1(q.z); s = s + sq1(q.w);
         }
     }
     return s;

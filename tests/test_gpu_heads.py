@@ -483,6 +483,39 @@ def test_append_of_rows_that_are_not_finite(lib, dev, D, staging):
         lib.sj_kvarn_layer_free(C.byref(B))
 
 
+# whole turns, parts, parts by LDS, odd addresses; runs of 7, 5 and 6 heads of keys and values a wavefront
+@pytest.mark.parametrize("D,H,n_head,n,t,n_rot,pad", [(128, 7, 2, 4211, sjk.BF16, 128, 0), (128, 5, 0, 4211, sjk.F32, 128, 0),
+                                                      (256, 5, 1, 2111, sjk.F32, 40, 0), (128, 6, 1, 4211, sjk.F16, 64, 0),
+                                                      (128, 7, 1, 4211, sjk.F32, 128, 3)])
+def test_large_append_with_rows_that_are_not_finite(lib, dev, D, H, n_head, n, t, n_rot, pad):
+    """calls so large that a wavefront stages more heads than it walks at once, and a number of them that is no multiple; rows
+    with infinities and NaNs of both signs in some of them"""
+    rng = np.random.default_rng(D + H + n)
+    A, B = (new_layer(lib, D, H, 0, 0, n_ubatch=4352) for _ in range(2))
+    va, vb = lib.sjk_layer_view(C.byref(A)), lib.sjk_layer_view(C.byref(B))
+    try:
+        p = Proj(dev, rng, n, n_head, H, D, t, True, n_rot, 0, pad=pad)
+        for specials in (False, True):
+            if specials:
+                flat = from_bits(p.x.host, t).copy()
+                at = rng.choice(p.x.index().ravel(), 200, replace=False)
+                flat[at] = rng.choice(np.array([np.inf, -np.inf, np.nan, -np.nan, 0.0], np.float32), 200)
+                p.x.host = to_bits(flat, t)
+                dev.upload(p.x.d, p.x.host)
+            want_q = p.two_steps(lib, vb, 100)
+            q, k, v = p.ptrs()
+            sjk.check(lib.sjk_hip_store_qkv(C.byref(va), 100, n, C.byref(p.m), None, q, k, v, p.q if n_head else None, None), "store_qkv")
+            dev.sync()
+            if n_head:
+                a, b = from_bits(p.q_out(), 0), from_bits(want_q, 0)
+                assert np.array_equal(p.q_out(), want_q) or (specials and np.array_equal(np.isnan(a), np.isnan(b)))
+            for got, want in zip(cache_bytes(dev, va), cache_bytes(dev, vb)):
+                assert np.array_equal(got, want), specials
+    finally:
+        lib.sj_kvarn_layer_free(C.byref(A))
+        lib.sj_kvarn_layer_free(C.byref(B))
+
+
 def test_append_at_positions_of_its_own_and_over_its_queries(lib, dev):
     """d_pos turns by other positions than the slots'; fp32 queries may be written over themselves"""
     rng = np.random.default_rng(21)
