@@ -604,8 +604,8 @@ int sjk_hip_seq_attend_batch(const sjk_hip_seq_job * jobs, int n_jobs, int il, i
 /* The sink entries [0, min(N, S)) and the staged rows of positions [B, N) of n_layers layers copied from src's buffers to dst's
  * slots of the same positions, in one launch for up to 64 layers; nothing else in dst is written. Records are not copied: dst's
  * view brings its own body or block table. The views agree in layout, KV heads, staging, sink type and S (capacities may
- * differ), buffers 4-byte aligned, each of dst's its own and none of src's. SJKVARN_ERR_ARG otherwise and for B < S, B inside a group or N < B with
- * B > S; SJKVARN_ERR_CAPACITY where [B, N) does not fit a ring. */
+ * differ), buffers 4-byte aligned, each of dst's its own and none of src's. SJKVARN_ERR_ARG otherwise and for B < S, B inside
+ * a group or N < B with B > S; SJKVARN_ERR_CAPACITY where [B, N) does not fit a ring. */
 int sjk_hip_fork(const sjk_hip_view * dst, const sjk_hip_view * src, int n_layers, uint32_t B, uint32_t N, void * stream);
 
 /* Blocks src_ids[i] of one pool's slab to blocks dst_ids[i] of another's (or the same) in every layer: block id of layer il lies
@@ -622,8 +622,8 @@ int sjk_hip_copy_blocks(uint8_t * d_dst, size_t dst_layer_bytes, uint32_t dst_bl
  * other streams. Where pos lies inside the sealed part the child starts at the group boundary below it, as
  * sj_kvarn_seq_truncate does; *kept (may be NULL) is the child's position count. The child is a new or reset sequence with the
  * parent's configuration (the status codes of sj_kvarn_seq_state_read otherwise; n_ctx and n_ubatch may differ:
- * SJKVARN_ERR_CAPACITY where the positions do not fit). SJKVARN_ERR_ARG for a child that is not empty or is the parent, or pos past the
- * parent's positions; SJKVARN_ERR_PENDING while a seal or a state restore of the parent, or any transfer of the child, is
+ * SJKVARN_ERR_CAPACITY where the positions do not fit). SJKVARN_ERR_ARG for a child that is not empty or is the parent, or
+ * pos past the parent's positions; SJKVARN_ERR_PENDING while a seal or a state restore of the parent, or any transfer of the child, is
  * pending; SJKVARN_ERR_POOL_FULL. A refused call changes nothing. */
 int sjk_hip_seq_fork(sj_kvarn_seq * child, sj_kvarn_seq * parent, uint32_t pos, uint32_t * kept, void * stream);
 

@@ -644,8 +644,8 @@ static int launch_typed(const HeadBatch & bt, int lpr, int mode, bool wide, unsi
 // The launch's shape. A wavefront goes through as many heads, up to HEAD_ITERS, as it takes for all wavefronts to be on the
 // device at once (16 a CU; the sines and cosines of a position serve its heads): a second, partly filled round of them costs a
 // 512-position append 7.1 -> 8.5 us, 1,237 positions x 64 heads of 80 10.8 -> 12.1. Its rows are adjacent positions, except in
-// calls of fewer positions than that, and where rows of fp32 go out: those of one position lie on end, and stores of 2 KB reach 5.0 TB/s where
-// four of 512 bytes reach 4.6. (Rows of 16 bits: 4.5 by head, 4.9 by position, whose sines also serve more heads.)
+// calls of fewer positions than that, and where rows of fp32 go out: those of one position lie on end, and stores of 2 KB
+// reach 5.0 TB/s where four of 512 bytes reach 4.6. (Rows of 16 bits: 4.5 by head, 4.9 by position, whose sines also serve more heads.)
 static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream_t st) {
     const int lpr = bt.D <= 64 ? 8 : bt.D <= 128 ? 16 : bt.D <= 256 ? 32 : 64, rpw = 64 / lpr;
     int64_t blocks[HEAD_PARTS];

@@ -723,9 +723,9 @@ void sj_kvarn_layer_attend_row(const sj_kvarn_layer * L, uint32_t B, uint32_t N,
 }
 
 // The byte ranges a truncation clears in one layer (sj_kvarn.h:1581-1603): the records of groups [B_new, B_old)
-// (in pool mode only the blocks the sequence holds, and with `pool` only those it holds alone), the sink entries of positions [resume, min(n_old, S)) and
-// the ring rows of positions [max(resume, S), n_old) that can still be resident (the last cap of them), as
-// contiguous runs.
+// (in pool mode only the blocks the sequence holds, and with `pool` only those it holds alone), the sink entries of
+// positions [resume, min(n_old, S)) and the ring rows of positions [max(resume, S), n_old) that can still be resident (the
+// last cap of them), as contiguous runs.
 static bool pool_shared(const sj_kvarn_pool * pool, uint32_t id);
 static void truncate_runs(const sj_kvarn_layer * L, uint32_t B_old, uint32_t B_new, uint32_t n_old, uint32_t resume,
                           std::vector<sjk::CopyRun> & runs, const sj_kvarn_pool * pool = nullptr) {

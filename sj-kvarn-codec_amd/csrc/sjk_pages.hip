@@ -95,9 +95,11 @@ extern "C" int sjk_hip_fork(const sjk_hip_view * dst, const sjk_hip_view * src, 
     const sjk_hip_view & s0 = src[0], & d0 = dst[0];
     if (s0.n_head_kv <= 0 || s0.lay.D <= 0 || s0.lay.G <= 0 || s0.cap == 0 || d0.cap == 0) return SJKVARN_ERR_ARG;
     if ((s0.staging != SJKVARN_STAGING_TQ6_0 && s0.staging != SJKVARN_STAGING_F16) ||
-        s0.stage_bytes != sj_kvarn_stage_row_bytes(s0.staging, s0.lay.D) || (s0.sink_type != SJKVARN_SINK_F16 && s0.sink_type != SJKVARN_SINK_INHERIT) || s0.stage_bytes == 0)
+        s0.stage_bytes != sj_kvarn_stage_row_bytes(s0.staging, s0.lay.D) || s0.stage_bytes == 0 ||
+        (s0.sink_type != SJKVARN_SINK_F16 && s0.sink_type != SJKVARN_SINK_INHERIT))
         return SJKVARN_ERR_ARG;
-    if (B < s0.S || (B - s0.S) % (uint32_t) s0.lay.G || (N < B && B > s0.S)) return refuse("sjk_hip_fork: B below S, inside a group or past N");
+    if (B < s0.S || (B - s0.S) % (uint32_t) s0.lay.G || (N < B && B > s0.S))
+        return refuse("sjk_hip_fork: B below S, inside a group or past N");
     for (int il = 0; il < n_layers; ++il)
         for (const sjk_hip_view * v : {dst + il, src + il}) {
             const sjk_hip_view & w = v == src + il ? s0 : d0;
@@ -140,8 +142,8 @@ extern "C" int sjk_hip_fork(const sjk_hip_view * dst, const sjk_hip_view * src, 
             bt.layer[k].sink = src[i0 + k].sink; bt.layer[k].ring = src[i0 + k].ring;
             bt.layer[k].to_sink = dst[i0 + k].sink; bt.layer[k].to_ring = dst[i0 + k].ring;
         }
-        hipLaunchKernelGGL(stream_past((uint64_t) n_layers * bytes) ? fork_kernel<true> : fork_kernel<false>, dim3((unsigned) at, (unsigned) nl),
-                           dim3(256), 0, (hipStream_t) stream, bt);
+        hipLaunchKernelGGL(stream_past((uint64_t) n_layers * bytes) ? fork_kernel<true> : fork_kernel<false>,
+                           dim3((unsigned) at, (unsigned) nl), dim3(256), 0, (hipStream_t) stream, bt);
         if (SJK_CHECK_LAUNCH()) return SJK_ERR_DEVICE;
     }
     return 0;
@@ -183,7 +185,8 @@ extern "C" int sjk_hip_copy_blocks(uint8_t * d_dst, size_t dst_layer_bytes, uint
     for (uint32_t i0 = 0; i0 < n; i0 += BLOCK_PAIRS) {
         const uint32_t k = n - i0 < (uint32_t) BLOCK_PAIRS ? n - i0 : (uint32_t) BLOCK_PAIRS;
         for (uint32_t i = 0; i < k; ++i) { bt.src[i] = src_ids[i0 + i]; bt.dst[i] = dst_ids[i0 + i]; }
-        hipLaunchKernelGGL(stream_past((uint64_t) n * (uint64_t) n_layers * block_bytes) ? copy_blocks_kernel<true> : copy_blocks_kernel<false>,
+        hipLaunchKernelGGL(stream_past((uint64_t) n * (uint64_t) n_layers * block_bytes) ? copy_blocks_kernel<true>
+                                                                                         : copy_blocks_kernel<false>,
                            dim3((unsigned) t, k, (unsigned) n_layers), dim3(256), 0, (hipStream_t) stream, bt);
         if (SJK_CHECK_LAUNCH()) return SJK_ERR_DEVICE;
     }
