@@ -630,6 +630,50 @@ def test_captured_append_replays_every_step(lib, dev):
         lib.sj_kvarn_layer_free(C.byref(B))
 
 
+def test_rows_past_32_bits(lib, dev):
+    """positions 3 GiB apart, read and written: the bits of rows on end"""
+    rng = np.random.default_rng(3)
+    n, heads, D, far = 3, 2, 128, 3 << 29        # elements of 2 bytes
+    x, o = Set(dev, rng, n, heads, D, sjk.BF16), Set(dev, rng, n, heads, D, sjk.BF16)
+    rope = make_rope(dev, {"n_rot": D, "layout": 0, "turns": turn_table(D)})
+    run_rows(lib, dev, [head_job(x, o, rope=1)], n, D, rope, pos0=9)
+    want = untouched(o)
+    row = heads * D * 2
+    big, out = (dev.alloc((n - 1) * far * 2 + row, zero=False).value for _ in range(2))
+    for i in range(n):
+        dev.upload(C.c_void_p(big + 2 * i * far), x.host[x.index()[i]])
+    run_rows(lib, dev, [sjk.HeadJob(big, out, far, D, far, D, x.t, x.t, heads, 1, 0, EPS, None, 0)], n, D, rope, pos0=9)
+    for i in range(n):
+        assert np.array_equal(dev.get(C.c_void_p(out + 2 * i * far), row, np.uint16), want[i].ravel())
+
+
+@pytest.mark.parametrize("staging", [0, 1])
+def test_slots_past_32_bits(lib, dev, staging):
+    """a ring of 5 GiB: the staged rows of a far slot are those of a small ring's"""
+    rng = np.random.default_rng(4 + staging)
+    D, H, n_head, n = 256, 8, 8, 21
+    A = new_layer(lib, D, H, staging, 0)
+    va = lib.sjk_layer_view(C.byref(A))
+    try:
+        entry = H * 2 * va.stage_bytes
+        vb = sjk.View.from_buffer_copy(va)
+        vb.cap = (5 << 30) // entry
+        vb.ring = dev.alloc(vb.cap * entry, zero=False).value
+        at = vb.cap - 40                         # its slot; the last of the n is 19 before the ring's end
+        pos0 = va.S + at
+        p = Proj(dev, rng, n, n_head, H, D, sjk.BF16, True, D, 0)
+        want_q = p.two_steps(lib, va, pos0)
+        q, k, v = p.ptrs()
+        sjk.check(lib.sjk_hip_store_qkv(C.byref(vb), pos0, n, C.byref(p.m), None, q, k, v, p.q, None), "store_qkv")
+        dev.sync()
+        assert at * entry > 1 << 32 and np.array_equal(p.q_out(), want_q)
+        small = cache_bytes(dev, va)[1].reshape(va.cap, entry)
+        got = dev.get(C.c_void_p(vb.ring + at * entry), n * entry, np.uint8).reshape(n, entry)
+        assert np.array_equal(got, small[(at + np.arange(n)) % va.cap])
+    finally:
+        lib.sj_kvarn_layer_free(C.byref(A))
+
+
 def test_two_streams_at_once(lib, dev):
     """two layers' appends from two streams at once, 20 times: the bytes of one after the other"""
     rng = np.random.default_rng(31)

@@ -109,6 +109,40 @@ def test_copy_blocks(lib, dev, block):
     assert np.array_equal(dev.get(da, a.nbytes, np.uint8), a)
 
 
+def test_pages_past_32_bits(lib, dev):
+    """blocks of a slab of 5 GiB and staged rows of a ring of 5 GiB"""
+    rng = np.random.default_rng(8)
+    block, n = 1 << 20, 5 << 10
+    slab = dev.alloc(block * n, zero=False)
+    far, near = rng.integers(0, 256, block, dtype=np.uint8), rng.integers(0, 256, block, dtype=np.uint8)
+    dev.upload(slab, far, offset=(n - 1) * block)
+    dev.upload(slab, near, offset=3 * block)
+    src, dst = (C.c_uint32 * 2)(n - 1, 3), (C.c_uint32 * 2)(7, n - 2)
+    sjk.check(lib.sjk_hip_copy_blocks(slab, block * n, n, slab, block * n, n, 1, block, src, dst, 2, None), "copy_blocks")
+    dev.sync()
+    assert np.array_equal(dev.get(C.c_void_p(slab.value + 7 * block), block, np.uint8), far)
+    assert np.array_equal(dev.get(C.c_void_p(slab.value + (n - 2) * block), block, np.uint8), near)
+
+    d, heads, small = 256, 8, 256
+    entry = heads * 2 * 2 * d
+    cap = (5 << 30) // entry
+    rows = rng.integers(0, 256, (200, entry), dtype=np.uint8)
+    sink = rng.integers(0, 256, S * heads * 4 * d, dtype=np.uint8)
+    at = (cap - 300) // 128 * 128                # slot and position of the first staged row
+    B = S + at
+    views = [raw_view(lib, dev, (sink, rng.integers(0, 256, small * entry, dtype=np.uint8)), d, heads, 1, 0, small) for _ in range(3)]
+    views[0].ring, views[0].cap = slab.value, cap
+    dev.upload(slab, rows, offset=at * entry)
+    sjk.check(lib.sjk_hip_fork(C.byref(views[1]), C.byref(views[0]), 1, B, B + 200, None), "fork")
+    dev.sync()
+    got = dev.get(C.c_void_p(views[1].ring), small * entry, np.uint8).reshape(small, entry)
+    assert at * entry > 1 << 32 and np.array_equal(got[(at + np.arange(200)) % small], rows)
+    dev.upload(slab, np.zeros_like(rows), offset=at * entry)
+    sjk.check(lib.sjk_hip_fork(C.byref(views[0]), C.byref(views[1]), 1, B, B + 200, None), "fork back")
+    dev.sync()
+    assert np.array_equal(dev.get(C.c_void_p(slab.value + at * entry), rows.nbytes, np.uint8).reshape(rows.shape), rows)
+
+
 def test_copy_more_blocks_than_a_launch_holds(lib, dev):
     rng = np.random.default_rng(1)
     n, block = 1500, 64
