@@ -523,6 +523,9 @@ __global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kerne
                     const float nsq = nf_batch ? walk<true, true>(row, xnw) : walk<false, true>(row);
                     const float norm = nsq != nsq ? nan_of(nsq) : __builtin_sqrtf(nsq);
                     const float inv = norm > 1e-10f ? 1.0f / norm : 0.0f;
+                    // a value of an infinite norm (rows with infinities, and finite rows whose rotation makes them) may be
+                    // infinity * 0, a NaN; no other can
+                    const bool inf = __any(norm == __builtin_inff());
                     wave_sync();
 #pragma unroll 1
                     for (int i = 0; i <= j; ++i) {
@@ -538,7 +541,7 @@ __global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kerne
                         for (int m = 0; m < 8; ++m) {
                             const float v = big ? z[m] * inv_i : 0.0f;
                             int code = level_of(v, s_cell);
-                            if (nf_batch && v != v) code = 63;
+                            if (inf && v != v) code = 63;
                             const float c = s_cent[code];
                             c2[m] = c * c;
                             qs |= (uint32_t) (code & 15) << (4 * m);
