@@ -82,7 +82,8 @@ SJK_DEV void turn(double u, float m, float sg, float & s, float & c) {
 // tq6_level by one look into a table: the line is cut into LV_CELLS cells so narrow that each holds at most one midpoint, which a
 // comparison then decides exactly. The cell of a value is a monotone function of it, the same for midpoints and values, so every
 // midpoint of a lower cell is below the value and every one of a higher cell above. (With the search's six dependent
-// reads 4,096 positions of 32 + 8 heads of 128 to tq6_0 take 6 us more.) Not for NaNs.
+// reads 4,096 positions of 32 + 8 heads of 128 to tq6_0 take 6 us more.) A NaN (infinity * 0 where a block's norm is
+// infinite) is level 63, as in the search: put into the last cell, where the comparison is false.
 constexpr int LV_CELLS = 128;
 constexpr float LV_SCALE = 200.0f;
 struct LevelCell { float mid; int base; };                 // the cell's midpoint, the midpoints of lower cells (a cell without one:
@@ -114,7 +115,7 @@ static_assert(level_table_ok(), "one midpoint a cell");
 static __constant__ LevelTable c_levels = level_table();
 
 SJK_DEV int level_of(float v, const LevelCell * cells) {
-    const LevelCell c = cells[(int) __builtin_amdgcn_fmed3f(level_at(v), 0.0f, 127.0f)];
+    const LevelCell c = cells[(int) __builtin_amdgcn_fmed3f(v != v ? 127.0f : level_at(v), 0.0f, 127.0f)];
     return c.base + (v < c.mid ? 0 : 1);
 }
 
@@ -168,31 +169,47 @@ template <bool WIDE> SJK_DEV void store_halves(uint16_t * o, const uint32_t (&h)
 // whether v is an infinity or a NaN
 SJK_DEV bool nonfinite(float v) { return __builtin_amdgcn_classf(v, 0x207); }
 
-// The rotation with the host's NaN rule in the rows where xn is set, through the wavefront's LDS (512 floats), a lane four pairs
-// of every stage: such rows are rare, so this is short rather than fast. The values of the other rows are hadamard_row's.
+// The rotation where some row comes out with a NaN, through the wavefront's LDS (512 floats): such rows are rare, so this is
+// short rather than fast. Rows where xn is set, with the host's NaN rule, a lane four pairs of every stage; each other row as the
+// row kernel rotates it, LPR / 8 values a lane in all lanes, so that the signs of NaNs that a finite row's overflow makes are its.
 template <int LPR> SJK_DEV void hadamard_rows_x(float (&x)[8], float * buf, int lane, float scale, bool xn) {
+    constexpr int V = LPR / 8;
     const int l = lane % LPR;
     float * row = buf + lane / LPR * (8 * LPR);
+    const uint64_t xn_rows = __ballot(xn);
     wave_sync();
 #pragma unroll
     for (int m = 0; m < 8; ++m) row[8 * l + m] = x[m];
     wave_sync();
 #pragma unroll 1
-    for (int h = 1; h < 8 * LPR; h *= 2) {
-#pragma unroll 1
-        for (int k = 4 * l; k < 4 * l + 4; ++k) {
-            const int j = 2 * (k & -h) + (k & (h - 1));
-            const float a = row[j], b = row[j + h];
-            row[j] = xn ? xadd(a, b) : a + b;
-            row[j + h] = xn ? xsub(a, b) : a - b;
-        }
-        wave_sync();
-    }
+    for (int r = 0; r < 64 / LPR; ++r) {
+        if (xn_rows >> (r * LPR) & 1) continue;
+        float * p = buf + r * (8 * LPR) + V * lane, y[V];
 #pragma unroll
-    for (int m = 0; m < 8; ++m) {
-        const float v = row[8 * l + m];
-        x[m] = xn ? xmul(v, scale) : v * scale;
+        for (int m = 0; m < V; ++m) y[m] = p[m];
+        hadamard_row<V, 64, false>(y, lane, scale);
+#pragma unroll
+        for (int m = 0; m < V; ++m) p[m] = y[m];
     }
+    wave_sync();
+    if (xn) {
+#pragma unroll 1
+        for (int h = 1; h < 8 * LPR; h *= 2) {
+#pragma unroll 1
+            for (int k = 4 * l; k < 4 * l + 4; ++k) {
+                const int j = 2 * (k & -h) + (k & (h - 1));
+                const float a = row[j], b = row[j + h];
+                row[j] = xadd(a, b);
+                row[j + h] = xsub(a, b);
+            }
+            wave_sync();
+        }
+#pragma unroll 1
+        for (int m = 0; m < 8; ++m) row[8 * l + m] = xmul(row[8 * l + m], scale);
+    }
+    wave_sync();
+#pragma unroll
+    for (int m = 0; m < 8; ++m) x[m] = row[8 * l + m];
     wave_sync();
 }
 
@@ -523,9 +540,6 @@ __global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kerne
                     const float nsq = nf_batch ? walk<true, true>(row, xnw) : walk<false, true>(row);
                     const float norm = nsq != nsq ? nan_of(nsq) : __builtin_sqrtf(nsq);
                     const float inv = norm > 1e-10f ? 1.0f / norm : 0.0f;
-                    // a value of an infinite norm (rows with infinities, and finite rows whose rotation makes them) may be
-                    // infinity * 0, a NaN; no other can
-                    const bool inf = __any(norm == __builtin_inff());
                     wave_sync();
 #pragma unroll 1
                     for (int i = 0; i <= j; ++i) {
@@ -540,8 +554,7 @@ __global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kerne
 #pragma unroll
                         for (int m = 0; m < 8; ++m) {
                             const float v = big ? z[m] * inv_i : 0.0f;
-                            int code = level_of(v, s_cell);
-                            if (inf && v != v) code = 63;
+                            const int code = level_of(v, s_cell);
                             const float c = s_cent[code];
                             c2[m] = c * c;
                             qs |= (uint32_t) (code & 15) << (4 * m);

@@ -28,7 +28,7 @@ OVERFLOWS = [((5, 6), 3e38), ((0, 1), -3e38), ((0, 127), 3e38), ((3, 5, 6), 3e38
 # whole turns, parts, parts by LDS, odd addresses, no turn
 @pytest.mark.parametrize("n_rot,pad", [(128, 0), (64, 0), (40, 0), (128, 3), (0, 0)])
 @pytest.mark.parametrize("D,t", [(128, sjk.F32), (256, sjk.F32), (128, sjk.BF16), (256, sjk.BF16)])
-@pytest.mark.parametrize("staging", [0])
+@pytest.mark.parametrize("staging", [0, 1])
 def test_append_of_rows_whose_rotation_overflows(lib, dev, D, t, staging, n_rot, pad):  # noqa: F811
     rng = np.random.default_rng(D + t + n_rot + pad)
     H, n_head, n = 4, 4, 2 * len(OVERFLOWS)
