@@ -22,6 +22,8 @@ constexpr int HEAD_PARTS = 3;          // sets of heads a launch: q, k, v
 constexpr int HEAD_SEQS = 32;          // sequences a launch
 constexpr int HEAD_ITERS = 8;          // heads a wavefront goes through at most
 constexpr int TQ_BATCH = 4;            // of them staged as tq6_0 together
+constexpr int TQ_UNROLL = 4;           // reads in flight of their walks (8 take 16 registers more: bf16 heads of 128 turned by half, 2,048
+                                       // positions, 24.6 us for 19.9; whole turns the same)
 enum { HP_ROWS = 0, HP_K = 1, HP_V = 2 };                               // where a part's rows go
 enum { HF_ROPE = 1, HF_ROT = 2, HF_BY_HEAD = 4 };
 enum { HM_ROWS = 0, HM_F16 = 1, HM_TQ6 = 2 };                           // a launch: plain rows only, or a cache's staging
@@ -82,8 +84,9 @@ SJK_DEV void turn(double u, float m, float sg, float & s, float & c) {
 // tq6_level by one look into a table: the line is cut into LV_CELLS cells so narrow that each holds at most one midpoint, which a
 // comparison then decides exactly. The cell of a value is a monotone function of it, the same for midpoints and values, so every
 // midpoint of a lower cell is below the value and every one of a higher cell above. (With the search's six dependent
-// reads 4,096 positions of 32 + 8 heads of 128 to tq6_0 take 6 us more.) A NaN (infinity * 0 where a block's norm is
-// infinite) is level 63, as in the search: put into the last cell, where the comparison is false.
+// reads 4,096 positions of 32 + 8 heads of 128 to tq6_0 take 6 us more.) Cells are counted downwards, by the negated value: the
+// hardware's median of a NaN and two others is their lesser, so a NaN (infinity * 0 where a block's norm is infinite) falls in the
+// highest cell, where the comparison is false, and gets level 63, as in the search.
 constexpr int LV_CELLS = 128;
 constexpr float LV_SCALE = 200.0f;
 struct LevelCell { float mid; int base; };                 // the cell's midpoint, the midpoints of lower cells (a cell without one:
@@ -99,8 +102,8 @@ constexpr LevelTable level_table() {
         t.cell[c].base = -1;
         for (int i = 0; i < 63; ++i) {
             const float m = __builtin_bit_cast(float, bits[i]);
-            if (level_cell(m) <= c) ++t.cell[c].base;
-            if (level_cell(m) == c) t.cell[c].mid = m;
+            if (level_cell(-m) >= c) ++t.cell[c].base;
+            if (level_cell(-m) == c) t.cell[c].mid = m;
         }
     }
     return t;
@@ -108,14 +111,14 @@ constexpr LevelTable level_table() {
 constexpr bool level_table_ok() {                          // no cell with two midpoints, midpoints in ascending order
     constexpr uint32_t bits[63] = SJK_TQ6_MIDPOINT_BITS_INIT;
     for (int i = 1; i < 63; ++i)
-        if (level_cell(__builtin_bit_cast(float, bits[i])) <= level_cell(__builtin_bit_cast(float, bits[i - 1]))) return false;
+        if (level_cell(-__builtin_bit_cast(float, bits[i])) >= level_cell(-__builtin_bit_cast(float, bits[i - 1]))) return false;
     return true;
 }
 static_assert(level_table_ok(), "one midpoint a cell");
 static __constant__ LevelTable c_levels = level_table();
 
 SJK_DEV int level_of(float v, const LevelCell * cells) {
-    const LevelCell c = cells[(int) __builtin_amdgcn_fmed3f(v != v ? 127.0f : level_at(v), 0.0f, 127.0f)];
+    const LevelCell c = cells[(int) __builtin_amdgcn_fmed3f(level_at(-v), 0.0f, 127.0f)];
     return c.base + (v < c.mid ? 0 : 1);
 }
 
@@ -169,47 +172,35 @@ template <bool WIDE> SJK_DEV void store_halves(uint16_t * o, const uint32_t (&h)
 // whether v is an infinity or a NaN
 SJK_DEV bool nonfinite(float v) { return __builtin_amdgcn_classf(v, 0x207); }
 
-// The rotation where some row comes out with a NaN, through the wavefront's LDS (512 floats): such rows are rare, so this is
-// short rather than fast. Rows where xn is set, with the host's NaN rule, a lane four pairs of every stage; each other row as the
-// row kernel rotates it, LPR / 8 values a lane in all lanes, so that the signs of NaNs that a finite row's overflow makes are its.
+// The rotation with the host's NaN rule in the rows where xn is set, through the wavefront's LDS (512 floats), a lane four pairs
+// of every stage: such rows are rare, so this is short rather than fast. The values of the other rows are hadamard_row's, signs of
+// NaNs included: as it is compiled, of two NaNs a sum keeps the upper one, a difference the lower one where the partner comes by
+// DPP (LPR / 8 values a lane in 64 lanes there) and the upper one where it comes by a row swap, and an upper one's sign is turned.
 template <int LPR> SJK_DEV void hadamard_rows_x(float (&x)[8], float * buf, int lane, float scale, bool xn) {
-    constexpr int V = LPR / 8;
     const int l = lane % LPR;
     float * row = buf + lane / LPR * (8 * LPR);
-    const uint64_t xn_rows = __ballot(xn);
     wave_sync();
 #pragma unroll
     for (int m = 0; m < 8; ++m) row[8 * l + m] = x[m];
     wave_sync();
 #pragma unroll 1
-    for (int r = 0; r < 64 / LPR; ++r) {
-        if (xn_rows >> (r * LPR) & 1) continue;
-        float * p = buf + r * (8 * LPR) + V * lane, y[V];
-#pragma unroll
-        for (int m = 0; m < V; ++m) y[m] = p[m];
-        hadamard_row<V, 64, false>(y, lane, scale);
-#pragma unroll
-        for (int m = 0; m < V; ++m) p[m] = y[m];
-    }
-    wave_sync();
-    if (xn) {
+    for (int h = 1; h < 8 * LPR; h *= 2) {
 #pragma unroll 1
-        for (int h = 1; h < 8 * LPR; h *= 2) {
-#pragma unroll 1
-            for (int k = 4 * l; k < 4 * l + 4; ++k) {
-                const int j = 2 * (k & -h) + (k & (h - 1));
-                const float a = row[j], b = row[j + h];
-                row[j] = xadd(a, b);
-                row[j + h] = xsub(a, b);
-            }
-            wave_sync();
+        for (int k = 4 * l; k < 4 * l + 4; ++k) {
+            const int j = 2 * (k & -h) + (k & (h - 1));
+            const float a = row[j], b = row[j + h];
+            const float n = -b;
+            const bool swap = h >= 16 * (LPR / 8);
+            row[j] = xn ? xadd(a, b) : b != b ? b : a + b;
+            row[j + h] = xn ? xsub(a, b) : swap && b != b ? n : a != a ? a : b != b ? n : a - b;
         }
-#pragma unroll 1
-        for (int m = 0; m < 8; ++m) row[8 * l + m] = xmul(row[8 * l + m], scale);
+        wave_sync();
     }
-    wave_sync();
 #pragma unroll
-    for (int m = 0; m < 8; ++m) x[m] = row[8 * l + m];
+    for (int m = 0; m < 8; ++m) {
+        const float v = row[8 * l + m];
+        x[m] = xn ? xmul(v, scale) : v * scale;
+    }
     wave_sync();
 }
 
@@ -537,7 +528,7 @@ __global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kerne
                     const int jw = min((lane & 15) / (16 / TB), j);            // the head this lane walks
                     const float * const row = blk + jw * (4 * BS);
                     const bool xnw = xn_batch >> jw & 1;
-                    const float nsq = nf_batch ? walk<true, true>(row, xnw) : walk<false, true>(row);
+                    const float nsq = nf_batch ? walk<true, true>(row, xnw) : walk<false, true, TQ_UNROLL>(row);
                     const float norm = nsq != nsq ? nan_of(nsq) : __builtin_sqrtf(nsq);
                     const float inv = norm > 1e-10f ? 1.0f / norm : 0.0f;
                     wave_sync();
@@ -572,7 +563,7 @@ __global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kerne
                         }
                     }
                     wave_sync();
-                    const float rn = __builtin_sqrtf(walk<false>(row));
+                    const float rn = __builtin_sqrtf(walk<false, false, TQ_UNROLL>(row));
                     const int h = head_at(it - j + jw, sub);
                     if (!f16_row && (lane & 15) % (16 / TB) == 0 && (ALL || (here && h < n_heads)))
                         *(uint16_t *) (d_base + h * d_head + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES) =

@@ -120,8 +120,9 @@ template <int V, int LPR> SJK_DEV void hadamard_finite(float (&x)[V], int lane, 
     for (int m = 0; m < V; ++m) x[m] = x[m] * scale;
 }
 
-// the sum of 128 values (SQUARED: of their squares) in index order; XN: the host's NaN rule where xn is set
-template <bool XN, bool SQUARED = false> SJK_DEV float walk(const float * sq, bool xn = true) {
+// the sum of 128 values (SQUARED: of their squares) in index order, UNROLL reads of four in flight; XN: the host's NaN rule where
+// xn is set
+template <bool XN, bool SQUARED = false, int UNROLL = 8> SJK_DEV float walk(const float * sq, bool xn = true) {
     const float4 * p = (const float4 *) sq;
     float s = 0.0f;
     if (XN) {
@@ -135,7 +136,7 @@ template <bool XN, bool SQUARED = false> SJK_DEV float walk(const float * sq, bo
         }
     } else {
         auto sq1 = [](float v) { return SQUARED ? v * v : v; };
-#pragma unroll 8
+#pragma unroll UNROLL
         for (int i = 0; i < 32; ++i) {
             const float4 q = p[i];
             s = s + sq1(q.x); s = s + sq1(q.y); s = s + sq1(q.z); s = s + sq1(q.w);
