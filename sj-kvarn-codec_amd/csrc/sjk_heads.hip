@@ -41,7 +41,7 @@ struct HeadSeq {
     const void * x[HEAD_PARTS];
     void * o[HEAD_PARTS];              // HP_ROWS: the part's rows; of a cache also [1] sink, [2] ring
     const int32_t * pos;
-    uint32_t pos0, S, cap;
+    uint32_t pos0, S, cap;             // pos0: with a descriptor, on top of its entry
 };
 
 struct HeadBatch {
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kerne
     const HeadPart & P = bt.part[pi];
     const HeadSeq & Q = bt.seq[si];
     if (bt.desc && bt.desc[SJK_DESC_QPOS0] < 0) return;
-    const uint32_t pos0 = bt.desc ? (uint32_t) bt.desc[SJK_DESC_QPOS0] : Q.pos0;
+    const uint32_t pos0 = Q.pos0 + (bt.desc ? (uint32_t) bt.desc[SJK_DESC_QPOS0] : 0u);
     const int n_heads = P.n_heads, step = P.flags & HF_BY_HEAD ? RPW : 1;
     const bool rope = P.flags & HF_ROPE, rot = P.flags & HF_ROT;
     float * buf = s_buf + wave * WS;
@@ -648,6 +648,25 @@ static int launch_typed(const HeadBatch & bt, int lpr, int mode, bool wide, unsi
     return launch_kind<T, HK_WHOLE>(bt, lpr, mode, grid, st);
 }
 
+// the table from position n on
+static void skip_positions(HeadBatch & bt, int n, size_t size) {
+    bt.n_pos -= n;
+    for (int k = 0; k < bt.n_seqs; ++k) {
+        HeadSeq & Q = bt.seq[k];
+        for (int p = 0; p < bt.n_parts; ++p) {
+            const HeadPart & P = bt.part[p];
+            if (!P.n_heads) continue;
+            Q.x[p] = (const uint8_t *) Q.x[p] + n * P.x_pos * (int64_t) size;
+            if (P.kind == HP_ROWS) Q.o[p] = (uint8_t *) Q.o[p] + n * P.o_pos * (int64_t) elem_size(P.o_type);
+        }
+        Q.pos0 += (uint32_t) n;
+        if (Q.pos) Q.pos += n;
+    }
+}
+
+// wavefronts of a launch, which has fewer than 2^32 threads
+constexpr int64_t MAX_WAVES = 0xffffffffll / (64 * HW) * HW;
+
 // The launch's shape. A wavefront goes through as many heads, up to HEAD_ITERS, as it takes for all wavefronts to be on the
 // device at once (16 a CU; the sines and cosines of a position serve its heads): a second, partly filled round of them costs a
 // 512-position append 7.1 -> 8.5 us, 1,237 positions x 64 heads of 80 10.8 -> 12.1. Its rows are adjacent positions, except in
@@ -660,7 +679,7 @@ static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream
     for (int p = 0; p < bt.n_parts; ++p) {
         HeadPart & P = bt.part[p];
         const bool by_head = bt.n_pos < rpw || (P.kind == HP_ROWS && P.o_type == SJK_F32 && P.n_heads % rpw == 0);
-        if (by_head) P.flags |= HF_BY_HEAD;
+        P.flags = by_head ? P.flags | HF_BY_HEAD : P.flags & ~HF_BY_HEAD;
         step[p] = by_head ? rpw : 1;                                       // heads an iteration takes on
         blocks[p] = by_head ? bt.n_pos : (bt.n_pos + rpw - 1) / rpw;
     }
@@ -684,6 +703,16 @@ static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream
     while (most <= HEAD_ITERS && !shape(most, (most + 1) / 2)) ++most;
     if (most > HEAD_ITERS) shape(HEAD_ITERS, HEAD_ITERS);
     if (!waves) return 0;
+    if (waves > MAX_WAVES) {                               // (8 channels of one head: from 2^29 positions on)
+        if (bt.n_pos <= 8) return refuse("head rows: more heads than a launch holds");
+        const int n = (bt.n_pos / 2 + 7) & ~7;
+        HeadBatch first = bt;
+        first.n_pos = n;
+        const int rc = launch_heads(first, type, mode, wide, st);
+        if (rc) return rc;
+        skip_positions(bt, n, elem_size(type));
+        return launch_heads(bt, type, mode, wide, st);
+    }
     bt.inv_D = 1.0f / (float) bt.D;
     bt.rot_scale = rot_scale(bt.D);
     const unsigned grid = (unsigned) ((waves + HW - 1) / HW);
@@ -692,10 +721,8 @@ static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream
     return launch_typed<__bf16>(bt, lpr, mode, wide, grid, st);
 }
 
-// rows of a launch are counted in 32 bits
-static bool rows_fit(uint64_t n_pos, uint64_t heads, uint64_t seqs) {
-    return n_pos <= 0x7fffffffu && n_pos * heads * seqs < 0x7fffff00u;
-}
+// rows of a sequence are counted in 32 bits
+static bool rows_fit(uint64_t n_pos, uint64_t heads) { return n_pos <= 0x7fffffffu && n_pos * heads < 0x7fffff00u; }
 
 }  // namespace sjk
 
@@ -720,7 +747,7 @@ extern "C" int sjk_hip_head_rows(const sjk_hip_head_job * jobs, int n_jobs, uint
         }
         heads += (uint64_t) J.n_heads;
     }
-    if (!rows_fit(n_pos, heads, 1)) return refuse("sjk_hip_head_rows: 2^31 rows or more");
+    if (!rows_fit(n_pos, heads)) return refuse("sjk_hip_head_rows: 2^31 rows or more");
     for (int k0 = 0; k0 < n_jobs;) {
         HeadBatch bt = {};
         bt.n_pos = (int) n_pos;
@@ -776,7 +803,7 @@ int qkv_ok(const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t pos0, uint32_
         set_error("sjk_hip_store_qkv: more positions than sink and ring hold at once");
         return SJKVARN_ERR_CAPACITY;
     }
-    if (!rows_fit(n_pos, (uint64_t) m.n_head + 2u * (uint64_t) H, HEAD_SEQS)) return refuse("sjk_hip_store_qkv: 2^31 rows or more");
+    if (!rows_fit(n_pos, (uint64_t) m.n_head + 2u * (uint64_t) H)) return refuse("sjk_hip_store_qkv: 2^31 rows or more");
     int rc = norm_ok(m.n_head ? m.d_q_norm : nullptr, m.eps);
     if (!rc) rc = norm_ok(m.d_k_norm, m.eps);
     if (!rc) rc = rope_ok(m.rope, D);
