@@ -460,9 +460,9 @@ typedef struct sjk_hip_head_job {
 } sjk_hip_head_job;
 
 /* n_pos positions of every job's heads (the queries and the keys of a layer, say) in one launch for up to three jobs of one
- * x_type (several where a call has more rows than a launch takes, 2^29 of up to 64 channels and one head). Fewer than 2^31 rows
- * in all jobs, SJKVARN_ERR_ARG otherwise. Head widths 1 to 512. Position i is d_pos[i] (device, int32) or, with d_pos NULL, pos0 + i. rope may be NULL if
- * no job turns. Sums, angles and products in 32 bits or more. */
+ * x_type (several where a call has more rows than a launch takes, 2^29 of up to 64 channels and one head). Head widths 1 to 512,
+ * fewer than 2^31 rows in all jobs. Position i is d_pos[i] (device, int32) or, with d_pos NULL, pos0 + i, below 2^32 - 1. rope may
+ * be NULL if no job turns. Sums, angles and products in 32 bits or more. */
 int sjk_hip_head_rows(const sjk_hip_head_job * jobs, int n_jobs, uint32_t n_pos, int D, const sjk_hip_rope * rope,
                       uint32_t pos0, const int32_t * d_pos, void * stream);
 

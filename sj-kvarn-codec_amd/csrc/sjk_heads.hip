@@ -734,6 +734,7 @@ extern "C" int sjk_hip_head_rows(const sjk_hip_head_job * jobs, int n_jobs, uint
     if (D < 1 || D > 512) return refuse("sjk_hip_head_rows: head widths 1 to 512");
     if (d_pos && (uintptr_t) d_pos % 4) return SJKVARN_ERR_ARG;
     uint64_t heads = 0;
+    bool turned = false;
     for (int k = 0; k < n_jobs; ++k) {
         const sjk_hip_head_job & J = jobs[k];
         if (!J.d_x || !J.d_out || J.n_heads < 0 || !type_ok(J.x_type) || !type_ok(J.out_type)) return SJKVARN_ERR_ARG;
@@ -746,8 +747,10 @@ extern "C" int sjk_hip_head_rows(const sjk_hip_head_job * jobs, int n_jobs, uint
             return SJK_ERR_UNSUPPORTED;
         }
         heads += (uint64_t) J.n_heads;
+        turned |= J.rope && rope->n_rot;
     }
     if (!rows_fit(n_pos, heads)) return refuse("sjk_hip_head_rows: 2^31 rows or more");
+    if (turned && !d_pos && (uint64_t) pos0 + n_pos > 0xffffffffull) return refuse("sjk_hip_head_rows: positions past 2^32 - 2");
     for (int k0 = 0; k0 < n_jobs;) {
         HeadBatch bt = {};
         bt.n_pos = (int) n_pos;
@@ -797,7 +800,7 @@ int qkv_ok(const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t pos0, uint32_
     if (((uintptr_t) d_k | (uintptr_t) d_v | (m.n_head ? (uintptr_t) d_q : 0)) % size || (uintptr_t) d_q_out % 4 ||
         (uintptr_t) d_pos % 4 || (((uintptr_t) v.sink | (uintptr_t) v.ring) & 1u))
         return SJKVARN_ERR_ARG;
-    if ((uint64_t) pos0 + n_pos > 0xffffffffull) return refuse("sjk_hip_store_qkv: positions past 2^32 - 1");
+    if ((uint64_t) pos0 + n_pos > 0xffffffffull) return refuse("sjk_hip_store_qkv: positions past 2^32 - 2");
     const uint64_t room = (uint64_t) v.cap + (pos0 < v.S ? v.S - pos0 : 0);
     if (n_pos > room) {
         set_error("sjk_hip_store_qkv: more positions than sink and ring hold at once");

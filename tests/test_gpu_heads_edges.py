@@ -8,8 +8,8 @@ import numpy as np
 import pytest
 
 import cabi  # noqa: F401
-from test_gpu_heads import (EPS, Proj, cache_bytes, dev, from_bits, lib, make_rope, new_layer, run_rows, sjk, to_bits,  # noqa: F401
-                            turn_table)
+from test_gpu_heads import (EPS, Proj, Set, cache_bytes, check_rows, dev, from_bits, head_job, lib, make_rope,  # noqa: F401
+                            new_layer, reference, run_rows, sjk, to_bits, turn_table, untouched)
 
 pytestmark = pytest.mark.gpu
 
@@ -125,3 +125,19 @@ def test_append_of_more_rows_than_a_launch_holds(lib, dev, dyn):  # noqa: F811
             assert np.array_equal(got.reshape(k, entry), want), w
     finally:
         lib.sj_kvarn_layer_free(C.byref(A))
+
+
+def test_turns_up_to_the_last_position(lib, dev):  # noqa: F811
+    """positions up to 2^32 - 2 by pos0; rows that are not turned, or by positions of their own, take any pos0"""
+    rng = np.random.default_rng(32)
+    D, n = 128, 255
+    r = {"n_rot": D, "layout": 0, "turns": turn_table(D)}
+    rope = make_rope(dev, r)
+    x, o = Set(dev, rng, n, 2, D, sjk.F32), Set(dev, rng, n, 2, D, sjk.F32)
+    run_rows(lib, dev, [head_job(x, o, rope=1)], n, D, rope, pos0=0xFFFFFF00)
+    ref, err = reference(x.values(), 0xFFFFFF00 + np.arange(n, dtype=np.int64), rope=r)
+    check_rows(untouched(o), sjk.F32, ref, err, "last positions")
+    run_rows(lib, dev, [head_job(x, o)], n, D, rope, pos0=0xFFFFFFFF)
+    assert np.array_equal(untouched(o), x.host[x.index()])
+    run_rows(lib, dev, [head_job(x, o, rope=1)], n, D, rope, pos0=0xFFFFFFFF, d_pos=dev.put(np.zeros(n, np.int32)))
+    assert np.array_equal(from_bits(untouched(o), sjk.F32), x.values())
