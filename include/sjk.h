@@ -605,8 +605,9 @@ int sjk_hip_seq_attend_batch(const sjk_hip_seq_job * jobs, int n_jobs, int il, i
 /* The sink entries [0, min(N, S)) and the staged rows of positions [B, N) of n_layers layers copied from src's buffers to dst's
  * slots of the same positions, in one launch for up to 64 layers; nothing else in dst is written. Records are not copied: dst's
  * view brings its own body or block table. The views agree in layout, KV heads, staging, sink type and S (capacities may
- * differ), buffers 4-byte aligned, each of dst's its own and none of src's. SJKVARN_ERR_ARG otherwise and for B < S, B inside
- * a group or N < B with B > S; SJKVARN_ERR_CAPACITY where [B, N) does not fit a ring. */
+ * differ), buffers 4-byte aligned, and no buffer of dst (S sink entries, cap ring slots) overlaps another of dst or one of src.
+ * SJKVARN_ERR_ARG otherwise and for B < S, B inside a group or N < B with B > S; SJKVARN_ERR_CAPACITY where [B, N) does not fit
+ * a ring. */
 int sjk_hip_fork(const sjk_hip_view * dst, const sjk_hip_view * src, int n_layers, uint32_t B, uint32_t N, void * stream);
 
 /* Blocks src_ids[i] of one pool's slab to blocks dst_ids[i] of another's (or the same) in every layer: block id of layer il lies

@@ -108,18 +108,29 @@ extern "C" int sjk_hip_fork(const sjk_hip_view * dst, const sjk_hip_view * src, 
                 v->sink_type != s0.sink_type || v->stage_bytes != s0.stage_bytes || v->S != s0.S || v->cap != w.cap)
                 return refuse("sjk_hip_fork: the views differ in layout, heads, staging, sink or (on one side) capacity");
         }
-    for (int i = 0; i < n_layers; ++i)                     // a layer's buffers written twice, or written and read
+    const uint64_t H = (uint64_t) s0.n_head_kv, entry = H * 2 * s0.stage_bytes;
+    const uint64_t sink_entry = s0.sink_type == SJKVARN_SINK_F16 ? H * 4 * (uint64_t) s0.lay.D : entry;
+    // each buffer of dst against every other buffer: none may be written twice, or written and read
+    const uint64_t ss = s0.S * sink_entry, sr = s0.cap * entry, dr = d0.cap * entry;
+    auto meet = [](const uint8_t * p, uint64_t np, const uint8_t * q, uint64_t nq) {
+        return (uint64_t) ((uintptr_t) p - (uintptr_t) q) + np - 1 < np + nq - 1;      // -np < p - q < nq
+    };
+    for (int i = 0; i < n_layers; ++i) {
+        const sjk_hip_view & d = dst[i];
+        bool bad = meet(d.sink, ss, d.ring, dr);
         for (int k = 0; k < n_layers; ++k)
-            if (dst[i].sink == src[k].sink || dst[i].ring == src[k].ring ||
-                (k < i && (dst[i].sink == dst[k].sink || dst[i].ring == dst[k].ring)))
-                return refuse("sjk_hip_fork: a buffer of dst is another layer's, or src's");
+            bad |= meet(d.sink, ss, src[k].sink, ss) | meet(d.sink, ss, src[k].ring, sr) | meet(d.ring, dr, src[k].sink, ss) |
+                   meet(d.ring, dr, src[k].ring, sr);
+        for (int k = 0; k < i; ++k)
+            bad |= meet(d.sink, ss, dst[k].sink, ss) | meet(d.sink, ss, dst[k].ring, dr) | meet(d.ring, dr, dst[k].sink, ss) |
+                   meet(d.ring, dr, dst[k].ring, dr);
+        if (bad) return refuse("sjk_hip_fork: a buffer of dst overlaps another of dst, or one of src");
+    }
     const uint32_t n = N > B ? N - B : 0;
     if (n > s0.cap || n > d0.cap) {
         set_error("sjk_hip_fork: the staged positions do not fit the ring");
         return SJKVARN_ERR_CAPACITY;
     }
-    const uint64_t H = (uint64_t) s0.n_head_kv, entry = H * 2 * s0.stage_bytes;
-    const uint64_t sink_entry = s0.sink_type == SJKVARN_SINK_F16 ? H * 4 * (uint64_t) s0.lay.D : entry;
     ForkBatch bt;
     const uint64_t sink = (uint64_t) (N < s0.S ? N : s0.S) * sink_entry, bytes = sink + n * entry;     // of a layer
     uint64_t at = tiles(sink / 4);

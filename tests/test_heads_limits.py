@@ -1,5 +1,5 @@
 """Calls between projections and cache, and those that move pages, that are refused before anything is launched (no GPU; every
-device pointer is fake): positions past 32 bits."""
+device pointer is fake): positions past 32 bits, buffers that overlap."""
 import ctypes as C
 import sys
 
@@ -17,3 +17,29 @@ def test_head_rows_positions_past_32_bits(lib):  # noqa: F811
     for n, pos0 in ((200, 0xFFFFFF80), (1, 0xFFFFFFFF), (2, 0xFFFFFFFE)):
         assert call(n, pos0) == ARG, (n, pos0)
     assert b"2^32" in lib.sjk_last_error() and call(0, 0xFFFFFFFF) == 0
+
+
+def test_fork_refuses_buffers_that_overlap(lib):  # noqa: F811
+    """a buffer of dst that is, or reaches into, another buffer of dst or one of src, of either kind, in any layer"""
+    MB = 1 << 20
+    sink, ring = 128 * 2 * 4 * 128, 256 * 2 * 2 * 98                    # bytes: 128 KiB, 98 KiB
+    src = [view(lib, sink=i * MB, ring=i * MB + MB // 2) for i in (1, 2)]
+    dst = [view(lib, sink=i * MB, ring=i * MB + MB // 2) for i in (11, 12)]
+
+    def call(d, s, n=200):
+        return lib.sjk_hip_fork((sjk.View * 2)(*d), (sjk.View * 2)(*s), 2, 128, n, None)
+
+    assert call(dst, src, 0) == 0
+    for il in (0, 1):
+        for name, size, starts in (("sink", sink, [v.sink for v in src] + [v.ring for v in src] + [dst[1 - il].sink, dst[1 - il].ring, dst[il].ring]),
+                                   ("ring", ring, [v.sink for v in src] + [v.ring for v in src] + [dst[1 - il].sink, dst[1 - il].ring, dst[il].sink])):
+            for k, at in enumerate(starts):
+                other = sink if at % MB == 0 else ring
+                for p, code in ((at, ARG), (at + other - 4, ARG), (at - size + 4, ARG), (at + other, 0), (at - size, 0)):
+                    d = [sjk.View.from_buffer_copy(v) for v in dst]
+                    setattr(d[il], name, p)
+                    assert call(d, src, 0) == code, (il, name, k, p - at)
+                    assert code == 0 or call(d, src) == code
+    other = [sjk.View.from_buffer_copy(v) for v in src]
+    other[1].sink, other[1].ring = src[0].sink, src[0].ring              # (src's own buffers are only read)
+    assert call(dst, other, 0) == 0
