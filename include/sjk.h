@@ -600,6 +600,7 @@ int sjk_hip_seq_attend_batch(const sjk_hip_seq_job * jobs, int n_jobs, int il, i
  * holders of its blocks. sj_kvarn_pool_release takes one holder off and frees the block with the last one; seq_truncate,
  * seq_reset, seq_free and a state restore release the blocks they drop in that way and clear only those that no one else holds
  * (sj_kvarn_layer_truncate on a pool sequence's layer knows no holders and clears every dropped record: use seq_truncate).
+ * The blocks of a pool that its caller put together have one holder each: forks on it copy the records.
  * These calls change the pool on the host: the caller orders them with each other and with commits on that pool. */
 
 /* The sink entries [0, min(N, S)) and the staged rows of positions [B, N) of n_layers layers copied from src's buffers to dst's

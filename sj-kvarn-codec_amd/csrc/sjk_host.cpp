@@ -7,7 +7,8 @@
 // host arrays: the free functions copy them to device buffers of their own call, the layer calls to
 // the layer's workspace, launch, and copy the result back (synchronous). There is no CPU path: a HIP
 // failure inside a void call (which has no status to return) aborts with a message. There is no
-// process-wide mutable state: every buffer belongs to a call or to a cache object.
+// process-wide mutable state but the list of the pools whose blocks are counted (pool_extra): every buffer belongs to a call or
+// to a cache object.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -726,11 +727,15 @@ void sj_kvarn_layer_attend_row(const sj_kvarn_layer * L, uint32_t B, uint32_t N,
 // (in pool mode only the blocks the sequence holds, and with `pool` only those it holds alone), the sink entries of
 // positions [resume, min(n_old, S)) and the ring rows of positions [max(resume, S), n_old) that can still be resident (the
 // last cap of them), as contiguous runs.
-static bool pool_shared(const sj_kvarn_pool * pool, uint32_t id);
+static uint32_t * pool_extra(const sj_kvarn_pool * pool);
+static bool pool_shared(const sj_kvarn_pool * pool, const uint32_t * extra, uint32_t id) {
+    return extra && id < pool->n_blocks && extra[id] != 0;
+}
 static void truncate_runs(const sj_kvarn_layer * L, uint32_t B_old, uint32_t B_new, uint32_t n_old, uint32_t resume,
                           std::vector<sjk::CopyRun> & runs, const sj_kvarn_pool * pool = nullptr) {
     const uint32_t S = L->cfg.sink, G = (uint32_t) L->cfg.group;
     const size_t H = (size_t) L->cfg.n_head_kv;
+    const uint32_t * extra = pool ? pool_extra(pool) : nullptr;
     auto add = [&](const uint8_t * p, size_t n) {
         if (!n) return;
         const uint64_t d = (uint64_t) (uintptr_t) p;
@@ -740,7 +745,7 @@ static void truncate_runs(const sj_kvarn_layer * L, uint32_t B_old, uint32_t B_n
     if (B_new < B_old)
         for (uint32_t g = (B_new - S) / G; g < (B_old - S) / G; ++g) {
             if (L->blocks && L->blocks[g] == SJKVARN_NO_BLOCK) continue;
-            if (L->blocks && pool && pool_shared(pool, L->blocks[g])) continue;
+            if (L->blocks && pool_shared(pool, extra, L->blocks[g])) continue;
             add(sj_kvarn_layer_record(L, g, 0), H * L->lay.bytes);
         }
     const uint32_t se = n_old < S ? n_old : S;
@@ -824,6 +829,35 @@ const char * sj_kvarn_strerror(int code) {
 // paged pool / sequence (sj_kvarn.h:1645-1809)
 // ---------------------------------------------------------------------------------------------------
 
+// The holders of a block beyond its first (sequences forked from the one that sealed it) lie behind the free list, in the same
+// allocation, so that the reference's struct stays as it is. Only sj_kvarn_pool_init makes such a list: the lists it made are kept
+// here, because a pool that its caller put together has n_blocks words and none behind them. Its blocks have one holder each.
+static std::mutex & pool_mutex = *new std::mutex;
+static std::vector<const uint32_t *> & pool_lists = *new std::vector<const uint32_t *>;
+
+static uint32_t * pool_extra(const sj_kvarn_pool * pool) {
+    std::lock_guard<std::mutex> g(pool_mutex);
+    for (const uint32_t * p : pool_lists)
+        if (p == pool->free_ids) return pool->free_ids + pool->n_blocks;
+    return nullptr;
+}
+
+static bool pool_note(const uint32_t * list) {
+    std::lock_guard<std::mutex> g(pool_mutex);
+    try { pool_lists.push_back(list); } catch (const std::bad_alloc &) { return false; }
+    return true;
+}
+
+static void pool_forget(const uint32_t * list) {
+    std::lock_guard<std::mutex> g(pool_mutex);
+    for (size_t i = 0; i < pool_lists.size(); ++i)
+        if (pool_lists[i] == list) {
+            pool_lists[i] = pool_lists.back();
+            pool_lists.pop_back();
+            return;
+        }
+}
+
 int sj_kvarn_pool_init(sj_kvarn_pool * pool, const sj_kvarn_config * cfg, int n_layers, uint32_t n_blocks) {
     memset(pool, 0, sizeof(*pool));
     if (n_layers <= 0 || n_blocks == 0 || cfg->n_head_kv <= 0) return SJKVARN_ERR_ARG;
@@ -836,7 +870,7 @@ int sj_kvarn_pool_init(sj_kvarn_pool * pool, const sj_kvarn_config * cfg, int n_
     const size_t body_b = (size_t) n_layers * n_blocks * (size_t) cfg->n_head_kv * pool->lay.bytes;
     pool->free_ids = (uint32_t *) malloc(2 * (size_t) n_blocks * sizeof(uint32_t));   // and the shared counts behind them
     if (!pool->free_ids || hipMalloc((void **) &pool->body, body_b) != hipSuccess ||
-        hipMemset(pool->body, 0, body_b) != hipSuccess) {
+        hipMemset(pool->body, 0, body_b) != hipSuccess || !pool_note(pool->free_ids)) {
         sj_kvarn_pool_free(pool);
         return SJKVARN_ERR_NOMEM;
     }
@@ -850,6 +884,7 @@ int sj_kvarn_pool_init(sj_kvarn_pool * pool, const sj_kvarn_config * cfg, int n_
 
 void sj_kvarn_pool_free(sj_kvarn_pool * pool) {
     if (pool->body) (void) hipFree(pool->body);
+    pool_forget(pool->free_ids);
     free(pool->free_ids);
     pool->body = nullptr;
     pool->free_ids = nullptr;
@@ -858,20 +893,17 @@ void sj_kvarn_pool_free(sj_kvarn_pool * pool) {
 
 uint32_t sj_kvarn_pool_alloc(sj_kvarn_pool * pool) { return pool->n_free ? pool->free_ids[--pool->n_free] : SJKVARN_NO_BLOCK; }
 
-// Holders of a block beyond its first (sequences forked from the one that sealed it): kept behind the free list, so that
-// the reference's struct stays as it is
-static uint32_t * pool_extra(const sj_kvarn_pool * pool) { return pool->free_ids + pool->n_blocks; }
-static bool pool_shared(const sj_kvarn_pool * pool, uint32_t id) { return id < pool->n_blocks && pool_extra(pool)[id] != 0; }
-
 void sj_kvarn_pool_release(sj_kvarn_pool * pool, uint32_t id) {
-    if (pool_shared(pool, id)) { --pool_extra(pool)[id]; return; }
+    uint32_t * extra = pool_extra(pool);
+    if (pool_shared(pool, extra, id)) { --extra[id]; return; }
     if (id != SJKVARN_NO_BLOCK && pool->n_free < pool->n_blocks) pool->free_ids[pool->n_free++] = id;
 }
 
 uint32_t sjk_hip_pool_refs(const sj_kvarn_pool * pool, uint32_t id) {
     if (!pool || !pool->free_ids || id >= pool->n_blocks) return 0;
     for (uint32_t i = 0; i < pool->n_free; ++i) if (pool->free_ids[i] == id) return 0;
-    return pool_extra(pool)[id] + 1u;
+    const uint32_t * extra = pool_extra(pool);
+    return extra ? extra[id] + 1u : 1u;
 }
 
 // the device copy of a sequence's block table lives in layers[0].work (shared by every layer): entries [g0, g1)
@@ -940,9 +972,10 @@ static int seq_release(sj_kvarn_seq * s, uint32_t g0, uint32_t g1) {
 
 // the blocks that releasing everything the sequence holds would free
 static uint32_t seq_held_alone(const sj_kvarn_seq * s) {
+    const uint32_t * extra = pool_extra(s->pool);
     uint32_t held = 0;
     for (uint32_t g = 0; g < s->layers[0].n_groups; ++g)
-        held += s->blocks[g] != SJKVARN_NO_BLOCK && !pool_shared(s->pool, s->blocks[g]);
+        held += s->blocks[g] != SJKVARN_NO_BLOCK && !pool_shared(s->pool, extra, s->blocks[g]);
     return held;
 }
 
@@ -1779,7 +1812,8 @@ int sjk_hip_seq_fork(sj_kvarn_seq * child, sj_kvarn_seq * parent, uint32_t pos, 
     const uint32_t n = sj_kvarn_policy_truncate(&pol, pos, nullptr), n_rec = (pol.B - S) / G;
     if (n > child->cfg.n_ctx || n_rec > child->layers[0].n_groups || (n > pol.B && n - pol.B > child->layers[0].cap))
         return SJKVARN_ERR_CAPACITY;
-    const bool share = child->pool && child->pool == parent->pool;
+    uint32_t * extra = child->pool && child->pool == parent->pool ? pool_extra(child->pool) : nullptr;
+    const bool share = extra != nullptr;
     if (child->pool && !share && child->pool->n_free < n_rec) return SJKVARN_ERR_POOL_FULL;
     for (uint32_t g = 0; parent->pool && g < n_rec; ++g)
         if (parent->blocks[g] >= parent->pool->n_blocks) return SJKVARN_ERR_ARG;
@@ -1794,7 +1828,7 @@ int sjk_hip_seq_fork(sj_kvarn_seq * child, sj_kvarn_seq * parent, uint32_t pos, 
     if (share) {
         for (uint32_t g = 0; g < n_rec; ++g) {
             child->blocks[g] = parent->blocks[g];
-            ++pool_extra(child->pool)[child->blocks[g]];
+            ++extra[child->blocks[g]];
         }
     } else {
         st = seq_reserve(child, 0, n_rec);
@@ -1865,13 +1899,14 @@ int sjk_hip_pool_compact(sj_kvarn_pool * pool, sj_kvarn_seq * const * seqs, int 
             if (id >= nb) return SJKVARN_ERR_ARG;
             ++held.p[id];
         }
+    uint32_t * extra = pool_extra(pool);
     bool ok = pool->n_free <= nb;
     for (uint32_t i = 0; ok && i < pool->n_free; ++i) {
         const uint32_t id = pool->free_ids[i];
         ok = id < nb && held.p[id] == 0 && where.p[id] == 0;
         if (ok) where.p[id] = SJKVARN_NO_BLOCK;                            // free
     }
-    for (uint32_t id = 0; ok && id < nb; ++id) ok = where.p[id] == SJKVARN_NO_BLOCK || held.p[id] == pool_extra(pool)[id] + 1u;
+    for (uint32_t id = 0; ok && id < nb; ++id) ok = where.p[id] == SJKVARN_NO_BLOCK || held.p[id] == (extra ? extra[id] : 0u) + 1u;
     if (!ok) {
         sjk::set_error("sjk_hip_pool_compact: a live block is not held by the given sequences alone");
         return SJKVARN_ERR_ARG;
@@ -1904,9 +1939,9 @@ int sjk_hip_pool_compact(sj_kvarn_pool * pool, sj_kvarn_seq * const * seqs, int 
         if (rc && !st) st = rc;
         rt_note_store(rt_of(s), (hipStream_t) stream);
     }
-    for (uint32_t i = 0; i < n; ++i) {
-        pool_extra(pool)[dst[i]] = pool_extra(pool)[src[i]];
-        pool_extra(pool)[src[i]] = 0;
+    for (uint32_t i = 0; extra && i < n; ++i) {
+        extra[dst[i]] = extra[src[i]];
+        extra[src[i]] = 0;
     }
     for (uint32_t i = 0; i < pool->n_free; ++i) pool->free_ids[i] = nb - 1u - i;
     if (moved) *moved = n;

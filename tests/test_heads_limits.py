@@ -1,5 +1,5 @@
 """Calls between projections and cache, and those that move pages, that are refused before anything is launched (no GPU; every
-device pointer is fake): positions past 32 bits, buffers that overlap."""
+device pointer is fake): positions past 32 bits, buffers that overlap; and pools that their caller put together."""
 import ctypes as C
 import sys
 
@@ -43,3 +43,20 @@ def test_fork_refuses_buffers_that_overlap(lib):  # noqa: F811
     other = [sjk.View.from_buffer_copy(v) for v in src]
     other[1].sink, other[1].ring = src[0].sink, src[0].ring              # (src's own buffers are only read)
     assert call(dst, other, 0) == 0
+
+
+def test_pool_put_together_by_its_caller(lib):  # noqa: F811
+    """a pool with a free list of the caller's own, n_blocks words: nothing behind the list is read or written, and every block
+    has one holder"""
+    for guard in (0, 1, 7, 0xFFFFFFFF):
+        ids = (C.c_uint32 * 12)(*([3, 2] + [guard] * 10))
+        pool = sjk.Pool()
+        pool.n_layers, pool.n_blocks, pool.n_free = 1, 4, 2
+        pool.free_ids = C.cast(ids, C.POINTER(C.c_uint32))
+        assert [lib.sjk_hip_pool_refs(C.byref(pool), i) for i in range(5)] == [1, 1, 0, 0, 0]
+        lib.sj_kvarn_pool_release(C.byref(pool), 1)
+        lib.sj_kvarn_pool_release(C.byref(pool), 0)
+        assert pool.n_free == 4 and list(ids) == [3, 2, 1, 0] + [guard] * 8
+        lib.sj_kvarn_pool_release(C.byref(pool), 0)              # full: nothing more
+        assert pool.n_free == 4 and list(ids) == [3, 2, 1, 0] + [guard] * 8
+        assert [lib.sj_kvarn_pool_alloc(C.byref(pool)) for _ in range(5)] == [0, 1, 2, 3, 0xFFFFFFFF]
