@@ -511,8 +511,9 @@ typedef struct sjk_hip_qkv_job {
 int sjk_hip_store_qkv_batch(const sjk_hip_qkv_job * jobs, int n_jobs, uint32_t n_pos, const sjk_hip_qkv * m, void * stream);
 
 /* The same for layer il of several sequences (a decode batch), as sjk_hip_seq_store_batch: each sequence's position count
- * is extended. SJKVARN_ERR_ARG for a bad layer index or a gap before pos0, SJKVARN_ERR_CAPACITY where the staged positions
- * (from the sealed end on) would not fit the ring, SJKVARN_ERR_ARG for a sequence given twice; a refused call stores nothing. */
+ * is extended. SJKVARN_ERR_ARG for a bad layer index, a gap before pos0 or a sequence given twice; SJKVARN_ERR_CAPACITY where the
+ * staged positions (from the sealed end on) would not fit the ring, and for positions of the sealed part whose ring slots hold
+ * staged ones. A refused call stores nothing. */
 typedef struct sjk_hip_seq_qkv_job {
     sj_kvarn_seq  * seq;
     uint32_t        pos0;

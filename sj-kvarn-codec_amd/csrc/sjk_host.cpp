@@ -1185,6 +1185,13 @@ int sjk_hip_seq_store_qkv_batch(const sjk_hip_seq_qkv_job * jobs, int n_jobs, in
             sjk::set_error("sjk_hip_seq_store_qkv_batch: more staged positions than the ring holds");
             return SJKVARN_ERR_CAPACITY;
         }
+        // positions [from, to) of the sealed part: their slots may hold nothing, or positions one or more turns of the ring later
+        const uint64_t S = s->cfg.sink, B = s->pol.B, cap = s->layers[il].cap, from = jobs[k].pos0 > S ? jobs[k].pos0 : S,
+                       to = end < B ? end : B;
+        if (cap && from < to && from + ((B - to) / cap + 1) * cap < s->n) {
+            sjk::set_error("sjk_hip_seq_store_qkv_batch: sealed positions whose ring slots hold staged ones");
+            return SJKVARN_ERR_CAPACITY;
+        }
         for (int i = 0; i < k; ++i)
             if (jobs[i].seq == s) {
                 sjk::set_error("sjk_hip_seq_store_qkv_batch: a sequence twice");

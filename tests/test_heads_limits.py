@@ -1,12 +1,12 @@
 """Calls between projections and cache, and those that move pages, that are refused before anything is launched (no GPU; every
-device pointer is fake): positions past 32 bits, buffers that overlap; and pools that their caller put together."""
+device pointer is fake): positions past 32 bits, buffers that overlap, sealed positions; and pools that their caller put together."""
 import ctypes as C
 import sys
 
 import cabi
 
 sys.path.insert(0, cabi.PKG)
-from test_heads_refusals import ARG, FAKE, job, lib, rope, sjk, view  # noqa: E402, F401
+from test_heads_refusals import ARG, CAPACITY, FAKE, job, lib, qkv, rope, sjk, view  # noqa: E402, F401
 
 
 def test_head_rows_positions_past_32_bits(lib):  # noqa: F811
@@ -60,3 +60,26 @@ def test_pool_put_together_by_its_caller(lib):  # noqa: F811
         lib.sj_kvarn_pool_release(C.byref(pool), 0)              # full: nothing more
         assert pool.n_free == 4 and list(ids) == [3, 2, 1, 0] + [guard] * 8
         assert [lib.sj_kvarn_pool_alloc(C.byref(pool)) for _ in range(5)] == [0, 1, 2, 3, 0xFFFFFFFF]
+
+
+def test_sequence_append_below_the_sealed_end(lib):  # noqa: F811
+    """positions of the sealed part whose ring slots hold staged positions are refused: storing them would write over those"""
+    L = sjk.Layer()
+    v = view(lib, cap=896)
+    L.lay, L.cap, L.stage_bytes, L.n_groups, L.ring, L.sink, L.body = v.lay, 896, v.stage_bytes, 64, v.ring, v.sink, v.body
+    L.cfg.staging, L.cfg.sink_type = v.staging, v.sink_type
+    L.cfg.head_dim, L.cfg.n_head_kv, L.cfg.group, L.cfg.sink, L.cfg.n_ctx = 128, 2, 128, 128, 8192
+    s = sjk.Seq()
+    s.n_layers, s.layers, s.cfg = 1, C.pointer(L), L.cfg
+    s.pol.sink, s.pol.group, s.pol.B, s.pol.B_pending, s.n = 128, 128, 128 + 1280, 128 + 1280, 128 + 1280 + 500
+    m = qkv()
+
+    def call(pos0, n):
+        j = sjk.SeqQkvJob(C.pointer(s), pos0, None, FAKE, FAKE, FAKE, FAKE)
+        return lib.sjk_hip_seq_store_qkv_batch(C.byref(j), 1, 0, n, C.byref(m), None)
+
+    # staged slots: positions 128 + [1280, 1780) at [384, 884); the sealed positions at them are 128 + [384, 884)
+    for pos0, n in ((128 + 384, 1), (128 + 883, 1), (128 + 380, 5), (128 + 883, 200), (128 + 300, 800), (0, 128 + 385)):
+        assert call(pos0, n) == CAPACITY, (pos0, n)
+    assert call(128 + 1280, 897) == CAPACITY and call(s.n + 1, 1) == ARG
+    assert call(128 + 384, 0) == 0 and s.n == 128 + 1780
