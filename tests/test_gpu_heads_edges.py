@@ -3,11 +3,13 @@ sink and behind it, alone in their wavefront and beside rows with infinities and
 sjk_hip_head_rows to fp32 followed by sjk_hip_layer_store, whose bytes the oracle pins. Calls of more rows than one launch
 holds (2^32 threads)."""
 import ctypes as C
+import os
+import re
 
 import numpy as np
 import pytest
 
-import cabi  # noqa: F401
+import cabi
 from test_gpu_heads import (EPS, Proj, Set, cache_bytes, check_rows, dev, from_bits, head_job, lib, make_rope,  # noqa: F401
                             new_layer, reference, run_rows, sjk, to_bits, turn_table, untouched)
 
@@ -141,3 +143,106 @@ def test_turns_up_to_the_last_position(lib, dev):  # noqa: F811
     assert np.array_equal(untouched(o), x.host[x.index()])
     run_rows(lib, dev, [head_job(x, o, rope=1)], n, D, rope, pos0=0xFFFFFFFF, d_pos=dev.put(np.zeros(n, np.int32)))
     assert np.array_equal(from_bits(untouched(o), sjk.F32), x.values())
+
+
+@pytest.mark.parametrize("D,n_rot,layout,rotate", [(128, 0, 0, 1), (256, 0, 0, 1), (64, 64, 0, 1), (512, 512, 1, 1), (128, 64, 0, 1), (128, 40, 0, 0),
+                                                   (80, 80, 0, 0), (96, 50, 1, 0), (33, 20, 0, 0), (7, 0, 0, 0), (128, 128, 0, 1)])
+@pytest.mark.parametrize("t_out", [sjk.F16, sjk.BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("norm", [False, True])
+def test_fp32_rows_to_16_bits(lib, dev, D, n_rot, layout, rotate, t_out, norm):  # noqa: F811
+    """the attention's output on its way to the output projection (the rotation alone, to 16 bits), and fp32 rows through every
+    other step, in calls of a few positions and of many, on 16-byte accesses and at any address"""
+    rng = np.random.default_rng(D + 1000 * n_rot + t_out)
+    r = {"n_rot": n_rot, "layout": layout, "turns": turn_table(n_rot)}
+    rope = make_rope(dev, r)
+    w = (1 + 0.25 * rng.standard_normal(D)).astype(np.float32)
+    for n, heads, offset in ((1, 3, 0), (3, 16, 0), (2, 5, 1), (301, 8, 0), (5, 1, 0)):
+        x, o = Set(dev, rng, n, heads, D, sjk.F32, offset=offset, scale=2.0), Set(dev, rng, n, heads, D, t_out, offset=offset)
+        run_rows(lib, dev, [head_job(x, o, rope=int(n_rot > 0), rotate=rotate, d_norm=dev.put(w).value if norm else None)], n, D, rope, pos0=4000)
+        ref, err = reference(x.values(), 4000 + np.arange(n), w=w if norm else None, rope=r, rotate=bool(rotate))
+        check_rows(untouched(o), t_out, ref, err, (n, heads, offset))
+
+
+def test_fp32_rows_past_the_range_of_16_bits(lib, dev):  # noqa: F811
+    """values past the type's largest become infinities, values below its smallest zeros or subnormal, NaNs stay NaNs: the one
+    rounding to nearest even that numpy makes"""
+    rng = np.random.default_rng(16)
+    D = 128
+    v = np.concatenate([np.float32([65504, 65519.99, 65520, -65520, 1e30, -3.3895e38, 3.4e38, 2 ** -14, 2 ** -24, 2 ** -25, 2.9802326e-08, 1e-45,
+                                    np.inf, -np.inf, np.nan, 0.0, -0.0]), (rng.integers(0, 1 << 32, 64 * D, dtype=np.uint64).astype(np.uint32)).view(np.float32)])
+    v = np.resize(v, (64, 1, D))
+    for t in (sjk.F16, sjk.BF16):
+        x, o = Set(dev, rng, 64, 1, D, sjk.F32), Set(dev, rng, 64, 1, D, t)
+        x.host[x.index()] = v.view(np.uint32)
+        dev.upload(x.d, x.host)
+        run_rows(lib, dev, [head_job(x, o)], 64, D)
+        got, want = from_bits(untouched(o), t), from_bits(to_bits(v, t), t)
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        assert np.array_equal(got[~np.isnan(got)], want[~np.isnan(want)]) and np.array_equal(np.signbit(got[got == 0]), np.signbit(want[want == 0]))
+
+
+def midpoints():
+    text = open(os.path.join(cabi.ROOT, "include", "sjk_tables.h")).read().replace("\\\n", " ")
+    bits = re.search(r"define\s+SJK_TQ6_MIDPOINT_BITS_INIT\s*\{(.*?)\}", text, re.S).group(1)
+    return np.array([int(x, 0) for x in re.findall(r"0x[0-9A-Fa-f]+", bits)], np.uint32).view(np.float32)
+
+
+def step_of(x):
+    """floats as integers, one apart from one float to the next (both zeros 0)"""
+    i = np.asarray(x, np.float32).view(np.int32).astype(np.int64)
+    return np.where(i < 0, -(i & 0x7FFFFFFF), i)
+
+
+def at_step(i):
+    return np.uint32(i if i >= 0 else 0x80000000 - i).view(np.float32)
+
+
+def test_levels_next_to_every_midpoint(lib, dev):  # noqa: F811
+    """blocks whose values over their norm are a midpoint, or one of the three floats on either side of it: the codes of
+    sjk_hip_layer_store, which searches the midpoints themselves. numpy makes the same fp32 operations, to see that every midpoint
+    is met from both sides and exactly"""
+    rng = np.random.default_rng(63)
+    mids = midpoints()
+    D, H = 128, 8
+
+    def block(i, scale):
+        """values mid[i] and mids[62 - i] a few floats apart, times scale, and one that brings the sum of squares to 1"""
+        x = np.zeros(D, np.float32)
+        near = []
+        for m in (mids[i], mids[(i + 21) % 63]):
+            for k in range(-3, 4):
+                near.append(at_step(step_of(m) + k))
+        near = np.array(near, np.float32)
+        x[1:1 + len(near)] = near
+        x[0] = np.sqrt(max(0.0, 1.0 - np.sum(near.astype(np.float64) ** 2)))
+        return (x * np.float32(scale)).astype(np.float32)
+
+    blocks = [block(i, 2.0 ** e * (1 + f)) for i in range(63) for e, f in ((0, 0), (3, 0), (-6, 0), (0, 0.1), (0, 0.37), (1, 0.71), (0, 1e-7), (0, -1e-7))]
+    blocks += [block(i, s) for i in range(63) for s in rng.uniform(0.5, 8, 24)]
+    rows = np.array(blocks + [np.zeros(D, np.float32)] * (-len(blocks) % (2 * H)), np.float32).reshape(-1, 2 * H, D)
+    nsq = np.zeros(rows.shape[:2], np.float32)
+    for c in range(D):
+        nsq += rows[..., c] * rows[..., c]
+    inv = np.float32(1) / np.maximum(np.sqrt(nsq), np.float32(1e-10))
+    met = (rows * inv[..., None]).astype(np.float32).ravel()
+    for m in mids:
+        assert {-1, 0, 1} <= set((step_of(met[np.abs(met - m) < 1e-6]) - step_of(m)).tolist()), m
+    n = len(rows)
+    A, B = (new_layer(lib, D, H, 0, 0, n_ubatch=256) for _ in range(2))
+    va, vb = lib.sjk_layer_view(C.byref(A)), lib.sjk_layer_view(C.byref(B))
+    try:
+        assert n <= va.cap
+        p = Proj(dev, rng, n, 0, H, D, sjk.F32, False, 0, 0, rotate_v=0)
+        p.m.rotate_qk = 0
+        p.x.host[p.x.index()] = rows.view(np.uint32)
+        dev.upload(p.x.d, p.x.host)
+        _, k, v = p.ptrs()
+        sjk.check(lib.sjk_hip_store_qkv(C.byref(va), 200, n, C.byref(p.m), None, None, k, v, None, None), "store_qkv")
+        dk, dv = (dev.put(np.ascontiguousarray(rows[:, a:a + H])) for a in (0, H))
+        sjk.check(lib.sjk_hip_layer_store(C.byref(vb), 200, n, dk, dv, 0, None), "layer_store")
+        dev.sync()
+        for got, want in zip(cache_bytes(dev, va), cache_bytes(dev, vb)):
+            assert np.array_equal(got, want)
+    finally:
+        lib.sj_kvarn_layer_free(C.byref(A))
+        lib.sj_kvarn_layer_free(C.byref(B))
