@@ -22,8 +22,8 @@ constexpr int HEAD_PARTS = 3;          // sets of heads a launch: q, k, v
 constexpr int HEAD_SEQS = 32;          // sequences a launch
 constexpr int HEAD_ITERS = 8;          // heads a wavefront goes through at most
 constexpr int TQ_BATCH = 4;            // of them staged as tq6_0 together
-constexpr int TQ_UNROLL = 4;           // reads in flight of their walks (8 take 16 registers more: bf16 heads of 128 turned by half, 2,048
-                                       // positions, 24.6 us for 19.9; whole turns the same)
+constexpr int TQ_UNROLL = 4;           // reads in flight of their walks (8 take 16 registers more: 2,048 positions of bf16 heads of
+                                       // 128 turned by half 24.6 us for 19.9, whole turns the same)
 enum { HP_ROWS = 0, HP_K = 1, HP_V = 2 };                               // where a part's rows go
 enum { HF_ROPE = 1, HF_ROT = 2, HF_BY_HEAD = 4 };
 enum { HM_ROWS = 0, HM_F16 = 1, HM_TQ6 = 2 };                           // a launch: plain rows only, or a cache's staging
@@ -211,7 +211,7 @@ enum { HK_WHOLE = 0,        // rows of 8 * LPR channels whose addresses and stri
        HK_ODD = 2,          // such accesses, a turn of halves over another number: pairs through LDS
        HK_ANY = 3 };        // rows of any width, address and stride, any turn, element by element (3,226 positions x 6 heads of 256
                             // turned over 232 channels: 25.7 us, 14.0 by HK_ODD)
-// (HK_WHOLE: 16 wavefronts a CU, as launch_heads counts on; tq6_0 takes the 128 registers that leaves, 130 without the bound)
+// (HK_WHOLE: 16 wavefronts a CU, as launch_heads counts on, 128 registers; tq6_0 takes 112 to 120 of them)
 template <typename T, int LPR, int MODE, int KIND>
 __global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kernel(const HeadBatch bt) {
     // Lanes behind the last row take the last row again, and lanes behind a row's channels its first ones, and write the same
@@ -668,10 +668,13 @@ static void skip_positions(HeadBatch & bt, int n, size_t size) {
 constexpr int64_t MAX_WAVES = 0xffffffffll / (64 * HW) * HW;
 
 // The launch's shape. A wavefront goes through as many heads, up to HEAD_ITERS, as it takes for all wavefronts to be on the
-// device at once (16 a CU; the sines and cosines of a position serve its heads): a second, partly filled round of them costs a
-// 512-position append 7.1 -> 8.5 us, 1,237 positions x 64 heads of 80 10.8 -> 12.1. Its rows are adjacent positions, except in
-// calls of fewer positions than that, and where rows of fp32 go out: those of one position lie on end, and stores of 2 KB
-// reach 5.0 TB/s where four of 512 bytes reach 4.6. (Rows of 16 bits: 4.5 by head, 4.9 by position, whose sines also serve more heads.)
+// device at once (the sines and cosines of a position serve its heads): a second, partly filled round of them costs a
+// 512-position append 7.1 -> 8.5 us, 1,237 positions x 64 heads of 80 10.8 -> 12.1. 16 wavefronts a CU are counted on, which the
+// kernels for whole turns are bound to. 24 of the others have the registers for 12 (most HK_ODD ones from fp32 and fp16 rows; to
+// tq6_0 HK_ODD, HK_ANY, and HK_PART but for 16-bit rows of 128): their calls of 12 to 16 a CU take a second round all the same.
+// A wavefront's rows are adjacent positions, except in calls of fewer positions than that, and where rows of fp32 go out: those of
+// one position lie on end, and stores of 2 KB reach 5.0 TB/s where four of 512 bytes reach 4.6. (Rows of 16 bits: 4.5 by head,
+// 4.9 by position, whose sines also serve more heads.)
 static int launch_heads(HeadBatch & bt, int type, int mode, bool wide, hipStream_t st) {
     const int lpr = bt.D <= 64 ? 8 : bt.D <= 128 ? 16 : bt.D <= 256 ? 32 : 64, rpw = 64 / lpr;
     int64_t blocks[HEAD_PARTS];
