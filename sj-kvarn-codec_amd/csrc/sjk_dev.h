@@ -241,6 +241,10 @@ int qkv_ok(const sjk_hip_view & v, const sjk_hip_qkv & m, uint32_t pos0, uint32_
 
 // the text sjk_last_error() returns on the calling thread (sjk_host.cpp)
 void set_error(const char * what);
+inline int refuse(const char * what) {
+    set_error(what);
+    return SJKVARN_ERR_ARG;
+}
 
 // partial slots that sjk_hip_workspace_bytes provides: every attention launch fits (sjk_attend3.hip)
 int ws_slots(int n_head_kv);

@@ -579,11 +579,6 @@ __global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kerne
     else heads(Int<HO_HALF>());
 }
 
-static int refuse(const char * what) {
-    set_error(what);
-    return SJKVARN_ERR_ARG;
-}
-
 static size_t elem_size(int type) { return type == SJK_F32 ? 4 : 2; }
 static bool type_ok(int type) { return type == SJK_F32 || type == SJK_F16 || type == SJK_BF16; }
 // rows at p with strides in elements of `size` bytes can be read and written 16 bytes at a time

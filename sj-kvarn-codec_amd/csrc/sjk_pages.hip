@@ -80,10 +80,6 @@ template <bool STREAM> __global__ __launch_bounds__(256) void copy_blocks_kernel
 static bool stream_past(uint64_t bytes) { return bytes > ((uint64_t) 64 << 20); }
 
 static uint64_t tiles(uint64_t words) { return (words + TILE_WORDS - 1) / TILE_WORDS; }
-static int refuse(const char * what) {
-    set_error(what);
-    return SJKVARN_ERR_ARG;
-}
 
 }  // namespace sjk
 

@@ -25,10 +25,10 @@ template <int LM> SJK_DEV float lane_xor(float v, int lane) {
     }
 }
 
-// Hadamard of one row (sj_kvarn.h:735-752): stages h < V inside the lane, stages h >= V between lanes l and l ^ (h / V)
-// (the lower partner keeps a + b, the upper a - b, a = the lower value), then one multiply by 1/sqrt(V * LPR). XN: the
+// Hadamard of one row of 64 V values (sj_kvarn.h:735-752): stages h < V inside the lane, stages h >= V between lanes l and
+// l ^ (h / V) (the lower partner keeps a + b, the upper a - b, a = the lower value), then one multiply by 1/sqrt(64 V). XN: the
 // host's NaN rule (a row holding an infinity or a NaN).
-template <int V, int LPR, bool XN>
+template <int V, bool XN>
 SJK_DEV void hadamard_row(float (&x)[V], int lane, float scale) {
     auto add = [&](float a, float b) { return XN ? xadd(a, b) : a + b; };
     auto sub = [&](float a, float b) { return XN ? xsub(a, b) : a - b; };
@@ -43,7 +43,7 @@ SJK_DEV void hadamard_row(float (&x)[V], int lane, float scale) {
             }
     if (XN) {
 #pragma unroll
-        for (int lm = 1; lm < LPR; lm *= 2) {
+        for (int lm = 1; lm < 64; lm *= 2) {
             const bool upper = (lane & lm) != 0;
 #pragma unroll
             for (int m = 0; m < V; ++m) {
@@ -62,12 +62,12 @@ SJK_DEV void hadamard_row(float (&x)[V], int lane, float scale) {
                 x[m] = upper ? o - x[m] : x[m] + o;
             }
         };
-        if constexpr (LPR > 1) stage(1, [&](float v) { return lane_xor<1>(v, lane); });
-        if constexpr (LPR > 2) stage(2, [&](float v) { return lane_xor<2>(v, lane); });
-        if constexpr (LPR > 4) stage(4, [&](float v) { return lane_xor<4>(v, lane); });
-        if constexpr (LPR > 8) stage(8, [&](float v) { return lane_xor<8>(v, lane); });
+        stage(1, [&](float v) { return lane_xor<1>(v, lane); });
+        stage(2, [&](float v) { return lane_xor<2>(v, lane); });
+        stage(4, [&](float v) { return lane_xor<4>(v, lane); });
+        stage(8, [&](float v) { return lane_xor<8>(v, lane); });
 #pragma unroll
-        for (int lm = 16; lm < LPR; lm *= 2) {
+        for (int lm = 16; lm < 64; lm *= 2) {
             const bool upper = (lane & lm) != 0;
 #pragma unroll
             for (int m = 0; m < V; ++m) {
@@ -83,8 +83,9 @@ SJK_DEV void hadamard_row(float (&x)[V], int lane, float scale) {
     for (int m = 0; m < V; ++m) x[m] = XN ? xmul(x[m], scale) : x[m] * scale;
 }
 
-// hadamard_row<V, LPR, false> for rows whose result is finite: a stage across lanes is the lane's own value with its sign
-// turned in the upper partner, added to the partner's value as the addition's DPP operand (two instructions a value for four).
+// The same of a row of V * LPR values in LPR lanes, for rows whose result is finite: a stage across lanes is the lane's own value
+// with its sign turned in the upper partner, added to the partner's value as the addition's DPP operand (two instructions a value
+// for four).
 // A NaN on the way may come out with another sign.
 template <int V, int LPR> SJK_DEV void hadamard_finite(float (&x)[V], int lane, float scale) {
 #pragma unroll

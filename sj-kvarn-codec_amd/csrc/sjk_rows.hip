@@ -117,8 +117,8 @@ __global__ __launch_bounds__(64 * NW) void rows_kernel(const RowBatch bt) {
     for (int m = 0; m < V; ++m) nf |= (f_bits(x[m]) & 0x7F800000u) == 0x7F800000u;
     const bool xn = __any(nf);
     if (live && j.rotate) {
-        if (xn) hadamard_row<V, 64, true>(x, lane, j.rot_scale);
-        else hadamard_row<V, 64, false>(x, lane, j.rot_scale);
+        if (xn) hadamard_row<V, true>(x, lane, j.rot_scale);
+        else hadamard_row<V, false>(x, lane, j.rot_scale);
     }
     const bool tq = live && mode == OUT_TQ6;
     bool any_tq = tq;
