@@ -22,8 +22,6 @@ constexpr int HEAD_PARTS = 3;          // sets of heads a launch: q, k, v
 constexpr int HEAD_SEQS = 32;          // sequences a launch
 constexpr int HEAD_ITERS = 8;          // heads a wavefront goes through at most
 constexpr int TQ_BATCH = 4;            // of them staged as tq6_0 together
-constexpr int TQ_UNROLL = 4;           // reads in flight of their walks (8 take 16 registers more: 2,048 positions of bf16 heads of
-                                       // 128 turned by half 24.6 us for 19.9, whole turns the same)
 enum { HP_ROWS = 0, HP_K = 1, HP_V = 2 };                               // where a part's rows go
 enum { HF_ROPE = 1, HF_ROT = 2, HF_BY_HEAD = 4 };
 enum { HM_ROWS = 0, HM_F16 = 1, HM_TQ6 = 2 };                           // a launch: plain rows only, or a cache's staging
@@ -86,7 +84,8 @@ SJK_DEV void turn(double u, float m, float sg, float & s, float & c) {
 // midpoint of a lower cell is below the value and every one of a higher cell above. (With the search's six dependent
 // reads 4,096 positions of 32 + 8 heads of 128 to tq6_0 take 6 us more.) Cells are counted downwards, by the negated value: the
 // hardware's median of a NaN and two others is their lesser, so a NaN (infinity * 0 where a block's norm is infinite) falls in the
-// highest cell, where the comparison is false, and gets level 63, as in the search.
+// highest cell, where the comparison is false, and gets level 63, as in the search (with a test of its own in its place, 16-bit rows
+// of 128 turned in part have 12 wavefronts a CU for 16: 2,048 positions 24.6 us for 19.5, 512 12.9 for 10.0).
 constexpr int LV_CELLS = 128;
 constexpr float LV_SCALE = 200.0f;
 struct LevelCell { float mid; int base; };                 // the cell's midpoint, the midpoints of lower cells (a cell without one:
@@ -211,7 +210,7 @@ enum { HK_WHOLE = 0,        // rows of 8 * LPR channels whose addresses and stri
        HK_ODD = 2,          // such accesses, a turn of halves over another number: pairs through LDS
        HK_ANY = 3 };        // rows of any width, address and stride, any turn, element by element (3,226 positions x 6 heads of 256
                             // turned over 232 channels: 25.7 us, 14.0 by HK_ODD)
-// (HK_WHOLE: 16 wavefronts a CU, as launch_heads counts on, 128 registers; tq6_0 takes 112 to 120 of them)
+// (HK_WHOLE: 16 wavefronts a CU, as launch_heads counts on, 128 registers; tq6_0 takes 120 to 128 of them)
 template <typename T, int LPR, int MODE, int KIND>
 __global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kernel(const HeadBatch bt) {
     // Lanes behind the last row take the last row again, and lanes behind a row's channels its first ones, and write the same
@@ -224,6 +223,9 @@ __global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kerne
     constexpr int BS = 132;                                // floats from a 128-value block to the next (walks: other banks)
     constexpr int TB = MODE == HM_TQ6 ? TQ_BATCH : 1;      // heads staged together
     constexpr int WS = MODE == HM_TQ6 ? TB * 4 * BS : 512; // floats of a wavefront's LDS
+    // reads in flight of a tq6_0 walk: 4 take 16 registers less and calls of few wavefronts 0.4 us more (64 positions 6.8 -> 7.3), so
+    // only where 8 do not fit the bound above
+    constexpr int UNROLL = KIND == HK_WHOLE && LPR == 16 && sizeof(T) == 4 ? 4 : 8;
     __shared__ alignas(16) float s_buf[HW * WS];
     __shared__ LevelCell s_cell[MODE == HM_TQ6 ? LV_CELLS : 1];
     __shared__ float s_cent[MODE == HM_TQ6 ? 64 : 1];
@@ -528,7 +530,7 @@ __global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kerne
                     const int jw = min((lane & 15) / (16 / TB), j);            // the head this lane walks
                     const float * const row = blk + jw * (4 * BS);
                     const bool xnw = xn_batch >> jw & 1;
-                    const float nsq = nf_batch ? walk<true, true>(row, xnw) : walk<false, true, TQ_UNROLL>(row);
+                    const float nsq = nf_batch ? walk<true, true>(row, xnw) : walk<false, true, UNROLL>(row);
                     const float norm = nsq != nsq ? nan_of(nsq) : __builtin_sqrtf(nsq);
                     const float inv = norm > 1e-10f ? 1.0f / norm : 0.0f;
                     wave_sync();
@@ -563,7 +565,7 @@ __global__ __launch_bounds__(64 * HW, KIND == HK_WHOLE ? 4 : 1) void heads_kerne
                         }
                     }
                     wave_sync();
-                    const float rn = __builtin_sqrtf(walk<false, false, TQ_UNROLL>(row));
+                    const float rn = __builtin_sqrtf(walk<false, false, UNROLL>(row));
                     const int h = head_at(it - j + jw, sub);
                     if (!f16_row && (lane & 15) % (16 / TB) == 0 && (ALL || (here && h < n_heads)))
                         *(uint16_t *) (d_base + h * d_head + (size_t) (l >> 4) * SJKVARN_TQ6_BLOCK_BYTES) =
@@ -666,7 +668,8 @@ constexpr int64_t MAX_WAVES = 0xffffffffll / (64 * HW) * HW;
 // device at once (the sines and cosines of a position serve its heads): a second, partly filled round of them costs a
 // 512-position append 7.1 -> 8.5 us, 1,237 positions x 64 heads of 80 10.8 -> 12.1. 16 wavefronts a CU are counted on, which the
 // kernels for whole turns are bound to. 24 of the others have the registers for 12 (most HK_ODD ones from fp32 and fp16 rows; to
-// tq6_0 HK_ODD, HK_ANY, and HK_PART but for 16-bit rows of 128): their calls of 12 to 16 a CU take a second round all the same.
+// tq6_0 HK_ODD, HK_ANY, and HK_PART but for 16-bit rows of 128; HK_ODD of fp32 rows of 256 for 8): their calls of 12 to 16 a CU
+// take a second round all the same.
 // A wavefront's rows are adjacent positions, except in calls of fewer positions than that, and where rows of fp32 go out: those of
 // one position lie on end, and stores of 2 KB reach 5.0 TB/s where four of 512 bytes reach 4.6. (Rows of 16 bits: 4.5 by head,
 // 4.9 by position, whose sines also serve more heads.)
