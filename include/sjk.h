@@ -492,7 +492,8 @@ int sjk_hip_store_qkv(const sjk_hip_view * v, uint32_t pos0, uint32_t n_pos, con
                       const void * d_q, const void * d_k, const void * d_v, float * d_q_out, void * stream);
 
 /* The same with pos0 = d_desc[SJK_DESC_QPOS0] read on the device when the kernel runs (sjk_hip_layer_store_dyn): one
- * captured graph takes every step. A negative entry writes nothing, d_q_out included. */
+ * captured graph takes every step. A negative entry writes nothing, d_q_out included. SJKVARN_ERR_ARG for more rows than one launch
+ * holds (2^27 positions of one KV head of 128). */
 int sjk_hip_store_qkv_dyn(const sjk_hip_view * v, const int32_t * d_desc, uint32_t n_pos, const sjk_hip_qkv * m,
                           const int32_t * d_pos, const void * d_q, const void * d_k, const void * d_v, float * d_q_out,
                           void * stream);

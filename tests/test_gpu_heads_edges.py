@@ -94,7 +94,7 @@ def test_more_rows_than_a_launch_holds(lib, dev):  # noqa: F811
 @pytest.mark.parametrize("dyn", [False, True])
 def test_append_of_more_rows_than_a_launch_holds(lib, dev, dyn):  # noqa: F811
     """2^27 positions of one head of 128 to tq6_0, a ring of 26 GB, every position from the same projection row: the staged rows
-    are those of small calls"""
+    are those of small calls. By descriptor one launch takes what it holds, and more is refused"""
     rng = np.random.default_rng(27)
     D, k, pos0 = 128, 500, 40
     n = (1 << 27) + 4003
@@ -111,7 +111,11 @@ def test_append_of_more_rows_than_a_launch_holds(lib, dev, dyn):  # noqa: F811
         if dyn:
             desc = np.zeros(16, np.int32)
             desc[4] = pos0 + big.S
-            rc = lib.sjk_hip_store_qkv_dyn(C.byref(big), dev.put(desc), n, C.byref(p.m), None, None, kp, vp, None, None)
+            d_desc = dev.put(desc)
+            assert lib.sjk_hip_store_qkv_dyn(C.byref(big), d_desc, n, C.byref(p.m), None, None, kp, vp, None, None) == -100
+            n -= 4100                                    # the most that one launch holds, and less
+            big.cap = n
+            rc = lib.sjk_hip_store_qkv_dyn(C.byref(big), d_desc, n, C.byref(p.m), None, None, kp, vp, None, None)
         else:
             rc = lib.sjk_hip_store_qkv(C.byref(big), pos0 + big.S, n, C.byref(p.m), None, None, kp, vp, None, None)
         sjk.check(rc, "store_qkv")
