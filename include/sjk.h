@@ -595,6 +595,117 @@ int sjk_hip_seq_state_finish(sj_kvarn_seq * s, size_t * written);
 int sjk_hip_seq_attend_batch(const sjk_hip_seq_job * jobs, int n_jobs, int il, int n_q, int n_head, float scale,
                              void * stream);
 
+/* ---- part of a long context, and drafted tokens (no counterpart in the reference, whose attention reads the whole context and
+ * whose positions follow each other) ---- */
+
+/* Attention over some of the sealed groups. For every query position and KV head, sjk_hip_select_groups lists the `top` groups
+ * whose keys can reach the highest scores, and sjk_hip_attend_groups attends over the sink, the listed groups and the
+ * staged tail (positions from B on, causal among themselves).
+ *
+ * A group's score comes from its record's scale tables alone. With codes in [c0, c1] (0 and 2^bits - 1, or the K codebook's
+ * least and greatest value) a key is K[t, d] = (c Kscale[d] + Kzero[d]) Ktok[t], so with
+ *   u = sum_d q_d Kzero_d + w_d Kscale_d,   w_d = c1 q_d for q_d > 0, else c0 q_d,
+ * no token's product with q is above u max Ktok (u >= 0) or u min Ktok (u < 0). The score is the largest such bound of the KV head's
+ * query heads, in 64 bits (for scores that are multiplied by a scale above zero). The greatest scores are taken, of equal ones the lower
+ * group; a score that is not a number is above all others. d_sel [n_q][n_head_kv][top] (int32) is in ascending order, -1 where there are fewer
+ * groups than top.
+ *
+ * sjk_hip_attend_groups takes any ascending list: an entry that is no sealed group, or not above the entry before it, adds nothing.
+ * With all groups listed the result is sjk_hip_attend's up to rounding. d_out [n_q][n_head][D] of out_type (SJK_F32, _F16, _BF16), rotated basis; weights keep 22 bits and sums 32. A row that
+ * sees nothing is zero. Infinities and NaNs of staged positions that a row does not see do not reach it.
+ *
+ * Query positions lie behind the sealed part: with B > S, qpos0 + 1 >= B, N >= B, and B at a group's end (SJKVARN_ERR_ARG otherwise).
+ * d_q is fp32 [n_q][n_head][D], 16-byte aligned, and does not overlap d_out. Both use v->work as sjk_hip_attend does. A selection's
+ * scores lie there too: SJKVARN_ERR_CAPACITY where one position's (8 bytes a group and KV head) do not fit. More
+ * staged positions than the ring holds are SJKVARN_ERR_CAPACITY. Views outside the attention kernels: SJK_ERR_UNSUPPORTED. */
+int sjk_hip_select_groups(const sjk_hip_view * v, uint32_t B, uint32_t N, uint32_t qpos0, int n_q, int n_head, const float * d_q,
+                          int top, int32_t * d_sel, void * stream);
+int sjk_hip_attend_groups(const sjk_hip_view * v, uint32_t B, uint32_t N, uint32_t qpos0, int n_q, int n_head, const float * d_q,
+                          float scale, const int32_t * d_sel, int top, int out_type, void * d_out, void * stream);
+
+/* The same with B, N and qpos0 from the device descriptor (SJK_DESC_B, _N, _QPOS0) when the kernels run, on a launch that does not
+ * depend on them: one captured graph takes every step. n_max bounds N. A descriptor that the view cannot hold, or whose
+ * positions do not lie behind the sealed part, gives lists of -1 and NaN rows. */
+int sjk_hip_select_groups_dyn(const sjk_hip_view * v, const int32_t * d_desc, uint32_t n_max, int n_q, int n_head, const float * d_q,
+                              int top, int32_t * d_sel, void * stream);
+int sjk_hip_attend_groups_dyn(const sjk_hip_view * v, const int32_t * d_desc, uint32_t n_max, int n_q, int n_head, const float * d_q,
+                              float scale, const int32_t * d_sel, int top, int out_type, void * d_out, void * stream);
+
+/* n_jobs independent calls with one n_q, n_head and top in as few launches as the kernels take (16 jobs a selection, 8 tiles of 16 query
+ * rows an attention). Views of a selection agree in layout and KV heads. d_out is not used by a selection. */
+typedef struct sjk_hip_groups_job {
+    sjk_hip_view  v;
+    uint32_t      B, N, qpos0;
+    const float * d_q;
+    int32_t     * d_sel;
+    void        * d_out;
+} sjk_hip_groups_job;
+int sjk_hip_select_groups_batch(const sjk_hip_groups_job * jobs, int n_jobs, int n_q, int n_head, int top, void * stream);
+int sjk_hip_attend_groups_batch(const sjk_hip_groups_job * jobs, int n_jobs, int n_q, int n_head, float scale, int top, int out_type,
+                                void * stream);
+
+/* The same for layer il of several sequences: positions pos0 .. pos0 + n_q - 1 of seq, which are stored (pos0 + n_q <= its count). */
+typedef struct sjk_hip_seq_groups_job {
+    sj_kvarn_seq * seq;
+    uint32_t       pos0;
+    const float  * d_q;
+    int32_t      * d_sel;
+    void         * d_out;
+} sjk_hip_seq_groups_job;
+int sjk_hip_seq_select_groups_batch(const sjk_hip_seq_groups_job * jobs, int n_jobs, int il, int n_q, int n_head, int top, void * stream);
+int sjk_hip_seq_attend_groups_batch(const sjk_hip_seq_groups_job * jobs, int n_jobs, int il, int n_q, int n_head, float scale, int top,
+                                    int out_type, void * stream);
+
+/* Attention of drafted nodes. A tree (or any set) of n_nodes drafted tokens is stored behind the context like positions base ..
+ * base + n_nodes - 1 (sjk_hip_store_qkv, whose d_pos turns each node by its depth). Query row i sees positions [0, base) and those nodes j
+ * whose bit is set in d_seen: bit j % 64 of word i * ceil(n_nodes / 64) + j / 64 (uint64, device), its ancestors and itself say;
+ * bits past the nodes are ignored. Rows and nodes need not be the same tokens: n_q rows may be the last level of a tree, and a row may see
+ * no node. Sealed groups are read whole; base is not below the sealed end (B > S: base >= B, SJKVARN_ERR_ARG otherwise). Everything else is as for
+ * sjk_hip_attend_groups; the values of a node reach no row that does not see it, whatever they are. */
+int sjk_hip_attend_tree(const sjk_hip_view * v, uint32_t B, uint32_t base, int n_nodes, int n_q, int n_head, const float * d_q, float scale,
+                        const uint64_t * d_seen, int out_type, void * d_out, void * stream);
+
+/* The same with B and base = d_desc[SJK_DESC_QPOS0] read on the device (SJK_DESC_N is not read); n_max bounds base + n_nodes. */
+int sjk_hip_attend_tree_dyn(const sjk_hip_view * v, const int32_t * d_desc, uint32_t n_max, int n_nodes, int n_q, int n_head,
+                            const float * d_q, float scale, const uint64_t * d_seen, int out_type, void * d_out, void * stream);
+
+typedef struct sjk_hip_tree_job {
+    sjk_hip_view     v;
+    uint32_t         B, base;
+    const uint64_t * d_seen;
+    const float    * d_q;
+    void           * d_out;
+} sjk_hip_tree_job;
+int sjk_hip_attend_tree_batch(const sjk_hip_tree_job * jobs, int n_jobs, int n_nodes, int n_q, int n_head, float scale, int out_type,
+                              void * stream);
+
+/* The same for layer il of several sequences whose nodes are stored (base + n_nodes <= the position count). */
+typedef struct sjk_hip_seq_tree_job {
+    sj_kvarn_seq   * seq;
+    uint32_t         base;
+    const uint64_t * d_seen;
+    const float    * d_q;
+    void           * d_out;
+} sjk_hip_seq_tree_job;
+int sjk_hip_seq_attend_tree_batch(const sjk_hip_seq_tree_job * jobs, int n_jobs, int il, int n_nodes, int n_q, int n_head, float scale,
+                                  int out_type, void * stream);
+
+/* The accepted path becomes the context: in every one of n_layers layers the stored row of node d_path[i] (device, int32) moves to position
+ * base + i, in place, one launch for up to 64 layers. The path ascends; it ends at n_path entries or at the first that is no node
+ * above the entry before it (-1, say), so a launch need not know its length. Rows of the positions behind it stay as they are. The views agree
+ * in heads, staging, sink and capacity. A row that moves from a ring of 6-bit rows into an fp16 sink becomes the fp16 values of what
+ * the ring holds. SJKVARN_ERR_CAPACITY for more staged nodes than the ring has slots. _dyn: base = d_desc[SJK_DESC_QPOS0], a negative
+ * one moves nothing. */
+int sjk_hip_accept(const sjk_hip_view * views, int n_layers, uint32_t base, int n_nodes, const int32_t * d_path, int n_path, void * stream);
+int sjk_hip_accept_dyn(const sjk_hip_view * views, int n_layers, const int32_t * d_desc, int n_nodes, const int32_t * d_path, int n_path,
+                       void * stream);
+
+/* The same for a sequence whose last positions, from base on, are drafted nodes: path is a host array, and the position count becomes
+ * base + n_path (n_path 0: all nodes are dropped). Enqueued on `stream` with no host wait; nothing is cleared. SJKVARN_ERR_ARG for a path
+ * that does not ascend or leaves the nodes, and for base past the count or below the sealed end; SJKVARN_ERR_PENDING while a
+ * state restore of the sequence is in flight. A refused call changes nothing. */
+int sjk_hip_seq_accept(sj_kvarn_seq * s, uint32_t base, const int32_t * path, int n_path, void * stream);
+
 /* ---- pages: from one sequence to another, and from place to place in a pool (no counterpart in the reference, whose
  * sequences own their blocks alone) ----
  *

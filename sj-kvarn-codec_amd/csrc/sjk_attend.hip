@@ -173,6 +173,128 @@ extern "C" int sjk_hip_attend_noalloc(const sjk_hip_view * v, uint32_t B, uint32
     return sjk_hip_attend(&w, B, N, qpos0, n_q, n_head, d_q, scale, d_out, stream);
 }
 
+// ---- attention over listed groups, and of drafted nodes (kernels: sjk_attend3.hip) ----
+
+int sjk::groups_ok(const sjk_hip_view & v, uint32_t B, uint32_t N, uint32_t qpos0, int n_q) {
+    if ((uint64_t) qpos0 + (uint64_t) n_q > 0xFFFFFFFFull) return SJKVARN_ERR_ARG;
+    if (B <= v.S) return 0;
+    if ((B - v.S) % 128u || N < B || qpos0 + 1u < B) return refuse("query positions before the sealed end, or a sealed end inside a group or past N");
+    return v.body ? 0 : SJKVARN_ERR_ARG;
+}
+
+// what both kinds ask of a call; end: the positions before it are read as far as the ring's or the sink's
+static int ext_ok(const char * who, const sjk_hip_view & v, uint32_t B, uint64_t end, int n_q, int n_head, const float * q, int out_type,
+                  const void * out) {
+    if (!q || !out || ((uintptr_t) q & 15u) || n_q <= 0 || n_head <= 0 || v.n_head_kv <= 0 || n_head % v.n_head_kv || !v.work ||
+        out_type < SJK_F32 || out_type > SJK_BF16 || ((uintptr_t) out & (out_type == SJK_F32 ? 3u : 1u)))
+        return SJKVARN_ERR_ARG;
+    if (!sjk_attend3_supported(&v)) return unsupported(who);
+    if ((int64_t) n_q * n_head > 0x7fffffff || v.n_head_kv > n_cus()) return SJKVARN_ERR_ARG;
+    const uint64_t row = (uint64_t) n_q * (uint64_t) n_head * (uint64_t) v.lay.D;
+    const uintptr_t q0 = (uintptr_t) q, o0 = (uintptr_t) out;
+    if (q0 < o0 + row * (out_type == SJK_F32 ? 4u : 2u) && o0 < q0 + row * 4u) return refuse("the output lies over the queries");
+    const uint32_t bend = B < v.S ? v.S : B;
+    if (v.S && end && !v.sink) return SJKVARN_ERR_ARG;
+    if (end > bend) {
+        if (!v.ring || v.cap < 16u) return SJKVARN_ERR_ARG;
+        if (end - bend > v.cap) {
+            set_error("more staged positions than the ring holds");
+            return SJKVARN_ERR_CAPACITY;
+        }
+    }
+    return 0;
+}
+
+static int run_ext(const ExtCall * calls, int n, int n_q, int n_head, float scale, int top, int n_nodes, int out_type, void * stream) {
+    bool one = true;
+    for (int j = 1; j < n; ++j) one = one && same_shape(calls[j].v, calls[0].v);
+    if (one) return sjk_attend_ext(calls, n, n_q, n_head, scale, top, n_nodes, out_type, (hipStream_t) stream);
+    for (int j = 0; j < n; ++j)
+        if (const int rc = sjk_attend_ext(calls + j, 1, n_q, n_head, scale, top, n_nodes, out_type, (hipStream_t) stream)) return rc;
+    return 0;
+}
+
+constexpr int EXT_CALLS = 64;                    // calls handed on at a time
+
+extern "C" int sjk_hip_attend_groups_batch(const sjk_hip_groups_job * jobs, int n_jobs, int n_q, int n_head, float scale, int top,
+                                           int out_type, void * stream) {
+    if (n_jobs < 0 || (n_jobs > 0 && !jobs)) return SJKVARN_ERR_ARG;
+    for (int j = 0; j < n_jobs; ++j) {
+        const sjk_hip_groups_job & J = jobs[j];
+        if (!J.d_sel || ((uintptr_t) J.d_sel & 3u) || top <= 0) return SJKVARN_ERR_ARG;
+        const uint64_t last = (uint64_t) J.qpos0 + (uint64_t) (n_q > 0 ? n_q : 0);
+        if (const int rc = ext_ok("sjk_hip_attend_groups", J.v, J.B, J.N < last ? J.N : last, n_q, n_head, J.d_q, out_type, J.d_out)) return rc;
+        if (const int rc = groups_ok(J.v, J.B, J.N, J.qpos0, n_q)) return rc;
+    }
+    ExtCall c[EXT_CALLS];
+    for (int k0 = 0; k0 < n_jobs; k0 += EXT_CALLS) {
+        const int n = n_jobs - k0 < EXT_CALLS ? n_jobs - k0 : EXT_CALLS;
+        for (int k = 0; k < n; ++k) {
+            const sjk_hip_groups_job & J = jobs[k0 + k];
+            c[k] = ExtCall{J.v, J.B, J.N, J.qpos0, J.d_q, J.d_out, J.d_sel, nullptr};
+        }
+        if (const int rc = run_ext(c, n, n_q, n_head, scale, top, 0, out_type, stream)) return rc;
+    }
+    return 0;
+}
+
+extern "C" int sjk_hip_attend_groups(const sjk_hip_view * v, uint32_t B, uint32_t N, uint32_t qpos0, int n_q, int n_head, const float * d_q,
+                                     float scale, const int32_t * d_sel, int top, int out_type, void * d_out, void * stream) {
+    if (!v) return SJKVARN_ERR_ARG;
+    sjk_hip_groups_job J = {};
+    J.v = *v; J.B = B; J.N = N; J.qpos0 = qpos0; J.d_q = d_q; J.d_sel = (int32_t *) d_sel; J.d_out = d_out;
+    return sjk_hip_attend_groups_batch(&J, 1, n_q, n_head, scale, top, out_type, stream);
+}
+
+extern "C" int sjk_hip_attend_groups_dyn(const sjk_hip_view * v, const int32_t * d_desc, uint32_t n_max, int n_q, int n_head,
+                                         const float * d_q, float scale, const int32_t * d_sel, int top, int out_type, void * d_out,
+                                         void * stream) {
+    if (!v || !d_desc || ((uintptr_t) d_desc & 3u) || !d_sel || ((uintptr_t) d_sel & 3u) || top <= 0) return SJKVARN_ERR_ARG;
+    // the descriptor's place is checked on the device
+    if (const int rc = ext_ok("sjk_hip_attend_groups_dyn", *v, 0, n_max < v->S ? n_max : v->S, n_q, n_head, d_q, out_type, d_out)) return rc;
+    const ExtCall c = {*v, 0, 0, 0, d_q, d_out, d_sel, nullptr};
+    return sjk_attend_ext_dyn(c, d_desc, n_max, n_q, n_head, scale, top, 0, out_type, (hipStream_t) stream);
+}
+
+extern "C" int sjk_hip_attend_tree_batch(const sjk_hip_tree_job * jobs, int n_jobs, int n_nodes, int n_q, int n_head, float scale,
+                                         int out_type, void * stream) {
+    if (n_jobs < 0 || (n_jobs > 0 && !jobs) || n_nodes <= 0) return SJKVARN_ERR_ARG;
+    for (int j = 0; j < n_jobs; ++j) {
+        const sjk_hip_tree_job & J = jobs[j];
+        const uint64_t end = (uint64_t) J.base + (uint64_t) n_nodes;
+        if (!J.d_seen || ((uintptr_t) J.d_seen & 7u) || end + (uint64_t) (n_q > 0 ? n_q : 0) > 0xFFFFFFFFull) return SJKVARN_ERR_ARG;
+        if (const int rc = ext_ok("sjk_hip_attend_tree", J.v, J.B, end, n_q, n_head, J.d_q, out_type, J.d_out)) return rc;
+        if (J.B > J.v.S && (!J.v.body || (J.B - J.v.S) % 128u || J.base < J.B))
+            return refuse("sjk_hip_attend_tree: nodes before the sealed end, or a sealed end inside a group");
+    }
+    ExtCall c[EXT_CALLS];
+    for (int k0 = 0; k0 < n_jobs; k0 += EXT_CALLS) {
+        const int n = n_jobs - k0 < EXT_CALLS ? n_jobs - k0 : EXT_CALLS;
+        for (int k = 0; k < n; ++k) {
+            const sjk_hip_tree_job & J = jobs[k0 + k];
+            c[k] = ExtCall{J.v, J.B, J.base + (uint32_t) n_nodes, J.base, J.d_q, J.d_out, nullptr, J.d_seen};
+        }
+        if (const int rc = run_ext(c, n, n_q, n_head, scale, 0, n_nodes, out_type, stream)) return rc;
+    }
+    return 0;
+}
+
+extern "C" int sjk_hip_attend_tree(const sjk_hip_view * v, uint32_t B, uint32_t base, int n_nodes, int n_q, int n_head, const float * d_q,
+                                   float scale, const uint64_t * d_seen, int out_type, void * d_out, void * stream) {
+    if (!v) return SJKVARN_ERR_ARG;
+    const sjk_hip_tree_job J = {*v, B, base, d_seen, d_q, d_out};
+    return sjk_hip_attend_tree_batch(&J, 1, n_nodes, n_q, n_head, scale, out_type, stream);
+}
+
+extern "C" int sjk_hip_attend_tree_dyn(const sjk_hip_view * v, const int32_t * d_desc, uint32_t n_max, int n_nodes, int n_q, int n_head,
+                                       const float * d_q, float scale, const uint64_t * d_seen, int out_type, void * d_out, void * stream) {
+    if (!v || !d_desc || ((uintptr_t) d_desc & 3u) || n_nodes <= 0 || !d_seen || ((uintptr_t) d_seen & 7u)) return SJKVARN_ERR_ARG;
+    if ((uint64_t) n_max + (uint64_t) (n_q > 0 ? n_q : 0) > 0xFFFFFFFFull) return SJKVARN_ERR_ARG;
+    if (const int rc = ext_ok("sjk_hip_attend_tree_dyn", *v, 0, n_max < v->S ? n_max : v->S, n_q, n_head, d_q, out_type, d_out)) return rc;
+    const ExtCall c = {*v, 0, 0, 0, d_q, d_out, nullptr, d_seen};
+    return sjk_attend_ext_dyn(c, d_desc, n_max, n_q, n_head, scale, 0, n_nodes, out_type, (hipStream_t) stream);
+}
+
 namespace sjk {
 // K and V rows of positions pos0 .. pos0+n_pos-1 of KV head h (the region resolver on its own)
 __global__ void kv_rows_kernel(sjk_hip_view v, uint32_t B, uint32_t pos0, uint32_t n_pos, int h, float * out_k,

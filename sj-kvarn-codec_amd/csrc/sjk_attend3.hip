@@ -108,11 +108,58 @@ struct A3Args {
     int rec_a, rec_b;             // 4/4 kernel: records per wavefront (rec_b unused)
 };
 
+// A job of the calls with a list of groups or a mask of drafted nodes (sjk_hip_attend_groups, sjk_hip_attend_tree). Their kernels
+// are the instances of the templates below on this type; the others' code does not know it. Every query position sees every
+// sealed group whole, so no record has an edge.
+struct A3Ext : A3Args {
+    const int32_t * sel;          // [H][top] groups of the tile's position, ascending, or null (all groups)
+    const uint64_t * seen;        // [n_q][words] bit j: node j (position base + j) is seen, or null (causal)
+    int top, words, n_nodes;
+    uint32_t n_grp, base;         // sealed groups; first node
+    int out_type;                 // SJK_F32, _F16, _BF16 (out is not a float's otherwise)
+};
+template <typename Args> constexpr bool is_ext = std::is_same<Args, A3Ext>::value;
+
+// The group of entry c of KV head h's records, or -1 for an entry that names none: outside the sealed part, or not above the
+// entry before it (in an ascending list no group counts twice).
+SJK_DEV int ext_group(const A3Ext & a, int h, int c) {
+    if (!a.sel) return c;
+    const int32_t * s = a.sel + (size_t) h * a.top;
+    const int g = __builtin_amdgcn_readfirstlane(s[c]), before = c ? __builtin_amdgcn_readfirstlane(s[c - 1]) : -1;
+    return g > before && (uint32_t) g < a.n_grp ? g : -1;
+}
+// The 16 positions from p0 on that row n of the tile sees of the nodes and of what lies before them (a bit each)
+SJK_DEV uint32_t ext_seen(const A3Ext & a, int n, uint32_t p0) {
+    if (p0 + 16u <= a.base) return 0xFFFFu;
+    const uint64_t * m = a.seen + (size_t) ((a.row0 + (n < a.n_rows ? n : 0)) / a.gq) * a.words;
+    if (p0 < a.base) {
+        const uint32_t k = a.base - p0;          // 1 .. 15 positions before the first node
+        return ((uint32_t) (m[0] << k) | ((1u << k) - 1u)) & 0xFFFFu;
+    }
+    const uint32_t r = p0 - a.base, i = r >> 6, s = r & 63u;
+    if (i >= (uint32_t) a.words) return 0u;
+    uint64_t x = m[i] >> s;
+    if (s > 48u && i + 1u < (uint32_t) a.words) x |= m[i + 1] << (64u - s);
+    return (uint32_t) x & 0xFFFFu;
+}
+// Two codes c (halves of x, c < 2^b) as the exact fp16 values c - 2^(b - 1): with 0x6400 above them they are 1024 + c. The products
+// of a record's sums then have both signs: with codes 0 .. 2^b - 1 the zero points take back nearly all of a sum over many
+// tokens, and with it the matrix unit's rounding of every product at the sum's own last place (1e-4 of the result at 1,024
+// positions, 5e-6 without).
+SJK_DEV uint32_t middle2(uint32_t x, int b) {
+    typedef _Float16 hf2 __attribute__((ext_vector_type(2)));
+    const _Float16 m = (_Float16) (-1024.0f - (float) (1 << (b - 1)));
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(hf2, x | 0x64006400u) + hf2{m, m});
+}
+// bit 15 / 31: the low / high half is an infinity or a NaN
+SJK_DEV uint32_t nonfinite2(uint32_t w) { return ((w & 0x7FFF7FFFu) + 0x04000400u) & 0x80008000u; }
+
 // Q' operands are read in the QK phase, P' operands in the PV phase of a record, with a barrier between
 // the last QK read and the first P' write, so they share their LDS
 union QPOps {
     uint16_t qb[2][8][4][A3_Q][8];               // Q' hi / lo in B-operand order [hl][k-step][lane group][query][slot]
     u4 pa[4][64];                                // P' A operands (fp16) of the four 32-token k-steps
+    u4 pe[2][4][64];                             // the same as hi and lo parts (A3Ext)
 };
 
 
@@ -842,8 +889,9 @@ __device__ __attribute__((always_inline)) inline void a4_records(const A3Args & 
 // trellis record workgroups
 // ------------------------------------------------------------------------------------------------
 
-template <int BK, int BV, int D, typename Lds>
-__device__ __attribute__((always_inline)) inline void a3_trellis(const A3Args & a, Lds & S, int h, int wgi, int r0, int r1) {
+template <int BK, int BV, int D, typename Args, typename Lds>
+__device__ __attribute__((always_inline)) inline void a3_trellis(const Args & a, Lds & S, int h, int wgi, int r0, int r1) {
+    constexpr bool EXT = is_ext<Args>;
     static_assert(D == 128 || D == 256, "head dimension of the trellis kernel");
     constexpr int CPT = D / 16;                  // channels per Q' builder thread
     constexpr int NJW = D / 64;                  // PV channel tiles per wavefront
@@ -855,8 +903,15 @@ __device__ __attribute__((always_inline)) inline void a3_trellis(const A3Args & 
     // the first record's loads go out before anything else
     constexpr int NV = RL::BYTES / 16, PF = (NV + A3_NT - 1) / A3_NT;
     u4 pf[PF];
+    int held = -1;                               // EXT: the entry whose record is in the registers
     auto fetch = [&](int c) {
-        const uint32_t gi = (a.sink_end + (uint32_t) c * 128u - V.S) / 128u;
+        uint32_t gi = (a.sink_end + (uint32_t) c * 128u - V.S) / 128u;
+        if constexpr (EXT) {
+            const int e = ext_group(a, h, c);
+            if (e < 0) return;
+            gi = (uint32_t) e;
+            held = c;
+        }
         const uint32_t blk = V.blocks ? V.blocks[gi] : gi;
         const u4 * src = (const u4 *) (V.body + ((size_t) blk * H + h) * RL::BYTES);
 #pragma unroll
@@ -938,6 +993,12 @@ __device__ __attribute__((always_inline)) inline void a3_trellis(const A3Args & 
 
 
     for (int c = r0; c < r1; ++c) {
+        if constexpr (EXT) {                     // an entry that names no group; the next one's record is not there yet
+            if (held != c) {
+                if (c + 1 < r1) fetch(c + 1);
+                continue;
+            }
+        }
         prio_by_progress(c - r0, r1 - r0);
         const uint32_t p0 = a.sink_end + (uint32_t) c * 128u;
         __syncthreads();
@@ -996,6 +1057,13 @@ __device__ __attribute__((always_inline)) inline void a3_trellis(const A3Args & 
             acl[0] = f4{0.0f, 0.0f, 0.0f, 0.0f};
             acl[1] = acl[0];
         }
+        f4 tot[2];
+        if constexpr (EXT) {
+            tot[0] = acc[0];
+            tot[1] = acc[1];
+            acc[0] = acl[0];
+            acc[1] = acl[0];
+        }
         // two k-steps (16 channels) at a time: all stream words, then all pair lookups, then the MFMAs, so
         // that each batch waits for LDS twice instead of once per channel
 #pragma unroll
@@ -1029,6 +1097,14 @@ __device__ __attribute__((always_inline)) inline void a3_trellis(const A3Args & 
                 acc[1] = mfma32(A1, Bh, acc[1]);
                 acl[1] = mfma32(A1, Bl, acl[1]);
             }
+            if constexpr (EXT) {                 // as the scalar bodies: 64 channels in sums of their own
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) { tot[tt] = tot[tt] + acc[tt]; acc[tt] = f4{0.0f, 0.0f, 0.0f, 0.0f}; }
+            }
+        }
+        if constexpr (EXT) {
+            acc[0] = tot[0];
+            acc[1] = tot[1];
         }
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) acc[tt] = acc[tt] + acl[tt];
@@ -1042,7 +1118,7 @@ __device__ __attribute__((always_inline)) inline void a3_trellis(const A3Args & 
                 sc[2 * i + 1] = mul_hi(acc[1][i], kt[i]) * a.sc2;
             }
         }
-        if (p0 + 128u > qend_min) {
+        if (!EXT && p0 + 128u > qend_min) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (p0 + (uint32_t) (tok0 + k) >= qend) sc[k] = -__builtin_inff();
@@ -1073,18 +1149,29 @@ __device__ __attribute__((always_inline)) inline void a3_trellis(const A3Args & 
 #pragma unroll
         for (int k = 0; k < 8; ++k) sc[k] = sc[k] * psc;
         {
-            u4 Ah;
+            u4 Ah, Al;
             float cv = 0.0f;
             const u4 vs = *(const u4 *) (s.rec + P::VSC + 2 * tok0);
             const u4 vz = *(const u4 *) (s.rec + P::VZE + 2 * tok0);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                Ah[u] = mul_pk(sc[2 * u], sc[2 * u + 1], vs[u]);
+                if constexpr (EXT) {
+                    const u2 hl = mul_split(sc[2 * u], sc[2 * u + 1], vs[u]);
+                    Ah[u] = hl.x;
+                    Al[u] = hl.y;
+                } else {
+                    Ah[u] = mul_pk(sc[2 * u], sc[2 * u + 1], vs[u]);
+                }
                 cv = fma_lo(sc[2 * u], vz[u], cv);
                 cv = fma_hi(sc[2 * u + 1], vz[u], cv);
             }
             cv = rows_sum(cv);
-            s.op.pa[w][lane] = Ah;
+            if constexpr (EXT) {
+                s.op.pe[0][w][lane] = Ah;
+                s.op.pe[1][w][lane] = Al;
+            } else {
+                s.op.pa[w][lane] = Ah;
+            }
             if (g == 0) s.cvp[w][n] = cv;
         }
         float arow[4];
@@ -1100,9 +1187,12 @@ __device__ __attribute__((always_inline)) inline void a3_trellis(const A3Args & 
 #pragma unroll
         for (int jj = 0; jj < NJW; ++jj) vchw[jj] = *(const uint16_t *) (s.rec + P::VCH + 2 * (16 * (NJW * w + jj) + n));
         __syncthreads();
-        u4 Ah[4];
+        u4 Ah[4], Al[4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) Ah[m] = s.op.pa[m][lane];
+        for (int m = 0; m < 4; ++m) {
+            Ah[m] = EXT ? s.op.pe[0][m][lane] : s.op.pa[m][lane];
+            if (EXT) Al[m] = s.op.pe[1][m][lane];
+        }
         f4 crow;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1125,6 +1215,7 @@ __device__ __attribute__((always_inline)) inline void a3_trellis(const A3Args & 
 #pragma unroll
                 for (int u = 0; u < 4; ++u) Bv[u] = *(const uint32_t *) ((const uint8_t *) s.tv + ((x >> (2 * BV * u)) & VM4));
                 t = mfma32(Ah[m], Bv, t);
+                if constexpr (EXT) t = mfma32(Al[m], Bv, t);
             }
             const float vc = h2f(vchw[jj]) * pinv;
 #pragma unroll
@@ -1174,8 +1265,11 @@ SJK_DEV void tq6_pairs8(const uint8_t * blk, int c8, const u2 * pt, u4 & vh, u4 
 // fin(O, m, l, chan) writes the wavefronts' state as the workgroup's partial (chan(j, n): channel of O tile j,
 // column n).
 // D: head dimension (128 or 256); NB = D / 128 tq6_0 blocks per row, O tiles 8 NB.
-template <int DEPTH, int D, typename Lds, typename Fin>
-__device__ __attribute__((always_inline)) inline void a3_rows(const A3Args & a, Lds & S, int h, int wgr, Fin fin) {
+// A3Ext: the mask of drafted nodes, and a position gives nothing to the rows that do not see it, whatever its values are (a tree's
+// branches do not see each other's rows).
+template <int DEPTH, int D, typename Args, typename Lds, typename Fin>
+__device__ __attribute__((always_inline)) inline void a3_rows(const Args & a, Lds & S, int h, int wgr, Fin fin) {
+    constexpr bool EXT = is_ext<Args>;
     static_assert(D == 128 || D == 256, "head dimension of the row path");
     constexpr int NB = D / 128;
     auto & s = S.w;
@@ -1353,6 +1447,15 @@ __device__ __attribute__((always_inline)) inline void a3_rows(const A3Args & a, 
                 }
             }
             float sc[4];
+            uint32_t see = 0xFu;                 // EXT: the positions p0 + 4 g + i that row n sees
+            if constexpr (EXT) {
+                see = a.seen ? ext_seen(a, n, p0) >> (4 * g) : 0xFu;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t p = p0 + (uint32_t) (4 * g + i);
+                    if (!(p < p1 && p < qend)) see &= ~(1u << i);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = 4 * g + i;
@@ -1365,7 +1468,7 @@ __device__ __attribute__((always_inline)) inline void a3_rows(const A3Args & a, 
                     if (NB == 2) raw += h2f(*(const uint16_t *) (row + SJKVARN_TQ6_BLOCK_BYTES)) * acc[NB - 1][i];
                 }
                 const uint32_t p = p0 + (uint32_t) r;
-                sc[i] = (p < p1 && p < qend) ? raw * r_sc2 : -__builtin_inff();
+                sc[i] = (EXT ? (see >> i & 1u) != 0u : p < p1 && p < qend) ? raw * r_sc2 : -__builtin_inff();
             }
             const float alpha = softmax_update<4>(sc, m_run, l_run);
             float arow[4];
@@ -1390,6 +1493,7 @@ __device__ __attribute__((always_inline)) inline void a3_rows(const A3Args & a, 
                         float nrm = 1.0f;
                         if (!F16) nrm = h2f(*(const uint16_t *) (st + r * RS + VO + b * SJKVARN_TQ6_BLOCK_BYTES));
                         x[e] = sc[2 * pr + e] * nrm;
+                        if (EXT && !F16 && !(see >> (2 * pr + e) & 1u)) x[e] = 0.0f;
                     }
                     const u2 hl = split2(x[0], x[1]);
                     Ph[b][pr] = hl.x;
@@ -1416,6 +1520,35 @@ __device__ __attribute__((always_inline)) inline void a3_rows(const A3Args & a, 
                         vl[k] = u4{0, 0, 0, 0};
                     } else {
                         tq6_pairs8(st + (4 * g + k) * RS + VO + b * SJKVARN_TQ6_BLOCK_BYTES, n, s.pt, vh[k], vl[k]);
+                    }
+                }
+                // fp16 values are shared by the rows of a product: those that are not finite leave it, and are added to the
+                // rows that see them
+                if constexpr (EXT && F16) {
+                    uint32_t nf = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) nf |= nonfinite2(vh[k][u]);
+                    if (__builtin_expect(__any(nf != 0u), 0)) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) vh[k][u] &= ~((nonfinite2(vh[k][u]) >> 15) * 0xFFFFu);
+#pragma unroll 1
+                        for (int t = 0; t < A3_CH && p0 + (uint32_t) t < p1; ++t) {
+                            const float wt = (see >> (t & 3) & 1u) ? ((t & 2) ? ((t & 1) ? sc[3] : sc[2]) : ((t & 1) ? sc[1] : sc[0])) : -1.0f;
+                            const u4 v = *(const __attribute__((address_space(1))) u4 *) (row_of(p0 + (uint32_t) t) + 2 * D + 2 * (128 * b + 8 * n));
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float wi = __shfl(wt, 16 * (t >> 2) + 4 * g + i, 64);
+#pragma unroll
+                                for (int jj = 0; jj < 8; ++jj) {
+                                    const uint32_t x = (v[jj >> 1] >> (16 * (jj & 1))) & 0xFFFFu;
+                                    if (nonfinite2(x) && !(wi < 0.0f)) O[8 * b + jj][i] += wi * h2f(x);
+                                }
+                            }
+                        }
                     }
                 }
 #pragma unroll
@@ -1451,18 +1584,19 @@ __device__ __attribute__((always_inline)) inline void a3_rows(const A3Args & a, 
 // Up to A3_MAXJ calls (jobs: one layer view, its context and query rows each) share one launch; the
 // x workgroups of job j are [wg_base[j], wg_base[j+1]). The jobs sit in the kernel arguments.
 constexpr int A3_MAXJ = 8;
-struct A3Batch {
-    A3Args job[A3_MAXJ];
+template <typename Args> struct A3BatchT {
+    Args job[A3_MAXJ];
     int wg_base[A3_MAXJ + 1];
     int slot_base[A3_MAXJ + 1];  // 4/4 kernel: first CU slot of each job
     int n_jobs;
     int n_slots;                 // 4/4 kernel: CU slots of the launch (one workgroup each)
 };
 
-static_assert(sizeof(A3Batch) <= 4096, "the job table travels in the kernel arguments");
+struct A3Batch : A3BatchT<A3Args> {};
+static_assert(sizeof(A3Batch) <= 4096 && sizeof(A3BatchT<A3Ext>) <= 4096, "the job table travels in the kernel arguments");
 
 // unrolled over the table, so that its loads go out together
-SJK_DEV int a3_job_of(const A3Batch & b, int x) {
+template <typename Args> SJK_DEV int a3_job_of(const A3BatchT<Args> & b, int x) {
     int j = 0;
 #pragma unroll
     for (int k = 1; k < A3_MAXJ; ++k) j += (k < b.n_jobs && x >= b.wg_base[k]) ? 1 : 0;
@@ -1472,7 +1606,7 @@ SJK_DEV int a3_job_of(const A3Batch & b, int x) {
 // per job: workgroups [0, n_row_wg) stream the sink and the tail, the others sealed records (trellis
 // body with BK / BV bits)
 // workgroup wg of job a (KV head blockIdx.y)
-template <int BK, int BV, int D> __device__ __attribute__((always_inline)) inline void attend3_job(const A3Args & a, int wg) {
+template <int BK, int BV, int D, typename Args> __device__ __attribute__((always_inline)) inline void attend3_job(const Args & a, int wg) {
     __shared__ A3LdsT<TrLds<BK, BV, D>> s;
     const int h = blockIdx.y;
     if (wg >= a.n_wg) return;                    // a fixed grid (sjk_hip_attend_dyn) may exceed the plan's split
@@ -1501,10 +1635,17 @@ __global__ __launch_bounds__(A3_NT) __attribute__((amdgpu_waves_per_eu(2))) void
 // w, w + 4, ...; every load is issued before any is used (one round trip for up to 64 per wave)
 constexpr int A3_CMB_MAX = 256;
 
+// element `at` of an output of the type: rounded once, to nearest even
+SJK_DEV void store_out(float * out, size_t at, int type, float y) {
+    if (type == SJK_F32) out[at] = y;
+    else if (type == SJK_F16) ((_Float16 *) out)[at] = (_Float16) y;
+    else ((__bf16 *) out)[at] = (__bf16) y;
+}
+
 // Log-sum-exp merge of the partials of one (query row qi, KV head h, channels 64 qt .. 64 qt + 63): wave w takes
 // partials w, w + 4, ...; every load is issued before any is used (one round trip for up to 64 per wave).
 // sm / sl / so: LDS for the four waves' results. Partials of 16 rows x (D + 2) floats.
-template <int D> SJK_DEV void combine_row(const A3Args & a, int h, int qi, int qt, float * sm, float * sl, float * so) {
+template <int D, typename Args> SJK_DEV void combine_row(const Args & a, int h, int qi, int qt, float * sm, float * sl, float * so) {
     constexpr int PS = A3_Q * (D + 2);
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int d = qt * 64 + lane;
@@ -1550,7 +1691,8 @@ template <int D> SJK_DEV void combine_row(const A3Args & a, int h, int qi, int q
             }
         }
         const int r = a.row0 + qi, iq = r / a.gq, hq = h * a.gq + r % a.gq;
-        a.out[((size_t) iq * a.n_head + hq) * D + d] = Ls == 0.0f ? 0.0f : Os / Ls;
+        if constexpr (is_ext<Args>) store_out(a.out, ((size_t) iq * a.n_head + hq) * D + d, a.out_type, Ls == 0.0f ? 0.0f : Os / Ls);
+        else a.out[((size_t) iq * a.n_head + hq) * D + d] = Ls == 0.0f ? 0.0f : Os / Ls;
     }
 }
 
@@ -1636,24 +1778,27 @@ template <int D> constexpr int sc_tts() { return D / 4 + 16; }
 // the largest staged scalar record (4/3 or 3/4: a 4-bit side, a padded 3-bit side, the scale tables)
 template <int D> constexpr int sc_rec_max() { return 64 * D + 128 * (3 * D / 8 + 4) + 6 * D + 768; }
 
-template <int D> struct ScRec {
-    alignas(16) uint8_t rec[sc_rec_max<D>()];    // the staged record: K payload | V payload | scale tables
-    alignas(16) uint16_t tv[SC_NW][32][sc_tts<D>()];    // per wavefront: 32 tokens x its channels of V codes
+// NP: 2 with the P' operands as hi and lo parts (A3Ext); B44: 4/4 records, whose V needs no table
+template <int D, int NP = 1, bool B44 = false> struct ScRec {
+    alignas(16) uint8_t rec[B44 ? RecLay4<D>::BYTES : sc_rec_max<D>()];    // the staged record: K payload | V payload | scale tables
+    alignas(16) uint16_t tv[B44 ? 1 : SC_NW][32][sc_tts<D>()];    // per wavefront: 32 tokens x its channels of V codes
     alignas(16) uint16_t qb[2][D / 32][4][A3_Q][8];      // Q' hi / lo in B-operand order [hl][ks][g][query][slot]
     alignas(16) u4 pa[4][64];                    // P' A operands of the four 32-token k-steps
+    alignas(16) u4 pl[NP == 2 ? 4 : 0][64];
     float corr[SC_NW][A3_Q];
     float wmax[SC_NW][A3_Q];
     float cvp[SC_NW][A3_Q];
     float wl[SC_NW][A3_Q];
 };
-template <int D> struct ScLds {                  // the record path's tables, or the row path's merge area
+template <int D, int NP = 1, bool B44 = false> struct ScLds {                  // the record path's tables, or the row path's merge area
     union {
-        ScRec<D> s;
+        ScRec<D, NP, B44> s;
         f4 merge[SC_NW][D / 16 * 64];
     };
 };
-template <int D> using AScLds = A3LdsT<ScLds<D>, SC_NW>;
-static_assert(sizeof(AScLds<256>) <= 80 * 1024 && sizeof(AScLds<128>) <= 80 * 1024, "LDS of two workgroups per CU");
+template <int D, int NP = 1, bool B44 = false> using AScLds = A3LdsT<ScLds<D, NP, B44>, SC_NW>;
+static_assert(sizeof(AScLds<256>) <= 80 * 1024 && sizeof(AScLds<128>) <= 80 * 1024 && sizeof(AScLds<256, 2>) <= 80 * 1024 &&
+              sizeof(AScLds<256, 2, true>) <= 80 * 1024, "LDS of two workgroups per CU");
 static_assert(sc_rec_max<256>() == 31488 && sc_rec_max<128>() == 16384, "largest staged scalar records");
 
 // where the parts of a scalar record sit once staged (token-major rows padded by one dword; an odd dword count)
@@ -1679,9 +1824,10 @@ SJK_DEV ScStage sc_stage(const sj_kvarn_layout & l) {
     return st;
 }
 
-template <int D>
-__device__ __attribute__((always_inline)) inline void asc_records(const A3Args & a, AScLds<D> & S, int h, int wgi, int r0, int r1) {
+template <int D, bool B44, typename Args, typename Lds>
+__device__ __attribute__((always_inline)) inline void asc_records(const Args & a, Lds & S, int h, int wgi, int r0, int r1) {
     static_assert(D == 128 || D == 256, "head dimension of the scalar-body kernel");
+    constexpr bool EXT = is_ext<Args>;
     constexpr int NKS = D / 32;                  // QK k-steps
     constexpr int NJW = D / 64;                  // PV channel tiles per wavefront
     constexpr int G8W = D / 32;                  // 8-channel groups per wavefront
@@ -1692,16 +1838,23 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
     const sjk_hip_view & V = a.v;
     const sj_kvarn_layout & L = V.lay;
     const int H = V.n_head_kv;
-    const int bk = L.bits_k, bv = L.bits_v;
+    const int bk = B44 ? 4 : L.bits_k, bv = B44 ? 4 : L.bits_v;
     const uint32_t RB = L.bytes;
     const ScStage st = sc_stage(L);
     // the record's bytes, 16 per thread and step (every record is a whole number of 16-byte units, at most
     // 4/3 or 3/4: 112 D + 6 D + 768 bytes); the next record waits in registers while this one is computed
-    constexpr int PF = ((112 * D + 6 * D + 768) / 16 + SC_NT - 1) / SC_NT;
+    constexpr int PF = (((B44 ? 128 : 112) * D + 6 * D + 768) / 16 + SC_NT - 1) / SC_NT;
     const int nv = (int) (RB / 16u);
     u4 pf[PF];
+    int held = -1;                               // EXT: the entry whose record is in the registers
     auto fetch = [&](int c) {
-        const uint32_t gi = (a.sink_end + (uint32_t) c * 128u - V.S) / 128u;
+        uint32_t gi = (a.sink_end + (uint32_t) c * 128u - V.S) / 128u;
+        if constexpr (EXT) {
+            const int e = ext_group(a, h, c);
+            if (e < 0) return;
+            gi = (uint32_t) e;
+            held = c;
+        }
         const uint32_t blk = V.blocks ? V.blocks[gi] : gi;
         const u4 * src = (const u4 *) (V.body + ((size_t) blk * H + h) * RB);
 #pragma unroll
@@ -1760,6 +1913,12 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
     uint16_t (*tvw)[sc_tts<D>()] = s.tv[w];      // this wavefront's V table: 32 tokens x its D / 4 channels
 
     for (int c = r0; c < r1; ++c) {
+        if constexpr (EXT) {                     // an entry that names no group; the next one's record is not there yet
+            if (held != c) {
+                if (c + 1 < r1) fetch(c + 1);
+                continue;
+            }
+        }
         prio_by_progress(c - r0, r1 - r0);
         const uint32_t p0 = a.sink_end + (uint32_t) c * 128u;
         __syncthreads();                         // the previous record's readers are done
@@ -1804,8 +1963,14 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
                 u4 hi, lo;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    corr = fma_lo(qv[e][2 * j], kz2[j], corr);
-                    corr = fma_hi(qv[e][2 * j + 1], kz2[j], corr);
+                    if constexpr (EXT) {         // the zero point of codes around 0
+                        const float mid = (float) (1 << (bk - 1));
+                        corr = __builtin_fmaf(qv[e][2 * j], __builtin_fmaf(mid, h2f(ks2[j] & 0xFFFFu), h2f(kz2[j] & 0xFFFFu)), corr);
+                        corr = __builtin_fmaf(qv[e][2 * j + 1], __builtin_fmaf(mid, h2f(ks2[j] >> 16), h2f(kz2[j] >> 16)), corr);
+                    } else {
+                        corr = fma_lo(qv[e][2 * j], kz2[j], corr);
+                        corr = fma_hi(qv[e][2 * j + 1], kz2[j], corr);
+                    }
                     const u2 hl = mul_split(qv[e][2 * j], qv[e][2 * j + 1], ks2[j]);
                     hi[j] = hl.x;
                     lo[j] = hl.y;
@@ -1821,6 +1986,15 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
         f4 acc[2], acl[2];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) { acc[tt] = f4{0.0f, 0.0f, 0.0f, 0.0f}; acl[tt] = acc[tt]; }
+        // EXT: 64 channels at a time in sums of their own, so that a product is rounded at their last place
+        f4 tot[2] = {acc[0], acc[0]};
+        auto cut = [&](int ks) {
+            if constexpr (EXT)
+                if (ks & 1) {
+#pragma unroll
+                    for (int tt = 0; tt < 2; ++tt) { tot[tt] = tot[tt] + acc[tt]; acc[tt] = f4{0.0f, 0.0f, 0.0f, 0.0f}; }
+                }
+        };
         if (bk == 4) {
             const uint32_t sh = 4u * (uint32_t) ((n >> 3) + 2 * (g & 1));
 #pragma unroll
@@ -1832,10 +2006,11 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
                     const u4 W = *(const u4 *) (s.rec + 4 * (tile * 32 + 4 * (n & 7)));
                     u4 A;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) A[j] = (W[j] >> sh) & 0x000F000Fu;
+                    for (int j = 0; j < 4; ++j) A[j] = EXT ? middle2((W[j] >> sh) & 0x000F000Fu, 4) : (W[j] >> sh) & 0x000F000Fu;
                     acc[tt] = mfma32(A, Bh, acc[tt]);
                     acl[tt] = mfma32(A, Bl, acl[tt]);
                 }
+                cut(ks);
             }
         } else {
             const uint32_t hm = ((1u << (4 * bk)) - 1u) << 16, cm = ((1u << bk) - 1u) * M2;
@@ -1851,11 +2026,16 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
                     const uint32_t y = x ^ (hm & ((x << (16 - 4 * bk)) ^ x));   // a bit-field insert
                     u4 A;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) A[j] = (y >> (bk * j)) & cm;
+                    for (int j = 0; j < 4; ++j) A[j] = EXT ? middle2((y >> (bk * j)) & cm, bk) : (y >> (bk * j)) & cm;
                     acc[tt] = mfma32(A, Bh, acc[tt]);
                     acl[tt] = mfma32(A, Bl, acl[tt]);
                 }
+                cut(ks);
             }
+        }
+        if constexpr (EXT) {
+            acc[0] = tot[0];
+            acc[1] = tot[1];
         }
         // ---- scores (log2 units): S = Ktok * (sum_d Q' c + sum_d Q Kzero) * scale * log2 e; lane (n, g) holds
         // query n, tokens 32w + 16tt + 4g + i ----
@@ -1864,7 +2044,7 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
             float ck = 0.0f;
 #pragma unroll
             for (int k = 0; k < SC_NW; ++k) ck += s.corr[k][n];
-            const float cs = ck * a.sc2, s24 = a.sc2 * 0x1p24f;
+            const float cs = ck * a.sc2, s24 = EXT ? a.sc2 : a.sc2 * 0x1p24f;
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt) {
                 f4 x;
@@ -1877,7 +2057,7 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
                 sc[4 * tt + 3] = mul_hi(x[3], kt.y);
             }
         }
-        if (p0 + 128u > qend_min) {
+        if (!EXT && p0 + 128u > qend_min) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (p0 + (uint32_t) (32 * w + 16 * (e >> 2) + 4 * g + (e & 3)) >= qend) sc[e] = -__builtin_inff();
@@ -1917,13 +2097,29 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
             const int t0 = 32 * w + 16 * tt + 4 * g;
             const u2 vs = *(const u2 *) (ksc + o_vsc + 2 * t0);
             const u2 vz = *(const u2 *) (ksc + o_vze + 2 * t0);
-            const u2 ah = u2{mul_pk(sc[4 * tt], sc[4 * tt + 1], vs.x), mul_pk(sc[4 * tt + 2], sc[4 * tt + 3], vs.y)};
-            cv = fma_lo(sc[4 * tt], vz.x, cv);
-            cv = fma_hi(sc[4 * tt + 1], vz.x, cv);
-            cv = fma_lo(sc[4 * tt + 2], vz.y, cv);
-            cv = fma_hi(sc[4 * tt + 3], vz.y, cv);
+            u2 ah, al;
+            if constexpr (EXT) {
+                const u2 x = mul_split(sc[4 * tt], sc[4 * tt + 1], vs.x), y = mul_split(sc[4 * tt + 2], sc[4 * tt + 3], vs.y);
+                ah = u2{x.x, y.x};
+                al = u2{x.y, y.y};
+            } else {
+                ah = u2{mul_pk(sc[4 * tt], sc[4 * tt + 1], vs.x), mul_pk(sc[4 * tt + 2], sc[4 * tt + 3], vs.y)};
+            }
+            if constexpr (EXT) {                 // the zero point of codes around 0: Vzero + 2^(bv - 1) Vscale
+                const float mid = (float) (1 << (bv - 1));
+                cv = __builtin_fmaf(sc[4 * tt], __builtin_fmaf(mid, h2f(vs.x & 0xFFFFu), h2f(vz.x & 0xFFFFu)), cv);
+                cv = __builtin_fmaf(sc[4 * tt + 1], __builtin_fmaf(mid, h2f(vs.x >> 16), h2f(vz.x >> 16)), cv);
+                cv = __builtin_fmaf(sc[4 * tt + 2], __builtin_fmaf(mid, h2f(vs.y & 0xFFFFu), h2f(vz.y & 0xFFFFu)), cv);
+                cv = __builtin_fmaf(sc[4 * tt + 3], __builtin_fmaf(mid, h2f(vs.y >> 16), h2f(vz.y >> 16)), cv);
+            } else {
+                cv = fma_lo(sc[4 * tt], vz.x, cv);
+                cv = fma_hi(sc[4 * tt + 1], vz.x, cv);
+                cv = fma_lo(sc[4 * tt + 2], vz.y, cv);
+                cv = fma_hi(sc[4 * tt + 3], vz.y, cv);
+            }
             // P' A operand of k-step w: tokens 16 tt + 4g + i of it are k-group 2 tt + g / 2, slots 4 (g & 1) + i
             *(u2 *) ((uint8_t *) &s.pa[w][16 * (2 * tt + (g >> 1)) + n] + 8 * (g & 1)) = ah;
+            if constexpr (EXT) *(u2 *) ((uint8_t *) &s.pl[w][16 * (2 * tt + (g >> 1)) + n] + 8 * (g & 1)) = al;
         }
         psum = rows_sum(psum);
         cv = rows_sum(cv);
@@ -1952,7 +2148,7 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
                 float cr = 0.0f;
 #pragma unroll
                 for (int k = 0; k < SC_NW; ++k) cr += s.cvp[k][4 * g + i];
-                cvr[i] = cr * 0x1p-24f;
+                cvr[i] = EXT ? cr : cr * 0x1p-24f;
             }
 #pragma unroll
             for (int jj = 0; jj < NJW; ++jj) t[jj] = cvr;
@@ -1965,6 +2161,8 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
             constexpr int NK = G8W / 2;          // 16-byte table writes per lane and k-step
             for (int ks = 0; ks < 4; ++ks) {
                 const u4 Ap = s.pa[ks][lane];
+                u4 Al;
+                if constexpr (EXT) Al = s.pl[ks][lane];
                 if constexpr (V4) {
                     // fragment order, V side (a = channel, b = token; sj_kvarn.h:807-833): the B operand of lane
                     // (n, g), channel 16 J + n x tokens 8g .. 8g + 7 of the k-step, is words 4 (n & 7) .. +3 of
@@ -1977,8 +2175,9 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
                         const u4 W = *(const u4 *) (s.rec + st.vp + 4 * (tile * 32 + 4 * (n & 7)));
                         u4 Bv;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) Bv[j] = (W[j] >> sh) & 0x000F000Fu;
+                        for (int j = 0; j < 4; ++j) Bv[j] = EXT ? middle2((W[j] >> sh) & 0x000F000Fu, 4) : (W[j] >> sh) & 0x000F000Fu;
                         t[jj] = mfma32(Ap, Bv, t[jj]);
+                        if constexpr (EXT) t[jj] = mfma32(Al, Bv, t[jj]);
                     }
                 } else {
                     // token-major: the 8 codes of channel group cg of token tk are the bits 8 cg bv .. + 8 bv of its
@@ -2002,6 +2201,10 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
                         for (int j = 0; j < 4; ++j)
                             pk[j] = __builtin_amdgcn_ubfe(x, (uint32_t) (2 * j * bv), (uint32_t) bv) |
                                     (__builtin_amdgcn_ubfe(x, (uint32_t) ((2 * j + 1) * bv), (uint32_t) bv) << 16);
+                        if constexpr (EXT) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) pk[j] = middle2(pk[j], bv);
+                        }
                         *(u4 *) &tvw[tl][8 * lg] = pk;
                     }
                     // no wait: one wavefront's LDS instructions execute in order, so its transposing reads below see
@@ -2015,18 +2218,20 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
                         const u2 b0 = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_hf4) &tvw[row][col]));
                         const u2 b1 = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_hf4) &tvw[row + 4][col]));
                         t[jj] = mfma32(Ap, u4{b0.x, b0.y, b1.x, b1.y}, t[jj]);
+                        if constexpr (EXT) t[jj] = mfma32(Al, u4{b0.x, b0.y, b1.x, b1.y}, t[jj]);
                     }
                 }
             }
         };
-        if (bv == 4) pv_steps(std::true_type{});
+        if constexpr (B44) pv_steps(std::true_type{});
+        else if (bv == 4) pv_steps(std::true_type{});
         else pv_steps(std::false_type{});
 #pragma unroll
         for (int jj = 0; jj < NJW; ++jj) {
             const int d = 16 * (NJW * w + jj) + n;
             // Vch index v_ch_idx(d) (sj_kvarn.h:843-849) for a fragment-order V, the channel otherwise
             const int vi = bv == 4 ? (d & 7) * (D / 8) + (d >> 4) * 2 + ((d >> 3) & 1) : d;
-            const float vch = h2f(*(const uint16_t *) (ksc + o_vch + 2 * vi)) * pinv * 0x1p24f;
+            const float vch = h2f(*(const uint16_t *) (ksc + o_vch + 2 * vi)) * pinv * (EXT ? 1.0f : 0x1p24f);
 #pragma unroll
             for (int i = 0; i < 4; ++i) O[jj][i] = __builtin_fmaf(vch, t[jj][i], O[jj][i]);
         }
@@ -2051,8 +2256,8 @@ __device__ __attribute__((always_inline)) inline void asc_records(const A3Args &
 
 // workgroup wg of job a (KV head blockIdx.y): row workgroups [0, n_row_wg) stream the sink and the tail, the others
 // rec_per_wg records each
-template <int D> __device__ __attribute__((always_inline)) inline void attendsc_job(const A3Args & a, int wg) {
-    __shared__ AScLds<D> s;
+template <int D, bool B44 = false, typename Args> __device__ __attribute__((always_inline)) inline void attendsc_job(const Args & a, int wg) {
+    __shared__ AScLds<D, is_ext<Args> ? 2 : 1, B44> s;
     const int h = blockIdx.y;
     if (wg >= a.n_wg) return;                    // a fixed grid (sjk_hip_attend_dyn) may exceed the plan's split
     asm volatile("" ::"s"(a.n_row_wg), "s"(a.rec_per_wg), "s"(a.n_rec), "s"(a.sink_end), "s"(a.v.S), "s"(a.v.n_head_kv),
@@ -2071,7 +2276,7 @@ template <int D> __device__ __attribute__((always_inline)) inline void attendsc_
     } else {
         const int r0 = (wg - a.n_row_wg) * a.rec_per_wg;
         const int r1 = r0 + a.rec_per_wg < a.n_rec ? r0 + a.rec_per_wg : a.n_rec;
-        asc_records<D>(a, s, h, wg, r0, r1);
+        asc_records<D, B44>(a, s, h, wg, r0, r1);
     }
 }
 
@@ -2242,7 +2447,7 @@ __host__ __device__ static void a3_split(A3Args & a, double unit, double chunk_c
 // record and row workgroups up, so the proportional unit can ask for a few workgroups more than the two per CU
 // that are resident at once, and those few then run as a second round after the others (at D = 128, 8 KV heads,
 // 100K: 65 workgroups per head for 64 slots took 82 us against 63 us for a split within them).
-__host__ __device__ static double a3_fit_unit(const A3Args * jobs, int n_jobs, double unit, double chunk_cost, int slots) {
+template <typename Args> __host__ __device__ static double a3_fit_unit(const Args * jobs, int n_jobs, double unit, double chunk_cost, int slots) {
     int least = 0;                               // one row and one record workgroup per job at the most
     for (int j = 0; j < n_jobs; ++j) {
         const int k = (jobs[j].n_chunk > 0) + (jobs[j].n_rec > 0);
@@ -2322,9 +2527,10 @@ __host__ __device__ static void a4_split(A3Args & a, int slots) {
 // to aim at), each job split into its workgroups, and the job table's bases; the descriptor path runs the same
 // code on the device, so that both make the same split. SJK_ERR_UNSUPPORTED when a job would have more partials
 // than the combine merges.
-__host__ __device__ static int a3_assign(A3Batch & bt, int body, int H, int slots) {
-    const bool a4 = body == 44;
-    const double cc = a4 ? A4_CHUNK_COST : a3_chunk_cost(body, (int) bt.job[0].v.lay.D);
+// (A3Ext: 4/4 records go through the scalar bodies' kernel, a workgroup a record: a list is short)
+template <typename Args> __host__ __device__ static int a3_assign(A3BatchT<Args> & bt, int body, int H, int slots) {
+    const bool a4 = body == 44 && !is_ext<Args>;
+    const double cc = a4 ? A4_CHUNK_COST : a3_chunk_cost(body == 44 ? 55 : body, (int) bt.job[0].v.lay.D);
     double total = 0.0;
     for (int j = 0; j < bt.n_jobs; ++j) total += bt.job[j].n_rec + cc * bt.job[j].n_chunk;
     double unit = total / slots > 1.0 ? total / slots : 1.0;
@@ -2339,7 +2545,7 @@ __host__ __device__ static int a3_assign(A3Batch & bt, int body, int H, int slot
     bt.wg_base[0] = 0;
     bt.slot_base[0] = 0;
     for (int j = 0; j < bt.n_jobs; ++j) {
-        A3Args & a = bt.job[j];
+        Args & a = bt.job[j];
         if (a4) {
             const int share = total > 0.0 ? (int) ((a.n_rec + cc * a.n_chunk) / total * slots + 1e-6) : 1;
             a4_split(a, share < 1 ? 1 : share);
@@ -2662,3 +2868,255 @@ extern "C" int sjk_hip_attend_dyn(const sjk_hip_view * v, const int32_t * d_desc
     }
     return 0;
 }
+
+// ------------------------------------------------------------------------------------------------
+// attention over listed groups, and of drafted nodes (A3Ext)
+// ------------------------------------------------------------------------------------------------
+//
+// The kernels are the trellis and scalar bodies' own (4/4 records take the scalar one's: a record per workgroup at a time, so that a
+// short list spreads over the device), with the weights P' as hi and lo parts, so that an output keeps the precision of 32 bits.
+// A tile of a list's call is one query position (16 of its heads): each position has a list of its own per KV head.
+
+namespace sjk {
+
+template <int D, bool B44>
+__global__ __launch_bounds__(SC_NT) __attribute__((amdgpu_waves_per_eu(2))) void ext_scalar_kernel(const A3BatchT<A3Ext> b) {
+    const int j = a3_job_of(b, blockIdx.x);
+    attendsc_job<D, B44>(b.job[j], (int) blockIdx.x - b.wg_base[j]);
+}
+template <int D, bool B44>
+__global__ __launch_bounds__(SC_NT) __attribute__((amdgpu_waves_per_eu(2))) void ext_scalar_kernel_dyn(const A3BatchT<A3Ext> * __restrict__ b) {
+    if ((int) blockIdx.x >= b->wg_base[b->n_jobs]) return;
+    const int j = a3_job_of(*b, blockIdx.x);
+    attendsc_job<D, B44>(b->job[j], (int) blockIdx.x - b->wg_base[j]);
+}
+template <int BK, int BV, int D>
+__global__ __launch_bounds__(A3_NT) __attribute__((amdgpu_waves_per_eu(2))) void ext_trellis_kernel(const A3BatchT<A3Ext> b) {
+    const int j = a3_job_of(b, blockIdx.x);
+    attend3_job<BK, BV, D>(b.job[j], (int) blockIdx.x - b.wg_base[j]);
+}
+template <int BK, int BV, int D>
+__global__ __launch_bounds__(A3_NT) __attribute__((amdgpu_waves_per_eu(2))) void ext_trellis_kernel_dyn(const A3BatchT<A3Ext> * __restrict__ b) {
+    if ((int) blockIdx.x >= b->wg_base[b->n_jobs]) return;
+    const int j = a3_job_of(*b, blockIdx.x);
+    attend3_job<BK, BV, D>(b->job[j], (int) blockIdx.x - b->wg_base[j]);
+}
+
+template <int D> __global__ __launch_bounds__(A3_NT) void ext_combine(const A3BatchT<A3Ext> b) {
+    __shared__ float s_M[4], s_L[4], s_O[4][64];
+    constexpr int NQ = D / 64;
+    const A3Ext & a = b.job[blockIdx.z / NQ];
+    if ((int) blockIdx.x >= a.n_rows) return;
+    combine_row<D>(a, blockIdx.y, blockIdx.x, blockIdx.z % NQ, s_M, s_L, &s_O[0][0]);
+}
+
+// What a call is, for its plan on the host or on the device
+struct ExtArgs {
+    ExtCall c;
+    const int32_t * desc;                        // B, N and qpos0 (a tree's first node) from the device, or null
+    uint32_t n_max;
+    int n_q, n_head, top, n_nodes, out_type, body, slots;
+    int tile0, n_tiles;                          // the launch's tiles
+    float scale;
+};
+static_assert(sizeof(ExtArgs) <= 4096 - 64, "the call travels in the kernel arguments");
+
+__host__ __device__ static int ext_tiles(const ExtArgs & e) {
+    const int gq = e.n_head / e.c.v.n_head_kv;
+    return e.c.sel ? e.n_q * ((gq + A3_Q - 1) / A3_Q) : (e.n_q * gq + A3_Q - 1) / A3_Q;
+}
+
+// tile k of the call, before the split
+__host__ __device__ static void ext_plan(const ExtArgs & e, A3Ext & a, int k) {
+    const sjk_hip_view & v = e.c.v;
+    const int gq = e.n_head / v.n_head_kv, rows = e.n_q * gq;
+    int row0 = A3_Q * k, n_rows = rows - row0 < A3_Q ? rows - row0 : A3_Q, pos = 0;
+    if (e.c.sel) {
+        const int per = (gq + A3_Q - 1) / A3_Q, piece = k % per;
+        pos = k / per;
+        row0 = pos * gq + A3_Q * piece;
+        n_rows = gq - A3_Q * piece < A3_Q ? gq - A3_Q * piece : A3_Q;
+    }
+    a = A3Ext{};
+    // every row of a tree's call sees up to N; what it sees of the nodes is the mask's
+    a3_plan(a, &v, e.c.B, e.c.N, e.c.seen ? e.c.N - 1u : e.c.qpos0, e.n_q, e.n_head, e.c.q, e.scale, (float *) e.c.out, row0, n_rows);
+    a.n_grp = (uint32_t) a.n_rec;
+    a.out_type = e.out_type;
+    if (e.c.sel) {
+        a.sel = e.c.sel + (size_t) pos * v.n_head_kv * e.top;
+        a.top = e.top;
+        if (a.n_rec > e.top) a.n_rec = e.top;
+    }
+    if (e.c.seen) {
+        a.seen = e.c.seen;
+        a.n_nodes = e.n_nodes;
+        a.words = (e.n_nodes + 63) / 64;
+        a.base = e.c.N - (uint32_t) e.n_nodes;
+    }
+}
+
+// the descriptor into the call: can the view hold it
+SJK_DEV bool ext_desc(ExtArgs & e) {
+    const int32_t iB = e.desc[SJK_DESC_B], iN = e.desc[SJK_DESC_N], iQ = e.desc[SJK_DESC_QPOS0];
+    const sjk_hip_view & v = e.c.v;
+    const uint64_t last = (uint64_t) (uint32_t) iQ + (uint32_t) (e.c.seen ? e.n_nodes : e.n_q);
+    const uint64_t N = e.c.seen ? last : (uint64_t) (uint32_t) iN;
+    const uint32_t B = (uint32_t) iB, bend = B < v.S ? v.S : B;
+    const uint64_t pend = N < last ? N : last;
+    const bool ok = iB >= 0 && iN >= 0 && iQ >= 0 && N <= e.n_max && (B <= v.S || ((B - v.S) % 128u == 0u && B <= N &&
+                    (uint64_t) (uint32_t) iQ + (e.c.seen ? 0u : 1u) >= B && v.body)) &&
+                    (pend <= bend || (v.ring && v.cap >= 16u && pend - bend <= v.cap));
+    e.c.B = ok ? B : 0u;
+    e.c.N = ok ? (uint32_t) N : 1u;
+    e.c.qpos0 = ok ? (uint32_t) iQ : 0u;
+    return ok;
+}
+
+// The job table of a descriptor's launch, written by one workgroup into the view's workspace (as attend_plan_kernel's)
+__global__ __launch_bounds__(64) void ext_plan_kernel(const ExtArgs e0, float * part, A3BatchT<A3Ext> * plan) {
+    __shared__ A3BatchT<A3Ext> bt;
+    if (threadIdx.x == 0) {
+        ExtArgs e = e0;
+        const bool ok = ext_desc(e);
+        bt.n_jobs = e.n_tiles;
+        size_t used = 0;
+        for (int k = 0; k < e.n_tiles; ++k) {
+            ext_plan(e, bt.job[k], e.tile0 + k);
+            if (!ok) { bt.job[k].n_rec = 0; bt.job[k].n_chunk = 0; bt.job[k].sink_chunks = 0; }
+        }
+        a3_assign(bt, e.body, e.c.v.n_head_kv, e.slots);
+        for (int k = 0; k < e.n_tiles; ++k) {
+            bt.job[k].part = part + used * ws_slot_floats(e.c.v.lay.D);
+            used += (size_t) e.c.v.n_head_kv * (size_t) bt.job[k].n_wg;
+            if (!ok) bt.job[k].n_nodes = -1;     // NaN rows
+        }
+    }
+    __syncthreads();
+    static_assert(sizeof(A3BatchT<A3Ext>) % 4 == 0 && sizeof(A3BatchT<A3Ext>) <= WS_PLAN_BYTES, "the table in its place");
+    const uint32_t * src = (const uint32_t *) &bt;
+    uint32_t * dst = (uint32_t *) plan;
+    for (int i = (int) threadIdx.x; i < (int) (sizeof(bt) / 4); i += 64) dst[i] = src[i];
+}
+
+template <int D> __global__ __launch_bounds__(A3_NT) void ext_combine_dyn(const A3BatchT<A3Ext> * __restrict__ b) {
+    __shared__ float s_M[4], s_L[4], s_O[4][64];
+    constexpr int NQ = D / 64;
+    const int z = (int) blockIdx.z / NQ, cb = (int) blockIdx.z % NQ;
+    const A3Ext & a = b->job[z];
+    if ((int) blockIdx.x >= a.n_rows) return;
+    if (a.n_nodes < 0) {
+        const int r = a.row0 + (int) blockIdx.x;
+        if (threadIdx.x < 64)
+            store_out(a.out, ((size_t) (r / a.gq) * a.n_head + (int) blockIdx.y * a.gq + r % a.gq) * D + 64 * cb + (int) threadIdx.x, a.out_type,
+                      __builtin_nanf(""));
+        return;
+    }
+    combine_row<D>(a, blockIdx.y, blockIdx.x, cb, s_M, s_L, &s_O[0][0]);
+}
+
+// one launch of the body's kernel over `grid`, from a table in the arguments (bt) or in memory (tp)
+static int ext_kernels(int body, int D, dim3 grid, dim3 cgrid, const A3BatchT<A3Ext> * bt, const A3BatchT<A3Ext> * tp, hipStream_t st) {
+#define SJK_EXT(K, KD, NT)                                          \
+    do {                                                            \
+        if (bt) hipLaunchKernelGGL(K, grid, dim3(NT), 0, st, *bt);  \
+        else hipLaunchKernelGGL(KD, grid, dim3(NT), 0, st, tp);     \
+    } while (0)
+    const bool d1 = D == 128;
+    switch (body) {
+    case 44:
+        if (d1) SJK_EXT((ext_scalar_kernel<128, true>), (ext_scalar_kernel_dyn<128, true>), SC_NT);
+        else SJK_EXT((ext_scalar_kernel<256, true>), (ext_scalar_kernel_dyn<256, true>), SC_NT);
+        break;
+    case 55:
+        if (d1) SJK_EXT((ext_scalar_kernel<128, false>), (ext_scalar_kernel_dyn<128, false>), SC_NT);
+        else SJK_EXT((ext_scalar_kernel<256, false>), (ext_scalar_kernel_dyn<256, false>), SC_NT);
+        break;
+    case 33:
+        if (d1) SJK_EXT((ext_trellis_kernel<3, 3, 128>), (ext_trellis_kernel_dyn<3, 3, 128>), A3_NT);
+        else SJK_EXT((ext_trellis_kernel<3, 3, 256>), (ext_trellis_kernel_dyn<3, 3, 256>), A3_NT);
+        break;
+    case 32:
+        if (d1) SJK_EXT((ext_trellis_kernel<3, 2, 128>), (ext_trellis_kernel_dyn<3, 2, 128>), A3_NT);
+        else SJK_EXT((ext_trellis_kernel<3, 2, 256>), (ext_trellis_kernel_dyn<3, 2, 256>), A3_NT);
+        break;
+    case 22:
+        if (d1) SJK_EXT((ext_trellis_kernel<2, 2, 128>), (ext_trellis_kernel_dyn<2, 2, 128>), A3_NT);
+        else SJK_EXT((ext_trellis_kernel<2, 2, 256>), (ext_trellis_kernel_dyn<2, 2, 256>), A3_NT);
+        break;
+    default: return SJK_ERR_UNSUPPORTED;
+    }
+    if (d1) {
+        if (bt) hipLaunchKernelGGL(ext_combine<128>, cgrid, dim3(A3_NT), 0, st, *bt);
+        else hipLaunchKernelGGL(ext_combine_dyn<128>, cgrid, dim3(A3_NT), 0, st, tp);
+    } else {
+        if (bt) hipLaunchKernelGGL(ext_combine<256>, cgrid, dim3(A3_NT), 0, st, *bt);
+        else hipLaunchKernelGGL(ext_combine_dyn<256>, cgrid, dim3(A3_NT), 0, st, tp);
+    }
+#undef SJK_EXT
+    return SJK_CHECK_LAUNCH();
+}
+
+static int ext_launch(A3BatchT<A3Ext> & bt, int body, int H, hipStream_t st) {
+    if (a3_assign(bt, body, H, a3_slots(H))) return SJK_ERR_UNSUPPORTED;
+    void * ws[A3_MAXJ];
+    size_t used[A3_MAXJ];
+    int n_ws = 0;
+    for (int j = 0; j < bt.n_jobs; ++j) {
+        A3Ext & a = bt.job[j];
+        int k = 0;
+        while (k < n_ws && ws[k] != a.v.work) ++k;
+        if (k == n_ws) { ws[n_ws] = a.v.work; used[n_ws] = 0; ++n_ws; }
+        a.part = ws_part(a.v) + used[k] * ws_slot_floats(a.v.lay.D);
+        used[k] += (size_t) H * (size_t) a.n_wg;
+        if (used[k] > ws_part_slots(a.v)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
+    }
+    const int D = bt.job[0].v.lay.D;
+    return ext_kernels(body, D, dim3((unsigned) bt.wg_base[bt.n_jobs], (unsigned) H),
+                       dim3(A3_Q, (unsigned) H, (unsigned) (D / 64 * bt.n_jobs)), &bt, nullptr, st);
+}
+
+int sjk_attend_ext(const ExtCall * calls, int n, int n_q, int n_head, float scale, int top, int n_nodes, int out_type, hipStream_t st) {
+    const int body = a3_body(calls[0].v.lay), H = calls[0].v.n_head_kv;
+    // a workspace smaller than it should be is found before anything is launched
+    for (int j = 0; j < n; ++j)
+        if (ws_part_slots(calls[j].v) < (size_t) ws_slots(H)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
+    A3BatchT<A3Ext> bt = {};
+    for (int j = 0; j < n; ++j) {
+        ExtArgs e = {};
+        e.c = calls[j];
+        e.n_q = n_q; e.n_head = n_head; e.top = top; e.n_nodes = n_nodes; e.out_type = out_type; e.scale = scale;
+        const int nt = ext_tiles(e);
+        for (int k = 0; k < nt; ++k) {
+            ext_plan(e, bt.job[bt.n_jobs++], k);
+            if (bt.n_jobs == A3_MAXJ || (j + 1 == n && k + 1 == nt)) {
+                if (const int rc = ext_launch(bt, body, H, st)) return rc;
+                bt = A3BatchT<A3Ext>{};
+            }
+        }
+    }
+    return 0;
+}
+
+int sjk_attend_ext_dyn(const ExtCall & call, const int32_t * desc, uint32_t n_max, int n_q, int n_head, float scale, int top, int n_nodes,
+                       int out_type, hipStream_t st) {
+    ExtArgs e = {};
+    e.c = call;
+    e.desc = desc; e.n_max = n_max;
+    e.n_q = n_q; e.n_head = n_head; e.top = top; e.n_nodes = n_nodes; e.out_type = out_type; e.scale = scale;
+    const int H = call.v.n_head_kv, D = call.v.lay.D;
+    e.body = a3_body(call.v.lay);
+    e.slots = a3_slots(H);
+    if (ws_part_slots(call.v) < (size_t) ws_slots(H)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
+    const int nt = ext_tiles(e);
+    A3BatchT<A3Ext> * plan = (A3BatchT<A3Ext> *) ws_plan(call.v);
+    for (e.tile0 = 0; e.tile0 < nt; e.tile0 += A3_MAXJ) {
+        e.n_tiles = nt - e.tile0 < A3_MAXJ ? nt - e.tile0 : A3_MAXJ;
+        hipLaunchKernelGGL(ext_plan_kernel, dim3(1), dim3(64), 0, st, e, ws_part(call.v), plan);
+        // the most workgroups per KV head that a table's jobs take: two each for the rounding of its split, 7 for its alignment
+        const dim3 grid((unsigned) (e.slots + 9 * e.n_tiles), (unsigned) H);
+        if (const int rc = ext_kernels(e.body, D, grid, dim3(A3_Q, (unsigned) H, (unsigned) (D / 64 * e.n_tiles)), nullptr, plan, st)) return rc;
+    }
+    return 0;
+}
+
+}  // namespace sjk

@@ -256,6 +256,25 @@ int sjk_prefill(const sjk_hip_view & v, const int32_t * desc, uint32_t n_max, ui
                 int n_q, int n_head, const float * d_q, float scale, float * d_out, hipStream_t st);
 // whether that kernel takes the call: the body, the number of query rows, the buffers
 bool sjk_prefill_takes(const sjk_hip_view & v, int body, int n_q, int n_head, const float * d_q, const float * d_out);
+
+// A call with a list of groups per (position, KV head) (sel) or a mask of drafted nodes (seen: N is the end of the nodes), sjk_attend3.hip;
+// the entry points have checked it. out: of out_type.
+struct ExtCall {
+    sjk_hip_view v;
+    uint32_t B, N, qpos0;
+    const float * q;
+    void * out;
+    const int32_t * sel;
+    const uint64_t * seen;
+};
+int sjk_attend_ext(const ExtCall * calls, int n, int n_q, int n_head, float scale, int top, int n_nodes, int out_type, hipStream_t st);
+int sjk_attend_ext_dyn(const ExtCall & call, const int32_t * desc, uint32_t n_max, int n_q, int n_head, float scale, int top, int n_nodes,
+                       int out_type, hipStream_t st);
+// sjk_hip_accept with the path on the device or on the host (sjk_pages.hip)
+int accept_rows(const sjk_hip_view * views, int n_layers, const int32_t * d_desc, uint32_t base, int n_nodes, const int32_t * d_path,
+                const int32_t * host, int n_path, hipStream_t st);
+// the place of a call over groups: every position behind the sealed part (sjk_attend.hip)
+int groups_ok(const sjk_hip_view & v, uint32_t B, uint32_t N, uint32_t qpos0, int n_q);
 }  // namespace sjk
 
 #define SJK_CHECK_LAUNCH() (hipPeekAtLastError() == hipSuccess ? 0 : SJK_ERR_DEVICE)

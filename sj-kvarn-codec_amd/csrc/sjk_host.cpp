@@ -16,6 +16,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <memory>
 #include <mutex>
 #include <new>
 #include <thread>
@@ -1224,6 +1225,51 @@ int sjk_hip_seq_store_qkv_batch(const sjk_hip_seq_qkv_job * jobs, int n_jobs, in
     return 0;
 }
 
+// ---- listed groups and drafted nodes, for layer il of several sequences ----
+
+// the views' jobs of a sequences' call (null: nothing to do, or rc says why)
+static std::unique_ptr<sjk_hip_groups_job[]> seq_groups_jobs(const sjk_hip_seq_groups_job * jobs, int n_jobs, int il, int n_q, int & rc) {
+    std::unique_ptr<sjk_hip_groups_job[]> out;
+    rc = n_jobs < 0 || (n_jobs > 0 && !jobs) ? SJKVARN_ERR_ARG : 0;
+    if (rc || !n_jobs) return out;
+    out.reset(new (std::nothrow) sjk_hip_groups_job[(size_t) n_jobs]);
+    if (!out) rc = SJKVARN_ERR_NOMEM;
+    for (int k = 0; !rc && k < n_jobs; ++k) {
+        const sjk_hip_seq_groups_job & J = jobs[k];
+        if (!J.seq || il < 0 || il >= J.seq->n_layers || n_q <= 0 || (uint64_t) J.pos0 + (uint64_t) n_q > J.seq->n) rc = SJKVARN_ERR_ARG;
+        else out[k] = sjk_hip_groups_job{sjk_layer_view(&J.seq->layers[il]), J.seq->pol.B, J.seq->n, J.pos0, J.d_q, J.d_sel, J.d_out};
+    }
+    if (rc) out.reset();
+    return out;
+}
+
+int sjk_hip_seq_select_groups_batch(const sjk_hip_seq_groups_job * jobs, int n_jobs, int il, int n_q, int n_head, int top, void * stream) {
+    int rc;
+    const auto g = seq_groups_jobs(jobs, n_jobs, il, n_q, rc);
+    return g ? sjk_hip_select_groups_batch(g.get(), n_jobs, n_q, n_head, top, stream) : rc;
+}
+
+int sjk_hip_seq_attend_groups_batch(const sjk_hip_seq_groups_job * jobs, int n_jobs, int il, int n_q, int n_head, float scale, int top,
+                                    int out_type, void * stream) {
+    int rc;
+    const auto g = seq_groups_jobs(jobs, n_jobs, il, n_q, rc);
+    return g ? sjk_hip_attend_groups_batch(g.get(), n_jobs, n_q, n_head, scale, top, out_type, stream) : rc;
+}
+
+int sjk_hip_seq_attend_tree_batch(const sjk_hip_seq_tree_job * jobs, int n_jobs, int il, int n_nodes, int n_q, int n_head, float scale,
+                                  int out_type, void * stream) {
+    if (n_jobs < 0 || (n_jobs > 0 && !jobs)) return SJKVARN_ERR_ARG;
+    if (!n_jobs) return 0;
+    std::unique_ptr<sjk_hip_tree_job[]> g(new (std::nothrow) sjk_hip_tree_job[(size_t) n_jobs]);
+    if (!g) return SJKVARN_ERR_NOMEM;
+    for (int k = 0; k < n_jobs; ++k) {
+        const sjk_hip_seq_tree_job & J = jobs[k];
+        if (!J.seq || il < 0 || il >= J.seq->n_layers || n_nodes <= 0 || (uint64_t) J.base + (uint64_t) n_nodes > J.seq->n) return SJKVARN_ERR_ARG;
+        g[k] = sjk_hip_tree_job{sjk_layer_view(&J.seq->layers[il]), J.seq->pol.B, J.base, J.d_seen, J.d_q, J.d_out};
+    }
+    return sjk_hip_attend_tree_batch(g.get(), n_jobs, n_nodes, n_q, n_head, scale, out_type, stream);
+}
+
 // ---------------------------------------------------------------------------------------------------
 // sequence state stream (sj_kvarn.h:1811-2034): byte layout of the reference; the device pieces are
 // gathered / scattered on the device and cross to the host in 64 MB chunks
@@ -1793,6 +1839,38 @@ static int same_config(const sj_kvarn_seq * a, const sj_kvarn_seq * b) {
     if (t->staging != c->staging) return SJKVARN_ERR_STAGING;
     if (t->tail != c->tail || t->tail_max != c->tail_max || t->flush_chunk != c->flush_chunk) return SJKVARN_ERR_TAIL;
     if (a->n_layers != b->n_layers) return SJKVARN_ERR_N_LAYERS;
+    return 0;
+}
+
+int sjk_hip_seq_accept(sj_kvarn_seq * s, uint32_t base, const int32_t * path, int n_path, void * stream) {
+    if (!s || !s->layers || n_path < 0 || (n_path > 0 && !path) || base > s->n) return SJKVARN_ERR_ARG;
+    if (s->pol.B > s->cfg.sink && base < s->pol.B) {
+        sjk::set_error("sjk_hip_seq_accept: nodes before the sealed end");
+        return SJKVARN_ERR_ARG;
+    }
+    const uint32_t n_nodes = s->n - base;
+    for (int i = 0; i < n_path; ++i)
+        if (path[i] < 0 || (uint32_t) path[i] >= n_nodes || path[i] > 65535 || (i && path[i] <= path[i - 1])) {
+            sjk::set_error("sjk_hip_seq_accept: the path does not ascend, or leaves the nodes");
+            return SJKVARN_ERR_ARG;
+        }
+    Rt * r = rt_of(s);
+    if (!r) return SJKVARN_ERR_ARG;
+    if (r->job && !r->job->out) {
+        sjk::set_error("sjk_hip_seq_accept: a state restore of the sequence is in flight");
+        return SJKVARN_ERR_PENDING;
+    }
+    int moved = n_path;                          // the entries that stay where they are need no move
+    while (moved > 0 && path[moved - 1] == moved - 1) --moved;
+    if (moved > 0) {
+        std::unique_ptr<sjk_hip_view[]> v(new (std::nothrow) sjk_hip_view[(size_t) s->n_layers]);
+        if (!v) return SJKVARN_ERR_NOMEM;
+        for (int il = 0; il < s->n_layers; ++il) v[il] = sjk_layer_view(&s->layers[il]);
+        const int rc = sjk::accept_rows(v.get(), s->n_layers, nullptr, base, (int) n_nodes, nullptr, path, n_path, (hipStream_t) stream);
+        if (rc) return rc;
+        rt_note_store(r, (hipStream_t) stream);
+    }
+    s->n = base + (uint32_t) n_path;
     return 0;
 }
 

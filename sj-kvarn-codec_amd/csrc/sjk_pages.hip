@@ -1,5 +1,5 @@
-// sjk_pages.hip - pages of a cache from one place to another: the sink and staged rows of a fork (sjk_hip_fork) and
-// record blocks of a pool (sjk_hip_copy_blocks).
+// sjk_pages.hip - pages of a cache from one place to another: the sink and staged rows of a fork (sjk_hip_fork),
+// record blocks of a pool (sjk_hip_copy_blocks), and the rows of accepted drafted tokens (sjk_hip_accept).
 //
 // Both are copies bound by HBM (6.0 TB/s read and written for 574 MB of blocks, where a large plain copy reaches 4.7-5.4).
 // A workgroup takes one tile of one run, each thread TILE_U 16-byte loads in flight before its stores (two or eight of them: 3%
@@ -80,6 +80,137 @@ template <bool STREAM> __global__ __launch_bounds__(256) void copy_blocks_kernel
 static bool stream_past(uint64_t bytes) { return bytes > ((uint64_t) 64 << 20); }
 
 static uint64_t tiles(uint64_t words) { return (words + TILE_WORDS - 1) / TILE_WORDS; }
+
+// ---- accept: rows base + path[i] to positions base + i, in place ----
+//
+// path ascends, so path[i] >= i: a row is never written before those that are copied from it at lower positions have been
+// read, if a workgroup reads ACC_ROWS rows of its columns, waits, writes them and goes on. A call moves little (5 rows of 16 layers
+// of 4 KV heads of 256: 125 KB) and is bound by its launch and two round trips; a column is 16 bytes of one row of one layer.
+constexpr int ACC_LAYERS = 64, ACC_COLS = 16, ACC_U = 4, ACC_ROWS = 256 / ACC_COLS * ACC_U, ACC_PATH = 320;
+struct AcceptBatch {
+    struct { uint8_t * sink, * ring; } layer[ACC_LAYERS];
+    const int32_t * path;                        // device, or null: the list below
+    const int32_t * desc;                        // base from the device descriptor, or null
+    uint32_t base, S, cap, n_nodes, n_path, to;  // rows go to base + to + i
+    uint32_t sink_row, ring_row;                 // bytes of a position's row
+    int D, H, side;                              // (rows of two formats) channels, KV heads, staged bytes of K or V
+    uint16_t list[ACC_PATH];
+};
+static_assert(sizeof(AcceptBatch) <= 4096, "the table travels in the kernel arguments");
+
+SJK_DEV uint8_t * acc_row(const AcceptBatch & b, int il, uint32_t p) {
+    return p < b.S ? b.layer[il].sink + (size_t) p * b.sink_row : b.layer[il].ring + (size_t) ((p - b.S) % b.cap) * b.ring_row;
+}
+SJK_DEV uint32_t acc_node(const AcceptBatch & b, uint32_t i) {
+    return b.path ? (uint32_t) b.path[i] : (uint32_t) b.list[i];
+}
+// the call's first position; false: it moves nothing
+SJK_DEV bool acc_base(const AcceptBatch & b, uint32_t & base) {
+    base = b.base;
+    if (!b.desc) return true;
+    const int32_t q = b.desc[SJK_DESC_QPOS0];
+    base = (uint32_t) q;
+    return q >= 0;
+}
+// entries of the path up to the first that is no node above the one before it
+SJK_DEV uint32_t acc_len(const AcceptBatch & b, uint32_t * s_len) {
+    if (threadIdx.x == 0) *s_len = b.n_path;
+    __syncthreads();
+    uint32_t first = b.n_path;
+    for (uint32_t i = threadIdx.x; i < b.n_path && i < first; i += blockDim.x) {
+        const int64_t x = (int32_t) acc_node(b, i), before = i ? (int64_t) (int32_t) acc_node(b, i - 1) : -1;
+        if (x <= before || x >= (int64_t) b.n_nodes) first = i;
+    }
+    if (first < b.n_path) atomicMin(s_len, first);
+    __syncthreads();
+    return *s_len;
+}
+// rows [from, to) of the path, n words of each, columns of this thread's workgroup: dst and src rows of i by row(i)
+template <typename Src, typename Dst>
+SJK_DEV void acc_move(uint32_t from, uint32_t to, uint32_t words, uint32_t col0, Src src, Dst dst) {
+    const uint32_t w = 4u * (col0 + threadIdx.x % ACC_COLS), r = threadIdx.x / ACC_COLS;
+    const bool in = w < words, whole = w + 4u <= words;
+    for (uint32_t i0 = from; i0 < to; i0 += ACC_ROWS) {
+        uint32_t v[ACC_U][4];
+#pragma unroll
+        for (int u = 0; u < ACC_U; ++u) {
+            const uint32_t i = i0 + u * (256 / ACC_COLS) + r;
+            if (i >= to || !in) continue;
+            const uint32_t * p = (const uint32_t *) src(i) + w;
+            if (whole) {
+                const word4_t x = *(const word4_t *) p;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[u][k] = x[k];
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[u][k] = w + k < words ? p[k] : 0u;
+            }
+        }
+        __syncthreads();                         // every row of this turn has been read
+#pragma unroll
+        for (int u = 0; u < ACC_U; ++u) {
+            const uint32_t i = i0 + u * (256 / ACC_COLS) + r;
+            if (i >= to || !in) continue;
+            uint32_t * p = (uint32_t *) dst(i) + w;
+            if (whole) {
+                *(word4_t *) p = word4_t{v[u][0], v[u][1], v[u][2], v[u][3]};
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (w + k < words) p[k] = v[u][k];
+            }
+        }
+    }
+}
+
+// sink and ring rows of one format, or a path that lies in one of them: grid (columns, layers)
+__global__ __launch_bounds__(256) void accept_kernel(const AcceptBatch b) {
+    __shared__ uint32_t s_len;
+    uint32_t base;
+    if (!acc_base(b, base)) return;
+    const uint32_t len = acc_len(b, &s_len);
+    const int il = (int) blockIdx.y;
+    // (fp16 sink rows and 6-bit ring rows: a descriptor whose nodes lie in the sink is the next kernel's)
+    const uint32_t words = (base < b.S ? b.sink_row : b.ring_row) / 4u;
+    acc_move(0, len, words, blockIdx.x * ACC_COLS, [&](uint32_t i) { return acc_row(b, il, base + acc_node(b, i)); },
+             [&](uint32_t i) { return acc_row(b, il, base + b.to + i); });
+}
+
+// An fp16 sink in front of a ring of 6-bit rows, nodes on both sides of its end: grid (KV heads, layers). Sink rows first, then the
+// ring's rows that go to the sink, as fp16 values of what the ring holds (centroid x norm, one rounding to fp32 and one to
+// fp16), then the rest; a step reads what the one before it does not write.
+__global__ __launch_bounds__(256) void accept_mixed_kernel(const AcceptBatch b) {
+    __shared__ uint32_t s_len, s_ns;
+    uint32_t base;
+    if (!acc_base(b, base)) return;
+    const uint32_t len = acc_len(b, &s_len);
+    const int h = (int) blockIdx.x, il = (int) blockIdx.y;
+    const uint32_t S = b.S, first = base + b.to;
+    if (threadIdx.x == 0) s_ns = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < len; i += 256)
+        if (base + acc_node(b, i) < S) atomicMax(&s_ns, i + 1u);       // nodes ascend: a prefix of the path
+    __syncthreads();
+    const uint32_t ns = s_ns, nd = first >= S ? 0u : S - first < len ? S - first : len;      // destinations in the sink
+    const uint32_t sw = (uint32_t) b.D, rw = (uint32_t) b.side / 2u;       // words of a head's sink and ring rows (K | V)
+    auto sink = [&](uint32_t p) { return b.layer[il].sink + (size_t) p * b.sink_row + (size_t) h * 4u * (size_t) b.D; };
+    auto ring = [&](uint32_t p) { return b.layer[il].ring + (size_t) ((p - S) % b.cap) * b.ring_row + (size_t) h * 2u * (size_t) b.side; };
+    for (uint32_t c = 0; 4u * c < sw; c += ACC_COLS)
+        acc_move(0, ns, sw, c, [&](uint32_t i) { return sink(base + acc_node(b, i)); }, [&](uint32_t i) { return sink(first + i); });
+    __syncthreads();
+    const uint32_t nv = 2u * (uint32_t) b.D;
+    for (uint32_t e = threadIdx.x; e < (nd > ns ? nd - ns : 0u) * nv; e += 256) {
+        const uint32_t i = ns + e / nv, d = e % nv, side = d / (uint32_t) b.D, j = d % (uint32_t) b.D;
+        const uint8_t * blk = ring(base + acc_node(b, i)) + side * (uint32_t) b.side + (j >> 7) * SJKVARN_TQ6_BLOCK_BYTES;
+        const uint32_t k = j & 127u;
+        const int code = ((blk[2 + (k >> 1)] >> (4 * (k & 1))) & 15) | (((blk[66 + (k >> 2)] >> (2 * (k & 3))) & 3) << 4);
+        ((uint16_t *) sink(first + i))[d] = f32_to_f16(xmul(tq6_cent(code), f16_to_f32((uint16_t) (blk[0] | (blk[1] << 8)))));
+    }
+    __syncthreads();
+    const uint32_t from = nd > ns ? nd : ns;
+    for (uint32_t c = 0; 4u * c < rw; c += ACC_COLS)
+        acc_move(from, len, rw, c, [&](uint32_t i) { return ring(base + acc_node(b, i)); }, [&](uint32_t i) { return ring(first + i); });
+}
 
 }  // namespace sjk
 
@@ -198,4 +329,71 @@ extern "C" int sjk_hip_copy_blocks(uint8_t * d_dst, size_t dst_layer_bytes, uint
         if (SJK_CHECK_LAUNCH()) return SJK_ERR_DEVICE;
     }
     return 0;
+}
+
+// The checks of an accept and its launches. host: the path (then d_path is null), in pieces that the arguments hold; a piece's rows go
+// where the ones before it end.
+namespace sjk {
+int accept_rows(const sjk_hip_view * views, int n_layers, const int32_t * d_desc, uint32_t base, int n_nodes, const int32_t * d_path,
+                const int32_t * host, int n_path, hipStream_t st) {
+    if (n_layers < 0 || (n_layers > 0 && !views) || n_nodes < 0 || n_path < 0) return SJKVARN_ERR_ARG;
+    if (!n_layers || !n_path || !n_nodes) return 0;
+    if ((!d_path && !host) || ((uintptr_t) d_path & 3u) || ((uintptr_t) d_desc & 3u)) return SJKVARN_ERR_ARG;
+    const sjk_hip_view & v0 = views[0];
+    if (v0.n_head_kv <= 0 || v0.n_head_kv > 65535 || v0.lay.D <= 0 || (v0.staging != SJKVARN_STAGING_TQ6_0 && v0.staging != SJKVARN_STAGING_F16) ||
+        v0.stage_bytes != sj_kvarn_stage_row_bytes(v0.staging, v0.lay.D) || v0.stage_bytes == 0 ||
+        (v0.sink_type != SJKVARN_SINK_F16 && v0.sink_type != SJKVARN_SINK_INHERIT))
+        return SJKVARN_ERR_ARG;
+    for (int il = 0; il < n_layers; ++il) {
+        const sjk_hip_view & v = views[il];
+        if ((v.S && !v.sink) || (v.cap && !v.ring) || (((uintptr_t) v.sink | (uintptr_t) v.ring) & 3u)) return SJKVARN_ERR_ARG;
+        if (v.lay.D != v0.lay.D || v.n_head_kv != v0.n_head_kv || v.staging != v0.staging || v.sink_type != v0.sink_type ||
+            v.stage_bytes != v0.stage_bytes || v.S != v0.S || v.cap != v0.cap)
+            return refuse("sjk_hip_accept: the views differ in heads, staging, sink or capacity");
+    }
+    const uint64_t end = (uint64_t) base + (uint64_t) n_nodes;
+    if (!d_desc && end > 0xFFFFFFFFull) return SJKVARN_ERR_ARG;
+    // staged nodes have a slot each (a descriptor's nodes may all be staged)
+    const uint64_t staged = d_desc ? (uint64_t) n_nodes : end <= v0.S ? 0 : end - (base > v0.S ? base : v0.S);
+    if (staged > v0.cap) {
+        set_error("sjk_hip_accept: more nodes than the ring holds");
+        return SJKVARN_ERR_CAPACITY;
+    }
+    AcceptBatch b;
+    const uint32_t H = (uint32_t) v0.n_head_kv;
+    b.path = d_path; b.desc = d_desc;
+    b.base = base; b.S = v0.S; b.cap = v0.cap ? v0.cap : 1u; b.n_nodes = (uint32_t) n_nodes;
+    b.D = v0.lay.D; b.H = v0.n_head_kv; b.side = (int) v0.stage_bytes;
+    b.ring_row = H * 2u * (uint32_t) v0.stage_bytes;
+    b.sink_row = v0.sink_type == SJKVARN_SINK_F16 ? H * 4u * (uint32_t) b.D : b.ring_row;
+    const bool mixed = b.sink_row != b.ring_row && v0.S && (d_desc ? true : base < v0.S && end > v0.S);
+    const uint32_t row = b.sink_row > b.ring_row ? b.sink_row : b.ring_row, cols = (row / 4u + 4u * ACC_COLS - 1u) / (4u * ACC_COLS);
+    const int step = d_path ? n_path : ACC_PATH;
+    for (int i0 = 0; i0 < n_path; i0 += step) {
+        const int k = n_path - i0 < step ? n_path - i0 : step;
+        b.n_path = (uint32_t) k;
+        b.to = (uint32_t) i0;
+        for (int i = 0; host && i < k; ++i) b.list[i] = (uint16_t) host[i0 + i];
+        for (int l0 = 0; l0 < n_layers; l0 += ACC_LAYERS) {
+            const int nl = n_layers - l0 < ACC_LAYERS ? n_layers - l0 : ACC_LAYERS;
+            for (int il = 0; il < nl; ++il) { b.layer[il].sink = views[l0 + il].sink; b.layer[il].ring = views[l0 + il].ring; }
+            if (mixed) hipLaunchKernelGGL(accept_mixed_kernel, dim3(H, (unsigned) nl), dim3(256), 0, st, b);
+            else hipLaunchKernelGGL(accept_kernel, dim3(cols, (unsigned) nl), dim3(256), 0, st, b);
+            if (SJK_CHECK_LAUNCH()) return SJK_ERR_DEVICE;
+        }
+    }
+    return 0;
+}
+}  // namespace sjk
+
+extern "C" int sjk_hip_accept(const sjk_hip_view * views, int n_layers, uint32_t base, int n_nodes, const int32_t * d_path, int n_path,
+                              void * stream) {
+    if (n_path > 0 && !d_path) return SJKVARN_ERR_ARG;
+    return accept_rows(views, n_layers, nullptr, base, n_nodes, d_path, nullptr, n_path, (hipStream_t) stream);
+}
+
+extern "C" int sjk_hip_accept_dyn(const sjk_hip_view * views, int n_layers, const int32_t * d_desc, int n_nodes, const int32_t * d_path,
+                                  int n_path, void * stream) {
+    if (!d_desc || (n_path > 0 && !d_path)) return SJKVARN_ERR_ARG;
+    return accept_rows(views, n_layers, d_desc, 0, n_nodes, d_path, nullptr, n_path, (hipStream_t) stream);
 }

@@ -121,6 +121,22 @@ class SeqQkvJob(C.Structure):
                 ("d_q_out", vp)]
 
 
+class GroupsJob(C.Structure):
+    _fields_ = [("v", View), ("B", C.c_uint32), ("N", C.c_uint32), ("qpos0", C.c_uint32), ("d_q", vp), ("d_sel", vp), ("d_out", vp)]
+
+
+class SeqGroupsJob(C.Structure):
+    _fields_ = [("seq", C.POINTER(Seq)), ("pos0", C.c_uint32), ("d_q", vp), ("d_sel", vp), ("d_out", vp)]
+
+
+class TreeJob(C.Structure):
+    _fields_ = [("v", View), ("B", C.c_uint32), ("base", C.c_uint32), ("d_seen", vp), ("d_q", vp), ("d_out", vp)]
+
+
+class SeqTreeJob(C.Structure):
+    _fields_ = [("seq", C.POINTER(Seq)), ("base", C.c_uint32), ("d_seen", vp), ("d_q", vp), ("d_out", vp)]
+
+
 LP, CP, PP, LYP, PLP, SQP = (C.POINTER(Layout), C.POINTER(Config), C.POINTER(Policy), C.POINTER(Layer),
                              C.POINTER(Pool), C.POINTER(Seq))
 
@@ -225,6 +241,27 @@ SIGNATURES = {
     "sjk_hip_store_qkv_dyn": (C.c_int, [C.POINTER(View), vp, C.c_uint32, C.POINTER(Qkv), vp, vp, vp, vp, vp, vp]),
     "sjk_hip_store_qkv_batch": (C.c_int, [C.POINTER(QkvJob), C.c_int, C.c_uint32, C.POINTER(Qkv), vp]),
     "sjk_hip_seq_store_qkv_batch": (C.c_int, [C.POINTER(SeqQkvJob), C.c_int, C.c_int, C.c_uint32, C.POINTER(Qkv), vp]),
+    "sjk_hip_select_groups": (C.c_int, [C.POINTER(View), C.c_uint32, C.c_uint32, C.c_uint32, C.c_int, C.c_int, vp, C.c_int, vp, vp]),
+    "sjk_hip_attend_groups": (C.c_int, [C.POINTER(View), C.c_uint32, C.c_uint32, C.c_uint32, C.c_int, C.c_int, vp, C.c_float, vp,
+                                        C.c_int, C.c_int, vp, vp]),
+    "sjk_hip_select_groups_dyn": (C.c_int, [C.POINTER(View), vp, C.c_uint32, C.c_int, C.c_int, vp, C.c_int, vp, vp]),
+    "sjk_hip_attend_groups_dyn": (C.c_int, [C.POINTER(View), vp, C.c_uint32, C.c_int, C.c_int, vp, C.c_float, vp, C.c_int, C.c_int, vp,
+                                            vp]),
+    "sjk_hip_select_groups_batch": (C.c_int, [C.POINTER(GroupsJob), C.c_int, C.c_int, C.c_int, C.c_int, vp]),
+    "sjk_hip_attend_groups_batch": (C.c_int, [C.POINTER(GroupsJob), C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, C.c_int, vp]),
+    "sjk_hip_seq_select_groups_batch": (C.c_int, [C.POINTER(SeqGroupsJob), C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp]),
+    "sjk_hip_seq_attend_groups_batch": (C.c_int, [C.POINTER(SeqGroupsJob), C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int,
+                                                  C.c_int, vp]),
+    "sjk_hip_attend_tree": (C.c_int, [C.POINTER(View), C.c_uint32, C.c_uint32, C.c_int, C.c_int, C.c_int, vp, C.c_float, vp, C.c_int, vp,
+                                      vp]),
+    "sjk_hip_attend_tree_dyn": (C.c_int, [C.POINTER(View), vp, C.c_uint32, C.c_int, C.c_int, C.c_int, vp, C.c_float, vp, C.c_int, vp,
+                                          vp]),
+    "sjk_hip_attend_tree_batch": (C.c_int, [C.POINTER(TreeJob), C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, vp]),
+    "sjk_hip_seq_attend_tree_batch": (C.c_int, [C.POINTER(SeqTreeJob), C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int,
+                                                vp]),
+    "sjk_hip_accept": (C.c_int, [C.POINTER(View), C.c_int, C.c_uint32, C.c_int, vp, C.c_int, vp]),
+    "sjk_hip_accept_dyn": (C.c_int, [C.POINTER(View), C.c_int, vp, C.c_int, vp, C.c_int, vp]),
+    "sjk_hip_seq_accept": (C.c_int, [SQP, C.c_uint32, C.POINTER(C.c_int32), C.c_int, vp]),
     "sjk_hip_fork": (C.c_int, [C.POINTER(View), C.POINTER(View), C.c_int, C.c_uint32, C.c_uint32, vp]),
     "sjk_hip_copy_blocks": (C.c_int, [vp, C.c_size_t, C.c_uint32, vp, C.c_size_t, C.c_uint32, C.c_int, C.c_size_t, u32p, u32p,
                                       C.c_uint32, vp]),
