@@ -122,10 +122,11 @@ template <typename Args> constexpr bool is_ext = std::is_same<Args, A3Ext>::valu
 
 // The group of entry c of KV head h's records, or -1 for an entry that names none: outside the sealed part, or not above the
 // entry before it (in an ascending list no group counts twice).
+// (Through the constant address space, by scalar loads: a vector load would wait for a stream's loads in flight.)
 SJK_DEV int ext_group(const A3Ext & a, int h, int c) {
     if (!a.sel) return c;
-    const int32_t * s = a.sel + (size_t) h * a.top;
-    const int g = __builtin_amdgcn_readfirstlane(s[c]), before = c ? __builtin_amdgcn_readfirstlane(s[c - 1]) : -1;
+    const __attribute__((address_space(4))) int32_t * s = (const __attribute__((address_space(4))) int32_t *) (a.sel + (size_t) h * a.top);
+    const int g = s[c], before = c ? s[c - 1] : -1;
     return g > before && (uint32_t) g < a.n_grp ? g : -1;
 }
 // The 16 positions from p0 on that row n of the tile sees of the nodes and of what lies before them (a bit each)
@@ -530,8 +531,9 @@ SJK_DEV void lds_reads_done(f4 & x0, f4 & x1, f4 & x2, f4 & x3) {
     asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x0), "+v"(x1), "+v"(x2), "+v"(x3) :: "memory");
 }
 
-template <int D>
-__device__ __attribute__((always_inline)) inline void a4_records(const A3Args & a, A4Lds<D> & S, int h, int wgi, int ls) {
+template <int D, typename Args>
+__device__ __attribute__((always_inline)) inline void a4_records(const Args & a, A4Lds<D> & S, int h, int wgi, int ls) {
+    constexpr bool EXT = is_ext<Args>;
     using GM = A4Geom<D>;
     using RL = typename GM::RL;
     constexpr int NS = GM::NS, CPR = GM::CPR;
@@ -551,7 +553,11 @@ __device__ __attribute__((always_inline)) inline void a4_records(const A3Args & 
     // would have to wait for every load in flight (the compiler cannot order it against the stream)
     const __attribute__((address_space(4))) uint32_t * blocks = (const __attribute__((address_space(4))) uint32_t *) V.blocks;
     auto rec_base = [&](int r) {
-        const uint32_t gi = (a.sink_end + (uint32_t) r * 128u - V.S) / 128u;
+        uint32_t gi = (a.sink_end + (uint32_t) r * 128u - V.S) / 128u;
+        if constexpr (EXT) {                     // an entry that names no group streams group 0, and counts for nothing (live)
+            const int e = ext_group(a, h, r);
+            gi = e < 0 ? 0u : (uint32_t) e;
+        }
         const uint32_t blk = blocks ? blocks[gi] : gi;
         return V.body + ((size_t) blk * H + h) * RL::BYTES;
     };
@@ -632,6 +638,8 @@ __device__ __attribute__((always_inline)) inline void a4_records(const A3Args & 
         const bool last = i + 1 == nrec;
         const uint8_t * rb_after = (i + 2 < nrec) ? rec_base(r0 + i + 2) : nullptr;
         const uint32_t p0 = a.sink_end + (uint32_t) (r0 + i) * 128u;
+        bool live = true;
+        if constexpr (EXT) live = ext_group(a, h, r0 + i) >= 0;
         const int mb = GM::NMETA == 1 ? 0 : (i & 1);              // this record's scale buffer set
         const uint8_t * kmeta = kmeta_of(mb);
         const uint8_t * vmeta = vmeta_of(mb);
@@ -753,7 +761,12 @@ __device__ __attribute__((always_inline)) inline void a4_records(const A3Args & 
             sc[8 * p + 6] = mul_lo(xh[2], kb.y);
             sc[8 * p + 7] = mul_hi(xh[3], kb.y);
         }
-        if (p0 + 128u > qend_min) {
+        if constexpr (EXT) {
+            if (!live) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) sc[e] = -__builtin_inff();
+            }
+        } else if (p0 + 128u > qend_min) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
                 const uint32_t tok = (uint32_t) (32 * (e >> 3) + tbg + (e & 3) + 8 * ((e >> 2) & 1));
@@ -779,6 +792,7 @@ __device__ __attribute__((always_inline)) inline void a4_records(const A3Args & 
         // exp2(s - mk) = P * 2^k; a row with no visible token has only -inf scores, and exp2(-inf - 0) = 0
         const float mk = anyv ? m_new - (float) kx : 0.0f;
         float psum = 0.0f, cv = 0.0f;
+        float lost = 0.0f;                       // EXT: what the rounding of P' took, sum of P Vscale 2^k - P'
         u4 Ah[4];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
@@ -802,12 +816,26 @@ __device__ __attribute__((always_inline)) inline void a4_records(const A3Args & 
             cv = fma_hi(sc[8 * p + 5], vz1.x, cv);
             cv = fma_lo(sc[8 * p + 6], vz1.y, cv);
             cv = fma_hi(sc[8 * p + 7], vz1.y, cv);
+            if constexpr (EXT) {
+                const uint32_t vs[4] = {vs0.x, vs0.y, vs1.x, vs1.y};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    lost = fma_lo(sc[8 * p + 2 * u], vs[u], lost);
+                    lost = fma_hi(sc[8 * p + 2 * u + 1], vs[u], lost);
+                    lost = fma_lo(-1.0f, Ah[p][u], lost);
+                    lost = fma_hi(-1.0f, Ah[p][u], lost);
+                }
+            }
         }
+        // A weight's rounding is multiplied by its token's code, 0 .. 15; with 7.5 of it given back through the zero point the
+        // factor is -7.5 .. 7.5 (3.0e-4 -> 1.3e-4 of a result)
+        if constexpr (EXT) cv = __builtin_fmaf(7.5f, lost, cv);
         lds_reads_done();
         if constexpr (GM::NMETA == 1)
             if (!last) issue_kmeta(rb_next, 0);  // the K scales of this record have been read
         psum = rows_sum(psum);
         cv = rows_sum(cv);
+        if constexpr (EXT) cv = live ? cv : 0.0f;
         m_run = m_new;
         l_run = l_run * alpha + psum * pinv;
         {   // unconditional: behind a branch the compiler kept O in two register sets (128 moves per record)
@@ -861,7 +889,8 @@ __device__ __attribute__((always_inline)) inline void a4_records(const A3Args & 
 #pragma unroll
             for (int jj = 0; jj < 2; ++jj) {
                 const int J = 2 * J2 + jj;
-                const float v0 = h2f(vch[jj] & 0xFFFFu) * pinv * 0x1p24f, v1 = h2f(vch[jj] >> 16) * pinv * 0x1p20f;
+                float v0 = h2f(vch[jj] & 0xFFFFu) * pinv * 0x1p24f, v1 = h2f(vch[jj] >> 16) * pinv * 0x1p20f;
+                if constexpr (EXT) { v0 = live ? v0 : 0.0f; v1 = live ? v1 : 0.0f; }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     O[2 * J][r] = __builtin_fmaf(v0, t[2 * jj][r], O[2 * J][r]);
@@ -1584,10 +1613,12 @@ __device__ __attribute__((always_inline)) inline void a3_rows(const Args & a, Ld
 // Up to A3_MAXJ calls (jobs: one layer view, its context and query rows each) share one launch; the
 // x workgroups of job j are [wg_base[j], wg_base[j+1]). The jobs sit in the kernel arguments.
 constexpr int A3_MAXJ = 8;
+// (A3Ext: 13, what the kernel arguments hold; 8 drafted trees of 12 nodes and more are 24 tiles and more)
+template <typename Args> constexpr int maxj = is_ext<Args> ? 13 : A3_MAXJ;
 template <typename Args> struct A3BatchT {
-    Args job[A3_MAXJ];
-    int wg_base[A3_MAXJ + 1];
-    int slot_base[A3_MAXJ + 1];  // 4/4 kernel: first CU slot of each job
+    Args job[maxj<Args>];
+    int wg_base[maxj<Args> + 1];
+    int slot_base[maxj<Args> + 1];  // 4/4 kernel: first CU slot of each job
     int n_jobs;
     int n_slots;                 // 4/4 kernel: CU slots of the launch (one workgroup each)
 };
@@ -1599,7 +1630,7 @@ static_assert(sizeof(A3Batch) <= 4096 && sizeof(A3BatchT<A3Ext>) <= 4096, "the j
 template <typename Args> SJK_DEV int a3_job_of(const A3BatchT<Args> & b, int x) {
     int j = 0;
 #pragma unroll
-    for (int k = 1; k < A3_MAXJ; ++k) j += (k < b.n_jobs && x >= b.wg_base[k]) ? 1 : 0;
+    for (int k = 1; k < maxj<Args>; ++k) j += (k < b.n_jobs && x >= b.wg_base[k]) ? 1 : 0;
     return __builtin_amdgcn_readfirstlane(j);
 }
 
@@ -1711,7 +1742,7 @@ template <int D> __global__ __launch_bounds__(A3_NT) void attend3_combine(const 
 // CU slot loc of job a. The job must sit in memory the compiler may read again at any time (kernel arguments, or a
 // plan written before the launch), not in registers: a spill would be a vector memory operation inside the
 // streams' hand-counted vmcnt waits.
-template <int D> __device__ __attribute__((always_inline)) inline void attend4_slot(const A3Args & a, int loc) {
+template <int D, typename Args> __device__ __attribute__((always_inline)) inline void attend4_slot(const Args & a, int loc) {
     __shared__ A4Lds<D> s;
     asm volatile("" ::"s"(a.slots), "s"(a.rec_slots), "s"(a.rec_a), "s"(a.n_rec), "s"(a.sink_end), "s"(a.v.S),
                  "s"(a.v.n_head_kv), "s"(a.v.body), "s"(a.v.blocks), "s"(a.n_chunk), "s"(a.sink_chunks), "s"(a.body_end),
@@ -1839,6 +1870,8 @@ __device__ __attribute__((always_inline)) inline void asc_records(const Args & a
     const sj_kvarn_layout & L = V.lay;
     const int H = V.n_head_kv;
     const int bk = B44 ? 4 : L.bits_k, bv = B44 ? 4 : L.bits_v;
+    bool fine = false;                           // EXT: the weights' low parts too
+    if constexpr (EXT) fine = B44 || a.out_type == SJK_F32;
     const uint32_t RB = L.bytes;
     const ScStage st = sc_stage(L);
     // the record's bytes, 16 per thread and step (every record is a whole number of 16-byte units, at most
@@ -2098,7 +2131,7 @@ __device__ __attribute__((always_inline)) inline void asc_records(const Args & a
             const u2 vs = *(const u2 *) (ksc + o_vsc + 2 * t0);
             const u2 vz = *(const u2 *) (ksc + o_vze + 2 * t0);
             u2 ah, al;
-            if constexpr (EXT) {
+            if (EXT && fine) {
                 const u2 x = mul_split(sc[4 * tt], sc[4 * tt + 1], vs.x), y = mul_split(sc[4 * tt + 2], sc[4 * tt + 3], vs.y);
                 ah = u2{x.x, y.x};
                 al = u2{x.y, y.y};
@@ -2119,7 +2152,7 @@ __device__ __attribute__((always_inline)) inline void asc_records(const Args & a
             }
             // P' A operand of k-step w: tokens 16 tt + 4g + i of it are k-group 2 tt + g / 2, slots 4 (g & 1) + i
             *(u2 *) ((uint8_t *) &s.pa[w][16 * (2 * tt + (g >> 1)) + n] + 8 * (g & 1)) = ah;
-            if constexpr (EXT) *(u2 *) ((uint8_t *) &s.pl[w][16 * (2 * tt + (g >> 1)) + n] + 8 * (g & 1)) = al;
+            if (EXT && fine) *(u2 *) ((uint8_t *) &s.pl[w][16 * (2 * tt + (g >> 1)) + n] + 8 * (g & 1)) = al;
         }
         psum = rows_sum(psum);
         cv = rows_sum(cv);
@@ -2156,13 +2189,13 @@ __device__ __attribute__((always_inline)) inline void asc_records(const Args & a
         const int tl = lane & 31;
         // the 4-bit / token-major choice is made once, outside the k-step loop: inside it, the k-steps' LDS reads
         // are issued together instead of one group per branch
-        auto pv_steps = [&](auto v4) {
-            constexpr bool V4 = decltype(v4)::value;
+        auto pv_steps = [&](auto v4, auto low) {
+            constexpr bool V4 = decltype(v4)::value, LOW = decltype(low)::value;
             constexpr int NK = G8W / 2;          // 16-byte table writes per lane and k-step
             for (int ks = 0; ks < 4; ++ks) {
                 const u4 Ap = s.pa[ks][lane];
                 u4 Al;
-                if constexpr (EXT) Al = s.pl[ks][lane];
+                if constexpr (LOW) Al = s.pl[ks][lane];
                 if constexpr (V4) {
                     // fragment order, V side (a = channel, b = token; sj_kvarn.h:807-833): the B operand of lane
                     // (n, g), channel 16 J + n x tokens 8g .. 8g + 7 of the k-step, is words 4 (n & 7) .. +3 of
@@ -2177,7 +2210,7 @@ __device__ __attribute__((always_inline)) inline void asc_records(const Args & a
 #pragma unroll
                         for (int j = 0; j < 4; ++j) Bv[j] = EXT ? middle2((W[j] >> sh) & 0x000F000Fu, 4) : (W[j] >> sh) & 0x000F000Fu;
                         t[jj] = mfma32(Ap, Bv, t[jj]);
-                        if constexpr (EXT) t[jj] = mfma32(Al, Bv, t[jj]);
+                        if constexpr (LOW) t[jj] = mfma32(Al, Bv, t[jj]);
                     }
                 } else {
                     // token-major: the 8 codes of channel group cg of token tk are the bits 8 cg bv .. + 8 bv of its
@@ -2218,14 +2251,25 @@ __device__ __attribute__((always_inline)) inline void asc_records(const Args & a
                         const u2 b0 = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_hf4) &tvw[row][col]));
                         const u2 b1 = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_hf4) &tvw[row + 4][col]));
                         t[jj] = mfma32(Ap, u4{b0.x, b0.y, b1.x, b1.y}, t[jj]);
-                        if constexpr (EXT) t[jj] = mfma32(Al, u4{b0.x, b0.y, b1.x, b1.y}, t[jj]);
+                        if constexpr (LOW) t[jj] = mfma32(Al, u4{b0.x, b0.y, b1.x, b1.y}, t[jj]);
                     }
                 }
             }
         };
-        if constexpr (B44) pv_steps(std::true_type{});
-        else if (bv == 4) pv_steps(std::true_type{});
-        else pv_steps(std::false_type{});
+        if constexpr (B44) {
+            pv_steps(std::true_type{}, std::true_type{});
+        } else if constexpr (EXT) {
+            if (bv == 4) {
+                if (fine) pv_steps(std::true_type{}, std::true_type{});
+                else pv_steps(std::true_type{}, std::false_type{});
+            } else {
+                if (fine) pv_steps(std::false_type{}, std::true_type{});
+                else pv_steps(std::false_type{}, std::false_type{});
+            }
+        } else {
+            if (bv == 4) pv_steps(std::true_type{}, std::false_type{});
+            else pv_steps(std::false_type{}, std::false_type{});
+        }
 #pragma unroll
         for (int jj = 0; jj < NJW; ++jj) {
             const int d = 16 * (NJW * w + jj) + n;
@@ -2523,14 +2567,44 @@ __host__ __device__ static void a4_split(A3Args & a, int slots) {
     a.rec_per_wg = 0;
 }
 
+// The split of a job of listed groups: `share` workgroups of its KV head, a whole number of records for each record workgroup and
+// of chunks for each wavefront of the row workgroups; the split whose longer side is least, the fewest workgroups that reach it.
+// EXT_CHUNK: a wavefront's chunk in records of a workgroup. 0.5 / 0.7 / 0.9 / 1.05 / 1.2: 25.1 / 25.0 / 25.1 / 22.0 / 22.0 us for 64
+// groups and 5.7K staged positions of one sequence (D = 256), 42.1 / 34.1 / 33.7 / 33.7 / 37.8 for 32 groups and 517 of 8 (3/3, D = 128).
+constexpr double EXT_CHUNK = 1.05;
+__host__ __device__ static void ext_split(A3Args & a, int share) {
+    int rec = 0, row = 0, per = 0;
+    if (a.n_rec && a.n_chunk) {
+        if (share < 2) share = 2;
+        double best = 1e30;
+        for (int k = (a.n_rec + share - 2) / (share - 1); k <= a.n_rec; ++k) {
+            const int r = (a.n_rec + k - 1) / k;
+            const int steps = (a.n_chunk + 4 * (share - r) - 1) / (4 * (share - r));
+            const double cost = k > EXT_CHUNK * steps ? k : EXT_CHUNK * steps;
+            if (cost < best - 1e-9) { best = cost; per = k; rec = r; row = (a.n_chunk + 4 * steps - 1) / (4 * steps); }
+            if (k >= best) break;
+        }
+    } else if (a.n_rec) {
+        per = (a.n_rec + share - 1) / share;
+        rec = (a.n_rec + per - 1) / per;
+    } else {
+        row = (a.n_chunk + 3) / 4 < share ? (a.n_chunk + 3) / 4 : share;
+        if (row < 1) row = 1;                        // nothing visible: one empty partial per head
+    }
+    a.rec_per_wg = per > 0 ? per : 1;
+    a.n_row_wg = row;
+    a.n_rec_wg = rec;
+    a.n_wg = row + rec;
+}
+
 // The launch's work shared out over the jobs of bt (slots: 4/4 CU slots per KV head, else workgroups per KV head
 // to aim at), each job split into its workgroups, and the job table's bases; the descriptor path runs the same
 // code on the device, so that both make the same split. SJK_ERR_UNSUPPORTED when a job would have more partials
 // than the combine merges.
-// (A3Ext: 4/4 records go through the scalar bodies' kernel, a workgroup a record: a list is short)
+// (body 45: 4/4 records through the scalar bodies' kernel, see ext_body)
 template <typename Args> __host__ __device__ static int a3_assign(A3BatchT<Args> & bt, int body, int H, int slots) {
-    const bool a4 = body == 44 && !is_ext<Args>;
-    const double cc = a4 ? A4_CHUNK_COST : a3_chunk_cost(body == 44 ? 55 : body, (int) bt.job[0].v.lay.D);
+    const bool a4 = body == 44;
+    const double cc = a4 ? A4_CHUNK_COST : a3_chunk_cost(body == 45 ? 55 : body, (int) bt.job[0].v.lay.D);
     double total = 0.0;
     for (int j = 0; j < bt.n_jobs; ++j) total += bt.job[j].n_rec + cc * bt.job[j].n_chunk;
     double unit = total / slots > 1.0 ? total / slots : 1.0;
@@ -2549,6 +2623,9 @@ template <typename Args> __host__ __device__ static int a3_assign(A3BatchT<Args>
         if (a4) {
             const int share = total > 0.0 ? (int) ((a.n_rec + cc * a.n_chunk) / total * slots + 1e-6) : 1;
             a4_split(a, share < 1 ? 1 : share);
+        } else if constexpr (is_ext<Args>) {
+            const int share = total > 0.0 ? (int) ((a.n_rec + cc * a.n_chunk) / total * slots + 1e-6) : 1;
+            ext_split(a, share < 1 ? 1 : share);
         } else {
             a3_split(a, unit, cc);
         }
@@ -2873,8 +2950,8 @@ extern "C" int sjk_hip_attend_dyn(const sjk_hip_view * v, const int32_t * d_desc
 // attention over listed groups, and of drafted nodes (A3Ext)
 // ------------------------------------------------------------------------------------------------
 //
-// The kernels are the trellis and scalar bodies' own (4/4 records take the scalar one's: a record per workgroup at a time, so that a
-// short list spreads over the device), with the weights P' as hi and lo parts, so that an output keeps the precision of 32 bits.
+// The kernels are the bodies' own; those of the trellis and scalar bodies take the weights P' as hi and lo parts here, so that an
+// output keeps the precision of 32 bits (ext_body: which kernel takes 4/4 records).
 // A tile of a list's call is one query position (16 of its heads): each position has a list of its own per KV head.
 
 namespace sjk {
@@ -2902,6 +2979,26 @@ __global__ __launch_bounds__(A3_NT) __attribute__((amdgpu_waves_per_eu(2))) void
     attend3_job<BK, BV, D>(b->job[j], (int) blockIdx.x - b->wg_base[j]);
 }
 
+template <int D>
+__global__ __launch_bounds__(A4_NT) __attribute__((amdgpu_waves_per_eu(2))) void ext_stream_kernel(const A3BatchT<A3Ext> b) {
+    const int slot = (int) blockIdx.x;
+    int j = 0;
+#pragma unroll
+    for (int k = 1; k < maxj<A3Ext>; ++k) j += (k < b.n_jobs && slot >= b.slot_base[k]) ? 1 : 0;
+    j = __builtin_amdgcn_readfirstlane(j);
+    attend4_slot<D>(b.job[j], slot - b.slot_base[j]);
+}
+template <int D>
+__global__ __launch_bounds__(A4_NT) __attribute__((amdgpu_waves_per_eu(2))) void ext_stream_kernel_dyn(const A3BatchT<A3Ext> * __restrict__ b) {
+    const int slot = (int) blockIdx.x;
+    if (slot >= b->n_slots) return;
+    int j = 0;
+#pragma unroll
+    for (int k = 1; k < maxj<A3Ext>; ++k) j += (k < b->n_jobs && slot >= b->slot_base[k]) ? 1 : 0;
+    j = __builtin_amdgcn_readfirstlane(j);
+    attend4_slot<D>(b->job[j], slot - b->slot_base[j]);
+}
+
 template <int D> __global__ __launch_bounds__(A3_NT) void ext_combine(const A3BatchT<A3Ext> b) {
     __shared__ float s_M[4], s_L[4], s_O[4][64];
     constexpr int NQ = D / 64;
@@ -2924,6 +3021,13 @@ static_assert(sizeof(ExtArgs) <= 4096 - 64, "the call travels in the kernel argu
 __host__ __device__ static int ext_tiles(const ExtArgs & e) {
     const int gq = e.n_head / e.c.v.n_head_kv;
     return e.c.sel ? e.n_q * ((gq + A3_Q - 1) / A3_Q) : (e.n_q * gq + A3_Q - 1) / A3_Q;
+}
+
+// tiles of a launch: the call's in as few launches as there can be, each about as many (16 tiles as 8 and 8, not 13 and 3: 289 against
+// 329 us at 100K)
+static int ext_per_launch(int tiles) {
+    const int launches = (tiles + maxj<A3Ext> - 1) / maxj<A3Ext>;
+    return (tiles + launches - 1) / launches;
 }
 
 // tile k of the call, before the split
@@ -3015,6 +3119,7 @@ template <int D> __global__ __launch_bounds__(A3_NT) void ext_combine_dyn(const 
 }
 
 // one launch of the body's kernel over `grid`, from a table in the arguments (bt) or in memory (tp)
+// (the grid of a body's kernels: x workgroups for each KV head in y, or CU slots of all heads in x)
 static int ext_kernels(int body, int D, dim3 grid, dim3 cgrid, const A3BatchT<A3Ext> * bt, const A3BatchT<A3Ext> * tp, hipStream_t st) {
 #define SJK_EXT(K, KD, NT)                                          \
     do {                                                            \
@@ -3024,6 +3129,10 @@ static int ext_kernels(int body, int D, dim3 grid, dim3 cgrid, const A3BatchT<A3
     const bool d1 = D == 128;
     switch (body) {
     case 44:
+        if (d1) SJK_EXT(ext_stream_kernel<128>, ext_stream_kernel_dyn<128>, A4_NT);
+        else SJK_EXT(ext_stream_kernel<256>, ext_stream_kernel_dyn<256>, A4_NT);
+        break;
+    case 45:
         if (d1) SJK_EXT((ext_scalar_kernel<128, true>), (ext_scalar_kernel_dyn<128, true>), SC_NT);
         else SJK_EXT((ext_scalar_kernel<256, true>), (ext_scalar_kernel_dyn<256, true>), SC_NT);
         break;
@@ -3056,10 +3165,21 @@ static int ext_kernels(int body, int D, dim3 grid, dim3 cgrid, const A3BatchT<A3
     return SJK_CHECK_LAUNCH();
 }
 
+// The kernel of a body: as a3_body, but 4/4 records of a 32-bit output go through the scalar bodies' kernel (45), which keeps the
+// weights' low parts; the streaming wavefronts round them to fp16 once (3e-4 of a result where that one has 4e-7, the rounding
+// of a 16-bit output 2e-4 or 2e-3).
+static int ext_body(const sj_kvarn_layout & l, int out_type) {
+    const int body = a3_body(l);
+    return body == 44 && out_type == SJK_F32 ? 45 : body;
+}
+static int ext_slots(int body, int H) {
+    return body == 44 ? (n_cus() / H > 0 ? n_cus() / H : 1) : a3_slots(H);
+}
+
 static int ext_launch(A3BatchT<A3Ext> & bt, int body, int H, hipStream_t st) {
-    if (a3_assign(bt, body, H, a3_slots(H))) return SJK_ERR_UNSUPPORTED;
-    void * ws[A3_MAXJ];
-    size_t used[A3_MAXJ];
+    if (a3_assign(bt, body, H, ext_slots(body, H))) return SJK_ERR_UNSUPPORTED;
+    void * ws[maxj<A3Ext>];
+    size_t used[maxj<A3Ext>];
     int n_ws = 0;
     for (int j = 0; j < bt.n_jobs; ++j) {
         A3Ext & a = bt.job[j];
@@ -3071,16 +3191,20 @@ static int ext_launch(A3BatchT<A3Ext> & bt, int body, int H, hipStream_t st) {
         if (used[k] > ws_part_slots(a.v)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
     }
     const int D = bt.job[0].v.lay.D;
-    return ext_kernels(body, D, dim3((unsigned) bt.wg_base[bt.n_jobs], (unsigned) H),
+    return ext_kernels(body, D, body == 44 ? dim3((unsigned) bt.n_slots) : dim3((unsigned) bt.wg_base[bt.n_jobs], (unsigned) H),
                        dim3(A3_Q, (unsigned) H, (unsigned) (D / 64 * bt.n_jobs)), &bt, nullptr, st);
 }
 
 int sjk_attend_ext(const ExtCall * calls, int n, int n_q, int n_head, float scale, int top, int n_nodes, int out_type, hipStream_t st) {
-    const int body = a3_body(calls[0].v.lay), H = calls[0].v.n_head_kv;
+    const int body = ext_body(calls[0].v.lay, out_type), H = calls[0].v.n_head_kv;
     // a workspace smaller than it should be is found before anything is launched
     for (int j = 0; j < n; ++j)
         if (ws_part_slots(calls[j].v) < (size_t) ws_slots(H)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
     A3BatchT<A3Ext> bt = {};
+    ExtArgs e0 = {};
+    e0.c = calls[0];
+    e0.n_q = n_q; e0.n_head = n_head;
+    const int per = ext_per_launch(n * ext_tiles(e0));
     for (int j = 0; j < n; ++j) {
         ExtArgs e = {};
         e.c = calls[j];
@@ -3088,7 +3212,7 @@ int sjk_attend_ext(const ExtCall * calls, int n, int n_q, int n_head, float scal
         const int nt = ext_tiles(e);
         for (int k = 0; k < nt; ++k) {
             ext_plan(e, bt.job[bt.n_jobs++], k);
-            if (bt.n_jobs == A3_MAXJ || (j + 1 == n && k + 1 == nt)) {
+            if (bt.n_jobs == per || (j + 1 == n && k + 1 == nt)) {
                 if (const int rc = ext_launch(bt, body, H, st)) return rc;
                 bt = A3BatchT<A3Ext>{};
             }
@@ -3104,16 +3228,17 @@ int sjk_attend_ext_dyn(const ExtCall & call, const int32_t * desc, uint32_t n_ma
     e.desc = desc; e.n_max = n_max;
     e.n_q = n_q; e.n_head = n_head; e.top = top; e.n_nodes = n_nodes; e.out_type = out_type; e.scale = scale;
     const int H = call.v.n_head_kv, D = call.v.lay.D;
-    e.body = a3_body(call.v.lay);
-    e.slots = a3_slots(H);
+    e.body = ext_body(call.v.lay, out_type);
+    e.slots = ext_slots(e.body, H);
     if (ws_part_slots(call.v) < (size_t) ws_slots(H)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
     const int nt = ext_tiles(e);
     A3BatchT<A3Ext> * plan = (A3BatchT<A3Ext> *) ws_plan(call.v);
-    for (e.tile0 = 0; e.tile0 < nt; e.tile0 += A3_MAXJ) {
-        e.n_tiles = nt - e.tile0 < A3_MAXJ ? nt - e.tile0 : A3_MAXJ;
+    const int per = ext_per_launch(nt);
+    for (e.tile0 = 0; e.tile0 < nt; e.tile0 += per) {
+        e.n_tiles = nt - e.tile0 < per ? nt - e.tile0 : per;
         hipLaunchKernelGGL(ext_plan_kernel, dim3(1), dim3(64), 0, st, e, ws_part(call.v), plan);
         // the most workgroups per KV head that a table's jobs take: two each for the rounding of its split, 7 for its alignment
-        const dim3 grid((unsigned) (e.slots + 9 * e.n_tiles), (unsigned) H);
+        const dim3 grid = e.body == 44 ? dim3((unsigned) (H * (e.slots + 2 * e.n_tiles))) : dim3((unsigned) (e.slots + 9 * e.n_tiles), (unsigned) H);
         if (const int rc = ext_kernels(e.body, D, grid, dim3(A3_Q, (unsigned) H, (unsigned) (D / 64 * e.n_tiles)), nullptr, plan, st)) return rc;
     }
     return 0;

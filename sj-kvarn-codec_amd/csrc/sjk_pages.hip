@@ -86,7 +86,7 @@ static uint64_t tiles(uint64_t words) { return (words + TILE_WORDS - 1) / TILE_W
 // path ascends, so path[i] >= i: a row is never written before those that are copied from it at lower positions have been
 // read, if a workgroup reads ACC_ROWS rows of its columns, waits, writes them and goes on. A call moves little (5 rows of 16 layers
 // of 4 KV heads of 256: 125 KB) and is bound by its launch and two round trips; a column is 16 bytes of one row of one layer.
-constexpr int ACC_LAYERS = 64, ACC_COLS = 16, ACC_U = 4, ACC_ROWS = 256 / ACC_COLS * ACC_U, ACC_PATH = 320;
+constexpr int ACC_LAYERS = 160, ACC_COLS = 16, ACC_U = 8, ACC_ROWS = 256 / ACC_COLS * ACC_U, ACC_PATH = 512;
 struct AcceptBatch {
     struct { uint8_t * sink, * ring; } layer[ACC_LAYERS];
     const int32_t * path;                        // device, or null: the list below
@@ -96,14 +96,23 @@ struct AcceptBatch {
     int D, H, side;                              // (rows of two formats) channels, KV heads, staged bytes of K or V
     uint16_t list[ACC_PATH];
 };
+constexpr int ACC_HELD = 1024;                   // path entries that a workgroup holds in LDS
 static_assert(sizeof(AcceptBatch) <= 4096, "the table travels in the kernel arguments");
 
-SJK_DEV uint8_t * acc_row(const AcceptBatch & b, int il, uint32_t p) {
-    return p < b.S ? b.layer[il].sink + (size_t) p * b.sink_row : b.layer[il].ring + (size_t) ((p - b.S) % b.cap) * b.ring_row;
-}
-SJK_DEV uint32_t acc_node(const AcceptBatch & b, uint32_t i) {
-    return b.path ? (uint32_t) b.path[i] : (uint32_t) b.list[i];
-}
+// A workgroup's place in the call: its first position, that position's slot, and the path's first entries in LDS
+struct AccPlace {
+    const AcceptBatch & b;
+    uint32_t base, slot0;
+    const uint32_t * held;
+    __device__ __forceinline__ uint32_t node(uint32_t i) const {
+        return i < (uint32_t) ACC_HELD ? held[i] : b.path ? (uint32_t) b.path[i] : (uint32_t) b.list[i];
+    }
+    // slot of position base + k; k is less than the ring's slots
+    __device__ __forceinline__ uint32_t slot(uint32_t k) const {
+        const uint32_t s = base < b.S ? base + k - b.S : slot0 + k;
+        return s < b.cap ? s : s - b.cap;
+    }
+};
 // the call's first position; false: it moves nothing
 SJK_DEV bool acc_base(const AcceptBatch & b, uint32_t & base) {
     base = b.base;
@@ -113,13 +122,16 @@ SJK_DEV bool acc_base(const AcceptBatch & b, uint32_t & base) {
     return q >= 0;
 }
 // entries of the path up to the first that is no node above the one before it
-SJK_DEV uint32_t acc_len(const AcceptBatch & b, uint32_t * s_len) {
+SJK_DEV uint32_t acc_len(const AcceptBatch & b, uint32_t * held, uint32_t * s_len) {
+    auto entry = [&](uint32_t i) { return b.path ? (uint32_t) b.path[i] : (uint32_t) b.list[i]; };
     if (threadIdx.x == 0) *s_len = b.n_path;
     __syncthreads();
     uint32_t first = b.n_path;
-    for (uint32_t i = threadIdx.x; i < b.n_path && i < first; i += blockDim.x) {
-        const int64_t x = (int32_t) acc_node(b, i), before = i ? (int64_t) (int32_t) acc_node(b, i - 1) : -1;
-        if (x <= before || x >= (int64_t) b.n_nodes) first = i;
+    for (uint32_t i = threadIdx.x; i < b.n_path; i += blockDim.x) {
+        const uint32_t e = entry(i);
+        const int64_t x = (int32_t) e, before = i ? (int64_t) (int32_t) entry(i - 1) : -1;
+        if (i < (uint32_t) ACC_HELD) held[i] = e;
+        if ((x <= before || x >= (int64_t) b.n_nodes) && i < first) first = i;
     }
     if (first < b.n_path) atomicMin(s_len, first);
     __syncthreads();
@@ -165,51 +177,53 @@ SJK_DEV void acc_move(uint32_t from, uint32_t to, uint32_t words, uint32_t col0,
 
 // sink and ring rows of one format, or a path that lies in one of them: grid (columns, layers)
 __global__ __launch_bounds__(256) void accept_kernel(const AcceptBatch b) {
-    __shared__ uint32_t s_len;
+    __shared__ uint32_t s_len, held[ACC_HELD];
     uint32_t base;
     if (!acc_base(b, base)) return;
-    const uint32_t len = acc_len(b, &s_len);
+    const uint32_t len = acc_len(b, held, &s_len);
     const int il = (int) blockIdx.y;
-    // (fp16 sink rows and 6-bit ring rows: a descriptor whose nodes lie in the sink is the next kernel's)
-    const uint32_t words = (base < b.S ? b.sink_row : b.ring_row) / 4u;
-    acc_move(0, len, words, blockIdx.x * ACC_COLS, [&](uint32_t i) { return acc_row(b, il, base + acc_node(b, i)); },
-             [&](uint32_t i) { return acc_row(b, il, base + b.to + i); });
+    const AccPlace P = {b, base, base < b.S ? 0u : (base - b.S) % b.cap, held};
+    uint8_t * sink = b.layer[il].sink, * ring = b.layer[il].ring;
+    auto row = [&](uint32_t k) { return base + k < b.S ? sink + (size_t) (base + k) * b.sink_row : ring + (size_t) P.slot(k) * b.ring_row; };
+    acc_move(0, len, (base < b.S ? b.sink_row : b.ring_row) / 4u, blockIdx.x * ACC_COLS, [&](uint32_t i) { return row(P.node(i)); },
+             [&](uint32_t i) { return row(b.to + i); });
 }
 
 // An fp16 sink in front of a ring of 6-bit rows, nodes on both sides of its end: grid (KV heads, layers). Sink rows first, then the
 // ring's rows that go to the sink, as fp16 values of what the ring holds (centroid x norm, one rounding to fp32 and one to
 // fp16), then the rest; a step reads what the one before it does not write.
 __global__ __launch_bounds__(256) void accept_mixed_kernel(const AcceptBatch b) {
-    __shared__ uint32_t s_len, s_ns;
+    __shared__ uint32_t s_len, s_ns, held[ACC_HELD];
     uint32_t base;
     if (!acc_base(b, base)) return;
-    const uint32_t len = acc_len(b, &s_len);
+    const uint32_t len = acc_len(b, held, &s_len);
     const int h = (int) blockIdx.x, il = (int) blockIdx.y;
+    const AccPlace P = {b, base, base < b.S ? 0u : (base - b.S) % b.cap, held};
     const uint32_t S = b.S, first = base + b.to;
     if (threadIdx.x == 0) s_ns = 0;
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < len; i += 256)
-        if (base + acc_node(b, i) < S) atomicMax(&s_ns, i + 1u);       // nodes ascend: a prefix of the path
+        if (base + P.node(i) < S) atomicMax(&s_ns, i + 1u);            // nodes ascend: a prefix of the path
     __syncthreads();
     const uint32_t ns = s_ns, nd = first >= S ? 0u : S - first < len ? S - first : len;      // destinations in the sink
     const uint32_t sw = (uint32_t) b.D, rw = (uint32_t) b.side / 2u;       // words of a head's sink and ring rows (K | V)
-    auto sink = [&](uint32_t p) { return b.layer[il].sink + (size_t) p * b.sink_row + (size_t) h * 4u * (size_t) b.D; };
-    auto ring = [&](uint32_t p) { return b.layer[il].ring + (size_t) ((p - S) % b.cap) * b.ring_row + (size_t) h * 2u * (size_t) b.side; };
+    auto sink = [&](uint32_t k) { return b.layer[il].sink + (size_t) (base + k) * b.sink_row + (size_t) h * 4u * (size_t) b.D; };
+    auto ring = [&](uint32_t k) { return b.layer[il].ring + (size_t) P.slot(k) * b.ring_row + (size_t) h * 2u * (size_t) b.side; };
     for (uint32_t c = 0; 4u * c < sw; c += ACC_COLS)
-        acc_move(0, ns, sw, c, [&](uint32_t i) { return sink(base + acc_node(b, i)); }, [&](uint32_t i) { return sink(first + i); });
+        acc_move(0, ns, sw, c, [&](uint32_t i) { return sink(P.node(i)); }, [&](uint32_t i) { return sink(b.to + i); });
     __syncthreads();
     const uint32_t nv = 2u * (uint32_t) b.D;
     for (uint32_t e = threadIdx.x; e < (nd > ns ? nd - ns : 0u) * nv; e += 256) {
         const uint32_t i = ns + e / nv, d = e % nv, side = d / (uint32_t) b.D, j = d % (uint32_t) b.D;
-        const uint8_t * blk = ring(base + acc_node(b, i)) + side * (uint32_t) b.side + (j >> 7) * SJKVARN_TQ6_BLOCK_BYTES;
+        const uint8_t * blk = ring(P.node(i)) + side * (uint32_t) b.side + (j >> 7) * SJKVARN_TQ6_BLOCK_BYTES;
         const uint32_t k = j & 127u;
         const int code = ((blk[2 + (k >> 1)] >> (4 * (k & 1))) & 15) | (((blk[66 + (k >> 2)] >> (2 * (k & 3))) & 3) << 4);
-        ((uint16_t *) sink(first + i))[d] = f32_to_f16(xmul(tq6_cent(code), f16_to_f32((uint16_t) (blk[0] | (blk[1] << 8)))));
+        ((uint16_t *) sink(b.to + i))[d] = f32_to_f16(xmul(tq6_cent(code), f16_to_f32((uint16_t) (blk[0] | (blk[1] << 8)))));
     }
     __syncthreads();
     const uint32_t from = nd > ns ? nd : ns;
     for (uint32_t c = 0; 4u * c < rw; c += ACC_COLS)
-        acc_move(from, len, rw, c, [&](uint32_t i) { return ring(base + acc_node(b, i)); }, [&](uint32_t i) { return ring(first + i); });
+        acc_move(from, len, rw, c, [&](uint32_t i) { return ring(P.node(i)); }, [&](uint32_t i) { return ring(b.to + i); });
 }
 
 }  // namespace sjk

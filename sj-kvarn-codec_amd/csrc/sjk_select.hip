@@ -18,7 +18,6 @@ typedef double d4 __attribute__((ext_vector_type(4)));
 constexpr int SEL_MAXJ = 16;
 constexpr int SEL_NT = 256;
 constexpr int SEL_GT = 16;                       // groups of a score tile
-constexpr int PICK_NT = 1024;
 
 struct SelJob {
     const uint8_t * body;
@@ -36,6 +35,7 @@ struct SelArgs {
     int H, n_head, gq, n_q, top, frag;
     int pos0, n_pos;                             // the launch's positions [pos0, pos0 + n_pos) of n_q
     int pb;                                      // positions of a score tile: 16 / gq, at least one
+    int tpw;                                     // score tiles of a workgroup
     double c0, c1;
 };
 static_assert(sizeof(SelArgs) <= 4096, "the jobs travel in the kernel arguments");
@@ -56,38 +56,9 @@ SJK_DEV int k_index(int d, int D, int frag) {
     return frag ? (j & 3) * (D / 4) + (d >> 4) * 4 + (j >> 2) * 2 + (d & 1) : d;
 }
 
-// scores: grid (16-group tiles, KV heads, jobs x position tiles). The wavefronts of a workgroup take a quarter of the channels
-// each (a tile's loads are one round trip); lane (m, k) loads group m's tables at channels 8 k .. 8 k + 7 of every 32, its A operands.
-template <int D>
-__global__ __launch_bounds__(SEL_NT) void score_kernel(const SelArgs a) {
-    constexpr int NC = D / 128;                  // 8-channel loads of a lane per table
-    __shared__ float qs[16][D + 4];              // query rows in the tables' channel order
-    __shared__ double part[4][16][17];
-    __shared__ double bound[16][17];             // [group][row]
-    const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, k = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n_pt = (a.n_pos + a.pb - 1) / a.pb, j = (int) blockIdx.z / n_pt, pt = (int) blockIdx.z % n_pt;
-    const int h = (int) blockIdx.y;
-    const uint32_t n = sel_groups(a, j), g0 = blockIdx.x * SEL_GT;
-    if (g0 >= n) return;
-    const SelJob & J = a.job[j];
-    auto table = [&](uint32_t gi) {              // groups past the end repeat the last one
-        gi = gi < n ? gi : n - 1;
-        const uint32_t blk = J.blocks ? J.blocks[gi] : gi;
-        return J.body + ((size_t) blk * a.H + h) * a.rec_bytes + a.k_scale;
-    };
-    const uint8_t * tb = table(g0 + (uint32_t) m);
-    u4 ks[NC], kz[NC];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const int i = (D / 4) * w + 32 * c + 8 * k;
-        ks[c] = *(const u4 *) (tb + 2 * i);
-        kz[c] = *(const u4 *) (tb + 2 * D + 2 * i);
-    }
-    // thread (group tid / 16, sixteenth of its Ktok)
-    const int gi = tid >> 4, r16 = tid & 15;
-    const u4 kt = *(const u4 *) (table(g0 + (uint32_t) gi) + 4 * D + 16 * r16);
-    float lo = __builtin_inff(), hi = -__builtin_inff(), bad = 0.0f;
+// least and greatest Ktok of a group from the eighths that its 16 lanes (a DPP row) hold; bad: a NaN if one of them is
+SJK_DEV void tok_range(const u4 & kt, float & lo, float & hi, float & bad) {
+    lo = __builtin_inff(); hi = -__builtin_inff(); bad = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const float x = h2f((kt[e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
@@ -95,65 +66,130 @@ __global__ __launch_bounds__(SEL_NT) void score_kernel(const SelArgs a) {
         hi = fmaxf(hi, x);
         if (x != x) bad = x;
     }
+    lo = fminf(lo, dpp<0x128>(lo)); hi = fmaxf(hi, dpp<0x128>(hi)); bad += dpp<0x128>(bad);
+    lo = fminf(lo, dpp<0x124>(lo)); hi = fmaxf(hi, dpp<0x124>(hi)); bad += dpp<0x124>(bad);
+    lo = fminf(lo, dpp<0x122>(lo)); hi = fmaxf(hi, dpp<0x122>(hi)); bad += dpp<0x122>(bad);
+    lo = fminf(lo, dpp<0x121>(lo)); hi = fmaxf(hi, dpp<0x121>(hi)); bad += dpp<0x121>(bad);
+}
+
+// scores: grid (runs of tpw 16-group tiles, KV heads, jobs x position tiles). The wavefronts of a workgroup take a quarter of the
+// channels each; lane (m, k) loads group m's tables at channels 8 k .. 8 k + 7 of every 32, its A operands, a tile ahead.
+template <int D>
+__global__ __launch_bounds__(SEL_NT) __attribute__((amdgpu_waves_per_eu(D == 128 ? 4 : 2))) void score_kernel(const SelArgs a) {
+    constexpr int NC = D / 128;                  // 8-channel loads of a lane per table
+    __shared__ float qs[16][D + 4];              // query rows in the tables' channel order
+    __shared__ double part[2][4][16][17];        // (two tiles' sums: one barrier a tile)
+    __shared__ double bound[16][17];             // [group][row]
+    const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, k = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n_pt = (a.n_pos + a.pb - 1) / a.pb, j = (int) blockIdx.z / n_pt, pt = (int) blockIdx.z % n_pt;
+    const int h = (int) blockIdx.y;
+    const uint32_t n = sel_groups(a, j), first = blockIdx.x * (uint32_t) a.tpw * SEL_GT;
+    if (first >= n) return;
+    const uint32_t end = first + (uint32_t) a.tpw * SEL_GT < n ? first + (uint32_t) a.tpw * SEL_GT : n;
+    const SelJob & J = a.job[j];
+    auto table = [&](uint32_t gi) {              // groups past the end repeat the last one
+        gi = gi < n ? gi : n - 1;
+        const uint32_t blk = J.blocks ? J.blocks[gi] : gi;
+        return J.body + ((size_t) blk * a.H + h) * a.rec_bytes + a.k_scale;
+    };
+    const int gi = tid >> 4, r16 = tid & 15;     // (group, row) of the sums; (group, sixteenth of its Ktok)
+    u4 ks[NC], kz[NC], kt;
+    auto load = [&](uint32_t g0) {
+        const uint8_t * tb = table(g0 + (uint32_t) m);
 #pragma unroll
-    for (int s = 1; s < 16; s <<= 1) {
-        lo = fminf(lo, __shfl_xor(lo, s, 64));
-        hi = fmaxf(hi, __shfl_xor(hi, s, 64));
-        bad += __shfl_xor(bad, s, 64);           // a NaN stays one
-    }
+        for (int c = 0; c < NC; ++c) {
+            const int i = (D / 4) * w + 32 * c + 8 * k;
+            ks[c] = *(const u4 *) (tb + 2 * i);
+            kz[c] = *(const u4 *) (tb + 2 * D + 2 * i);
+        }
+        kt = *(const u4 *) (table(g0 + (uint32_t) gi) + 4 * D + 16 * r16);
+    };
+    load(first);
     // query rows of the tile's positions: 16 at a time (one position of more than 16 heads takes several turns)
     const int p0 = a.pos0 + pt * a.pb, np = a.pos0 + a.n_pos - p0 < a.pb ? a.pos0 + a.n_pos - p0 : a.pb;
     const int rows = np * a.gq;
-    double best = -__builtin_inf();              // thread (group gi, position r16 < np)
-    for (int r0 = 0; r0 < rows; r0 += 16) {
-        __syncthreads();
-        {
-            constexpr int PT = D / 16;
-            const int r = r0 + gi < rows ? r0 + gi : rows - 1;
-            const float * src = J.q + ((size_t) (p0 + r / a.gq) * a.n_head + h * a.gq + r % a.gq) * D + PT * r16;
+    auto stage = [&](int r0) {
+        constexpr int PT = D / 16;
+        const int r = r0 + gi < rows ? r0 + gi : rows - 1;
+        const float * src = J.q + ((size_t) (p0 + r / a.gq) * a.n_head + h * a.gq + r % a.gq) * D + PT * r16;
 #pragma unroll
-            for (int e = 0; e < PT; e += 4) {
-                const float4 x = *(const float4 *) (src + e);
-                const float v[4] = {x.x, x.y, x.z, x.w};
+        for (int e = 0; e < PT; e += 4) {
+            const float4 x = *(const float4 *) (src + e);
+            const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                for (int u = 0; u < 4; ++u) qs[gi][k_index(PT * r16 + e + u, D, a.frag)] = v[u];
-            }
+            for (int u = 0; u < 4; ++u) qs[gi][k_index(PT * r16 + e + u, D, a.frag)] = v[u];
         }
-        __syncthreads();
-        d4 acc = {0.0, 0.0, 0.0, 0.0}, acw = acc;
+    };
+    stage(0);
+    // B operands, of all tiles while a position tile has no more than 16 rows
+    double qd[NC][8], wd[NC][8];
+    auto rows_to_regs = [&]() {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const float * qr = &qs[m][(D / 4) * w + 32 * c + 8 * k];
             const f4 q0 = *(const f4 *) qr, q1 = *(const f4 *) (qr + 4);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const double q = (double) (e < 4 ? q0[e & 3] : q1[e & 3]);
-                const double wq = q > 0.0 ? q * a.c1 : q * a.c0;       // exact: 24 and 11 bits
-                const uint32_t sh = 16 * (e & 1);
-                acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double) h2f((kz[c][e >> 1] >> sh) & 0xFFFFu), q, acc, 0, 0, 0);
-                acw = __builtin_amdgcn_mfma_f64_16x16x4f64((double) h2f((ks[c][e >> 1] >> sh) & 0xFFFFu), wq, acw, 0, 0, 0);
+                qd[c][e] = (double) (e < 4 ? q0[e & 3] : q1[e & 3]);
+                wd[c][e] = qd[c][e] > 0.0 ? qd[c][e] * a.c1 : qd[c][e] * a.c0;       // exact: 24 and 11 bits
             }
         }
-        // lane (row m, k): groups 4 i + k
+    };
+    __syncthreads();
+    rows_to_regs();
+    int turn = 0;
+    for (uint32_t g0 = first; g0 < end; g0 += SEL_GT) {
+        double kzd[NC][8], ksd[NC][8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) part[w][4 * i + k][m] = acc[i] + acw[i];
-        __syncthreads();
-        {
-            const double u = (part[0][gi][r16] + part[1][gi][r16]) + (part[2][gi][r16] + part[3][gi][r16]);
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                kzd[c][e] = (double) h2f((kz[c][e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
+                ksd[c][e] = (double) h2f((ks[c][e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
+            }
+        const u4 kt0 = kt;
+        if (g0 + SEL_GT < end) load(g0 + SEL_GT);
+        float lo, hi, bad;
+        tok_range(kt0, lo, hi, bad);
+        double best = -__builtin_inf();          // thread (group gi, position r16 < np)
+        for (int r0 = 0; r0 < rows; r0 += 16) {
+            if (rows > 16 && (g0 > first || r0 > 0)) {
+                __syncthreads();                 // the rows before these have been read
+                stage(r0);
+                __syncthreads();
+                rows_to_regs();
+            }
+            d4 acc = {0.0, 0.0, 0.0, 0.0}, acw = acc;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(kzd[c][e], qd[c][e], acc, 0, 0, 0);
+                    acw = __builtin_amdgcn_mfma_f64_16x16x4f64(ksd[c][e], wd[c][e], acw, 0, 0, 0);
+                }
+            // lane (row m, k): groups 4 i + k
+            double (*pw)[16][17] = part[turn & 1];
+            ++turn;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pw[w][4 * i + k][m] = acc[i] + acw[i];
+            __syncthreads();
+            const double u = (pw[0][gi][r16] + pw[1][gi][r16]) + (pw[2][gi][r16] + pw[3][gi][r16]);
+            wave_sync();                         // a group's rows stay in its wavefront
             bound[gi][r16] = bad != 0.0f ? (double) bad : u >= 0.0 ? u * (double) hi : u * (double) lo;
-        }
-        __syncthreads();
-        const int nr = rows - r0 < 16 ? rows - r0 : 16;
-        if (r16 < np) {                          // the rows of position r16 in this turn (all of them, unless there are several)
-            const int a0 = a.gq <= 16 ? r16 * a.gq : 0, a1 = a.gq <= 16 ? a0 + a.gq : nr;
-            for (int r = a0; r < a1; ++r) {
-                const double x = bound[gi][r];
-                best = x > best || x != x ? x : best;                  // a NaN stays: no number is greater
+            wave_sync();
+            const int nr = rows - r0 < 16 ? rows - r0 : 16;
+            if (r16 < np) {                      // the rows of position r16 in this turn (all of them, unless there are several)
+                const int a0 = a.gq <= 16 ? r16 * a.gq : 0, a1 = a.gq <= 16 ? a0 + a.gq : nr;
+                for (int r = a0; r < a1; ++r) {
+                    const double x = bound[gi][r];
+                    best = x > best || x != x ? x : best;              // a NaN stays: no number is greater
+                }
             }
         }
+        if (r16 < np && g0 + (uint32_t) gi < n)
+            J.score[((size_t) (p0 - a.pos0 + r16) * a.H + h) * a.stride + g0 + gi] = best;
     }
-    if (r16 < np && g0 + (uint32_t) gi < n)
-        J.score[((size_t) (p0 - a.pos0 + r16) * a.H + h) * a.stride + g0 + gi] = best;
 }
 
 // scores as unsigned numbers of the same order; -0 counts as 0, a NaN is above all (a group whose bound is not a number is
@@ -165,12 +201,15 @@ SJK_DEV uint64_t sel_key(double x) {
 }
 
 // The list of one (position, KV head): the border is found digit by digit from the highest bit in which the keys differ, until the
-// keys that share the border's digits are just those still wanted; then one pass in order of the groups.
-__global__ __launch_bounds__(PICK_NT) void pick_kernel(const SelArgs a) {
+// keys that share the border's digits are just those still wanted; then the places of the taken ones in order of the groups.
+// NT threads; KPT: keys per thread, adjacent groups, in registers, or 0: read again for every digit.
+template <int NT, int KPT>
+__global__ __launch_bounds__(NT) void pick_kernel(const SelArgs a) {
+    constexpr int NW = NT / 64, NK = KPT ? KPT : 8;
     __shared__ uint32_t hist[256];
-    __shared__ uint64_t s_or, s_first;
+    __shared__ unsigned long long s_or;
     __shared__ uint32_t s_digit, s_left, s_all;
-    __shared__ uint32_t w_sel[PICK_NT / 64], w_tie[PICK_NT / 64];
+    __shared__ uint32_t w_sel[NW], w_tie[NW];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int j = (int) blockIdx.y, list = (int) blockIdx.x;           // list = position x H + KV head
     const SelJob & J = a.job[j];
@@ -178,35 +217,52 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(const SelArgs a) {
     int32_t * out = J.sel + ((size_t) a.pos0 * a.H + list) * top;
     const double * sc = J.score + (size_t) list * a.stride;
     if (n <= top) {
-        for (uint32_t i = tid; i < top; i += PICK_NT) out[i] = i < n ? (int32_t) i : -1;
+        for (uint32_t i = tid; i < top; i += NT) out[i] = i < n ? (int32_t) i : -1;
         return;
     }
-    // the bits in which any key differs from the first
-    if (tid == 0) { s_or = 0; s_first = sel_key(sc[0]); }
+    // keys of a turn of NT x NK groups; keys past the end are 0, below every key of a number
+    uint64_t key[NK];
+    auto load = [&](uint32_t i0) {
+#pragma unroll
+        for (int e = 0; e < NK; ++e) {
+            const uint32_t i = i0 + (uint32_t) tid * NK + e;
+            key[e] = i < n ? sel_key(sc[i]) : 0;
+        }
+    };
+    const uint64_t first = sel_key(sc[0]);
+    load(0);
+    if (tid == 0) s_or = 0;
     __syncthreads();
-    {
-        const uint64_t first = s_first;
+    {   // the bits in which any key differs from the first
         uint64_t d = 0;
-        for (uint32_t i = tid; i < n; i += PICK_NT) d |= sel_key(sc[i]) ^ first;
+        for (uint32_t i0 = 0; i0 < n; i0 += NT * NK) {
+            if (!KPT && i0) load(i0);
+#pragma unroll
+            for (int e = 0; e < NK; ++e)
+                if (i0 + (uint32_t) tid * NK + e < n) d |= key[e] ^ first;
+        }
 #pragma unroll
         for (int s = 1; s < 64; s <<= 1) {
             const uint32_t lo = __shfl_xor((uint32_t) d, s, 64), hi = __shfl_xor((uint32_t) (d >> 32), s, 64);
             d |= lo | ((uint64_t) hi << 32);
         }
-        if (lane == 0 && d) atomicOr((unsigned long long *) &s_or, (unsigned long long) d);
+        if (lane == 0 && d) atomicOr(&s_or, (unsigned long long) d);
     }
     __syncthreads();
-    // border: keys with key >> shift above pre >> shift are taken, of those equal to it the first `left`
+    // border: keys with key >> shift above pre are taken, of those equal to it the first `left`
     int shift = s_or ? 64 - (int) __clzll((long long) s_or) : 0;       // the digits above are the same in all keys
-    uint64_t pre = shift < 64 ? s_first >> shift : 0;
+    uint64_t pre = shift < 64 ? first >> shift : 0;
     uint32_t left = top;
     while (shift > 0) {
         const int bits = shift < 8 ? shift : 8, sh = shift - bits;
-        for (int i = tid; i < 256; i += PICK_NT) hist[i] = 0;
+        if (tid < 256) hist[tid] = 0;
         __syncthreads();
-        for (uint32_t i = tid; i < n; i += PICK_NT) {
-            const uint64_t key = sel_key(sc[i]);
-            if (shift == 64 || (key >> shift) == pre) atomicAdd(&hist[(uint32_t) (key >> sh) & ((1u << bits) - 1u)], 1u);
+        for (uint32_t i0 = 0; i0 < n; i0 += NT * NK) {
+            if (!KPT) load(i0);
+#pragma unroll
+            for (int e = 0; e < NK; ++e)
+                if (i0 + (uint32_t) tid * NK + e < n && (shift == 64 || (key[e] >> shift) == pre))
+                    atomicAdd(&hist[(uint32_t) (key[e] >> sh) & ((1u << bits) - 1u)], 1u);
         }
         __syncthreads();
         if (tid < 64) {                          // digits 4 lane .. 4 lane + 3: how many keys have a higher one
@@ -229,33 +285,45 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(const SelArgs a) {
         __syncthreads();
         pre = (shift == 64 ? 0 : pre << bits) | s_digit;
         left = s_left;
-        const uint32_t all = s_all;
         shift = sh;
-        __syncthreads();
-        if (all == left) break;
+        if (s_all == left) break;                // (the next writes of s_* are two barriers away)
     }
     uint32_t done = 0, ties = 0;
-    for (uint32_t i0 = 0; i0 < n; i0 += PICK_NT) {
-        const uint32_t i = i0 + (uint32_t) tid;
-        const uint64_t key = i < n ? sel_key(sc[i]) >> shift : 0;
-        const bool tie = i < n && key == pre;
-        const uint64_t below = (1ull << lane) - 1ull, mt = __ballot(tie);
-        if (lane == 0) w_tie[w] = (uint32_t) __popcll(mt);
-        __syncthreads();
-        uint32_t t0 = ties, tt = 0;
+    for (uint32_t i0 = 0; i0 < n; i0 += NT * NK) {
+        if (!KPT) load(i0);
+        // this thread's counts of taken and of equal keys, and those of the threads before it
+        uint32_t nt = 0, ng = 0;
 #pragma unroll
-        for (int x = 0; x < PICK_NT / 64; ++x) { if (x < w) t0 += w_tie[x]; tt += w_tie[x]; }
-        const bool take = (i < n && key > pre) || (tie && t0 + (uint32_t) __popcll(mt & below) < left);
-        const uint64_t ms = __ballot(take);
-        if (lane == 0) w_sel[w] = (uint32_t) __popcll(ms);
-        __syncthreads();
-        uint32_t at = done, ss = 0;
+        for (int e = 0; e < NK; ++e) {
+            const bool in = i0 + (uint32_t) tid * NK + e < n;
+            nt += in && (key[e] >> shift) == pre;
+            ng += in && (key[e] >> shift) > pre;
+        }
+        uint32_t both = ng | (nt << 16), inc = both;                   // at most 512 of a wavefront
 #pragma unroll
-        for (int x = 0; x < PICK_NT / 64; ++x) { if (x < w) at += w_sel[x]; ss += w_sel[x]; }
-        if (take) out[at + (uint32_t) __popcll(ms & below)] = (int32_t) i;
-        done += ss;
-        ties += tt;
+        for (int s = 1; s < 64; s <<= 1) {
+            const uint32_t o = __shfl_up(inc, s, 64);
+            if (lane >= s) inc += o;
+        }
+        __syncthreads();                         // the last turn's counts have been read
+        if (lane == 63) { w_sel[w] = inc & 0xFFFFu; w_tie[w] = inc >> 16; }
         __syncthreads();
+        uint32_t g = done + (inc & 0xFFFFu) - ng, t = ties + (inc >> 16) - nt;
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+            if (x < w) { g += w_sel[x]; t += w_tie[x]; }
+            done += w_sel[x];
+            ties += w_tie[x];
+        }
+#pragma unroll
+        for (int e = 0; e < NK; ++e) {
+            const uint32_t i = i0 + (uint32_t) tid * NK + e;
+            if (i >= n) continue;
+            const uint64_t kk = key[e] >> shift;
+            if (kk > pre || (kk == pre && t < left)) out[g + (t < left ? t : left)] = (int32_t) i;
+            g += kk > pre;
+            t += kk == pre;
+        }
     }
 }
 
@@ -323,11 +391,20 @@ static int sel_launch(SelArgs & a, const sjk_hip_view & v, int n_jobs, size_t ro
     for (a.pos0 = 0; a.pos0 < a.n_q; a.pos0 += chunk) {
         a.n_pos = a.n_q - a.pos0 < chunk ? a.n_q - a.pos0 : chunk;
         if (scored) {
-            const dim3 grid((most + SEL_GT - 1) / SEL_GT, (unsigned) a.H, (unsigned) (n_jobs * ((a.n_pos + a.pb - 1) / a.pb)));
+            // a tile a workgroup up to 8 of them a CU (two rounds), then runs of up to 16 that are all on the device at once
+            // (1M positions of 8 KV heads, 4,000 tiles: runs of 4 25.6 -> 22 us)
+            const uint64_t tiles = (most + SEL_GT - 1) / SEL_GT, others = (uint64_t) a.H * (uint64_t) (n_jobs * ((a.n_pos + a.pb - 1) / a.pb));
+            const uint64_t cus = (uint64_t) n_cus(), run = (tiles * others + 4u * cus - 1) / (4u * cus);
+            a.tpw = tiles * others <= 8u * cus ? 1 : run > 16 ? 16 : (int) run;
+            const dim3 grid((unsigned) ((tiles + a.tpw - 1) / a.tpw), (unsigned) a.H, (unsigned) (others / (uint64_t) a.H));
             if (l.D == 128) hipLaunchKernelGGL(score_kernel<128>, grid, dim3(SEL_NT), 0, st, a);
             else hipLaunchKernelGGL(score_kernel<256>, grid, dim3(SEL_NT), 0, st, a);
         }
-        hipLaunchKernelGGL(pick_kernel, dim3((unsigned) (a.n_pos * a.H), (unsigned) n_jobs), dim3(PICK_NT), 0, st, a);
+        const dim3 lists((unsigned) (a.n_pos * a.H), (unsigned) n_jobs);
+        if (most <= 256u) hipLaunchKernelGGL((pick_kernel<256, 1>), lists, dim3(256), 0, st, a);
+        else if (most <= 1024u) hipLaunchKernelGGL((pick_kernel<256, 4>), lists, dim3(256), 0, st, a);
+        else if (most <= 8192u) hipLaunchKernelGGL((pick_kernel<1024, 8>), lists, dim3(1024), 0, st, a);
+        else hipLaunchKernelGGL((pick_kernel<1024, 0>), lists, dim3(1024), 0, st, a);
         if (SJK_CHECK_LAUNCH()) return SJK_ERR_DEVICE;
     }
     return 0;
