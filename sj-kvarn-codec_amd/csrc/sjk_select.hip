@@ -73,7 +73,8 @@ SJK_DEV void tok_range(const u4 & kt, float & lo, float & hi, float & bad) {
 }
 
 // scores: grid (runs of tpw 16-group tiles, KV heads, jobs x position tiles). The wavefronts of a workgroup take a quarter of the
-// channels each; lane (m, k) loads group m's tables at channels 8 k .. 8 k + 7 of every 32, its A operands, a tile ahead.
+// channels each; lane (m, k) loads group m's tables at channels 8 k .. 8 k + 7 of every 32, its A operands. Four workgroups a CU hide
+// each other's loads at D = 128 (tables loaded a tile ahead took registers for three: no faster).
 template <int D>
 __global__ __launch_bounds__(SEL_NT) __attribute__((amdgpu_waves_per_eu(D == 128 ? 4 : 2))) void score_kernel(const SelArgs a) {
     constexpr int NC = D / 128;                  // 8-channel loads of a lane per table
@@ -140,18 +141,8 @@ __global__ __launch_bounds__(SEL_NT) __attribute__((amdgpu_waves_per_eu(D == 128
     rows_to_regs();
     int turn = 0;
     for (uint32_t g0 = first; g0 < end; g0 += SEL_GT) {
-        double kzd[NC][8], ksd[NC][8];
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                kzd[c][e] = (double) h2f((kz[c][e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
-                ksd[c][e] = (double) h2f((ks[c][e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
-            }
-        const u4 kt0 = kt;
-        if (g0 + SEL_GT < end) load(g0 + SEL_GT);
         float lo, hi, bad;
-        tok_range(kt0, lo, hi, bad);
+        tok_range(kt, lo, hi, bad);
         double best = -__builtin_inf();          // thread (group gi, position r16 < np)
         for (int r0 = 0; r0 < rows; r0 += 16) {
             if (rows > 16 && (g0 > first || r0 > 0)) {
@@ -165,8 +156,11 @@ __global__ __launch_bounds__(SEL_NT) __attribute__((amdgpu_waves_per_eu(D == 128
             for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(kzd[c][e], qd[c][e], acc, 0, 0, 0);
-                    acw = __builtin_amdgcn_mfma_f64_16x16x4f64(ksd[c][e], wd[c][e], acw, 0, 0, 0);
+                    const uint32_t sh = 16 * (e & 1);
+                    uint32_t z = kz[c][e >> 1], s = ks[c][e >> 1];
+                    asm volatile("" : "+v"(z), "+v"(s));               // converted here: 32 registers of doubles less, no spill
+                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double) h2f((z >> sh) & 0xFFFFu), qd[c][e], acc, 0, 0, 0);
+                    acw = __builtin_amdgcn_mfma_f64_16x16x4f64((double) h2f((s >> sh) & 0xFFFFu), wd[c][e], acw, 0, 0, 0);
                 }
             // lane (row m, k): groups 4 i + k
             double (*pw)[16][17] = part[turn & 1];
@@ -181,12 +175,14 @@ __global__ __launch_bounds__(SEL_NT) __attribute__((amdgpu_waves_per_eu(D == 128
             const int nr = rows - r0 < 16 ? rows - r0 : 16;
             if (r16 < np) {                      // the rows of position r16 in this turn (all of them, unless there are several)
                 const int a0 = a.gq <= 16 ? r16 * a.gq : 0, a1 = a.gq <= 16 ? a0 + a.gq : nr;
+#pragma unroll 1
                 for (int r = a0; r < a1; ++r) {
                     const double x = bound[gi][r];
                     best = x > best || x != x ? x : best;              // a NaN stays: no number is greater
                 }
             }
         }
+        if (g0 + SEL_GT < end) load(g0 + SEL_GT);
         if (r16 < np && g0 + (uint32_t) gi < n)
             J.score[((size_t) (p0 - a.pos0 + r16) * a.H + h) * a.stride + g0 + gi] = best;
     }
