@@ -3023,11 +3023,26 @@ __host__ __device__ static int ext_tiles(const ExtArgs & e) {
     return e.c.sel ? e.n_q * ((gq + A3_Q - 1) / A3_Q) : (e.n_q * gq + A3_Q - 1) / A3_Q;
 }
 
-// tiles of a launch: the call's in as few launches as there can be, each about as many (16 tiles as 8 and 8, not 13 and 3: 289 against
-// 329 us at 100K)
-static int ext_per_launch(int tiles) {
-    const int launches = (tiles + maxj<A3Ext> - 1) / maxj<A3Ext>;
-    return (tiles + launches - 1) / launches;
+// Tiles of a launch: as few launches as there can be, each with about as many tiles (16 as 8 and 8, not 13 and 3: 289 against 329 us
+// at 100K), but more launches of fewer 4/4 tiles where a tile's CU slots would be too few to share out between its records and its
+// rows: by the steps of a4_split, a launch's fixed part at EXT_FIXED records of a wavefront (12 tiles of 8 KV heads at 100K, D = 128:
+// 495 us as one launch of 2 slots a tile and head).
+constexpr double EXT_FIXED = 2.2;
+static int ext_per_launch(int tiles, int body, int slots, int n_rec, int n_chunk) {
+    const int least = (tiles + maxj<A3Ext> - 1) / maxj<A3Ext>;
+    if (body != 44) return (tiles + least - 1) / least;
+    int best = 0;
+    double cost = 0.0;
+    for (int l = least; l <= tiles && l <= least + 8; ++l) {
+        const int per = (tiles + l - 1) / l;
+        A3Args a = {};
+        a.n_rec = n_rec; a.n_chunk = n_chunk;
+        a4_split(a, slots / per > 1 ? slots / per : 1);
+        const double rows = a.n_row_wg ? A4_CHUNK_UNIT * (double) ((n_chunk + A4_NW * a.n_row_wg - 1) / (A4_NW * a.n_row_wg)) : 0.0;
+        const double c = l * (EXT_FIXED + (a.rec_a > rows ? a.rec_a : rows));
+        if (best == 0 || c < cost - 1e-9) { best = per; cost = c; }
+    }
+    return best;
 }
 
 // tile k of the call, before the split
@@ -3200,11 +3215,25 @@ int sjk_attend_ext(const ExtCall * calls, int n, int n_q, int n_head, float scal
     // a workspace smaller than it should be is found before anything is launched
     for (int j = 0; j < n; ++j)
         if (ws_part_slots(calls[j].v) < (size_t) ws_slots(H)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
+    bool wide = calls[0].seen != nullptr;
+    for (int j = 0; wide && j < n; ++j) wide = sjk_prefill_takes_tree(calls[j].v, body, calls[j].N, n_q, n_head, out_type);
+    if (wide) {
+        for (int j = 0; j < n; ++j)
+            if (const int rc = sjk_prefill_tree(calls[j], nullptr, 0, n_q, n_head, scale, n_nodes, out_type, st)) return rc;
+        return 0;
+    }
     A3BatchT<A3Ext> bt = {};
-    ExtArgs e0 = {};
-    e0.c = calls[0];
-    e0.n_q = n_q; e0.n_head = n_head;
-    const int per = ext_per_launch(n * ext_tiles(e0));
+    int n_rec = 0, n_chunk = 0, tiles = 0;       // of the longest call
+    for (int j = 0; j < n; ++j) {
+        ExtArgs e = {};
+        e.c = calls[j];
+        e.n_q = n_q; e.n_head = n_head; e.top = top; e.n_nodes = n_nodes;
+        ext_plan(e, bt.job[0], 0);
+        n_rec = bt.job[0].n_rec > n_rec ? bt.job[0].n_rec : n_rec;
+        n_chunk = bt.job[0].n_chunk > n_chunk ? bt.job[0].n_chunk : n_chunk;
+        tiles += ext_tiles(e);
+    }
+    const int per = ext_per_launch(tiles, body, ext_slots(body, H), n_rec, n_chunk);
     for (int j = 0; j < n; ++j) {
         ExtArgs e = {};
         e.c = calls[j];
@@ -3231,9 +3260,11 @@ int sjk_attend_ext_dyn(const ExtCall & call, const int32_t * desc, uint32_t n_ma
     e.body = ext_body(call.v.lay, out_type);
     e.slots = ext_slots(e.body, H);
     if (ws_part_slots(call.v) < (size_t) ws_slots(H)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
+    if (call.seen && sjk_prefill_takes_tree(call.v, e.body, 0, n_q, n_head, out_type))
+        return sjk_prefill_tree(call, desc, n_max, n_q, n_head, scale, n_nodes, out_type, st);
     const int nt = ext_tiles(e);
     A3BatchT<A3Ext> * plan = (A3BatchT<A3Ext> *) ws_plan(call.v);
-    const int per = ext_per_launch(nt);
+    const int most = e.body == 44 ? A3_MAXJ : maxj<A3Ext>, launches = (nt + most - 1) / most, per = (nt + launches - 1) / launches;
     for (e.tile0 = 0; e.tile0 < nt; e.tile0 += per) {
         e.n_tiles = nt - e.tile0 < per ? nt - e.tile0 : per;
         hipLaunchKernelGGL(ext_plan_kernel, dim3(1), dim3(64), 0, st, e, ws_part(call.v), plan);

@@ -55,6 +55,12 @@ constexpr int PF_COST_CH = 3, PF_COST_REC = 4;
 // it takes 38.1 against 35.3 us at 600 positions, with 1 head 38.5 against 32.0 at 1,500. At 128 rows it takes up to twice as
 // long on short contexts. The line is on rows and heads alone: a captured call does not know its context.
 constexpr int PF_MIN_ROWS = 256, PF_MIN_ROWS_HEADS = 8;
+// Trees of drafted nodes (16-bit outputs): from 256 rows on at every length, and from 64 rows on where rows x heads x positions
+// reach 24M (a captured call does not know its context: rows alone). Against the 16-row kernel: 256 rows of 4 heads, D = 256, 37 / 36
+// us at 300 positions, 55 / 59 at 8.7K, 219 / 288 at 100K; 96 of 8 heads, D = 128, 35 / 26 at 8.7K, 61 / 79 at 42K; 64 of 4, D = 256, 44 / 21
+// at 8.7K, 85 / 79 at 100K; 192 of 1, D = 128, 53 / 43 at 100K, of 2 72 / 83.
+constexpr int PF_TREE_ROWS = 256, PF_TREE_SOME = 64;
+constexpr uint64_t PF_TREE_WORK = 24u << 20;
 
 struct PreArgs {
     sjk_hip_view v;
@@ -70,6 +76,34 @@ struct PreArgs {
                                                  // tile; then [2][n_wg][32] (m, l): of that segment, and of one that starts a
                                                  // tile and does not end it (its O is in out)
 };
+
+// A call of drafted nodes (sjk_hip_attend_tree with a 16-bit output and many rows): the instances of the templates below on this type.
+// Every row sees all positions before `base`, and the nodes of its mask behind it.
+struct PreTree : PreArgs {
+    const uint64_t * seen;                       // [n_q][words]
+    int words, n_nodes, out_type;                // N is base + n_nodes
+    float * first;                               // [H][n_tile][32][D]: O of a segment that starts a tile and does not end it
+                                                 // (where the other calls have it in their 32-bit output)
+};
+template <typename Args> constexpr bool is_tree = std::is_same<Args, PreTree>::value;
+// the 32 positions from p0 on that query position iq sees (a bit each). The mask's place is read from the kernel's arguments each
+// time: held over the loops it would push other scalars into vector registers.
+SJK_DEV uint32_t tree_seen(int iq, uint32_t base, uint32_t p0) {
+    if (p0 + 32u <= base) return ~0u;
+    auto arg = (const __attribute__((address_space(4))) PreTree *) __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(arg));
+    const struct { const uint64_t * seen; int words; } a = {arg->seen, arg->words};
+    const uint64_t * m = a.seen + (size_t) iq * a.words;
+    if (p0 < base) {
+        const uint32_t k = base - p0;            // 1 .. 31 positions before the first node
+        return (uint32_t) (m[0] << k) | ((1u << k) - 1u);
+    }
+    const uint32_t r = p0 - base, i = r >> 6, s = r & 63u;
+    if (i >= (uint32_t) a.words) return 0u;
+    uint64_t x = m[i] >> s;
+    if (s > 32u && i + 1u < (uint32_t) a.words) x |= m[i + 1] << (64u - s);
+    return (uint32_t) x;
+}
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef float f2v __attribute__((ext_vector_type(2)));
@@ -135,12 +169,23 @@ struct PreCtx {
     uint32_t cost;
     bool ok;
 };
-SJK_DEV PreCtx pre_ctx(const PreArgs & a, int tile) {
+template <typename Args> SJK_DEV PreCtx pre_ctx(const Args & a, int tile) {
     uint32_t B = a.B, N = a.N, q0 = a.qpos0;
     PreCtx c;
     c.ok = true;
     const uint32_t S = a.v.S;
-    if (a.desc) {                                // the test of the 16-row path: NaN rows if the view cannot hold it
+    if constexpr (is_tree<Args>) {
+        if (a.desc) {
+            const int32_t iB = a.desc[SJK_DESC_B], iQ = a.desc[SJK_DESC_QPOS0];
+            const uint64_t end = (uint64_t) (uint32_t) iQ + (uint32_t) a.n_nodes;
+            B = (uint32_t) iB; q0 = (uint32_t) iQ;
+            const uint32_t bend = B < S ? S : B;
+            c.ok = iB >= 0 && iQ >= 0 && end <= a.n_max && (B <= S || ((B - S) % 128u == 0u && B <= q0 && a.v.body)) &&
+                   (end <= bend || (a.v.ring && a.v.cap >= 16u && end - bend <= a.v.cap));
+            N = (uint32_t) end;
+            if (!c.ok) { B = 0; N = 0; q0 = 0; }
+        }
+    } else if (a.desc) {                                // the test of the 16-row path: NaN rows if the view cannot hold it
         const int32_t iB = a.desc[SJK_DESC_B], iN = a.desc[SJK_DESC_N], iQ = a.desc[SJK_DESC_QPOS0];
         B = (uint32_t) iB; N = (uint32_t) iN; q0 = (uint32_t) iQ;
         const uint32_t end = q0 + (uint32_t) a.n_q, pend = N < end ? N : end, bend = B < S ? S : B;
@@ -149,8 +194,8 @@ SJK_DEV PreCtx pre_ctx(const PreArgs & a, int tile) {
         if (!c.ok) { B = 0; N = 0; q0 = 0; }
     }
     const int last = PF_ROWS * tile + PF_ROWS < a.rows ? PF_ROWS * tile + PF_ROWS - 1 : a.rows - 1;
-    const uint32_t end = q0 + (uint32_t) (last / a.gq) + 1u;
-    c.N = N; c.qpos0 = q0;
+    const uint32_t end = is_tree<Args> ? N : q0 + (uint32_t) (last / a.gq) + 1u;
+    c.N = N; c.qpos0 = q0;                       // (a tree: its first node)
     c.pend = N < end ? N : end;
     c.sink_end = c.pend < S ? c.pend : S;
     uint32_t Bb = B < S ? S : B;
@@ -170,7 +215,7 @@ SJK_DEV PreCtx pre_ctx(const PreArgs & a, int tile) {
 // Costs of the tiles before `tile` and of all tiles of a KV head (every head has the same): computed by each wavefront,
 // 64 tiles at a time. With find, `tile` is instead the tile whose cost range holds y, and before its start.
 struct PrePos { uint64_t before, total; int tile; };
-SJK_DEV PrePos pre_scan(const PreArgs & a, int tile, bool find, uint64_t y) {
+template <typename Args> SJK_DEV PrePos pre_scan(const Args & a, int tile, bool find, uint64_t y) {
     const int lane = threadIdx.x & 63;
     PrePos r = {0, 0, tile};
     uint64_t run = 0;
@@ -228,8 +273,15 @@ SJK_DEV void dma16(gptr src, uint8_t * dst) {
 }
 SJK_DEV void vm_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-template <int D>
-__global__ __launch_bounds__(PF_NT) __attribute__((amdgpu_waves_per_eu(2))) void prefill_kernel(const PreArgs a) {
+// an output value of the call's type
+SJK_DEV void tree_out(const PreTree & a, size_t at, float y) {
+    if (a.out_type == SJK_F16) ((_Float16 *) a.out)[at] = (_Float16) y;
+    else ((__bf16 *) a.out)[at] = (__bf16) y;
+}
+
+template <int D, typename Args>
+__global__ __launch_bounds__(PF_NT) __attribute__((amdgpu_waves_per_eu(2))) void prefill_kernel(const Args a) {
+    constexpr bool TREE = is_tree<Args>;
     static_assert(D == 128 || D == 256, "head dimension of the prefill kernel");
     constexpr int NB = D / 128, NT = D / 32, NC = D / 16;        // tq6_0 blocks of a row, O tiles, K steps
     using RL4 = RecLay<4, 4, D>;
@@ -273,7 +325,7 @@ __global__ __launch_bounds__(PF_NT) __attribute__((amdgpu_waves_per_eu(2))) void
         // of the records' 32-bit rows keeps its own
         __syncthreads();
         if (tid < PF_ROWS) {
-            const uint32_t e = c.qpos0 + (uint32_t) ((r0 + tid) / a.gq) + 1u;
+            const uint32_t e = TREE ? c.N : c.qpos0 + (uint32_t) ((r0 + tid) / a.gq) + 1u;
             L.see[tid] = tid < nr ? (e < c.N ? e : c.N) : 0u;
         }
         {
@@ -309,7 +361,7 @@ __global__ __launch_bounds__(PF_NT) __attribute__((amdgpu_waves_per_eu(2))) void
             }
         }
         __syncthreads();
-        uint32_t qend_min = c.qpos0 + (uint32_t) (r0 / a.gq) + 1u;   // visible to every live row
+        uint32_t qend_min = TREE ? c.N : c.qpos0 + (uint32_t) (r0 / a.gq) + 1u;   // visible to every live row (but for a mask)
         if (qend_min > c.N) qend_min = c.N;
 
         // the wavefront's part: the steps whose first cost unit lies in [ca, cb)
@@ -488,14 +540,16 @@ __global__ __launch_bounds__(PF_NT) __attribute__((amdgpu_waves_per_eu(2))) void
                     const float rs = L.rs[m];
                     // positions that the row does not see: no score, and nothing of their values, whose infinities and NaNs
                     // would make a NaN with a weight of zero (dead: a bit per score)
-                    const bool edge = p1 - p0 < PF_CH || p1 > qend_min;
+                    const bool edge = p1 - p0 < PF_CH || p1 > (TREE ? c.qpos0 : qend_min);
                     uint32_t dead = 0;
                     if (edge) {
                         const uint32_t qend = L.see[m];
+                        uint32_t bits = ~0u;
+                        if constexpr (TREE) bits = tree_seen((r0 + (m < nr ? m : 0)) / a.gq, c.qpos0, p0) >> (4 * h);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const uint32_t p = p0 + (uint32_t) (8 * (i >> 2) + 4 * h + (i & 3));
-                            if (p >= p1 || p >= qend) {
+                            if (p >= p1 || p >= qend || (TREE && !(bits >> (8 * (i >> 2) + (i & 3)) & 1u))) {
                                 sc[i] = -__builtin_inff();
                                 dead |= 1u << i;
                             }
@@ -907,8 +961,10 @@ __global__ __launch_bounds__(PF_NT) __attribute__((amdgpu_waves_per_eu(2))) void
             }
             const bool whole = from == 0 && to == c.cost;
             const int rq = r0 + r, iq = rq / a.gq, hq = head * a.gq + rq % a.gq;
-            float * dst = from == 0 ? a.out + ((size_t) iq * a.n_head + hq) * D
-                                    : a.part + ((size_t) lw * PF_ROWS + r) * D;
+            const size_t at = ((size_t) iq * a.n_head + hq) * D;
+            float * dst = from == 0 ? a.out + at : a.part + ((size_t) lw * PF_ROWS + r) * D;
+            if constexpr (TREE)
+                if (from == 0) dst = a.first + (((size_t) head * a.n_tile + tile) * PF_ROWS + r) * D;
             const float inv = whole ? (ls == 0.0f ? 0.0f : 1.0f / ls) : 1.0f;
 #pragma unroll
             for (int p = 0; p < NT / 2; ++p) {
@@ -927,8 +983,14 @@ __global__ __launch_bounds__(PF_NT) __attribute__((amdgpu_waves_per_eu(2))) void
                     for (int i = 0; i < 4; ++i) y[i] = __builtin_fmaf(fac[k], z[i], y[i]);
                 }
                 if (r < nr) {
+                    if (TREE && whole) {
+                        if constexpr (TREE)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) dst[64 * p + 4 * c4 + i] = y[i] * inv;
+                            for (int i = 0; i < 4; ++i) tree_out(a, at + 64 * p + 4 * c4 + i, y[i] * inv);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) dst[64 * p + 4 * c4 + i] = y[i] * inv;
+                    }
                 }
                 __syncthreads();
             }
@@ -948,16 +1010,22 @@ __global__ __launch_bounds__(PF_NT) __attribute__((amdgpu_waves_per_eu(2))) void
 // The tiles that several workgroups took: grid (tiles, KV heads, D / 64), thread = (query row, 4 channels); eight
 // segments' loads at a time go out together (one after the other they were most of the call's fixed cost, 12 us at 9
 // segments a tile)
-template <int D> __global__ __launch_bounds__(PF_NT) void prefill_combine(const PreArgs a) {
+template <int D, typename Args> __global__ __launch_bounds__(PF_NT) void prefill_combine(const Args a) {
+    constexpr bool TREE = is_tree<Args>;
     constexpr int NS = 8;
     const int tid = threadIdx.x, r = tid >> 4, ch = 64 * (int) blockIdx.z + 4 * (tid & 15);
     const int tile = (int) blockIdx.x, head = (int) blockIdx.y, H = a.v.n_head_kv;
     const int rq = PF_ROWS * tile + r, iq = rq / a.gq, hq = head * a.gq + rq % a.gq;
     const PreCtx c = pre_ctx(a, tile);
-    float * o = a.out + ((size_t) iq * a.n_head + hq) * D + ch;
+    const size_t at = ((size_t) iq * a.n_head + hq) * D + ch;
+    float * o = a.out + at;
+    auto put = [&](int i, float y) {
+        if constexpr (TREE) tree_out(a, at + i, y);
+        else o[i] = y;
+    };
     if (!c.ok) {
         if (rq < a.rows)
-            for (int i = 0; i < 4; ++i) o[i] = __builtin_nanf("");
+            for (int i = 0; i < 4; ++i) put(i, __builtin_nanf(""));
         return;
     }
     const PrePos pos = pre_scan(a, tile, false, 0);
@@ -969,8 +1037,10 @@ template <int D> __global__ __launch_bounds__(PF_NT) void prefill_combine(const 
     const float * ml0 = mls + ((size_t) a.n_wg + w0) * PF_ROWS * 2;
     float M = ml0[0], ls = ml0[1];
     f4 y;
+    const float * from = o;
+    if constexpr (TREE) from = a.first + (((size_t) head * a.n_tile + tile) * PF_ROWS + r) * D + ch;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = o[i];
+    for (int i = 0; i < 4; ++i) y[i] = from[i];
     for (int k0 = w0 + 1; k0 <= w1; k0 += NS) {
         float mk[NS], lk[NS], Mn = M;
         f4 z[NS];
@@ -1003,7 +1073,7 @@ template <int D> __global__ __launch_bounds__(PF_NT) void prefill_combine(const 
     }
     const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = y[i] * inv;
+    for (int i = 0; i < 4; ++i) put(i, y[i] * inv);
 }
 
 // The kernel takes 4/4 bodies whose workspace holds one partial per CU and whose rows are not written where another
@@ -1019,9 +1089,9 @@ bool sjk_prefill_takes(const sjk_hip_view & v, int body, int n_q, int n_head, co
     return W * PF_ROWS * (size_t) v.lay.D + W * PF_ROWS * 4 <= ws_part_slots(v) * sf;
 }
 
-template <int D> static int launch_d(const PreArgs & a, hipStream_t st) {
-    hipLaunchKernelGGL(prefill_kernel<D>, dim3((unsigned) a.n_wg), dim3(PF_NT), 0, st, a);
-    hipLaunchKernelGGL(prefill_combine<D>, dim3((unsigned) a.n_tile, (unsigned) a.v.n_head_kv, (unsigned) (D / 64)), dim3(PF_NT), 0, st, a);
+template <int D, typename Args> static int launch_d(const Args & a, hipStream_t st) {
+    hipLaunchKernelGGL((prefill_kernel<D, Args>), dim3((unsigned) a.n_wg), dim3(PF_NT), 0, st, a);
+    hipLaunchKernelGGL((prefill_combine<D, Args>), dim3((unsigned) a.n_tile, (unsigned) a.v.n_head_kv, (unsigned) (D / 64)), dim3(PF_NT), 0, st, a);
     return SJK_CHECK_LAUNCH();
 }
 
@@ -1036,6 +1106,37 @@ int sjk_prefill(const sjk_hip_view & v, const int32_t * desc, uint32_t n_max, ui
     a.sc2 = scale * 1.4426950408889634f;
     a.q = d_q; a.out = d_out; a.part = ws_part(v);   // 256-byte aligned
     return v.lay.D == 128 ? launch_d<128>(a, st) : launch_d<256>(a, st);
+}
+
+// Where the first segments of a tree's tiles lie in the workspace: behind the partials, 16-byte aligned
+static size_t tree_first(int D) {
+    const size_t W = (size_t) n_cus();
+    return (W * PF_ROWS * (size_t) D + W * PF_ROWS * 4 + 3) & ~(size_t) 3;
+}
+static size_t tree_tiles(int n_q, int n_head, int H) { return ((size_t) n_q * (size_t) (n_head / H) + PF_ROWS - 1) / PF_ROWS; }
+
+bool sjk_prefill_takes_tree(const sjk_hip_view & v, int body, uint32_t N, int n_q, int n_head, int out_type) {
+    const int rows = n_q * (n_head / v.n_head_kv), D = v.lay.D;
+    if (body != 44 || out_type == SJK_F32) return false;
+    if (rows < PF_TREE_ROWS && (rows < PF_TREE_SOME || (uint64_t) rows * (uint64_t) v.n_head_kv * N < PF_TREE_WORK)) return false;
+    if (v.work_bytes < WS_PLAN_BYTES + ws_stage_bytes(D, v.n_head_kv)) return false;
+    if (v.staging != SJKVARN_STAGING_F16 && (((uintptr_t) v.sink | (uintptr_t) v.ring) & 3u)) return false;
+    return tree_first(D) + tree_tiles(n_q, n_head, v.n_head_kv) * (size_t) v.n_head_kv * PF_ROWS * (size_t) D <= ws_part_slots(v) * ws_slot_floats(D);
+}
+
+int sjk_prefill_tree(const ExtCall & e, const int32_t * desc, uint32_t n_max, int n_q, int n_head, float scale, int n_nodes, int out_type,
+                     hipStream_t st) {
+    PreTree a = {};
+    a.v = e.v; a.desc = desc; a.n_max = n_max; a.B = e.B; a.N = e.N; a.qpos0 = e.N - (uint32_t) n_nodes;
+    a.n_q = n_q; a.n_head = n_head; a.gq = n_head / e.v.n_head_kv;
+    a.rows = n_q * a.gq;
+    a.n_tile = (a.rows + PF_ROWS - 1) / PF_ROWS;
+    a.n_wg = n_cus();
+    a.sc2 = scale * 1.4426950408889634f;
+    a.q = e.q; a.out = (float *) e.out; a.part = ws_part(e.v);
+    a.seen = e.seen; a.words = (n_nodes + 63) / 64; a.n_nodes = n_nodes; a.out_type = out_type;
+    a.first = a.part + tree_first(e.v.lay.D);
+    return e.v.lay.D == 128 ? launch_d<128>(a, st) : launch_d<256>(a, st);
 }
 
 }  // namespace sjk
