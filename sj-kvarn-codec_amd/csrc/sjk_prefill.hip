@@ -55,8 +55,9 @@ constexpr int PF_COST_CH = 3, PF_COST_REC = 4;
 // it takes 38.1 against 35.3 us at 600 positions, with 1 head 38.5 against 32.0 at 1,500. At 128 rows it takes up to twice as
 // long on short contexts. The line is on rows and heads alone: a captured call does not know its context.
 constexpr int PF_MIN_ROWS = 256, PF_MIN_ROWS_HEADS = 8;
-// Trees of drafted nodes (16-bit outputs): from 256 rows on at every length, and from 64 rows on where rows x heads x positions
-// reach 24M (a captured call does not know its context: rows alone). Against the 16-row kernel: 256 rows of 4 heads, D = 256, 37 / 36
+// Trees of drafted nodes, BF16 outputs (weights of records are rounded to fp16 once, without the 16-row kernel's correction: beside
+// a rounding to bf16 that is nothing, of FP16 outputs it took the error from 2.0e-4 to 3.6e-4, so those stay with the 16-row
+// kernel): from 256 rows on at every length, and from 64 rows on where rows x heads x positions reach 24M (a captured call does not know its context: rows alone). Against the 16-row kernel: 256 rows of 4 heads, D = 256, 37 / 36
 // us at 300 positions, 55 / 59 at 8.7K, 219 / 288 at 100K; 96 of 8 heads, D = 128, 35 / 26 at 8.7K, 61 / 79 at 42K; 64 of 4, D = 256, 44 / 21
 // at 8.7K, 85 / 79 at 100K; 192 of 1, D = 128, 53 / 43 at 100K, of 2 72 / 83.
 constexpr int PF_TREE_ROWS = 256, PF_TREE_SOME = 64;
@@ -77,7 +78,7 @@ struct PreArgs {
                                                  // tile and does not end it (its O is in out)
 };
 
-// A call of drafted nodes (sjk_hip_attend_tree with a 16-bit output and many rows): the instances of the templates below on this type.
+// A call of drafted nodes (sjk_hip_attend_tree with a BF16 output and many rows): the instances of the templates below on this type.
 // Every row sees all positions before `base`, and the nodes of its mask behind it.
 struct PreTree : PreArgs {
     const uint64_t * seen;                       // [n_q][words]
@@ -1117,7 +1118,7 @@ static size_t tree_tiles(int n_q, int n_head, int H) { return ((size_t) n_q * (s
 
 bool sjk_prefill_takes_tree(const sjk_hip_view & v, int body, uint32_t N, int n_q, int n_head, int out_type) {
     const int rows = n_q * (n_head / v.n_head_kv), D = v.lay.D;
-    if (body != 44 || out_type == SJK_F32) return false;
+    if (body != 44 || out_type != SJK_BF16) return false;
     if (rows < PF_TREE_ROWS && (rows < PF_TREE_SOME || (uint64_t) rows * (uint64_t) v.n_head_kv * N < PF_TREE_WORK)) return false;
     if (v.work_bytes < WS_PLAN_BYTES + ws_stage_bytes(D, v.n_head_kv)) return false;
     if (v.staging != SJKVARN_STAGING_F16 && (((uintptr_t) v.sink | (uintptr_t) v.ring) & 3u)) return false;

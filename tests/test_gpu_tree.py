@@ -139,6 +139,69 @@ def test_many_rows(lib, dev, n_q, per, H):
     ctx.close()
 
 
+@pytest.mark.parametrize("D,H,per,staging,sink_type,n_groups,tail,base,n,n_q", [
+    (128, 1, 4, 0, 0, 0, 70, 0, 70, 70),             # no context: rows without nodes are zero
+    (256, 1, 8, 1, 0, 0, 150, 100, 50, 33),          # nodes across the sink's end
+    (128, 2, 3, 0, 1, 0, 300, 125, 175, 90),
+    (256, 2, 2, 0, 0, 3, 170, 0, 131, 131),          # several words a row
+    (128, 1, 16, 1, 0, 9, 200, 61, 129, 16),         # the ring has wrapped
+    (128, 8, 4, 0, 0, 2, 140, 5, 97, 64),
+])
+def test_rows_of_a_ubatch(lib, dev, D, H, per, staging, sink_type, n_groups, tail, base, n, n_q):
+    """256 rows per head and more (BF16 outputs: the 32-row kernel), eager and captured"""
+    rng = np.random.default_rng(n * n_q)
+    ctx = Ctx(lib, dev, D, H, (4, 4, 0), staging, sink_type, n_groups=n_groups, tail=tail, seed=12)
+    base += ctx.B if n_groups else 0
+    B = ctx.B if n_groups else 0 if base < S else S
+    K, V = ctx.rows(base + n, B=max(B, S))
+    mask = tree(rng, n)[n - n_q:]
+    mask[[0, 7, n_q - 1]] = False
+    q = queries(rng, n_q, H * per, D)
+    want, tol = attention(q, K, V, seen_of(mask, base, H), D ** -0.5)
+    bits = {}
+    for t in (sjk.F16, sjk.BF16):
+        bits[t] = run(lib, dev, ctx.view, B, base, mask, q, t, junk=rng).bits()
+        # weights of 16-bit outputs may be rounded to fp16 once (half a step of each), times values up to twice the largest off the zero point
+        got = parts.values(bits[t], t).reshape(q.shape)
+        check(got, want, tol + 2.0 ** -10 * np.abs(V).max(), t, t)
+        if base == 0:
+            assert (got[[0, 7, n_q - 1]] == 0).all()
+    st, desc = dev.stream(), dev.put(descriptor(0, 0, 0))
+    dq, dm = dev.put(q), dev.put(words(mask))
+    out = Out(dev, q.size, sjk.BF16)
+    n_max = base + n + 5
+    if B == 0 and n_max > S + ctx.L.cap:
+        n_max = S + ctx.L.cap
+    g = Graph(dev, st, [lambda: lib.sjk_hip_attend_tree_dyn(C.byref(ctx.view), desc, n_max, n, n_q, H * per, dq, D ** -0.5, dm, sjk.BF16, out.at, st)])
+    for d, ok in (((B, 0, base), 1), ((B, 0, -1), 0), ((B, 9, base), 1), ((B, 0, n_max - n + 1), 0), ((S + 64, 0, base), 0), ((B, 0, base), 1)):
+        dev.upload(desc, descriptor(*d))
+        run(lib, dev, ctx.view, B, base, mask, q, sjk.BF16).bits()         # eager work on the same workspace between the replays
+        g.replay()
+        if ok:
+            assert np.array_equal(out.bits(), bits[sjk.BF16]), d
+        else:
+            assert np.isnan(out.get()).all(), d
+    g.close()
+    ctx.close()
+
+
+@pytest.mark.parametrize("D,H,n_q,per,n_groups", [(128, 4, 64, 3, 260), (256, 8, 40, 2, 310)])
+def test_long_contexts_of_some_rows(lib, dev, D, H, n_q, per, n_groups):
+    """64 rows and more on contexts that are long enough for the 32-row kernel, against the FP32 output"""
+    rng = np.random.default_rng(n_q)
+    ctx = Ctx(lib, dev, D, H, (4, 4, 0), n_groups=n_groups, tail=150, seed=14)
+    assert n_q * per * H * ctx.N >= 24 << 20
+    most = max(np.abs(ctx.rows(ctx.N)[1]).max(), 1)
+    base = ctx.N - n_q
+    mask = tree(rng, n_q)
+    mask[9] = False
+    q = queries(rng, n_q, H * per, D)
+    want = run(lib, dev, ctx.view, ctx.B, base, mask, q).get()
+    for t in (sjk.F16, sjk.BF16):
+        check(run(lib, dev, ctx.view, ctx.B, base, mask, q, t).get(), want, 2.0 ** -10 * most, t, t)
+    ctx.close()
+
+
 def test_a_chain_is_causal_attention(lib, dev):
     rng = np.random.default_rng(2)
     D, H = 256, 2
