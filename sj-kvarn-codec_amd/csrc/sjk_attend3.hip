@@ -1828,6 +1828,26 @@ template <int D, int NP = 1, bool B44 = false> struct ScLds {                  /
     };
 };
 template <int D, int NP = 1, bool B44 = false> using AScLds = A3LdsT<ScLds<D, NP, B44>, SC_NW>;
+// A3Ext at D = 128: the row path's tables at this D's sizes, the merge's state in the record path's part, for three workgroups per CU
+struct RowLds128 {
+    alignas(16) uint8_t stage[SC_NW][A3_CH * 2 * SJKVARN_TQ6_BLOCK_BYTES];
+    alignas(16) uint16_t qb[2][4][4][A3_Q][8];
+    u2 pt[4096];
+    float cent[64];
+};
+template <bool B44> struct AScLds128 {
+    union {
+        ScLds<128, 2, B44> r;
+        RowLds128 w;
+        struct {
+            f4 merge[SC_NW][128 / 16 * 64];
+            float wm[SC_NW][A3_Q], wl[SC_NW][A3_Q], wf[SC_NW][A3_Q];
+        };
+    };
+};
+template <int D, typename Args, bool B44> using ScLdsOf =
+    typename std::conditional<!is_ext<Args>, AScLds<D, 1, B44>, typename std::conditional<D == 128, AScLds128<B44>, AScLds<D, 2, B44>>::type>::type;
+static_assert(sizeof(AScLds128<false>) <= 42 * 1280 && sizeof(AScLds128<true>) <= 42 * 1280, "LDS of three workgroups per CU");
 static_assert(sizeof(AScLds<256>) <= 80 * 1024 && sizeof(AScLds<128>) <= 80 * 1024 && sizeof(AScLds<256, 2>) <= 80 * 1024 &&
               sizeof(AScLds<256, 2, true>) <= 80 * 1024, "LDS of two workgroups per CU");
 static_assert(sc_rec_max<256>() == 31488 && sc_rec_max<128>() == 16384, "largest staged scalar records");
@@ -2301,7 +2321,7 @@ __device__ __attribute__((always_inline)) inline void asc_records(const Args & a
 // workgroup wg of job a (KV head blockIdx.y): row workgroups [0, n_row_wg) stream the sink and the tail, the others
 // rec_per_wg records each
 template <int D, bool B44 = false, typename Args> __device__ __attribute__((always_inline)) inline void attendsc_job(const Args & a, int wg) {
-    __shared__ AScLds<D, is_ext<Args> ? 2 : 1, B44> s;
+    __shared__ ScLdsOf<D, Args, B44> s;
     const int h = blockIdx.y;
     if (wg >= a.n_wg) return;                    // a fixed grid (sjk_hip_attend_dyn) may exceed the plan's split
     asm volatile("" ::"s"(a.n_row_wg), "s"(a.rec_per_wg), "s"(a.n_rec), "s"(a.sink_end), "s"(a.v.S), "s"(a.v.n_head_kv),
@@ -2625,7 +2645,7 @@ template <typename Args> __host__ __device__ static int a3_assign(A3BatchT<Args>
             a4_split(a, share < 1 ? 1 : share);
         } else if constexpr (is_ext<Args>) {
             const int share = total > 0.0 ? (int) ((a.n_rec + cc * a.n_chunk) / total * slots + 1e-6) : 1;
-            ext_split(a, share < 1 ? 1 : share);
+            ext_split(a, share < 1 ? 1 : share > A3_CMB_MAX ? A3_CMB_MAX : share);
         } else {
             a3_split(a, unit, cc);
         }
@@ -2957,12 +2977,12 @@ extern "C" int sjk_hip_attend_dyn(const sjk_hip_view * v, const int32_t * d_desc
 namespace sjk {
 
 template <int D, bool B44>
-__global__ __launch_bounds__(SC_NT) __attribute__((amdgpu_waves_per_eu(2))) void ext_scalar_kernel(const A3BatchT<A3Ext> b) {
+__global__ __launch_bounds__(SC_NT) __attribute__((amdgpu_waves_per_eu(D == 128 ? 3 : 2))) void ext_scalar_kernel(const A3BatchT<A3Ext> b) {
     const int j = a3_job_of(b, blockIdx.x);
     attendsc_job<D, B44>(b.job[j], (int) blockIdx.x - b.wg_base[j]);
 }
 template <int D, bool B44>
-__global__ __launch_bounds__(SC_NT) __attribute__((amdgpu_waves_per_eu(2))) void ext_scalar_kernel_dyn(const A3BatchT<A3Ext> * __restrict__ b) {
+__global__ __launch_bounds__(SC_NT) __attribute__((amdgpu_waves_per_eu(D == 128 ? 3 : 2))) void ext_scalar_kernel_dyn(const A3BatchT<A3Ext> * __restrict__ b) {
     if ((int) blockIdx.x >= b->wg_base[b->n_jobs]) return;
     const int j = a3_job_of(*b, blockIdx.x);
     attendsc_job<D, B44>(b->job[j], (int) blockIdx.x - b->wg_base[j]);
@@ -3028,9 +3048,10 @@ __host__ __device__ static int ext_tiles(const ExtArgs & e) {
 // rows: by the steps of a4_split, a launch's fixed part at EXT_FIXED records of a wavefront (12 tiles of 8 KV heads at 100K, D = 128:
 // 495 us as one launch of 2 slots a tile and head).
 constexpr double EXT_FIXED = 2.2;
-static int ext_per_launch(int tiles, int body, int slots, int n_rec, int n_chunk) {
+static int ext_per_launch(int tiles, int body, int H, int n_rec, int n_chunk) {
     const int least = (tiles + maxj<A3Ext> - 1) / maxj<A3Ext>;
     if (body != 44) return (tiles + least - 1) / least;
+    const int slots = n_cus() / H;
     int best = 0;
     double cost = 0.0;
     for (int l = least; l <= tiles && l <= least + 8; ++l) {
@@ -3187,25 +3208,45 @@ static int ext_body(const sj_kvarn_layout & l, int out_type) {
     const int body = a3_body(l);
     return body == 44 && out_type == SJK_F32 ? 45 : body;
 }
-static int ext_slots(int body, int H) {
-    return body == 44 ? (n_cus() / H > 0 ? n_cus() / H : 1) : a3_slots(H);
+// CU slots per KV head of a launch of `jobs` tiles: 4/4 one workgroup per CU, the others two, scalar records at D = 128 three (163
+// registers, 53,760 bytes of LDS; 32 groups of 8 sequences, 3/3: 28.6 us against 33.9 with two). room: the partials that the tiles'
+// workspace holds; a launch writes H (slots + 2 jobs) at most.
+static int ext_slots(int body, int D, int H, size_t room, int jobs) {
+    if (body == 44) return n_cus() / H > 0 ? n_cus() / H : 1;
+    const int two = (2 * n_cus() + H - 1) / H;
+    if (D != 128 || !(body == 45 || body == 55)) return two;
+    const int three = (3 * n_cus() + H - 1) / H, most = (int) (room / (size_t) H) - 2 * jobs;
+    return three < most ? three : two > most ? two : most;
 }
 
 static int ext_launch(A3BatchT<A3Ext> & bt, int body, int H, hipStream_t st) {
-    if (a3_assign(bt, body, H, ext_slots(body, H))) return SJK_ERR_UNSUPPORTED;
-    void * ws[maxj<A3Ext>];
-    size_t used[maxj<A3Ext>];
-    int n_ws = 0;
-    for (int j = 0; j < bt.n_jobs; ++j) {
-        A3Ext & a = bt.job[j];
-        int k = 0;
-        while (k < n_ws && ws[k] != a.v.work) ++k;
-        if (k == n_ws) { ws[n_ws] = a.v.work; used[n_ws] = 0; ++n_ws; }
-        a.part = ws_part(a.v) + used[k] * ws_slot_floats(a.v.lay.D);
-        used[k] += (size_t) H * (size_t) a.n_wg;
-        if (used[k] > ws_part_slots(a.v)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
-    }
     const int D = bt.job[0].v.lay.D;
+    bool one = true;                             // one workspace for all tiles: they share its partials
+    size_t room = ws_part_slots(bt.job[0].v);
+    for (int j = 1; j < bt.n_jobs; ++j) {
+        const size_t r = ws_part_slots(bt.job[j].v);
+        one = one && bt.job[j].v.work == bt.job[0].v.work;
+        room = r < room ? r : room;
+    }
+    // tiles on several workspaces: what three workgroups per CU write has to fit each of them, else two
+    for (int pass = one ? 1 : 0; pass < 2; ++pass) {
+        if (a3_assign(bt, body, H, ext_slots(body, D, H, one ? room : pass == 0 ? (size_t) 1 << 30 : 0, bt.n_jobs))) return SJK_ERR_UNSUPPORTED;
+        void * ws[maxj<A3Ext>];
+        size_t used[maxj<A3Ext>];
+        int n_ws = 0;
+        bool fits = true;
+        for (int j = 0; j < bt.n_jobs; ++j) {
+            A3Ext & a = bt.job[j];
+            int k = 0;
+            while (k < n_ws && ws[k] != a.v.work) ++k;
+            if (k == n_ws) { ws[n_ws] = a.v.work; used[n_ws] = 0; ++n_ws; }
+            a.part = ws_part(a.v) + used[k] * ws_slot_floats(D);
+            used[k] += (size_t) H * (size_t) a.n_wg;
+            fits = fits && used[k] <= ws_part_slots(a.v);
+        }
+        if (fits) break;
+        if (pass == 1) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
+    }
     return ext_kernels(body, D, body == 44 ? dim3((unsigned) bt.n_slots) : dim3((unsigned) bt.wg_base[bt.n_jobs], (unsigned) H),
                        dim3(A3_Q, (unsigned) H, (unsigned) (D / 64 * bt.n_jobs)), &bt, nullptr, st);
 }
@@ -3233,7 +3274,7 @@ int sjk_attend_ext(const ExtCall * calls, int n, int n_q, int n_head, float scal
         n_chunk = bt.job[0].n_chunk > n_chunk ? bt.job[0].n_chunk : n_chunk;
         tiles += ext_tiles(e);
     }
-    const int per = ext_per_launch(tiles, body, ext_slots(body, H), n_rec, n_chunk);
+    const int per = ext_per_launch(tiles, body, H, n_rec, n_chunk);
     for (int j = 0; j < n; ++j) {
         ExtArgs e = {};
         e.c = calls[j];
@@ -3258,7 +3299,6 @@ int sjk_attend_ext_dyn(const ExtCall & call, const int32_t * desc, uint32_t n_ma
     e.n_q = n_q; e.n_head = n_head; e.top = top; e.n_nodes = n_nodes; e.out_type = out_type; e.scale = scale;
     const int H = call.v.n_head_kv, D = call.v.lay.D;
     e.body = ext_body(call.v.lay, out_type);
-    e.slots = ext_slots(e.body, H);
     if (ws_part_slots(call.v) < (size_t) ws_slots(H)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
     if (call.seen && sjk_prefill_takes_tree(call.v, e.body, 0, n_q, n_head, out_type))
         return sjk_prefill_tree(call, desc, n_max, n_q, n_head, scale, n_nodes, out_type, st);
@@ -3267,6 +3307,7 @@ int sjk_attend_ext_dyn(const ExtCall & call, const int32_t * desc, uint32_t n_ma
     const int most = e.body == 44 ? A3_MAXJ : maxj<A3Ext>, launches = (nt + most - 1) / most, per = (nt + launches - 1) / launches;
     for (e.tile0 = 0; e.tile0 < nt; e.tile0 += per) {
         e.n_tiles = nt - e.tile0 < per ? nt - e.tile0 : per;
+        e.slots = ext_slots(e.body, D, H, ws_part_slots(call.v), e.n_tiles);
         hipLaunchKernelGGL(ext_plan_kernel, dim3(1), dim3(64), 0, st, e, ws_part(call.v), plan);
         // the most workgroups per KV head that a table's jobs take: two each for the rounding of its split, 7 for its alignment
         const dim3 grid = e.body == 44 ? dim3((unsigned) (H * (e.slots + 2 * e.n_tiles))) : dim3((unsigned) (e.slots + 9 * e.n_tiles), (unsigned) H);
