@@ -611,8 +611,9 @@ int sjk_hip_seq_attend_batch(const sjk_hip_seq_job * jobs, int n_jobs, int il, i
  * groups than top.
  *
  * sjk_hip_attend_groups takes any ascending list: an entry that is no sealed group, or not above the entry before it, adds nothing.
- * With all groups listed the result is sjk_hip_attend's up to rounding. d_out [n_q][n_head][D] of out_type (SJK_F32, _F16, _BF16), rotated basis; weights keep 22 bits and sums 32. A row that
- * sees nothing is zero. Infinities and NaNs of staged positions that a row does not see do not reach it.
+ * With all groups listed the result is sjk_hip_attend's up to rounding. d_out [n_q][n_head][D] of out_type (SJK_F32, _F16, _BF16), rotated
+ * basis. Sums and statistics have 32 bits; weights keep 22 bits for SJK_F32 outputs, those of 16-bit outputs are rounded to fp16 once
+ * on sealed records. A row that sees nothing is zero. Infinities and NaNs of staged positions that a row does not see do not reach it.
  *
  * Query positions lie behind the sealed part: with B > S, qpos0 + 1 >= B, N >= B, and B at a group's end (SJKVARN_ERR_ARG otherwise).
  * d_q is fp32 [n_q][n_head][D], 16-byte aligned, and does not overlap d_out. Both use v->work as sjk_hip_attend does. A selection's
@@ -631,8 +632,8 @@ int sjk_hip_select_groups_dyn(const sjk_hip_view * v, const int32_t * d_desc, ui
 int sjk_hip_attend_groups_dyn(const sjk_hip_view * v, const int32_t * d_desc, uint32_t n_max, int n_q, int n_head, const float * d_q,
                               float scale, const int32_t * d_sel, int top, int out_type, void * d_out, void * stream);
 
-/* n_jobs independent calls with one n_q, n_head and top in as few launches as the kernels take (16 jobs a selection, 8 tiles of 16 query
- * rows an attention). Views of a selection agree in layout and KV heads. d_out is not used by a selection. */
+/* n_jobs independent calls with one n_q, n_head and top in as few launches as the kernels take (16 jobs a selection; up to 13 tiles of
+ * 16 query rows an attention, where a list's tile is one position). Views of a selection agree in layout and KV heads. d_out is not used by a selection. */
 typedef struct sjk_hip_groups_job {
     sjk_hip_view  v;
     uint32_t      B, N, qpos0;
@@ -691,7 +692,7 @@ int sjk_hip_seq_attend_tree_batch(const sjk_hip_seq_tree_job * jobs, int n_jobs,
                                   int out_type, void * stream);
 
 /* The accepted path becomes the context: in every one of n_layers layers the stored row of node d_path[i] (device, int32) moves to position
- * base + i, in place, one launch for up to 64 layers. The path ascends; it ends at n_path entries or at the first that is no node
+ * base + i, in place, one launch for up to 160 layers. The path ascends; it ends at n_path entries or at the first that is no node
  * above the entry before it (-1, say), so a launch need not know its length. Rows of the positions behind it stay as they are. The views agree
  * in heads, staging, sink and capacity. A row that moves from a ring of 6-bit rows into an fp16 sink becomes the fp16 values of what
  * the ring holds. SJKVARN_ERR_CAPACITY for more staged nodes than the ring has slots. _dyn: base = d_desc[SJK_DESC_QPOS0], a negative

@@ -86,7 +86,7 @@ __global__ __launch_bounds__(SEL_NT) __attribute__((amdgpu_waves_per_eu(D == 128
     const int n_pt = (a.n_pos + a.pb - 1) / a.pb, j = (int) blockIdx.z / n_pt, pt = (int) blockIdx.z % n_pt;
     const int h = (int) blockIdx.y;
     const uint32_t n = sel_groups(a, j), first = blockIdx.x * (uint32_t) a.tpw * SEL_GT;
-    if (first >= n) return;
+    if (first >= n || n <= (uint32_t) a.top) return;                   // (all of its groups are listed, without scores)
     const uint32_t end = first + (uint32_t) a.tpw * SEL_GT < n ? first + (uint32_t) a.tpw * SEL_GT : n;
     const SelJob & J = a.job[j];
     auto table = [&](uint32_t gi) {              // groups past the end repeat the last one
@@ -346,7 +346,7 @@ using namespace sjk;
 extern "C" int sjk_attend3_supported(const sjk_hip_view * v);
 
 // what every form asks of a view and its call
-static int sel_args(const char * who, const sjk_hip_view & v, int n_q, int n_head, const float * q, int top, const int32_t * sel) {
+static int sel_args(const sjk_hip_view & v, int n_q, int n_head, const float * q, int top, const int32_t * sel) {
     if (!q || !sel || ((uintptr_t) q & 15u) || ((uintptr_t) sel & 3u) || n_q <= 0 || n_head <= 0 || top <= 0 || v.n_head_kv <= 0 ||
         n_head % v.n_head_kv)
         return SJKVARN_ERR_ARG;
@@ -354,8 +354,7 @@ static int sel_args(const char * who, const sjk_hip_view & v, int n_q, int n_hea
         set_error("the view is not one the attention kernels are built for (a layer's own layout)");
         return SJK_ERR_UNSUPPORTED;
     }
-    (void) who;
-    if (v.n_head_kv > 65535 || (int64_t) n_q * v.n_head_kv > 0x7fffffff) return SJKVARN_ERR_ARG;
+    if (v.n_head_kv > n_cus() || (int64_t) n_q * v.n_head_kv > 0x7fffffff) return SJKVARN_ERR_ARG;
     return 0;
 }
 
@@ -411,39 +410,38 @@ extern "C" int sjk_hip_select_groups_batch(const sjk_hip_groups_job * jobs, int 
     for (int k = 0; k < n_jobs; ++k) {
         const sjk_hip_groups_job & J = jobs[k];
         const sjk_hip_view & v = J.v, & v0 = jobs[0].v;
-        if (const int rc = sel_args("sjk_hip_select_groups", v, n_q, n_head, J.d_q, top, J.d_sel)) return rc;
+        if (const int rc = sel_args(v, n_q, n_head, J.d_q, top, J.d_sel)) return rc;
         if (const int rc = groups_ok(v, J.B, J.N, J.qpos0, n_q)) return rc;
         if (J.B > v.S && (J.B - v.S) / 128u > (uint32_t) top && !v.work) return SJKVARN_ERR_ARG;
         if (v.lay.D != v0.lay.D || v.lay.bits_k != v0.lay.bits_k || v.lay.bits_v != v0.lay.bits_v || v.lay.body != v0.lay.body ||
             v.n_head_kv != v0.n_head_kv)
             return refuse("sjk_hip_select_groups_batch: the views differ in layout or KV heads");
     }
-    // jobs that share a workspace (the layers of a sequence) share its room
+    // jobs with scores that share a workspace (the layers of a sequence) share its room
+    auto groups = [&](int k) { return jobs[k].B > jobs[k].v.S ? (jobs[k].B - jobs[k].v.S) / 128u : 0u; };
     for (int k0 = 0; k0 < n_jobs; k0 += SEL_MAXJ) {
         const int n = n_jobs - k0 < SEL_MAXJ ? n_jobs - k0 : SEL_MAXJ;
         SelArgs a = {};
         a.n_q = n_q; a.n_head = n_head; a.top = top;
         uint32_t most = 0;
         size_t room = ~(size_t) 0;
-        int shared[SEL_MAXJ], rank[SEL_MAXJ];
         for (int k = 0; k < n; ++k) {
             const sjk_hip_groups_job & J = jobs[k0 + k];
-            shared[k] = rank[k] = 0;
-            for (int i = 0; i < n; ++i)
-                if (jobs[k0 + i].v.work == J.v.work) {
-                    ++shared[k];
-                    if (i < k) ++rank[k];
-                }
-            const size_t r = sel_room(J.v) / (size_t) shared[k];
-            if (r < room) room = r;
             SelJob & s = a.job[k];
             s.body = J.v.body; s.blocks = J.v.blocks; s.q = J.d_q; s.sel = J.d_sel;
-            s.n = J.B > J.v.S ? (J.B - J.v.S) / 128u : 0u;
+            s.n = groups(k0 + k);
             if (s.n > most) most = s.n;
+            if (s.n <= (uint32_t) top) continue;
+            int shared = 0, rank = 0;
+            for (int i = 0; i < n; ++i)
+                if (groups(k0 + i) > (uint32_t) top && jobs[k0 + i].v.work == J.v.work) {
+                    ++shared;
+                    if (i < k) ++rank;
+                }
+            const size_t r = sel_room(J.v) / (size_t) shared;
+            if (r < room) room = r;
+            s.score = (double *) ws_part(J.v) + (size_t) rank * r;
         }
-        for (int k = 0; k < n; ++k)
-            a.job[k].score = jobs[k0 + k].v.work ? (double *) ws_part(jobs[k0 + k].v) + (size_t) rank[k] * (sel_room(jobs[k0 + k].v) / (size_t) shared[k])
-                                                 : nullptr;
         if (const int rc = sel_launch(a, jobs[k0].v, n, room, most, (hipStream_t) stream)) return rc;
     }
     return 0;
@@ -460,7 +458,7 @@ extern "C" int sjk_hip_select_groups(const sjk_hip_view * v, uint32_t B, uint32_
 extern "C" int sjk_hip_select_groups_dyn(const sjk_hip_view * v, const int32_t * d_desc, uint32_t n_max, int n_q, int n_head,
                                          const float * d_q, int top, int32_t * d_sel, void * stream) {
     if (!v || !d_desc || ((uintptr_t) d_desc & 3u)) return SJKVARN_ERR_ARG;
-    if (const int rc = sel_args("sjk_hip_select_groups_dyn", *v, n_q, n_head, d_q, top, d_sel)) return rc;
+    if (const int rc = sel_args(*v, n_q, n_head, d_q, top, d_sel)) return rc;
     const uint32_t most = n_max > v->S ? (n_max - v->S) / 128u : 0u;
     if (most && !v->body) return SJKVARN_ERR_ARG;
     if (most > (uint32_t) top && !v->work) return SJKVARN_ERR_ARG;

@@ -364,6 +364,61 @@ def test_batch_and_descriptor_forms(lib, dev):
         x.close()
 
 
+def test_lists_of_a_batch_of_many_lengths(lib, dev):
+    """jobs whose groups are all listed need no scores, nor a workspace; the others share theirs"""
+    rng = np.random.default_rng(14)
+    D, H, top = 128, 2, 20
+    lay = sjk.layout(D, G, 3, 3, 0)
+    recs = records(rng, lay, 300, H)
+    lengths = (300, 5, 0, 77, 20, 21, 150)
+    jobs = (sjk.GroupsJob * len(lengths))()
+    views = [fake_view(lib, dev, D, H, (3, 3, 0), recs, rng.permutation(300), work=n > top) for n in lengths]
+    views[3].work, views[6].work_bytes = views[0].work, views[6].work_bytes
+    views[1].work, views[1].work_bytes = dev.alloc(256).value, 256
+    q = [queries(rng, 3, 8, D) for _ in lengths]
+    sel = dev.put(np.full((len(lengths), 3, H, top), 77, np.int32))
+    for k, n in enumerate(lengths):
+        B = S + G * n
+        jobs[k] = sjk.GroupsJob(views[k], B, B + 3, B, dev.put(q[k]), C.c_void_p(sel.value + 4 * k * 3 * H * top), None)
+    sjk.check(lib.sjk_hip_select_groups_batch(jobs, len(lengths), 3, 8, top, None), "batch")
+    dev.sync()
+    got = dev.get(sel, 4 * len(lengths) * 3 * H * top, np.int32).reshape(len(lengths), 3, H, top)
+    for k, n in enumerate(lengths):
+        if n <= top:
+            assert (got[k] == np.concatenate([np.arange(n), np.full(top - n, -1)])).all(), n
+        else:
+            B = S + G * n
+            assert np.array_equal(got[k], select(lib, dev, views[k], B, B + 3, B, q[k], top, H)), n
+
+
+@pytest.mark.parametrize("bits", [(3, 3, 0), (4, 4, 0), (3, 3, 1)])
+def test_many_short_jobs_beside_a_long_one(lib, dev, bits):
+    """jobs on one workspace and on another's: a launch's partials fit each"""
+    rng = np.random.default_rng(15)
+    D, H, per, top = 128, 8, 2, 30
+    long, own = Ctx(lib, dev, D, H, bits, n_groups=30, tail=300, seed=70), Ctx(lib, dev, D, H, bits, tail=40, seed=71)
+    short = Ctx(lib, dev, D, H, bits, tail=25, seed=72)
+    ctxs = [long] + [short] * 11 + [own]
+    jobs, outs, qs = (sjk.GroupsJob * 13)(), [], []
+    for k, c in enumerate(ctxs):
+        v = sjk.View.from_buffer_copy(c.view)
+        if c is short:
+            v.work, v.work_bytes = long.view.work, long.view.work_bytes
+        q = queries(rng, 1, H * per, D)
+        sel = dev.put(np.broadcast_to(np.arange(30, dtype=np.int32), (H, top)).copy())
+        outs.append(Out(dev, q.size, sjk.F32))
+        qs.append(q)
+        jobs[k] = sjk.GroupsJob(v, c.B if c.n_groups else 0, c.N, c.N - 1, dev.put(q), sel, outs[-1].at)
+    sjk.check(lib.sjk_hip_attend_groups_batch(jobs, 13, 1, H * per, D ** -0.5, top, sjk.F32, None), "batch")
+    for k, c in enumerate(ctxs):
+        K, V = c.rows(c.N, B=max(jobs[k].B, S))
+        seen = np.ones((1, H, c.N), bool)
+        want, tol = attention(qs[k], K, V, seen, D ** -0.5)
+        check(outs[k].get().reshape(want.shape), want, tol, sjk.F32, k)
+    for c in (long, own, short):
+        c.close()
+
+
 def test_sequences(lib, dev):
     """a decode batch of sequences of one pool: selection and attention of a layer, against the views' calls"""
     rng = np.random.default_rng(30)
