@@ -1272,6 +1272,27 @@ SJK_DEV void tq6_pair_entry(uint32_t e, const float * cent, u2 & out) {
     out = split2(cent[c0], cent[c1]);
 }
 
+// The same table made by the compiler, for the instances that read it from memory (A3Ext)
+struct Tq6Pairs { alignas(16) uint32_t v[2 * 4096]; };
+constexpr Tq6Pairs tq6_pairs() {
+    constexpr uint32_t bits[64] = SJK_TQ6_CENTROID_BITS_INIT;
+    uint32_t hi[64] = {}, lo[64] = {};
+    for (int i = 0; i < 64; ++i) {
+        const float x = __builtin_bit_cast(float, bits[i]);
+        const _Float16 a = (_Float16) x, c = (_Float16) (x - (float) a);
+        hi[i] = __builtin_bit_cast(uint16_t, a);
+        lo[i] = __builtin_bit_cast(uint16_t, c);
+    }
+    Tq6Pairs t = {};
+    for (uint32_t e = 0; e < 4096; ++e) {
+        const uint32_t c0 = (e & 15u) | (((e >> 8) & 3u) << 4), c1 = ((e >> 4) & 15u) | (((e >> 10) & 3u) << 4);
+        t.v[2 * e] = hi[c0] | (hi[c1] << 16);
+        t.v[2 * e + 1] = lo[c0] | (lo[c1] << 16);
+    }
+    return t;
+}
+static __device__ const Tq6Pairs g_tq6_pairs = tq6_pairs();
+
 // 8 tq6_0 values (channels 8 c8 .. 8 c8 + 7 of a 128-value block; centroids, without the block norm) as fp16
 // hi and lo pairs, one pair-table lookup per two channels: pair u holds channels 2u, 2u+1
 SJK_DEV void tq6_pairs8(const uint8_t * blk, int c8, const u2 * pt, u4 & vh, u4 & vl) {
@@ -1379,6 +1400,13 @@ __device__ __attribute__((always_inline)) inline void a3_rows(const Args & a, Ld
     // chunk c, c + waves, ... of the wave's rank: with 8 waves (two per SIMD: waves w and w + 4), the first
     // waves of all SIMDs rank before the second ones, so that the chunks of a short last round go one per
     // SIMD (a SIMD with two 3-chunk waves ends ~5 us after one with a 3-chunk and a 2-chunk wave)
+    // A3Ext: the pair table comes from the caches, its loads ahead of the rows' (made in place it takes a workgroup 1.5 us)
+    u4 tab[EXT ? 4096 / (128 * NW) : 1];
+    if constexpr (EXT) {
+#pragma unroll
+        for (int k = 0; k < 4096 / (128 * NW); ++k) tab[k] = ((const u4 *) g_tq6_pairs.v)[tid + 64 * NW * k];
+        __builtin_amdgcn_sched_barrier(0);
+    }
     const int rank = NW == 8 ? (wu < 4 ? 4 * wgr + wu : 4 * a.n_row_wg + 4 * wgr + wu - 4) : wgr * NW + wu;
     int c = rank;
     if (c < r_nch) fetch(c, std::integral_constant<int, 0>{});
@@ -1399,14 +1427,19 @@ __device__ __attribute__((always_inline)) inline void a3_rows(const Args & a, Ld
             qx[e][1] = *(const float4 *) (qr + 4);
         }
     }
-    if (tid < 64) s.cent[tid] = tq6_cent(tid);
-    // the centroids are in LDS: each wave waits for its own LDS writes, then a bare s_barrier (__syncthreads
-    // would also wait for the loads in flight)
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    if constexpr (EXT) {
+#pragma unroll
+        for (int k = 0; k < 4096 / (128 * NW); ++k) ((u4 *) s.pt)[tid + 64 * NW * k] = tab[k];
+    } else {
+        if (tid < 64) s.cent[tid] = tq6_cent(tid);
+        // the centroids are in LDS: each wave waits for its own LDS writes, then a bare s_barrier (__syncthreads
+        // would also wait for the loads in flight)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
 #pragma unroll 4
-    for (int e = tid; e < 4096; e += 64 * NW) tq6_pair_entry((uint32_t) e, s.cent, s.pt[e]);
+        for (int e = tid; e < 4096; e += 64 * NW) tq6_pair_entry((uint32_t) e, s.cent, s.pt[e]);
+    }
     if (tid < D) {
         const int bq = tid & 15;
         const bool live = bq < a.n_rows;
@@ -1832,8 +1865,7 @@ template <int D, int NP = 1, bool B44 = false> using AScLds = A3LdsT<ScLds<D, NP
 struct RowLds128 {
     alignas(16) uint8_t stage[SC_NW][A3_CH * 2 * SJKVARN_TQ6_BLOCK_BYTES];
     alignas(16) uint16_t qb[2][4][4][A3_Q][8];
-    u2 pt[4096];
-    float cent[64];
+    alignas(16) u2 pt[4096];
 };
 template <bool B44> struct AScLds128 {
     union {
@@ -2318,11 +2350,10 @@ __device__ __attribute__((always_inline)) inline void asc_records(const Args & a
     }
 }
 
-// workgroup wg of job a (KV head blockIdx.y): row workgroups [0, n_row_wg) stream the sink and the tail, the others
+// workgroup wg of KV head h of job a: row workgroups [0, n_row_wg) stream the sink and the tail, the others
 // rec_per_wg records each
-template <int D, bool B44 = false, typename Args> __device__ __attribute__((always_inline)) inline void attendsc_job(const Args & a, int wg) {
+template <int D, bool B44 = false, typename Args> __device__ __attribute__((always_inline)) inline void attendsc_job(const Args & a, int h, int wg) {
     __shared__ ScLdsOf<D, Args, B44> s;
-    const int h = blockIdx.y;
     if (wg >= a.n_wg) return;                    // a fixed grid (sjk_hip_attend_dyn) may exceed the plan's split
     asm volatile("" ::"s"(a.n_row_wg), "s"(a.rec_per_wg), "s"(a.n_rec), "s"(a.sink_end), "s"(a.v.S), "s"(a.v.n_head_kv),
                  "s"(a.v.body), "s"(a.v.blocks), "s"(a.n_chunk), "s"(a.sink_chunks), "s"(a.body_end), "s"(a.pend));
@@ -2347,7 +2378,7 @@ template <int D, bool B44 = false, typename Args> __device__ __attribute__((alwa
 template <int D>
 __global__ __launch_bounds__(SC_NT) __attribute__((amdgpu_waves_per_eu(2))) void attendsc_kernel(const A3Batch b) {
     const int j = a3_job_of(b, blockIdx.x);
-    attendsc_job<D>(b.job[j], (int) blockIdx.x - b.wg_base[j]);
+    attendsc_job<D>(b.job[j], (int) blockIdx.y, (int) blockIdx.x - b.wg_base[j]);
 }
 
 
@@ -2856,11 +2887,11 @@ __global__ __launch_bounds__(SC_NT) __attribute__((amdgpu_waves_per_eu(2))) void
         const int x = (int) blockIdx.x;
         if (x >= plan->wg_base[plan->n_jobs]) return;
         const int j = a3_job_of(*plan, x);
-        attendsc_job<D>(plan->job[j], x - plan->wg_base[j]);
+        attendsc_job<D>(plan->job[j], (int) blockIdx.y, x - plan->wg_base[j]);
     } else {
         A3Args a;
         dyn_plan(c, a);
-        attendsc_job<D>(a, (int) blockIdx.x);
+        attendsc_job<D>(a, (int) blockIdx.y, (int) blockIdx.x);
     }
 }
 
@@ -2981,16 +3012,28 @@ extern "C" int sjk_hip_attend_dyn(const sjk_hip_view * v, const int32_t * d_desc
 
 namespace sjk {
 
+// A workgroup's place in a grid of (workgroups of the launch, KV heads): workgroups start one after the other (512 of them in 4.3 us), so the
+// heads take turns and a job's record workgroups, which take longest, come before its row workgroups
+SJK_DEV int ext_place(int & h) {
+    const uint32_t id = blockIdx.x + gridDim.x * blockIdx.y;
+    h = (int) (id % gridDim.y);
+    return (int) (id / gridDim.y);
+}
+SJK_DEV int ext_wg(const A3Ext & a, int i) { return i >= a.n_wg ? i : a.n_wg - 1 - i; }
+
 template <int D, bool B44>
 __global__ __launch_bounds__(SC_NT) __attribute__((amdgpu_waves_per_eu(D == 128 ? 3 : 2))) void ext_scalar_kernel(const A3BatchT<A3Ext> b) {
-    const int j = a3_job_of(b, blockIdx.x);
-    attendsc_job<D, B44>(b.job[j], (int) blockIdx.x - b.wg_base[j]);
+    int h;
+    const int x = ext_place(h), j = a3_job_of(b, x);
+    attendsc_job<D, B44>(b.job[j], h, ext_wg(b.job[j], x - b.wg_base[j]));
 }
 template <int D, bool B44>
 __global__ __launch_bounds__(SC_NT) __attribute__((amdgpu_waves_per_eu(D == 128 ? 3 : 2))) void ext_scalar_kernel_dyn(const A3BatchT<A3Ext> * __restrict__ b) {
-    if ((int) blockIdx.x >= b->wg_base[b->n_jobs]) return;
-    const int j = a3_job_of(*b, blockIdx.x);
-    attendsc_job<D, B44>(b->job[j], (int) blockIdx.x - b->wg_base[j]);
+    int h;
+    const int x = ext_place(h);
+    if (x >= b->wg_base[b->n_jobs]) return;
+    const int j = a3_job_of(*b, x);
+    attendsc_job<D, B44>(b->job[j], h, ext_wg(b->job[j], x - b->wg_base[j]));
 }
 template <int BK, int BV, int D>
 __global__ __launch_bounds__(A3_NT) __attribute__((amdgpu_waves_per_eu(2))) void ext_trellis_kernel(const A3BatchT<A3Ext> b) {
