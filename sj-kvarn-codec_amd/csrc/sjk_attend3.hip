@@ -3005,9 +3005,9 @@ extern "C" int sjk_hip_attend_dyn(const sjk_hip_view * v, const int32_t * d_desc
 // output keeps the precision of 32 bits (ext_body: which kernel takes 4/4 records).
 // A tile of a list's call is one query position (16 of its heads): each position has a list of its own per KV head.
 //
-// What bounds them: the streaming wavefronts HBM (384 of 3,100 groups for 3 positions, 8 KV heads of 128: 47.3 us for 173 MB, 3.65 TB/s); the
-// staged kernel of the scalar bodies latency where a workgroup has two records (64 of 736 groups, D = 256: 18.9 us, of them 4 for all
-// workgroups to start, 6 to the first record, 5 a record) and vector issue where it has more (32 groups of 8 sequences, 3/3: 24.9 us, 12 of them
+// What bounds them: the streaming wavefronts HBM (384 of 3,100 groups for 3 positions, 8 KV heads of 128: 47.1 us for 173 MB, 3.67 TB/s); the
+// staged kernel of the scalar bodies latency where a workgroup has two records (64 of 736 groups, D = 256: 17.8 us, of them 4 for all
+// workgroups to start, 6 to the first record, 5 a record) and vector issue where it has more (32 groups of 8 sequences, 3/3: 24.5 us, 12 of them
 // vector instructions). The combine takes 3.9 to 6.7 us more.
 
 namespace sjk {

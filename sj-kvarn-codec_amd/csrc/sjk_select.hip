@@ -10,8 +10,8 @@
 // Sums are 64-bit, on the fp64 matrix unit (v_mfma_f64_16x16x4: 16 groups x 16 query rows x 4 channels): a list is whole
 // numbers, and two scores next to its border must not change places with the order of a sum.
 //
-// What bounds it: few groups, its two launches (5.7 + 4.1 us); 8,000 groups of 8 KV heads of 128 for 4 positions, 22.3 us of scores (49 MB of
-// tables in pieces of 768 bytes, 9.5 us at a copy's rate, beside 6.9 us of fp64 products and as much of conversions) and 12.7 of lists (32
+// What bounds it: few groups, its two launches (5.7 + 3.9 us); 8,000 groups of 8 KV heads of 128 for 4 positions, 21.9 us of scores (49 MB of
+// tables in pieces of 768 bytes, 9.5 us at a copy's rate, beside 6.9 us of fp64 products and as much of conversions) and 11.8 of lists (32
 // workgroups, counts and barriers).
 #include "sjk_mfma.h"
 
@@ -206,7 +206,8 @@ SJK_DEV uint64_t sel_key(double x) {
 template <int NT, int KPT>
 __global__ __launch_bounds__(NT) void pick_kernel(const SelArgs a) {
     constexpr int NW = NT / 64, NK = KPT ? KPT : 8;
-    __shared__ uint32_t hist[256];
+    constexpr int HC = NT > 256 ? 8 : 1;         // counts per digit, one for every eighth lane: the first digits of most keys are alike
+    __shared__ uint32_t hist[256 * HC];
     __shared__ unsigned long long s_or;
     __shared__ uint32_t s_digit, s_left, s_all;
     __shared__ uint32_t w_sel[NW], w_tie[NW];
@@ -255,20 +256,25 @@ __global__ __launch_bounds__(NT) void pick_kernel(const SelArgs a) {
     uint32_t left = top;
     while (shift > 0) {
         const int bits = shift < 8 ? shift : 8, sh = shift - bits;
-        if (tid < 256) hist[tid] = 0;
+        for (int i = tid; i < 256 * HC; i += NT) hist[i] = 0;
         __syncthreads();
         for (uint32_t i0 = 0; i0 < n; i0 += NT * NK) {
             if (!KPT) load(i0);
 #pragma unroll
             for (int e = 0; e < NK; ++e)
                 if (i0 + (uint32_t) tid * NK + e < n && (shift == 64 || (key[e] >> shift) == pre))
-                    atomicAdd(&hist[(uint32_t) (key[e] >> sh) & ((1u << bits) - 1u)], 1u);
+                    atomicAdd(&hist[((uint32_t) (key[e] >> sh) & ((1u << bits) - 1u)) * HC + (lane & (HC - 1))], 1u);
         }
         __syncthreads();
         if (tid < 64) {                          // digits 4 lane .. 4 lane + 3: how many keys have a higher one
             uint32_t c[4], sum = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { c[e] = hist[4 * lane + e]; sum += c[e]; }
+            for (int e = 0; e < 4; ++e) {
+                c[e] = 0;
+#pragma unroll
+                for (int k = 0; k < HC; ++k) c[e] += hist[(4 * lane + e) * HC + k];
+                sum += c[e];
+            }
             uint32_t above = sum;                // of this lane and the ones after it
 #pragma unroll
             for (int s = 1; s < 64; s <<= 1) {
