@@ -827,6 +827,12 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
                 }
             }
         }
+        if constexpr (EXT) {
+            if (!live) {                         // a scale that is no number makes a NaN with a weight of zero
+#pragma unroll
+                for (int p = 0; p < 4; ++p) Ah[p] = u4{0u, 0u, 0u, 0u};
+            }
+        }
         // A weight's rounding is multiplied by its token's code, 0 .. 15; with 7.5 of it given back through the zero point the
         // factor is -7.5 .. 7.5 (3.0e-4 -> 1.3e-4 of a result)
         if constexpr (EXT) cv = __builtin_fmaf(7.5f, lost, cv);
@@ -3257,7 +3263,7 @@ static int ext_body(const sj_kvarn_layout & l, int out_type) {
     return body == 44 && out_type == SJK_F32 ? 45 : body;
 }
 // CU slots per KV head of a launch of `jobs` tiles: 4/4 one workgroup per CU, the others two, scalar records at D = 128 three (163
-// registers, 53,760 bytes of LDS; 32 groups of 8 sequences, 3/3: 28.6 us against 33.9 with two). room: the partials that the tiles'
+// registers, 53,504 bytes of LDS; 32 groups of 8 sequences, 3/3: 28.6 us against 33.9 with two). room: the partials that the tiles'
 // workspace holds; a launch writes H (slots + 2 jobs) at most.
 static int ext_slots(int body, int D, int H, size_t room, int jobs) {
     if (body == 44) return n_cus() / H > 0 ? n_cus() / H : 1;
@@ -3308,7 +3314,7 @@ int sjk_attend_ext(const ExtCall * calls, int n, int n_q, int n_head, float scal
     for (int j = 0; wide && j < n; ++j) wide = sjk_prefill_takes_tree(calls[j].v, body, calls[j].N, n_q, n_head, out_type);
     if (wide) {
         for (int j = 0; j < n; ++j)
-            if (const int rc = sjk_prefill_tree(calls[j], nullptr, 0, n_q, n_head, scale, n_nodes, out_type, st)) return rc;
+            if (const int rc = sjk_prefill_tree(calls[j], nullptr, 0, n_q, n_head, scale, n_nodes, st)) return rc;
         return 0;
     }
     A3BatchT<A3Ext> bt = {};
@@ -3349,7 +3355,7 @@ int sjk_attend_ext_dyn(const ExtCall & call, const int32_t * desc, uint32_t n_ma
     e.body = ext_body(call.v.lay, out_type);
     if (ws_part_slots(call.v) < (size_t) ws_slots(H)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
     if (call.seen && sjk_prefill_takes_tree(call.v, e.body, 0, n_q, n_head, out_type))
-        return sjk_prefill_tree(call, desc, n_max, n_q, n_head, scale, n_nodes, out_type, st);
+        return sjk_prefill_tree(call, desc, n_max, n_q, n_head, scale, n_nodes, st);
     const int nt = ext_tiles(e);
     A3BatchT<A3Ext> * plan = (A3BatchT<A3Ext> *) ws_plan(call.v);
     const int most = e.body == 44 ? A3_MAXJ : maxj<A3Ext>, launches = (nt + most - 1) / most, per = (nt + launches - 1) / launches;

@@ -267,9 +267,8 @@ struct ExtCall {
     const int32_t * sel;
     const uint64_t * seen;
 };
-// a tree's call with a 16-bit output and many query rows per KV head (sjk_prefill.hip), and whether that kernel takes it
-int sjk_prefill_tree(const ExtCall & e, const int32_t * desc, uint32_t n_max, int n_q, int n_head, float scale, int n_nodes, int out_type,
-                     hipStream_t st);
+// a tree's call with a BF16 output and many query rows per KV head (sjk_prefill.hip), and whether that kernel takes it
+int sjk_prefill_tree(const ExtCall & e, const int32_t * desc, uint32_t n_max, int n_q, int n_head, float scale, int n_nodes, hipStream_t st);
 bool sjk_prefill_takes_tree(const sjk_hip_view & v, int body, uint32_t N, int n_q, int n_head, int out_type);      // N: 0 if not known
 int sjk_attend_ext(const ExtCall * calls, int n, int n_q, int n_head, float scale, int top, int n_nodes, int out_type, hipStream_t st);
 int sjk_attend_ext_dyn(const ExtCall & call, const int32_t * desc, uint32_t n_max, int n_q, int n_head, float scale, int top, int n_nodes,

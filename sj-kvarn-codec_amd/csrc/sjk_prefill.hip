@@ -57,9 +57,10 @@ constexpr int PF_COST_CH = 3, PF_COST_REC = 4;
 constexpr int PF_MIN_ROWS = 256, PF_MIN_ROWS_HEADS = 8;
 // Trees of drafted nodes, BF16 outputs (weights of records are rounded to fp16 once, without the 16-row kernel's correction: beside
 // a rounding to bf16 that is nothing, of FP16 outputs it took the error from 2.0e-4 to 3.6e-4, so those stay with the 16-row
-// kernel): from 256 rows on at every length, and from 64 rows on where rows x heads x positions reach 24M (a captured call does not know its context: rows alone). Against the 16-row kernel: 256 rows of 4 heads, D = 256, 37 / 36
-// us at 300 positions, 55 / 59 at 8.7K, 219 / 288 at 100K; 96 of 8 heads, D = 128, 35 / 26 at 8.7K, 61 / 79 at 42K; 64 of 4, D = 256, 44 / 21
-// at 8.7K, 85 / 79 at 100K; 192 of 1, D = 128, 53 / 43 at 100K, of 2 72 / 83. 64 nodes x 16 heads of 256 at 100K: 226 us, 105 GFLOP of products at
+// kernel): from 256 rows on at every length, and from 64 rows on where rows x heads x positions reach 24M (a captured call does not
+// know its context: rows alone). Against the 16-row kernel: 256 rows of 4 heads, D = 256, 37 / 36 us at 300 positions, 55 / 59 at
+// 8.7K, 219 / 288 at 100K; 96 of 8 heads, D = 128, 35 / 26 at 8.7K, 61 / 79 at 42K; 64 of 4, D = 256, 44 / 21 at 8.7K, 85 / 79 at
+// 100K; 192 of 1, D = 128, 53 / 43 at 100K, of 2 72 / 83. 64 nodes x 16 heads of 256 at 100K: 226 us, 105 GFLOP of products at
 // 0.47 PFLOP/s, bound as the other calls are.
 constexpr int PF_TREE_ROWS = 256, PF_TREE_SOME = 64;
 constexpr uint64_t PF_TREE_WORK = 24u << 20;
@@ -83,7 +84,7 @@ struct PreArgs {
 // Every row sees all positions before `base`, and the nodes of its mask behind it.
 struct PreTree : PreArgs {
     const uint64_t * seen;                       // [n_q][words]
-    int words, n_nodes, out_type;                // N is base + n_nodes
+    int words, n_nodes;                          // N is base + n_nodes
     float * first;                               // [H][n_tile][32][D]: O of a segment that starts a tile and does not end it
                                                  // (where the other calls have it in their 32-bit output)
 };
@@ -275,11 +276,7 @@ SJK_DEV void dma16(gptr src, uint8_t * dst) {
 }
 SJK_DEV void vm_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// an output value of the call's type
-SJK_DEV void tree_out(const PreTree & a, size_t at, float y) {
-    if (a.out_type == SJK_F16) ((_Float16 *) a.out)[at] = (_Float16) y;
-    else ((__bf16 *) a.out)[at] = (__bf16) y;
-}
+SJK_DEV void tree_out(const PreTree & a, size_t at, float y) { ((__bf16 *) a.out)[at] = (__bf16) y; }
 
 template <int D, typename Args>
 __global__ __launch_bounds__(PF_NT) __attribute__((amdgpu_waves_per_eu(2))) void prefill_kernel(const Args a) {
@@ -1126,8 +1123,7 @@ bool sjk_prefill_takes_tree(const sjk_hip_view & v, int body, uint32_t N, int n_
     return tree_first(D) + tree_tiles(n_q, n_head, v.n_head_kv) * (size_t) v.n_head_kv * PF_ROWS * (size_t) D <= ws_part_slots(v) * ws_slot_floats(D);
 }
 
-int sjk_prefill_tree(const ExtCall & e, const int32_t * desc, uint32_t n_max, int n_q, int n_head, float scale, int n_nodes, int out_type,
-                     hipStream_t st) {
+int sjk_prefill_tree(const ExtCall & e, const int32_t * desc, uint32_t n_max, int n_q, int n_head, float scale, int n_nodes, hipStream_t st) {
     PreTree a = {};
     a.v = e.v; a.desc = desc; a.n_max = n_max; a.B = e.B; a.N = e.N; a.qpos0 = e.N - (uint32_t) n_nodes;
     a.n_q = n_q; a.n_head = n_head; a.gq = n_head / e.v.n_head_kv;
@@ -1136,7 +1132,7 @@ int sjk_prefill_tree(const ExtCall & e, const int32_t * desc, uint32_t n_max, in
     a.n_wg = n_cus();
     a.sc2 = scale * 1.4426950408889634f;
     a.q = e.q; a.out = (float *) e.out; a.part = ws_part(e.v);
-    a.seen = e.seen; a.words = (n_nodes + 63) / 64; a.n_nodes = n_nodes; a.out_type = out_type;
+    a.seen = e.seen; a.words = (n_nodes + 63) / 64; a.n_nodes = n_nodes;
     a.first = a.part + tree_first(e.v.lay.D);
     return e.v.lay.D == 128 ? launch_d<128>(a, st) : launch_d<256>(a, st);
 }

@@ -282,6 +282,36 @@ def test_attention_over_lists(lib, dev, D, H, per, bits, staging, sink_type):
     ctx.close()
 
 
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("bits", [(4, 4, 0), (3, 3, 0), (3, 3, 1)])
+def test_unlisted_groups_stay_out(lib, dev, D, bits):
+    """records that are not listed hold infinities and NaNs, the first group's among them; entries that name no group beside them"""
+    rng = np.random.default_rng(D + bits[0])
+    H, per, n = 2, 4, 9
+    ctx = Ctx(lib, dev, D, H, bits, n_groups=n, tail=30, seed=31)
+    lay = ctx.view.lay
+    q = queries(rng, 2, H * per, D)
+    sel = np.array([[[-1, 2, 3, 40, 7, -1], [-1, -1, -1, -1, -1, -1]], [[-3, -1, 5, 5, -1, 8], [1, 0, 2, 1, -1, 3]]], np.int32)
+    clean = [attend(lib, dev, ctx.view, ctx.B, ctx.N, ctx.N - 2, q, sel, t).bits() for t in (sjk.F32, sjk.F16, sjk.BF16)]
+    raw = dev.get(C.c_void_p(ctx.view.body), n * H * lay.bytes, np.uint8).reshape(n, H, lay.bytes)
+    bad = raw.copy()
+    for g in (0, 4, 6):
+        for h in range(H):
+            if (g, h) in ((0, 1),):
+                continue
+            for at, x in ((lay.k_scale, 0x7C00), (lay.k_zero, 0x7E00), (lay.k_tok, 0xFC00), (lay.v_ch, 0x7E00), (lay.v_scale, 0x7C00), (lay.v_zero, 0xFE00)):
+                bad[g, h, at + 10:at + 12] = np.array([x], np.uint16).view(np.uint8)
+    dev.upload(C.c_void_p(ctx.view.body), bad)
+    for t, want in zip((sjk.F32, sjk.F16, sjk.BF16), clean):
+        assert np.array_equal(attend(lib, dev, ctx.view, ctx.B, ctx.N, ctx.N - 2, q, sel, t).bits(), want), t
+    # the first group where it is an entry's own
+    sel[0, 0] = [0, 2, 3, 4, 7, 8]
+    got = parts.values(attend(lib, dev, ctx.view, ctx.B, ctx.N, ctx.N - 2, q, sel).bits(), sjk.F32).reshape(2, H, per, D)
+    assert not np.isfinite(got[0, 0]).any() and np.isfinite(got[0, 1]).all() and np.isfinite(got[1]).all()
+    dev.upload(C.c_void_p(ctx.view.body), raw)
+    ctx.close()
+
+
 def test_all_groups_listed_is_the_whole_context(lib, dev):
     """against sjk_hip_attend (its own tolerance), at a length where every workgroup has several records; and no groups at all"""
     rng = np.random.default_rng(3)
