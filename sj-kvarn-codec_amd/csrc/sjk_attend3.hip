@@ -3073,12 +3073,44 @@ __global__ __launch_bounds__(A4_NT) __attribute__((amdgpu_waves_per_eu(2))) void
     attend4_slot<D>(b->job[j], slot - b->slot_base[j]);
 }
 
-template <int D> __global__ __launch_bounds__(A3_NT) void ext_combine(const A3BatchT<A3Ext> b) {
+// Few partials a head (many tiles or short contexts share a launch): a wavefront merges a row by itself, four rows a workgroup
+constexpr int EXT_FEW = 32;
+template <int D> SJK_DEV void combine_few(const A3Ext & a, int h, int qi, int qt) {
+    constexpr int PS = A3_Q * (D + 2);
+    const int lane = threadIdx.x & 63, d = qt * 64 + lane;
+    const float * base = a.part + (size_t) h * a.n_wg * PS + qi * (D + 2);
+    float o[EXT_FEW];
+#pragma unroll
+    for (int k = 0; k < EXT_FEW; ++k) o[k] = k < a.n_wg ? base[(size_t) k * PS + 2 + d] : 0.0f;
+    float mk = -__builtin_inff(), lk = 0.0f;         // lane k holds (m, l) of partial k
+    if (lane < a.n_wg) {
+        mk = base[(size_t) lane * PS];
+        lk = base[(size_t) lane * PS + 1];
+    }
+    const float M = wave_max(mk);
+    const float f = (M == -__builtin_inff() || mk == -__builtin_inff()) ? 0.0f : __builtin_amdgcn_exp2f(mk - M);
+    const float L = wave_sum(f * lk);
+    float y = 0.0f;
+#pragma unroll
+    for (int k = 0; k < EXT_FEW; ++k)
+        if (k < a.n_wg) y = __builtin_fmaf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), k)), o[k], y);
+    const int r = a.row0 + qi, iq = r / a.gq, hq = h * a.gq + r % a.gq;
+    store_out(a.out, ((size_t) iq * a.n_head + hq) * D + d, a.out_type, L == 0.0f ? 0.0f : y / L);
+}
+// rows of block x: four where a job has few partials (blocks past 3 have none), else one
+template <int D> SJK_DEV void ext_combine_rows(const A3Ext & a, int cb) {
     __shared__ float s_M[4], s_L[4], s_O[4][64];
+    const int x = (int) blockIdx.x;
+    if (a.n_wg <= EXT_FEW) {
+        const int qi = 4 * x + __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
+        if (qi < a.n_rows) combine_few<D>(a, blockIdx.y, qi, cb);
+    } else if (x < a.n_rows) {
+        combine_row<D>(a, blockIdx.y, x, cb, s_M, s_L, &s_O[0][0]);
+    }
+}
+template <int D> __global__ __launch_bounds__(A3_NT) void ext_combine(const A3BatchT<A3Ext> b) {
     constexpr int NQ = D / 64;
-    const A3Ext & a = b.job[blockIdx.z / NQ];
-    if ((int) blockIdx.x >= a.n_rows) return;
-    combine_row<D>(a, blockIdx.y, blockIdx.x, blockIdx.z % NQ, s_M, s_L, &s_O[0][0]);
+    ext_combine_rows<D>(b.job[blockIdx.z / NQ], blockIdx.z % NQ);
 }
 
 // What a call is, for its plan on the host or on the device
@@ -3193,19 +3225,18 @@ __global__ __launch_bounds__(64) void ext_plan_kernel(const ExtArgs e0, float * 
 }
 
 template <int D> __global__ __launch_bounds__(A3_NT) void ext_combine_dyn(const A3BatchT<A3Ext> * __restrict__ b) {
-    __shared__ float s_M[4], s_L[4], s_O[4][64];
     constexpr int NQ = D / 64;
     const int z = (int) blockIdx.z / NQ, cb = (int) blockIdx.z % NQ;
     const A3Ext & a = b->job[z];
-    if ((int) blockIdx.x >= a.n_rows) return;
     if (a.n_nodes < 0) {
+        if ((int) blockIdx.x >= a.n_rows) return;
         const int r = a.row0 + (int) blockIdx.x;
         if (threadIdx.x < 64)
             store_out(a.out, ((size_t) (r / a.gq) * a.n_head + (int) blockIdx.y * a.gq + r % a.gq) * D + 64 * cb + (int) threadIdx.x, a.out_type,
                       __builtin_nanf(""));
         return;
     }
-    combine_row<D>(a, blockIdx.y, blockIdx.x, cb, s_M, s_L, &s_O[0][0]);
+    ext_combine_rows<D>(a, cb);
 }
 
 // one launch of the body's kernel over `grid`, from a table in the arguments (bt) or in memory (tp)
@@ -3301,8 +3332,10 @@ static int ext_launch(A3BatchT<A3Ext> & bt, int body, int H, hipStream_t st) {
         if (fits) break;
         if (pass == 1) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
     }
+    bool few = true;
+    for (int j = 0; j < bt.n_jobs; ++j) few = few && bt.job[j].n_wg <= EXT_FEW;
     return ext_kernels(body, D, body == 44 ? dim3((unsigned) bt.n_slots) : dim3((unsigned) bt.wg_base[bt.n_jobs], (unsigned) H),
-                       dim3(A3_Q, (unsigned) H, (unsigned) (D / 64 * bt.n_jobs)), &bt, nullptr, st);
+                       dim3(few ? A3_Q / 4 : A3_Q, (unsigned) H, (unsigned) (D / 64 * bt.n_jobs)), &bt, nullptr, st);
 }
 
 int sjk_attend_ext(const ExtCall * calls, int n, int n_q, int n_head, float scale, int top, int n_nodes, int out_type, hipStream_t st) {
