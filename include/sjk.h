@@ -612,8 +612,8 @@ int sjk_hip_seq_attend_batch(const sjk_hip_seq_job * jobs, int n_jobs, int il, i
  *
  * sjk_hip_attend_groups takes any ascending list: an entry that is no sealed group, or not above the entry before it, adds nothing.
  * With all groups listed the result is sjk_hip_attend's up to rounding. d_out [n_q][n_head][D] of out_type (SJK_F32, _F16, _BF16), rotated
- * basis. Sums and statistics have 32 bits; weights keep 22 bits for SJK_F32 outputs, those of 16-bit outputs are rounded to fp16 once
- * on sealed records. A row that sees nothing is zero. Infinities and NaNs of staged positions that a row does not see do not reach it.
+ * basis. Sums and statistics have 32 bits; weights keep 22 bits, those of SJK_BF16 outputs on scalar records are rounded to
+ * fp16 once. A row that sees nothing is zero. Infinities and NaNs of staged positions that a row does not see do not reach it.
  *
  * Query positions lie behind the sealed part: with B > S, qpos0 + 1 >= B, N >= B, and B at a group's end (SJKVARN_ERR_ARG otherwise).
  * d_q is fp32 [n_q][n_head][D], 16-byte aligned, and does not overlap d_out. Both use v->work as sjk_hip_attend does. A selection's

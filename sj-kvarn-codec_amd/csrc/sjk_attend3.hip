@@ -531,7 +531,8 @@ SJK_DEV void lds_reads_done(f4 & x0, f4 & x1, f4 & x2, f4 & x3) {
     asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x0), "+v"(x1), "+v"(x2), "+v"(x3) :: "memory");
 }
 
-template <int D, typename Args>
+// LOW (A3Ext, fp16 outputs): the weights P' as hi and lo parts
+template <int D, bool LOW, typename Args>
 __device__ __attribute__((always_inline)) inline void a4_records(const Args & a, A4Lds<D> & S, int h, int wgi, int ls) {
     constexpr bool EXT = is_ext<Args>;
     using GM = A4Geom<D>;
@@ -792,8 +793,7 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
         // exp2(s - mk) = P * 2^k; a row with no visible token has only -inf scores, and exp2(-inf - 0) = 0
         const float mk = anyv ? m_new - (float) kx : 0.0f;
         float psum = 0.0f, cv = 0.0f;
-        float lost = 0.0f;                       // EXT: what the rounding of P' took, sum of P Vscale 2^k - P'
-        u4 Ah[4];
+        u4 Ah[4], Al[LOW ? 4 : 1];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
 #pragma unroll
@@ -806,8 +806,18 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
             const u2 vs1 = *(const u2 *) (vmeta + GM::M_VSC + 2 * (32 * p + tbg + 8));
             const u2 vz0 = *(const u2 *) (vmeta + GM::M_VZE + 2 * (32 * p + tbg));
             const u2 vz1 = *(const u2 *) (vmeta + GM::M_VZE + 2 * (32 * p + tbg + 8));
-            Ah[p] = u4{mul_pk(sc[8 * p + 0], sc[8 * p + 1], vs0.x), mul_pk(sc[8 * p + 2], sc[8 * p + 3], vs0.y),
-                       mul_pk(sc[8 * p + 4], sc[8 * p + 5], vs1.x), mul_pk(sc[8 * p + 6], sc[8 * p + 7], vs1.y)};
+            if constexpr (LOW) {
+                const uint32_t vs[4] = {vs0.x, vs0.y, vs1.x, vs1.y};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const u2 hl = mul_split(sc[8 * p + 2 * u], sc[8 * p + 2 * u + 1], vs[u]);
+                    Ah[p][u] = hl.x;
+                    Al[p][u] = hl.y;
+                }
+            } else {
+                Ah[p] = u4{mul_pk(sc[8 * p + 0], sc[8 * p + 1], vs0.x), mul_pk(sc[8 * p + 2], sc[8 * p + 3], vs0.y),
+                           mul_pk(sc[8 * p + 4], sc[8 * p + 5], vs1.x), mul_pk(sc[8 * p + 6], sc[8 * p + 7], vs1.y)};
+            }
             cv = fma_lo(sc[8 * p + 0], vz0.x, cv);
             cv = fma_hi(sc[8 * p + 1], vz0.x, cv);
             cv = fma_lo(sc[8 * p + 2], vz0.y, cv);
@@ -816,26 +826,16 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
             cv = fma_hi(sc[8 * p + 5], vz1.x, cv);
             cv = fma_lo(sc[8 * p + 6], vz1.y, cv);
             cv = fma_hi(sc[8 * p + 7], vz1.y, cv);
-            if constexpr (EXT) {
-                const uint32_t vs[4] = {vs0.x, vs0.y, vs1.x, vs1.y};
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    lost = fma_lo(sc[8 * p + 2 * u], vs[u], lost);
-                    lost = fma_hi(sc[8 * p + 2 * u + 1], vs[u], lost);
-                    lost = fma_lo(-1.0f, Ah[p][u], lost);
-                    lost = fma_hi(-1.0f, Ah[p][u], lost);
-                }
-            }
         }
         if constexpr (EXT) {
             if (!live) {                         // a scale that is no number makes a NaN with a weight of zero
 #pragma unroll
-                for (int p = 0; p < 4; ++p) Ah[p] = u4{0u, 0u, 0u, 0u};
+                for (int p = 0; p < 4; ++p) {
+                    Ah[p] = u4{0u, 0u, 0u, 0u};
+                    if constexpr (LOW) Al[p] = Ah[p];
+                }
             }
         }
-        // A weight's rounding is multiplied by its token's code, 0 .. 15; with 7.5 of it given back through the zero point the
-        // factor is -7.5 .. 7.5 (3.0e-4 -> 1.3e-4 of a result)
-        if constexpr (EXT) cv = __builtin_fmaf(7.5f, lost, cv);
         lds_reads_done();
         if constexpr (GM::NMETA == 1)
             if (!last) issue_kmeta(rb_next, 0);  // the K scales of this record have been read
@@ -890,6 +890,10 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
                     const u4 b1 = u4{w0 & M1, w1 & M1, x0 & M1, x1 & M1};
                     t[2 * jj] = mfma32(Ah[p], b0, t[2 * jj]);
                     t[2 * jj + 1] = mfma32(Ah[p], b1, t[2 * jj + 1]);
+                    if constexpr (LOW) {
+                        t[2 * jj] = mfma32(Al[p], b0, t[2 * jj]);
+                        t[2 * jj + 1] = mfma32(Al[p], b1, t[2 * jj + 1]);
+                    }
                 }
             // O += Vch * 2^-k * t
 #pragma unroll
@@ -1781,7 +1785,7 @@ template <int D> __global__ __launch_bounds__(A3_NT) void attend3_combine(const 
 // CU slot loc of job a. The job must sit in memory the compiler may read again at any time (kernel arguments, or a
 // plan written before the launch), not in registers: a spill would be a vector memory operation inside the
 // streams' hand-counted vmcnt waits.
-template <int D, typename Args> __device__ __attribute__((always_inline)) inline void attend4_slot(const Args & a, int loc) {
+template <int D, bool LOW = false, typename Args> __device__ __attribute__((always_inline)) inline void attend4_slot(const Args & a, int loc) {
     __shared__ A4Lds<D> s;
     asm volatile("" ::"s"(a.slots), "s"(a.rec_slots), "s"(a.rec_a), "s"(a.n_rec), "s"(a.sink_end), "s"(a.v.S),
                  "s"(a.v.n_head_kv), "s"(a.v.body), "s"(a.v.blocks), "s"(a.n_chunk), "s"(a.sink_chunks), "s"(a.body_end),
@@ -1799,7 +1803,7 @@ template <int D, typename Args> __device__ __attribute__((always_inline)) inline
             });
         });
     else
-        a4_records<D>(a, s, h, ls, ls);
+        a4_records<D, LOW>(a, s, h, ls, ls);
 }
 
 template <int D>
@@ -1929,7 +1933,7 @@ __device__ __attribute__((always_inline)) inline void asc_records(const Args & a
     const int H = V.n_head_kv;
     const int bk = B44 ? 4 : L.bits_k, bv = B44 ? 4 : L.bits_v;
     bool fine = false;                           // EXT: the weights' low parts too
-    if constexpr (EXT) fine = B44 || a.out_type == SJK_F32;
+    if constexpr (EXT) fine = B44 || a.out_type != SJK_BF16;
     const uint32_t RB = L.bytes;
     const ScStage st = sc_stage(L);
     // the record's bytes, 16 per thread and step (every record is a whole number of 16-byte units, at most
@@ -3007,19 +3011,19 @@ extern "C" int sjk_hip_attend_dyn(const sjk_hip_view * v, const int32_t * d_desc
 // attention over listed groups, and of drafted nodes (A3Ext)
 // ------------------------------------------------------------------------------------------------
 //
-// The kernels are the bodies' own; those of the trellis and scalar bodies take the weights P' as hi and lo parts here, so that an
-// output keeps the precision of 32 bits (ext_body: which kernel takes 4/4 records).
+// The kernels are the bodies' own; they take the weights P' as hi and lo parts here, so that an output keeps the precision of 32 bits (but
+// for bf16 outputs of scalar records; ext_body: which kernel takes 4/4 records).
 // A tile of a list's call is one query position (16 of its heads): each position has a list of its own per KV head.
 //
-// What bounds them: the streaming wavefronts HBM (384 of 3,100 groups for 3 positions, 8 KV heads of 128: 47.1 us for 173 MB, 3.67 TB/s); the
-// staged kernel of the scalar bodies latency where a workgroup has two records (64 of 736 groups, D = 256: 17.8 us, of them 4 for all
-// workgroups to start, 6 to the first record, 5 a record) and vector issue where it has more (32 groups of 8 sequences, 3/3: 24.5 us, 12 of them
-// vector instructions). The combine takes 3.9 to 6.7 us more.
+// What bounds them: the streaming wavefronts HBM (384 of 3,100 groups for 3 positions, 8 KV heads of 128, fp16 out: 50 us for 173 MB, 3.4 TB/s); the
+// staged kernel of the scalar bodies latency where a workgroup has two records (64 of 736 groups, D = 256: 17.0 us, of them 6 to the
+// first record - arguments, list, record, one after the other - and 5 a record) and vector issue where it has more (32 groups of 8 sequences, 3/3: 24.2 us, 12 of them
+// vector instructions). The combine takes 3.9 to 4.7 us more.
 
 namespace sjk {
 
-// A workgroup's place in a grid of (workgroups of the launch, KV heads): workgroups start one after the other (512 of them in 4.3 us), so the
-// heads take turns and a job's record workgroups, which take longest, come before its row workgroups
+// A workgroup's place in a grid of (workgroups of the launch, KV heads): the heads take turns, and a job's record workgroups, which take
+// longest, come before its row workgroups (64 of 736 groups, D = 256: 22.0 -> 21.5 us; trees of many tiles 2 to 4%)
 SJK_DEV int ext_place(int & h) {
     const uint32_t id = blockIdx.x + gridDim.x * blockIdx.y;
     h = (int) (id % gridDim.y);
@@ -3053,16 +3057,16 @@ __global__ __launch_bounds__(A3_NT) __attribute__((amdgpu_waves_per_eu(2))) void
     attend3_job<BK, BV, D>(b->job[j], (int) blockIdx.x - b->wg_base[j]);
 }
 
-template <int D>
+template <int D, bool LOW>
 __global__ __launch_bounds__(A4_NT) __attribute__((amdgpu_waves_per_eu(2))) void ext_stream_kernel(const A3BatchT<A3Ext> b) {
     const int slot = (int) blockIdx.x;
     int j = 0;
 #pragma unroll
     for (int k = 1; k < maxj<A3Ext>; ++k) j += (k < b.n_jobs && slot >= b.slot_base[k]) ? 1 : 0;
     j = __builtin_amdgcn_readfirstlane(j);
-    attend4_slot<D>(b.job[j], slot - b.slot_base[j]);
+    attend4_slot<D, LOW>(b.job[j], slot - b.slot_base[j]);
 }
-template <int D>
+template <int D, bool LOW>
 __global__ __launch_bounds__(A4_NT) __attribute__((amdgpu_waves_per_eu(2))) void ext_stream_kernel_dyn(const A3BatchT<A3Ext> * __restrict__ b) {
     const int slot = (int) blockIdx.x;
     if (slot >= b->n_slots) return;
@@ -3070,7 +3074,7 @@ __global__ __launch_bounds__(A4_NT) __attribute__((amdgpu_waves_per_eu(2))) void
 #pragma unroll
     for (int k = 1; k < maxj<A3Ext>; ++k) j += (k < b->n_jobs && slot >= b->slot_base[k]) ? 1 : 0;
     j = __builtin_amdgcn_readfirstlane(j);
-    attend4_slot<D>(b->job[j], slot - b->slot_base[j]);
+    attend4_slot<D, LOW>(b->job[j], slot - b->slot_base[j]);
 }
 
 // Few partials a head (many tiles or short contexts share a launch): a wavefront merges a row by itself, four rows a workgroup
@@ -3241,7 +3245,7 @@ template <int D> __global__ __launch_bounds__(A3_NT) void ext_combine_dyn(const 
 
 // one launch of the body's kernel over `grid`, from a table in the arguments (bt) or in memory (tp)
 // (the grid of a body's kernels: x workgroups for each KV head in y, or CU slots of all heads in x)
-static int ext_kernels(int body, int D, dim3 grid, dim3 cgrid, const A3BatchT<A3Ext> * bt, const A3BatchT<A3Ext> * tp, hipStream_t st) {
+static int ext_kernels(int body, bool low, int D, dim3 grid, dim3 cgrid, const A3BatchT<A3Ext> * bt, const A3BatchT<A3Ext> * tp, hipStream_t st) {
 #define SJK_EXT(K, KD, NT)                                          \
     do {                                                            \
         if (bt) hipLaunchKernelGGL(K, grid, dim3(NT), 0, st, *bt);  \
@@ -3250,8 +3254,13 @@ static int ext_kernels(int body, int D, dim3 grid, dim3 cgrid, const A3BatchT<A3
     const bool d1 = D == 128;
     switch (body) {
     case 44:
-        if (d1) SJK_EXT(ext_stream_kernel<128>, ext_stream_kernel_dyn<128>, A4_NT);
-        else SJK_EXT(ext_stream_kernel<256>, ext_stream_kernel_dyn<256>, A4_NT);
+        if (low) {
+            if (d1) SJK_EXT((ext_stream_kernel<128, true>), (ext_stream_kernel_dyn<128, true>), A4_NT);
+            else SJK_EXT((ext_stream_kernel<256, true>), (ext_stream_kernel_dyn<256, true>), A4_NT);
+        } else {
+            if (d1) SJK_EXT((ext_stream_kernel<128, false>), (ext_stream_kernel_dyn<128, false>), A4_NT);
+            else SJK_EXT((ext_stream_kernel<256, false>), (ext_stream_kernel_dyn<256, false>), A4_NT);
+        }
         break;
     case 45:
         if (d1) SJK_EXT((ext_scalar_kernel<128, true>), (ext_scalar_kernel_dyn<128, true>), SC_NT);
@@ -3287,8 +3296,9 @@ static int ext_kernels(int body, int D, dim3 grid, dim3 cgrid, const A3BatchT<A3
 }
 
 // The kernel of a body: as a3_body, but 4/4 records of a 32-bit output go through the scalar bodies' kernel (45), which keeps the
-// weights' low parts; the streaming wavefronts round them to fp16 once (3e-4 of a result where that one has 4e-7, the rounding
-// of a 16-bit output 2e-4 or 2e-3).
+// weights' low parts and codes around zero (4e-7 of a result against float64). The streaming wavefronts of fp16 outputs keep the low parts
+// (2.2e-4, the output's own rounding 2.0e-4; without them 3.1e-4 and 46 instead of 50 us for 384 groups of 3 positions), those of bf16 outputs
+// round the weights to fp16 once (3e-4 beside the output's 1.7e-3).
 static int ext_body(const sj_kvarn_layout & l, int out_type) {
     const int body = a3_body(l);
     return body == 44 && out_type == SJK_F32 ? 45 : body;
@@ -3334,7 +3344,7 @@ static int ext_launch(A3BatchT<A3Ext> & bt, int body, int H, hipStream_t st) {
     }
     bool few = true;
     for (int j = 0; j < bt.n_jobs; ++j) few = few && bt.job[j].n_wg <= EXT_FEW;
-    return ext_kernels(body, D, body == 44 ? dim3((unsigned) bt.n_slots) : dim3((unsigned) bt.wg_base[bt.n_jobs], (unsigned) H),
+    return ext_kernels(body, bt.job[0].out_type == SJK_F16, D, body == 44 ? dim3((unsigned) bt.n_slots) : dim3((unsigned) bt.wg_base[bt.n_jobs], (unsigned) H),
                        dim3(few ? A3_Q / 4 : A3_Q, (unsigned) H, (unsigned) (D / 64 * bt.n_jobs)), &bt, nullptr, st);
 }
 
@@ -3398,7 +3408,7 @@ int sjk_attend_ext_dyn(const ExtCall & call, const int32_t * desc, uint32_t n_ma
         hipLaunchKernelGGL(ext_plan_kernel, dim3(1), dim3(64), 0, st, e, ws_part(call.v), plan);
         // the most workgroups per KV head that a table's jobs take: two each for the rounding of its split, 7 for its alignment
         const dim3 grid = e.body == 44 ? dim3((unsigned) (H * (e.slots + 2 * e.n_tiles))) : dim3((unsigned) (e.slots + 9 * e.n_tiles), (unsigned) H);
-        if (const int rc = ext_kernels(e.body, D, grid, dim3(A3_Q, (unsigned) H, (unsigned) (D / 64 * e.n_tiles)), nullptr, plan, st)) return rc;
+        if (const int rc = ext_kernels(e.body, out_type == SJK_F16, D, grid, dim3(A3_Q, (unsigned) H, (unsigned) (D / 64 * e.n_tiles)), nullptr, plan, st)) return rc;
     }
     return 0;
 }
