@@ -3015,9 +3015,9 @@ extern "C" int sjk_hip_attend_dyn(const sjk_hip_view * v, const int32_t * d_desc
 // for bf16 outputs of scalar records; ext_body: which kernel takes 4/4 records).
 // A tile of a list's call is one query position (16 of its heads): each position has a list of its own per KV head.
 //
-// What bounds them: the streaming wavefronts HBM (384 of 3,100 groups for 3 positions, 8 KV heads of 128, fp16 out: 50 us for 173 MB, 3.4 TB/s); the
-// staged kernel of the scalar bodies latency where a workgroup has two records (64 of 736 groups, D = 256: 17.0 us, of them 6 to the
-// first record - arguments, list, record, one after the other - and 5 a record) and vector issue where it has more (32 groups of 8 sequences, 3/3: 24.2 us, 12 of them
+// What bounds them: the streaming wavefronts HBM (384 of 3,100 groups for 3 positions, 8 KV heads of 128, fp16 out: 50.8 us for 173 MB, 3.4 TB/s); the
+// staged kernel of the scalar bodies latency where a workgroup has two records (64 of 736 groups, D = 256: 17.6 us, of them 6 to the
+// first record - arguments, list, record, one after the other - and 5 a record) and vector issue where it has more (32 groups of 8 sequences, 3/3: 24.4 us, 12 of them
 // vector instructions). The combine takes 3.9 to 4.7 us more.
 
 namespace sjk {
