@@ -610,7 +610,8 @@ int sjk_hip_seq_attend_batch(const sjk_hip_seq_job * jobs, int n_jobs, int il, i
  * group; a score that is not a number is above all others. d_sel [n_q][n_head_kv][top] (int32) is in ascending order, -1 where there are fewer
  * groups than top.
  *
- * sjk_hip_attend_groups takes any ascending list: an entry that is no sealed group, or not above the entry before it, adds nothing.
+ * sjk_hip_attend_groups takes any ascending list, longer than the groups are many or not: an entry that is no sealed group, or not above the
+ * entry before it, adds nothing, wherever it stands.
  * With all groups listed the result is sjk_hip_attend's up to rounding. d_out [n_q][n_head][D] of out_type (SJK_F32, _F16, _BF16), rotated
  * basis. Sums and statistics have 32 bits; weights keep 22 bits, those of SJK_BF16 outputs on scalar records are rounded to
  * fp16 once. A row that sees nothing is zero. Infinities and NaNs of staged positions that a row does not see do not reach it.

@@ -129,6 +129,32 @@ SJK_DEV int ext_group(const A3Ext & a, int h, int c) {
     const int g = s[c], before = c ? s[c - 1] : -1;
     return g > before && (uint32_t) g < a.n_grp ? g : -1;
 }
+// Records [r0, r1) of a job as entries of KV head h's list. A list of no more entries than there are groups is cut by its entries. A longer one is
+// cut by the groups that it names, so that a short context with lists of a fixed length is shared out by its groups: record r is
+// then the r-th entry that names one, wherever it stands, and the last range goes on to the last one that does. Every wavefront looks by
+// itself, 64 entries at a time (10 groups of 8 sequences, 3/3, lists of 64: 20.1 us; cut by entries 34).
+SJK_DEV void ext_range(const A3Ext & a, int h, int & r0, int & r1) {
+    if (!a.sel || a.n_rec >= a.top || r0 >= r1) return;
+    const int lane = (int) (threadIdx.x & 63);
+    const int32_t * s = a.sel + (size_t) h * a.top;
+    const uint32_t top = (uint32_t) a.top;
+    const bool last = r1 == a.n_rec;
+    uint32_t e0 = top, e1 = top;
+    int seen = 0;                                // entries that name a group before these 64
+    for (uint32_t i0 = 0; i0 < top && (e0 == top || e1 == top || last); i0 += 64) {
+        const uint32_t i = i0 + (uint32_t) lane;
+        const int g = i < top ? s[i] : -1, before = i && i < top ? s[i - 1] : -1;
+        const uint64_t m = __ballot(g > before && (uint32_t) g < a.n_grp);
+        const int n = seen + __popcll(m), at = seen + (int) __builtin_amdgcn_mbcnt_hi((uint32_t) (m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) m, 0));
+        const bool mine = (m >> lane) & 1u;
+        if (r0 >= seen && r0 < n) e0 = i0 + (uint32_t) __builtin_ctzll(__ballot(mine && at == r0));
+        if (last && m) e1 = i0 + 64u - (uint32_t) __builtin_clzll(m);
+        if (!last && r1 >= seen && r1 < n) e1 = i0 + (uint32_t) __builtin_ctzll(__ballot(mine && at == r1));
+        seen = n;
+    }
+    r0 = __builtin_amdgcn_readfirstlane((int) e0);
+    r1 = __builtin_amdgcn_readfirstlane((int) e1);
+}
 // The 16 positions from p0 on that row n of the tile sees of the nodes and of what lies before them (a bit each)
 SJK_DEV uint32_t ext_seen(const A3Ext & a, int n, uint32_t p0) {
     if (p0 + 16u <= a.base) return 0xFFFFu;
@@ -546,21 +572,30 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
     // those at the end has the same number, so that every SIMD, whichever two wavefronts it holds, has the same)
     const int per = a.rec_a;
     const int base = (ls * A4_NW + w) * per;
-    const int r0 = __builtin_amdgcn_readfirstlane(base < a.n_rec ? base : a.n_rec);
-    const int r1 = __builtin_amdgcn_readfirstlane(base + per < a.n_rec ? base + per : a.n_rec);
+    int r0 = __builtin_amdgcn_readfirstlane(base < a.n_rec ? base : a.n_rec);
+    int r1 = __builtin_amdgcn_readfirstlane(base + per < a.n_rec ? base + per : a.n_rec);
+    if constexpr (EXT) ext_range(a, h, r0, r1);  // entries of the list
     const int nrec = r1 - r0, C = CPR * nrec;
     uint8_t * ring = S.r.wv[w].ring[0];
     // the block table is read through the constant address space, i.e. by a scalar load: a vector load
     // would have to wait for every load in flight (the compiler cannot order it against the stream)
     const __attribute__((address_space(4))) uint32_t * blocks = (const __attribute__((address_space(4))) uint32_t *) V.blocks;
     auto rec_base = [&](int r) {
-        uint32_t gi = (a.sink_end + (uint32_t) r * 128u - V.S) / 128u;
-        if constexpr (EXT) {                     // an entry that names no group streams group 0, and counts for nothing (live)
-            const int e = ext_group(a, h, r);
-            gi = e < 0 ? 0u : (uint32_t) e;
-        }
+        const uint32_t gi = (a.sink_end + (uint32_t) r * 128u - V.S) / 128u;
         const uint32_t blk = blocks ? blocks[gi] : gi;
         return V.body + ((size_t) blk * H + h) * RL::BYTES;
+    };
+    // A3Ext: the record of entry e, or of the first one behind it that names a group (e is then that one's place); null: there is
+    // none. Entries that name no group are passed over: they cost a scalar load, and nothing of them is streamed.
+    auto rec_from = [&](int & e) -> const uint8_t * {
+        if constexpr (EXT)
+            for (; e < r1; ++e) {
+                const int gi = ext_group(a, h, e);
+                if (gi < 0) continue;
+                const uint32_t blk = blocks ? blocks[gi] : (uint32_t) gi;
+                return V.body + ((size_t) blk * H + h) * RL::BYTES;
+            }
+        return nullptr;
     };
     auto dma = [&](const uint8_t * src, uint8_t * dst) {
         __builtin_amdgcn_global_load_lds((const void *) src, SJK_LDS(dst), 16, 0, A4_POL);
@@ -604,8 +639,10 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
     // Only chunk 0 goes out with the scales before the barrier: every wavefront's first chunk then comes
     // ahead of the second and third chunks of all the others (the start is a burst of all wavefronts).
     const uint8_t * rb_cur = nullptr;
-    if (nrec > 0) {
-        rb_cur = rec_base(r0);
+    int e_cur = r0, e_next = r1;                 // A3Ext: the entries of rb_cur and rb_next
+    if constexpr (EXT) rb_cur = rec_from(e_cur);
+    if (EXT ? rb_cur != nullptr : nrec > 0) {
+        if constexpr (!EXT) rb_cur = rec_base(r0);
         issue_kmeta(rb_cur, 0);
         issue_vmeta(rb_cur, 0);
         issue_chunk(rb_cur, 0);
@@ -618,7 +655,8 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (nrec > 0) {
+    static_assert(A4_SLOTS <= CPR, "the first chunks are one record's");
+    if (EXT ? rb_cur != nullptr : nrec > 0) {
 #pragma unroll
         for (int c = 1; c < A4_SLOTS; ++c) issue_chunk(rb_cur, c);
     }
@@ -634,13 +672,16 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
     const uint32_t M0 = 0x000F000Fu, M1 = 0x00F000F0u;
     const float * qlane = &S.r.q[n][0];
 
-    const uint8_t * rb_next = (nrec > 1) ? rec_base(r0 + 1) : nullptr;
-    for (int i = 0; i < nrec; ++i) {
-        const bool last = i + 1 == nrec;
-        const uint8_t * rb_after = (i + 2 < nrec) ? rec_base(r0 + i + 2) : nullptr;
+    const uint8_t * rb_next = nullptr;
+    if constexpr (EXT) rb_next = rec_from(e_next = e_cur + 1);
+    else rb_next = (nrec > 1) ? rec_base(r0 + 1) : nullptr;
+    for (int i = 0; EXT ? rb_cur != nullptr : i < nrec; ++i) {
+        const bool last = EXT ? rb_next == nullptr : i + 1 == nrec;
+        int e_after = e_next + 1;
+        const uint8_t * rb_after = nullptr;
+        if constexpr (EXT) rb_after = rec_from(e_after);
+        else rb_after = (i + 2 < nrec) ? rec_base(r0 + i + 2) : nullptr;
         const uint32_t p0 = a.sink_end + (uint32_t) (r0 + i) * 128u;
-        bool live = true;
-        if constexpr (EXT) live = ext_group(a, h, r0 + i) >= 0;
         const int mb = GM::NMETA == 1 ? 0 : (i & 1);              // this record's scale buffer set
         const uint8_t * kmeta = kmeta_of(mb);
         const uint8_t * vmeta = vmeta_of(mb);
@@ -671,7 +712,12 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
             }
         };
         auto refill = [&](int c) {               // after chunk c has been read
-            if (c + A4_SLOTS < C) issue_chunk((c + A4_SLOTS) / CPR == i ? rb_cur : rb_next, c + A4_SLOTS);
+            if constexpr (EXT) {
+                const bool same = (c + A4_SLOTS) / CPR == i;
+                if (same || !last) issue_chunk(same ? rb_cur : rb_next, c + A4_SLOTS);
+            } else {
+                if (c + A4_SLOTS < C) issue_chunk((c + A4_SLOTS) / CPR == i ? rb_cur : rb_next, c + A4_SLOTS);
+            }
         };
 
         // ---- QK, one chunk of 64 channels at a time ----
@@ -682,7 +728,7 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             const int c = CPR * i + s;
-            if (s == 0) prio_by_progress(c, C);
+            if (s == 0) prio_by_progress(EXT ? CPR * (e_cur - r0) : c, C);
             wait_unit(s);
             const uint8_t * ck = ring + (c % A4_SLOTS) * A4_CHUNK + ((n >> 3) * 4 + g) * 128 + 16 * (n & 7);
             u4 kw[4];
@@ -762,12 +808,7 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
             sc[8 * p + 6] = mul_lo(xh[2], kb.y);
             sc[8 * p + 7] = mul_hi(xh[3], kb.y);
         }
-        if constexpr (EXT) {
-            if (!live) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) sc[e] = -__builtin_inff();
-            }
-        } else if (p0 + 128u > qend_min) {
+        if (!EXT && p0 + 128u > qend_min) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
                 const uint32_t tok = (uint32_t) (32 * (e >> 3) + tbg + (e & 3) + 8 * ((e >> 2) & 1));
@@ -827,21 +868,11 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
             cv = fma_lo(sc[8 * p + 6], vz1.y, cv);
             cv = fma_hi(sc[8 * p + 7], vz1.y, cv);
         }
-        if constexpr (EXT) {
-            if (!live) {                         // a scale that is no number makes a NaN with a weight of zero
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    Ah[p] = u4{0u, 0u, 0u, 0u};
-                    if constexpr (LOW) Al[p] = Ah[p];
-                }
-            }
-        }
         lds_reads_done();
         if constexpr (GM::NMETA == 1)
             if (!last) issue_kmeta(rb_next, 0);  // the K scales of this record have been read
         psum = rows_sum(psum);
         cv = rows_sum(cv);
-        if constexpr (EXT) cv = live ? cv : 0.0f;
         m_run = m_new;
         l_run = l_run * alpha + psum * pinv;
         {   // unconditional: behind a branch the compiler kept O in two register sets (128 moves per record)
@@ -865,7 +896,7 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
 #pragma unroll
         for (int J2 = 0; J2 < NS; ++J2) {
             const int c = CPR * i + NS + J2;
-            if (J2 == 0) prio_by_progress(c, C);
+            if (J2 == 0) prio_by_progress(EXT ? CPR * (e_cur - r0) + NS : c, C);
             wait_unit(NS + J2);
             const uint8_t * cvp = ring + (c % A4_SLOTS) * A4_CHUNK + ((g >> 1) * 4 + (n >> 3)) * 128 + 16 * (n & 7) + 8 * (g & 1);
             u2 vw[4][2];
@@ -899,8 +930,7 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
 #pragma unroll
             for (int jj = 0; jj < 2; ++jj) {
                 const int J = 2 * J2 + jj;
-                float v0 = h2f(vch[jj] & 0xFFFFu) * pinv * 0x1p24f, v1 = h2f(vch[jj] >> 16) * pinv * 0x1p20f;
-                if constexpr (EXT) { v0 = live ? v0 : 0.0f; v1 = live ? v1 : 0.0f; }
+                const float v0 = h2f(vch[jj] & 0xFFFFu) * pinv * 0x1p24f, v1 = h2f(vch[jj] >> 16) * pinv * 0x1p20f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     O[2 * J][r] = __builtin_fmaf(v0, t[2 * jj][r], O[2 * J][r]);
@@ -912,6 +942,8 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
             if (!last) issue_vmeta(rb_next, 0);  // the V scales of this record have been read (lgkmcnt above)
         rb_cur = rb_next;
         rb_next = rb_after;
+        e_cur = e_next;
+        e_next = e_after;
     }
     // the stream is done (its last wait was vmcnt(0)) and its LDS reads have returned: the wavefront's O
     // tiles go to its own area while the others still run. O tile j = 2J + m, column n holds channel
@@ -941,6 +973,7 @@ __device__ __attribute__((always_inline)) inline void a3_trellis(const Args & a,
     const int H = V.n_head_kv;
     // the first record's loads go out before anything else
     constexpr int NV = RL::BYTES / 16, PF = (NV + A3_NT - 1) / A3_NT;
+    if constexpr (EXT) ext_range(a, h, r0, r1);
     u4 pf[PF];
     int held = -1;                               // EXT: the entry whose record is in the registers
     auto fetch = [&](int c) {
@@ -1940,6 +1973,7 @@ __device__ __attribute__((always_inline)) inline void asc_records(const Args & a
     // 4/3 or 3/4: 112 D + 6 D + 768 bytes); the next record waits in registers while this one is computed
     constexpr int PF = (((B44 ? 128 : 112) * D + 6 * D + 768) / 16 + SC_NT - 1) / SC_NT;
     const int nv = (int) (RB / 16u);
+    if constexpr (EXT) ext_range(a, h, r0, r1);
     u4 pf[PF];
     int held = -1;                               // EXT: the entry whose record is in the registers
     auto fetch = [&](int c) {
@@ -3175,7 +3209,7 @@ __host__ __device__ static void ext_plan(const ExtArgs & e, A3Ext & a, int k) {
     if (e.c.sel) {
         a.sel = e.c.sel + (size_t) pos * v.n_head_kv * e.top;
         a.top = e.top;
-        if (a.n_rec > e.top) a.n_rec = e.top;
+        if (a.n_rec > e.top) a.n_rec = e.top;    // (the records to share out, not the entries to look at: ext_range)
     }
     if (e.c.seen) {
         a.seen = e.c.seen;

@@ -1,0 +1,95 @@
+"""Listed groups and drafted nodes at their edges, on the GPU: lists longer than the sealed groups are many, descriptors that hold more
+than the view or less than the call reads, selections whose jobs share a workspace, long paths and many layers of an acceptance."""
+import ctypes as C
+import sys
+
+import numpy as np
+import pytest
+
+import cabi
+import parts
+import test_gpu_groups as groups
+import test_gpu_tree as trees
+from parts import G, S, Ctx, Graph, Out, attention, check, descriptor
+
+sys.path.insert(0, cabi.PKG)
+import sjk  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+TYPES = (sjk.F32, sjk.F16, sjk.BF16)
+CAPACITY = -109
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return sjk.load()
+
+
+@pytest.fixture
+def dev():
+    d = sjk.Device()
+    yield d
+    d.sync()
+    d.free_all()
+
+
+# ---- lists ----
+
+def named(entries, n):
+    """the groups that a list names: entries of [0, n) that are above the entry before them"""
+    return [g for j, g in enumerate(entries) if 0 <= g < n and (j == 0 or g > entries[j - 1])]
+
+
+def spread(rng, n, top):
+    """an ascending list of `top` entries whose groups stand anywhere among repeats, -1 before the first"""
+    at = np.sort(rng.choice(top, min(n, top), replace=False))
+    x = np.full(top, -1)
+    for g, i in enumerate(at):
+        x[i:] = g
+    return x.tolist()
+
+
+@pytest.mark.parametrize("D,H,per", [(128, 2, 4), (256, 1, 5)])
+@pytest.mark.parametrize("bits", groups.BODIES, ids=groups.IDS)
+def test_lists_longer_than_the_groups(lib, dev, D, H, per, bits):
+    """every entry of a list counts, wherever it stands: -1 and repeats ahead of it, long runs of them, whole lists of them; eager, captured
+    and in a batch"""
+    rng = np.random.default_rng(D + 10 * bits[0] + bits[1])
+    n_q = 2
+    st = dev.stream()
+    for n, tops in ((1, (2, 40)), (2, (3, 300)), (3, (5, 6, 700))):
+        ctx = Ctx(lib, dev, D, H, bits, n_groups=n, tail=21, seed=40 + n)
+        K, V = ctx.rows(ctx.N)
+        qpos0 = ctx.N - n_q
+        for top in tops:
+            rows = [spread(rng, n, top) for _ in range(n_q * H)]
+            if top == 6:
+                rows[1] = [-1] * top
+            rows[0] = [-1] * (top - n) + list(range(n))               # the groups behind everything else
+            rows[-1] = [0] * (top - n + 1) + list(range(1, n))
+            pick = [rows[i * H:(i + 1) * H] for i in range(n_q)]
+            lists = [[named(x, n) for x in r] for r in pick]
+            assert lists[0][0] == list(range(n)) and lists[-1][-1] == list(range(n))
+            sel = np.array(pick, np.int32)
+            q = groups.queries(rng, n_q, H * per, D)
+            want, tol = attention(q, K, V, groups.seen_of(ctx, lists, n_q, qpos0), D ** -0.5)
+            for t in TYPES:
+                eager = groups.attend(lib, dev, ctx.view, ctx.B, ctx.N, qpos0, q, sel, t).bits()
+                check(parts.values(eager, t).reshape(q.shape), want, tol, t, (n, top, t))
+                out, desc = Out(dev, q.size, t), dev.put(descriptor(ctx.B, ctx.N, qpos0))
+                dq, ds = dev.put(q), dev.put(sel)
+                g = Graph(dev, st, [lambda: lib.sjk_hip_attend_groups_dyn(C.byref(ctx.view), desc, ctx.N + 9, n_q, H * per, dq, D ** -0.5, ds, top,
+                                                                          t, out.at, st)])
+                for _ in range(3):
+                    g.replay()
+                    assert np.array_equal(out.bits(), eager), (n, top, t)
+                    groups.attend(lib, dev, ctx.view, ctx.B, ctx.N, qpos0, q, sel, t).bits()
+                g.close()
+                jobs = (sjk.GroupsJob * 3)()
+                outs = [Out(dev, q.size, t) for _ in jobs]
+                for j, o in zip(jobs, outs):
+                    j.v, j.B, j.N, j.qpos0, j.d_q, j.d_sel, j.d_out = ctx.view, ctx.B, ctx.N, qpos0, dq, ds, o.at
+                sjk.check(lib.sjk_hip_attend_groups_batch(jobs, 3, n_q, H * per, D ** -0.5, top, t, None), "batch")
+                for o in outs:
+                    check(o.get().reshape(q.shape), want, tol, t, (n, top, t))
+        ctx.close()
