@@ -3227,7 +3227,7 @@ SJK_DEV bool ext_desc(ExtArgs & e) {
     const uint64_t N = e.c.seen ? last : (uint64_t) (uint32_t) iN;
     const uint32_t B = (uint32_t) iB, bend = B < v.S ? v.S : B;
     const uint64_t pend = N < last ? N : last;
-    const bool ok = iB >= 0 && iN >= 0 && iQ >= 0 && N <= e.n_max && (B <= v.S || ((B - v.S) % 128u == 0u && B <= N &&
+    const bool ok = iB >= 0 && (e.c.seen || iN >= 0) && iQ >= 0 && N <= e.n_max && (B <= v.S || ((B - v.S) % 128u == 0u && B <= N &&
                     (uint64_t) (uint32_t) iQ + (e.c.seen ? 0u : 1u) >= B && v.body)) &&
                     (pend <= bend || (v.ring && v.cap >= 16u && pend - bend <= v.cap));
     e.c.B = ok ? B : 0u;

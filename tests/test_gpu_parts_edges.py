@@ -93,3 +93,30 @@ def test_lists_longer_than_the_groups(lib, dev, D, H, per, bits):
                 for o in outs:
                     check(o.get().reshape(q.shape), want, tol, t, (n, top, t))
         ctx.close()
+
+
+# ---- descriptors ----
+
+@pytest.mark.parametrize("bits", [(4, 4, 0), (3, 3, 0), (2, 2, 1)])
+def test_a_tree_does_not_read_the_descriptors_n(lib, dev, bits):
+    """any N, below zero too, gives the eager call's bits, in every kernel behind the call"""
+    rng = np.random.default_rng(bits[0])
+    D, H, per = 128, 1, 8
+    ctx = Ctx(lib, dev, D, H, bits, n_groups=3, tail=70, seed=90)
+    st, desc = dev.stream(), dev.put(descriptor(0, 0, 0))
+    n_max = ctx.B + ctx.L.cap
+    for n in (9, 40):                                # 72 and 320 rows a head: the 32-row kernel takes the latter's BF16 output
+        base = ctx.N - n
+        mask, q = trees.tree(rng, n), groups.queries(rng, n, H * per, D)
+        dq, dm = dev.put(q), dev.put(trees.words(mask))
+        for t in TYPES:
+            out = Out(dev, q.size, t)
+            g = Graph(dev, st, [lambda: lib.sjk_hip_attend_tree_dyn(C.byref(ctx.view), desc, n_max, n, n, H * per, dq, D ** -0.5, dm, t, out.at, st)])
+            for N in (-7, 0, 2 ** 31 - 1, -2 ** 31, ctx.N):
+                want = trees.run(lib, dev, ctx.view, ctx.B, base, mask, q, t).bits()
+                dev.upload(desc, descriptor(ctx.B, N, base))
+                dev.sync()
+                g.replay()
+                assert np.array_equal(out.bits(), want), (n, t, N)
+            g.close()
+    ctx.close()
