@@ -99,7 +99,7 @@ def test_lists_longer_than_the_groups(lib, dev, D, H, per, bits):
 
 @pytest.mark.parametrize("bits", [(4, 4, 0), (3, 3, 0), (2, 2, 1)])
 def test_a_tree_does_not_read_the_descriptors_n(lib, dev, bits):
-    """any N, below zero too, gives the eager call's bits, in every kernel behind the call"""
+    """any N, below zero too, gives the same rows, those of the eager call, in every kernel behind the call"""
     rng = np.random.default_rng(bits[0])
     D, H, per = 128, 1, 8
     ctx = Ctx(lib, dev, D, H, bits, n_groups=3, tail=70, seed=90)
@@ -112,11 +112,19 @@ def test_a_tree_does_not_read_the_descriptors_n(lib, dev, bits):
         for t in TYPES:
             out = Out(dev, q.size, t)
             g = Graph(dev, st, [lambda: lib.sjk_hip_attend_tree_dyn(C.byref(ctx.view), desc, n_max, n, n, H * per, dq, D ** -0.5, dm, t, out.at, st)])
-            for N in (-7, 0, 2 ** 31 - 1, -2 ** 31, ctx.N):
+            first = None
+            for N in (ctx.N, -7, 0, 2 ** 31 - 1, -2 ** 31, ctx.N):
                 want = trees.run(lib, dev, ctx.view, ctx.B, base, mask, q, t).bits()
                 dev.upload(desc, descriptor(ctx.B, N, base))
                 dev.sync()
                 g.replay()
-                assert np.array_equal(out.bits(), want), (n, t, N)
+                got = out.bits()
+                first = got if first is None else first
+                assert np.array_equal(got, first), (n, t, N)
+                # an eager call of many tiles may cut them into other launches (other partial sums, within their roundings)
+                if n == 9 or bits[2] or t == sjk.BF16:
+                    assert np.array_equal(got, want), (n, t, N)
+                else:
+                    check(parts.values(got, t), parts.values(want, t), 2.0 ** -12 * np.abs(parts.values(want, t)).max(), t, (n, t, N))
             g.close()
     ctx.close()
