@@ -51,6 +51,9 @@ SJK_DEV uint32_t sel_groups(const SelArgs & a, int j) {
     const uint32_t b = (uint32_t) B;
     const bool ok = B >= 0 && N >= 0 && Q >= 0 && b <= (uint32_t) N && (uint32_t) N <= a.n_max && b > a.S && (b - a.S) % 128u == 0u &&
                     (uint32_t) Q + 1u >= b;
+    // staged positions that the call's rows see: as many as the ring holds
+    const uint64_t last = (uint64_t) (uint32_t) Q + (uint32_t) a.n_q, end = (uint64_t) (uint32_t) N < last ? (uint32_t) N : last;
+    if (ok && end > b && end - b > a.cap) return 0u;
     return ok ? (b - a.S) / 128u : 0u;
 }
 
@@ -422,6 +425,11 @@ extern "C" int sjk_hip_select_groups_batch(const sjk_hip_groups_job * jobs, int 
         const sjk_hip_view & v = J.v, & v0 = jobs[0].v;
         if (const int rc = sel_args(v, n_q, n_head, J.d_q, top, J.d_sel)) return rc;
         if (const int rc = groups_ok(v, J.B, J.N, J.qpos0, n_q)) return rc;
+        const uint32_t bend = J.B > v.S ? J.B : v.S, last = J.qpos0 + (uint32_t) n_q, end = J.N < last ? J.N : last;
+        if (end > bend && end - bend > v.cap) {
+            set_error("sjk_hip_select_groups: more staged positions than the ring holds");
+            return SJKVARN_ERR_CAPACITY;
+        }
         if (J.B > v.S && (J.B - v.S) / 128u > (uint32_t) top && !v.work) return SJKVARN_ERR_ARG;
         if (v.lay.D != v0.lay.D || v.lay.bits_k != v0.lay.bits_k || v.lay.bits_v != v0.lay.bits_v || v.lay.body != v0.lay.body ||
             v.n_head_kv != v0.n_head_kv)

@@ -128,3 +128,37 @@ def test_a_tree_does_not_read_the_descriptors_n(lib, dev, bits):
                     check(parts.values(got, t), parts.values(want, t), 2.0 ** -12 * np.abs(parts.values(want, t)).max(), t, (n, t, N))
             g.close()
     ctx.close()
+
+
+def test_descriptors_past_the_ring(lib, dev):
+    """more staged positions than the ring holds: lists of -1 where the attention gives NaN rows, and the last place that fits"""
+    rng = np.random.default_rng(3)
+    D, H, per, top, n = 128, 2, 3, 4, 9
+    lay = sjk.layout(D, G, 3, 3, 0)
+    v = groups.fake_view(lib, dev, D, H, (3, 3, 0), groups.records(rng, lay, n, H), np.arange(n))
+    B, cap = S + G * n, 256
+    q = groups.queries(rng, 3, H * per, D)
+    st = dev.stream()
+    desc, dq, sel, out = dev.put(descriptor(0, 0, 0)), dev.put(q), dev.alloc(3 * H * top * 4), Out(dev, q.size, sjk.F32)
+    g = Graph(dev, st, [lambda: lib.sjk_hip_select_groups_dyn(C.byref(v), desc, 1 << 20, 3, H * per, dq, top, sel, st),
+                        lambda: lib.sjk_hip_attend_groups_dyn(C.byref(v), desc, 1 << 20, 3, H * per, dq, D ** -0.5, sel, top, sjk.F32, out.at, st)])
+    lists = lambda: dev.get(sel, 3 * H * top * 4, np.int32).reshape(3, H, top)  # noqa: E731
+    for N, qpos0, ok in ((B + cap, B + cap - 3, 1), (B + cap + 1, B + cap - 2, 0), (1 << 20, B + 700, 0), (B + cap + 900, B + 5, 1), (B + 20, B + 700, 1),
+                         ((1 << 20) + 1, B + 5, 0), (B + 3, 2 ** 31 - 1, 1), (B + cap + 1, B + cap - 2, 0)):
+        dev.upload(desc, descriptor(B, N, qpos0))
+        dev.sync()
+        g.replay()
+        if ok:
+            want = groups.select(lib, dev, v, B, N, qpos0, q, top, H)
+            assert (want >= 0).all() and np.array_equal(lists(), want), (N, qpos0)
+            assert np.array_equal(out.bits(), groups.attend(lib, dev, v, B, N, qpos0, q, want).bits()), (N, qpos0)
+        else:
+            assert (lists() == -1).all() and np.isnan(out.get()).all(), (N, qpos0)
+    # nothing sealed: the list is -1 in any case, and a tail past the ring gives NaN rows
+    for N, qpos0, ok in ((S + cap, S + cap - 3, 1), (S + cap + 1, S + cap - 2, 0), (S + cap + 1, S, 1)):
+        dev.upload(desc, descriptor(S, N, qpos0))
+        dev.sync()
+        g.replay()
+        assert (lists() == -1).all()
+        assert np.isfinite(out.get()).all() if ok else np.isnan(out.get()).all(), (N, qpos0)
+    g.close()
