@@ -373,6 +373,11 @@ static int sel_args(const sjk_hip_view & v, int n_q, int n_head, const float * q
 
 static size_t sel_room(const sjk_hip_view & v) { return ws_part_slots(v) * ws_slot_floats(v.lay.D) * sizeof(float) / sizeof(double); }
 
+static int sel_full() {
+    set_error("sjk_hip_select_groups: the scores of one position do not fit the view's workspace");
+    return SJKVARN_ERR_CAPACITY;
+}
+
 // n_jobs <= SEL_MAXJ jobs of one shape; most: the largest number of groups any of them can have
 static int sel_launch(SelArgs & a, const sjk_hip_view & v, int n_jobs, size_t room, uint32_t most, hipStream_t st) {
     const sj_kvarn_layout & l = v.lay;
@@ -389,10 +394,7 @@ static int sel_launch(SelArgs & a, const sjk_hip_view & v, int n_jobs, size_t ro
     int chunk = a.n_q;                           // positions whose scores the workspaces hold at once
     if (scored) {
         const size_t fit = room / ((size_t) a.H * most);
-        if (fit == 0) {
-            set_error("sjk_hip_select_groups: the scores of one position do not fit the view's workspace");
-            return SJKVARN_ERR_CAPACITY;
-        }
+        if (fit == 0) return sel_full();
         if ((size_t) chunk > fit) chunk = (int) fit;
     }
     if (chunk > 2048) chunk = 2048;              // grid z: jobs x position tiles
@@ -435,30 +437,43 @@ extern "C" int sjk_hip_select_groups_batch(const sjk_hip_groups_job * jobs, int 
             v.n_head_kv != v0.n_head_kv)
             return refuse("sjk_hip_select_groups_batch: the views differ in layout or KV heads");
     }
-    // jobs with scores that share a workspace (the layers of a sequence) share its room
     auto groups = [&](int k) { return jobs[k].B > jobs[k].v.S ? (jobs[k].B - jobs[k].v.S) / 128u : 0u; };
-    for (int k0 = 0; k0 < n_jobs; k0 += SEL_MAXJ) {
-        const int n = n_jobs - k0 < SEL_MAXJ ? n_jobs - k0 : SEL_MAXJ;
+    auto scored = [&](int k) { return groups(k) > (uint32_t) top; };
+    // before the first launch: every job's scores of one position fit its workspace
+    for (int k = 0; k < n_jobs; ++k)
+        if (scored(k) && sel_room(jobs[k].v) < (size_t) jobs[k].v.n_head_kv * groups(k)) return sel_full();
+    // Jobs with scores that share a workspace (the layers of a sequence) share its room: the scores that each of the n jobs from k0 on
+    // may hold; most: the groups of the longest
+    auto share = [&](int k0, int n, uint32_t & most) {
+        size_t room = ~(size_t) 0;
+        most = 0;
+        for (int k = k0; k < k0 + n; ++k) {
+            if (groups(k) > most) most = groups(k);
+            if (!scored(k)) continue;
+            size_t on_it = 0;
+            for (int i = k0; i < k0 + n; ++i) on_it += scored(i) && jobs[i].v.work == jobs[k].v.work;
+            const size_t r = sel_room(jobs[k].v) / on_it;
+            if (r < room) room = r;
+        }
+        return room;
+    };
+    for (int k0 = 0, n; k0 < n_jobs; k0 += n) {
+        // as many jobs a launch as have room for the longest one's scores of a position; the next launch follows on the stream
+        uint32_t most;
+        n = n_jobs - k0 < SEL_MAXJ ? n_jobs - k0 : SEL_MAXJ;
+        size_t room = share(k0, n, most);
+        while (n > 1 && most > (uint32_t) top && room < (size_t) jobs[0].v.n_head_kv * most) room = share(k0, --n, most);
         SelArgs a = {};
         a.n_q = n_q; a.n_head = n_head; a.top = top;
-        uint32_t most = 0;
-        size_t room = ~(size_t) 0;
         for (int k = 0; k < n; ++k) {
             const sjk_hip_groups_job & J = jobs[k0 + k];
             SelJob & s = a.job[k];
             s.body = J.v.body; s.blocks = J.v.blocks; s.q = J.d_q; s.sel = J.d_sel;
             s.n = groups(k0 + k);
-            if (s.n > most) most = s.n;
-            if (s.n <= (uint32_t) top) continue;
-            int shared = 0, rank = 0;
-            for (int i = 0; i < n; ++i)
-                if (groups(k0 + i) > (uint32_t) top && jobs[k0 + i].v.work == J.v.work) {
-                    ++shared;
-                    if (i < k) ++rank;
-                }
-            const size_t r = sel_room(J.v) / (size_t) shared;
-            if (r < room) room = r;
-            s.score = (double *) ws_part(J.v) + (size_t) rank * r;
+            if (!scored(k0 + k)) continue;
+            size_t rank = 0;
+            for (int i = k0; i < k0 + k; ++i) rank += scored(i) && jobs[i].v.work == J.v.work;
+            s.score = (double *) ws_part(J.v) + rank * room;
         }
         if (const int rc = sel_launch(a, jobs[k0].v, n, room, most, (hipStream_t) stream)) return rc;
     }

@@ -162,3 +162,41 @@ def test_descriptors_past_the_ring(lib, dev):
         assert (lists() == -1).all()
         assert np.isfinite(out.get()).all() if ok else np.isnan(out.get()).all(), (N, qpos0)
     g.close()
+
+
+# ---- selections ----
+
+def test_selections_that_share_a_workspace(lib, dev):
+    """jobs of one workspace whose scores do not fit it together, beside jobs of their own: every list as alone. A job that does not fit at
+    all: no list of the batch is written."""
+    rng = np.random.default_rng(8)
+    D, H, n, top = 128, 2, 900, 20
+    lay = sjk.layout(D, G, 3, 3, 0)
+    recs = groups.records(rng, lay, 200, H)
+    head, slot = 4096 + ((H * D * 8 + 255) & ~255), 16 * (D + 2) * 4
+    shared = dev.alloc(head + 64 * slot)
+    own = dev.alloc(head + 64 * slot)
+    views, q, lengths = [], [], []
+    for k in range(37):
+        v = groups.fake_view(lib, dev, D, H, (3, 3, 0), recs, rng.integers(0, 200, n), work=False)
+        # the shared one holds the scores of 2 positions of 900 groups and 2 heads, the other of many
+        v.work, v.work_bytes = (own.value, head + 64 * slot) if k in (4, 20) else (shared.value, head + -(-(2 * H * n * 8) // slot) * slot)
+        views.append(v)
+        q.append(groups.queries(rng, 5, 8, D))
+        lengths.append(15 if k in (3, 30) else n - 20 * (k % 5))
+    dqs = [dev.put(x) for x in q]
+    sel = dev.put(np.full((37, 5, H, top), 77, np.int32))
+    size = 5 * H * top * 4
+    jobs = (sjk.GroupsJob * 37)()
+    for k in range(37):
+        B = S + G * lengths[k]
+        jobs[k] = sjk.GroupsJob(views[k], B, B + 5, B, dqs[k], C.c_void_p(sel.value + k * size), None)
+    want = np.stack([groups.select(lib, dev, views[k], jobs[k].B, jobs[k].N, jobs[k].qpos0, q[k], top, H) for k in range(37)])
+    sjk.check(lib.sjk_hip_select_groups_batch(jobs, 37, 5, 8, top, None), "batch")
+    dev.sync()
+    assert np.array_equal(dev.get(sel, 37 * size, np.int32).reshape(want.shape), want)
+    dev.upload(sel, np.full((37, 5, H, top), 77, np.int32))
+    jobs[36].v.work_bytes = head + slot
+    assert lib.sjk_hip_select_groups_batch(jobs, 37, 5, 8, top, None) == CAPACITY
+    dev.sync()
+    assert (dev.get(sel, 37 * size, np.int32) == 77).all()
