@@ -190,6 +190,7 @@ static int ext_ok(const char * who, const sjk_hip_view & v, uint32_t B, uint64_t
         return SJKVARN_ERR_ARG;
     if (!sjk_attend3_supported(&v)) return unsupported(who);
     if ((int64_t) n_q * n_head > 0x7fffffff || v.n_head_kv > n_cus()) return SJKVARN_ERR_ARG;
+    if (ws_part_slots(v) < (size_t) ws_slots(v.n_head_kv)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
     const uint64_t row = (uint64_t) n_q * (uint64_t) n_head * (uint64_t) v.lay.D;
     const uintptr_t q0 = (uintptr_t) q, o0 = (uintptr_t) out;
     if (q0 < o0 + row * (out_type == SJK_F32 ? 4u : 2u) && o0 < q0 + row * 4u) return refuse("the output lies over the queries");

@@ -3384,9 +3384,6 @@ static int ext_launch(A3BatchT<A3Ext> & bt, int body, int H, hipStream_t st) {
 
 int sjk_attend_ext(const ExtCall * calls, int n, int n_q, int n_head, float scale, int top, int n_nodes, int out_type, hipStream_t st) {
     const int body = ext_body(calls[0].v.lay, out_type), H = calls[0].v.n_head_kv;
-    // a workspace smaller than it should be is found before anything is launched
-    for (int j = 0; j < n; ++j)
-        if (ws_part_slots(calls[j].v) < (size_t) ws_slots(H)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
     bool wide = calls[0].seen != nullptr;
     for (int j = 0; wide && j < n; ++j) wide = sjk_prefill_takes_tree(calls[j].v, body, calls[j].N, n_q, n_head, out_type);
     if (wide) {
@@ -3430,7 +3427,6 @@ int sjk_attend_ext_dyn(const ExtCall & call, const int32_t * desc, uint32_t n_ma
     e.n_q = n_q; e.n_head = n_head; e.top = top; e.n_nodes = n_nodes; e.out_type = out_type; e.scale = scale;
     const int H = call.v.n_head_kv, D = call.v.lay.D;
     e.body = ext_body(call.v.lay, out_type);
-    if (ws_part_slots(call.v) < (size_t) ws_slots(H)) return refuse("the view's workspace is smaller than sjk_hip_workspace_bytes");
     if (call.seen && sjk_prefill_takes_tree(call.v, e.body, 0, n_q, n_head, out_type))
         return sjk_prefill_tree(call, desc, n_max, n_q, n_head, scale, n_nodes, st);
     const int nt = ext_tiles(e);
