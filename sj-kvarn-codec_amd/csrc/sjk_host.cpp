@@ -1850,7 +1850,7 @@ int sjk_hip_seq_accept(sj_kvarn_seq * s, uint32_t base, const int32_t * path, in
     }
     const uint32_t n_nodes = s->n - base;
     for (int i = 0; i < n_path; ++i)
-        if (path[i] < 0 || (uint32_t) path[i] >= n_nodes || path[i] > 65535 || (i && path[i] <= path[i - 1])) {
+        if (path[i] < 0 || (uint32_t) path[i] >= n_nodes || (i && path[i] <= path[i - 1])) {
             sjk::set_error("sjk_hip_seq_accept: the path does not ascend, or leaves the nodes");
             return SJKVARN_ERR_ARG;
         }

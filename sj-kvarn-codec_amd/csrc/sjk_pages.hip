@@ -95,9 +95,11 @@ struct AcceptBatch {
     uint32_t base, S, cap, n_nodes, n_path, to;  // rows go to base + to + i
     uint32_t sink_row, ring_row;                 // bytes of a position's row
     int D, H, side;                              // (rows of two formats) channels, KV heads, staged bytes of K or V
+    uint32_t list0;                              // the list's first node; its entries count from there
     uint16_t list[ACC_PATH];
 };
 constexpr int ACC_HELD = 1024;                   // path entries that a workgroup holds in LDS
+static_assert(ACC_PATH <= ACC_HELD, "a list is held whole");
 static_assert(sizeof(AcceptBatch) <= 4096, "the table travels in the kernel arguments");
 
 // A workgroup's place in the call: its first position, that position's slot, and the path's first entries in LDS
@@ -105,9 +107,7 @@ struct AccPlace {
     const AcceptBatch & b;
     uint32_t base, slot0;
     const uint32_t * held;
-    __device__ __forceinline__ uint32_t node(uint32_t i) const {
-        return i < (uint32_t) ACC_HELD ? held[i] : b.path ? (uint32_t) b.path[i] : (uint32_t) b.list[i];
-    }
+    __device__ __forceinline__ uint32_t node(uint32_t i) const { return i < (uint32_t) ACC_HELD ? held[i] : (uint32_t) b.path[i]; }
     // slot of position base + k; k is less than the ring's slots
     __device__ __forceinline__ uint32_t slot(uint32_t k) const {
         const uint32_t s = base < b.S ? base + k - b.S : slot0 + k;
@@ -124,7 +124,7 @@ SJK_DEV bool acc_base(const AcceptBatch & b, uint32_t & base) {
 }
 // entries of the path up to the first that is no node above the one before it
 SJK_DEV uint32_t acc_len(const AcceptBatch & b, uint32_t * held, uint32_t * s_len) {
-    auto entry = [&](uint32_t i) { return b.path ? (uint32_t) b.path[i] : (uint32_t) b.list[i]; };
+    auto entry = [&](uint32_t i) { return b.path ? (uint32_t) b.path[i] : b.list0 + b.list[i]; };
     if (threadIdx.x == 0) *s_len = b.n_path;
     __syncthreads();
     uint32_t first = b.n_path;
@@ -383,12 +383,16 @@ int accept_rows(const sjk_hip_view * views, int n_layers, const int32_t * d_desc
     b.sink_row = v0.sink_type == SJKVARN_SINK_F16 ? H * 4u * (uint32_t) b.D : b.ring_row;
     const bool mixed = b.sink_row != b.ring_row && v0.S && (d_desc ? true : base < v0.S && end > v0.S);
     const uint32_t row = b.sink_row > b.ring_row ? b.sink_row : b.ring_row, cols = (row / 4u + 4u * ACC_COLS - 1u) / (4u * ACC_COLS);
-    const int step = d_path ? n_path : ACC_PATH;
-    for (int i0 = 0; i0 < n_path; i0 += step) {
-        const int k = n_path - i0 < step ? n_path - i0 : step;
+    for (int i0 = 0, k; i0 < n_path; i0 += k) {
+        k = n_path - i0;
+        if (host) {                              // what the list holds: ACC_PATH entries, 65,536 nodes from its first on
+            if (k > ACC_PATH) k = ACC_PATH;
+            while (host[i0 + k - 1] - host[i0] > 65535) --k;
+        }
         b.n_path = (uint32_t) k;
         b.to = (uint32_t) i0;
-        for (int i = 0; host && i < k; ++i) b.list[i] = (uint16_t) host[i0 + i];
+        b.list0 = host ? (uint32_t) host[i0] : 0u;
+        for (int i = 0; host && i < k; ++i) b.list[i] = (uint16_t) (host[i0 + i] - host[i0]);
         for (int l0 = 0; l0 < n_layers; l0 += ACC_LAYERS) {
             const int nl = n_layers - l0 < ACC_LAYERS ? n_layers - l0 : ACC_LAYERS;
             for (int il = 0; il < nl; ++il) { b.layer[il].sink = views[l0 + il].sink; b.layer[il].ring = views[l0 + il].ring; }

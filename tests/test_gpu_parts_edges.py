@@ -200,3 +200,92 @@ def test_selections_that_share_a_workspace(lib, dev):
     assert lib.sjk_hip_select_groups_batch(jobs, 37, 5, 8, top, None) == CAPACITY
     dev.sync()
     assert (dev.get(sel, 37 * size, np.int32) == 77).all()
+
+
+# ---- acceptance ----
+
+def staged_views(dev, D, H, cap, NL, rings, sink):
+    """views of layers whose rings stand one after the other at `rings`"""
+    views = (sjk.View * NL)()
+    for il, v in enumerate(views):
+        v.lay = sjk.layout(D, G, 4, 4, 0)
+        v.n_head_kv, v.S, v.cap, v.stage_bytes = H, S, cap, D // 128 * 98
+        v.sink, v.ring = sink.value, rings.value + il * cap * H * 2 * v.stage_bytes
+    return views
+
+
+@pytest.mark.parametrize("NL", [160, 161, 321])
+def test_accept_in_more_layers_than_a_launch_takes(lib, dev, NL):
+    rng = np.random.default_rng(NL)
+    D, H, cap = 128, 1, 128
+    rings = rng.integers(0, 256, (NL, cap, H * 2 * 98), dtype=np.uint8)
+    buf, sink = dev.put(rings), dev.alloc(S * H * 4 * D)
+    views = staged_views(dev, D, H, cap, NL, buf, sink)
+    path = [1, 7, 8, 60, 99]
+    sjk.check(lib.sjk_hip_accept(views, NL, 1000, 100, dev.put(np.array(path, np.int32)), len(path), None), "accept")
+    dev.sync()
+    for i, p in enumerate(path):
+        rings[:, (1000 + i - S) % cap] = rings[:, (1000 + p - S) % cap]
+    assert np.array_equal(dev.get(buf, rings.nbytes, np.uint8), rings.ravel())
+
+
+@pytest.mark.parametrize("base", [9000, S - 20])
+@pytest.mark.parametrize("sink_type", [0, 1])
+def test_accept_of_long_paths(lib, dev, base, sink_type):
+    """a path on the device past what a workgroup holds of it, through the ring's end, and from the ring into the sink"""
+    rng = np.random.default_rng(base + sink_type)
+    D, H, cap, n, NL = 128, 2, 4096, 4000, 2
+    row = H * 2 * 98
+    rings = rng.integers(0, 256, (NL, cap, row), dtype=np.uint8)
+    rings.reshape(NL, cap, H * 2, 98)[..., 1] &= 0x3F                       # block norms that are numbers
+    sink_row = row if sink_type else H * 4 * D
+    sinks = rng.integers(0, 256, (NL, S, sink_row), dtype=np.uint8)
+    for path in (list(range(1, n)), np.sort(rng.choice(n, 2500, replace=False)).tolist()):
+        buf, sink = dev.put(rings), dev.put(sinks)
+        views = staged_views(dev, D, H, cap, NL, buf, sink)
+        for il, v in enumerate(views):
+            v.sink_type, v.sink = sink_type, sink.value + il * S * sink_row
+        want_s, want_r = sinks.copy(), rings.copy()
+
+        def to_half(x):
+            dp, fp = dev.put(np.ascontiguousarray(x)), dev.alloc(2 * H * D * 4)
+            sjk.check(lib.sjk_hip_unstage(0, dp, 98, fp, D, 2 * H, None), "unstage")
+            dev.sync()
+            return dev.get(fp, 2 * H * D * 4, np.float32).astype(np.float16).view(np.uint8)
+
+        for il in range(NL):
+            trees.accept_ref(want_s[il], want_r[il], S, cap, base, path, None if sink_type else to_half)
+        sjk.check(lib.sjk_hip_accept(views, NL, base, n, dev.put(np.array(path + [3], np.int32)), len(path) + 1, None), "accept")
+        dev.sync()
+        assert np.array_equal(dev.get(sink, sinks.nbytes, np.uint8), want_s.ravel())
+        assert np.array_equal(dev.get(buf, rings.nbytes, np.uint8), want_r.ravel())
+
+
+def test_a_sequence_accepts_long_paths_of_many_nodes(lib, dev):
+    """paths past what one launch's arguments hold, of nodes past 65,535, from the sink on"""
+    rng = np.random.default_rng(6)
+    D, H, n_pos = 128, 1, 66100
+    cfg = lib.sj_kvarn_config_default(D, H, 70000, 256)
+    cfg.tail, cfg.tail_max = 128, 128 * 520
+    s = sjk.Seq()
+    sjk.check(lib.sj_kvarn_seq_init(C.byref(s), C.byref(cfg), 1, None), "seq")
+    v = lib.sjk_layer_view(C.byref(s.layers[0]))
+    assert v.cap >= n_pos - S
+    dk, dv = (dev.put(rng.standard_normal((n_pos, H, D)).astype(np.float32)) for _ in range(2))
+    for p in range(0, n_pos, 4096):
+        m = min(4096, n_pos - p)
+        sjk.check(lib.sjk_hip_seq_store(C.byref(s), 0, p, m, dk.value + p * H * D * 4, dv.value + p * H * D * 4, 1, None), "store")
+    dev.sync()
+    row = H * 2 * 98
+    for base, pick in ((200, np.r_[[0, 2], 65530 + np.arange(0, 300, 7)]), (150, np.sort(rng.choice(65600, 1500, replace=False))),
+                       (400, np.arange(700) * 90 + 1)):
+        s.n = n_pos
+        path = pick.tolist()
+        ring = dev.get(C.c_void_p(v.ring), v.cap * row, np.uint8).reshape(v.cap, row)
+        for i, p in enumerate(path):
+            ring[(base + i - S) % v.cap] = ring[(base + p - S) % v.cap]
+        sjk.check(lib.sjk_hip_seq_accept(C.byref(s), base, (C.c_int32 * len(path))(*path), len(path), None), "accept")
+        dev.sync()
+        assert s.n == base + len(path)
+        assert np.array_equal(dev.get(C.c_void_p(v.ring), v.cap * row, np.uint8), ring.ravel()), base
+    lib.sj_kvarn_seq_free(C.byref(s))
