@@ -2586,7 +2586,7 @@ __host__ __device__ static void a3_split(A3Args & a, double unit, double chunk_c
 // record and row workgroups up, so the proportional unit can ask for a few workgroups more than the two per CU
 // that are resident at once, and those few then run as a second round after the others (at D = 128, 8 KV heads,
 // 100K: 65 workgroups per head for 64 slots took 82 us against 63 us for a split within them).
-template <typename Args> __host__ __device__ static double a3_fit_unit(const Args * jobs, int n_jobs, double unit, double chunk_cost, int slots) {
+__host__ __device__ static double a3_fit_unit(const A3Args * jobs, int n_jobs, double unit, double chunk_cost, int slots) {
     int least = 0;                               // one row and one record workgroup per job at the most
     for (int j = 0; j < n_jobs; ++j) {
         const int k = (jobs[j].n_chunk > 0) + (jobs[j].n_rec > 0);
@@ -2703,7 +2703,8 @@ template <typename Args> __host__ __device__ static int a3_assign(A3BatchT<Args>
     double total = 0.0;
     for (int j = 0; j < bt.n_jobs; ++j) total += bt.job[j].n_rec + cc * bt.job[j].n_chunk;
     double unit = total / slots > 1.0 ? total / slots : 1.0;
-    if (!a4) unit = a3_fit_unit(bt.job, bt.n_jobs, unit, cc, slots);
+    if constexpr (!is_ext<Args>)                 // (ext_split goes by shares)
+        if (!a4) unit = a3_fit_unit(bt.job, bt.n_jobs, unit, cc, slots);
     // tiles of one call (jobs on one view: the sequences of a pool share its body but not their block tables and
     // rings): they stream the same records
     bool tiles = bt.n_jobs > 1;
