@@ -557,7 +557,11 @@ SJK_DEV void lds_reads_done(f4 & x0, f4 & x1, f4 & x2, f4 & x3) {
     asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x0), "+v"(x1), "+v"(x2), "+v"(x3) :: "memory");
 }
 
-// LOW (A3Ext, fp16 outputs): the weights P' as hi and lo parts
+// LOW (A3Ext, fp16 outputs): the weights P' as hi and lo parts, and the V codes of both tiles of a pair at 2^-20. The matrix unit adds
+// products at the places that their operands' exponents name, and a subnormal operand has the exponent of the least normal number: of a
+// product with a code at 2^-24 the bits go up to 2^-10 sooner than its size says. Over tens of thousands of positions that was as much as
+// the rounding to fp16 (384 groups of 3 positions 2.8e-4 beside 2.0e-4, three seeds; every code at 2^-20 2.0 to 2.1e-4 and 48.2 ->
+// 48.9 us; at 2^-18 the same error; codes around zero, as the scalar bodies' kernel has them, the same and 53.5 us).
 template <int D, bool LOW, typename Args>
 __device__ __attribute__((always_inline)) inline void a4_records(const Args & a, A4Lds<D> & S, int h, int wgi, int ls) {
     constexpr bool EXT = is_ext<Args>;
@@ -670,6 +674,7 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
     const uint32_t qend_min = q_end(a, 0);       // q_end grows with the row over the live rows
     const int tbg = 16 * (g >> 1) + 4 * (g & 1); // first score token of the lane group in a 32-token step
     const uint32_t M0 = 0x000F000Fu, M1 = 0x00F000F0u;
+    constexpr float T0 = LOW ? 0x1p-20f : 0x1p-24f;    // scale of the V codes of a pair's first tile
     const float * qlane = &S.r.q[n][0];
 
     const uint8_t * rb_next = nullptr;
@@ -888,7 +893,7 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const float cr = __shfl(cv, 4 * g + r, 64);
-            c0v[r] = cr * 0x1p-24f;
+            c0v[r] = cr * T0;
             c1v[r] = cr * 0x1p-20f;
         }
 
@@ -917,7 +922,7 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
 #pragma unroll
                 for (int jj = 0; jj < 2; ++jj) {
                     const uint32_t w0 = vw[p][jj].x, w1 = vw[p][jj].y, x0 = w0 >> 8, x1 = w1 >> 8;
-                    const u4 b0 = u4{w0 & M0, w1 & M0, x0 & M0, x1 & M0};
+                    const u4 b0 = LOW ? u4{(w0 << 4) & M1, (w1 << 4) & M1, (w0 >> 4) & M1, (w1 >> 4) & M1} : u4{w0 & M0, w1 & M0, x0 & M0, x1 & M0};
                     const u4 b1 = u4{w0 & M1, w1 & M1, x0 & M1, x1 & M1};
                     t[2 * jj] = mfma32(Ah[p], b0, t[2 * jj]);
                     t[2 * jj + 1] = mfma32(Ah[p], b1, t[2 * jj + 1]);
@@ -930,7 +935,7 @@ __device__ __attribute__((always_inline)) inline void a4_records(const Args & a,
 #pragma unroll
             for (int jj = 0; jj < 2; ++jj) {
                 const int J = 2 * J2 + jj;
-                const float v0 = h2f(vch[jj] & 0xFFFFu) * pinv * 0x1p24f, v1 = h2f(vch[jj] >> 16) * pinv * 0x1p20f;
+                const float v0 = h2f(vch[jj] & 0xFFFFu) * pinv * (1.0f / T0), v1 = h2f(vch[jj] >> 16) * pinv * 0x1p20f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     O[2 * J][r] = __builtin_fmaf(v0, t[2 * jj][r], O[2 * J][r]);
@@ -3331,9 +3336,10 @@ static int ext_kernels(int body, bool low, int D, dim3 grid, dim3 cgrid, const A
 }
 
 // The kernel of a body: as a3_body, but 4/4 records of a 32-bit output go through the scalar bodies' kernel (45), which keeps the
-// weights' low parts and codes around zero (4e-7 of a result against float64). The streaming wavefronts of fp16 outputs keep the low parts
-// (2.2e-4, the output's own rounding 2.0e-4; without them 3.1e-4 and 46 instead of 50 us for 384 groups of 3 positions), those of bf16 outputs
-// round the weights to fp16 once (3e-4 beside the output's 1.7e-3).
+// weights' low parts and codes around zero (3e-7 to 4e-7 of a result against float64). The streaming wavefronts of fp16 outputs keep the
+// low parts too: their error is within 1% of the output's own rounding (2.00e-4 to 2.13e-4 beside 2.00e-4 to 2.12e-4 for 384 and for 64
+// groups, three seeds each, and a tree at 100K positions). Those of bf16 outputs round the weights to fp16 once (1.61e-3 beside 1.60e-3;
+// 1.69e-3 beside 1.67e-3 for 64 nodes at 100K).
 static int ext_body(const sj_kvarn_layout & l, int out_type) {
     const int body = a3_body(l);
     return body == 44 && out_type == SJK_F32 ? 45 : body;

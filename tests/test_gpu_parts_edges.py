@@ -289,3 +289,48 @@ def test_a_sequence_accepts_long_paths_of_many_nodes(lib, dev):
         assert s.n == base + len(path)
         assert np.array_equal(dev.get(C.c_void_p(v.ring), v.cap * row, np.uint8), ring.ravel()), base
     lib.sj_kvarn_seq_free(C.byref(s))
+
+
+# ---- precision ----
+
+@pytest.mark.parametrize("D,seed,flat", [(128, 1, 1.0), (128, 2, 0.5), (128, 3, 0.25), (256, 4, 0.5), (256, 5, 0.25)])
+def test_fp16_outputs_are_rounded_once(lib, dev, D, seed, flat):
+    """4/4 records, 384 listed groups and a tree of 64 rows, weights from uneven to nearly equal: an error at most a tenth above that of the exact result rounded to fp16 (what
+    is computed before the rounding is then within 0.46 of the rounding's error)"""
+    rng = np.random.default_rng(seed)
+    H, per, n = 2, 4, 400
+    lay = sjk.layout(D, G, 4, 4, 0)
+    recs = groups.records(rng, lay, n, H)
+    # values around zero: a row over many of them is far smaller than they are
+    vs = recs[:, :, lay.v_scale:lay.v_scale + 2 * G].copy().view(np.float16).astype(np.float64)
+    recs[:, :, lay.v_zero:lay.v_zero + 2 * G] = (-7.5 * vs).astype(np.float16).view(np.uint8)
+    v = groups.fake_view(lib, dev, D, H, (4, 4, 0), recs, rng.permutation(n))
+    B, N = S + G * n, S + G * n + 200
+    K, V = Ctx.rows(_Rows(lib, dev, D, H), N, view=v, B=B)
+    q = groups.queries(rng, 2, H * per, D)
+    sel = np.stack([np.sort(rng.choice(n, 384, replace=False)) for _ in range(2 * H)]).reshape(2, H, 384)
+    seen = np.zeros((2, H, N), bool)
+    for i in range(2):
+        seen[i, :, :S] = seen[i, :, B:N - 1 + i] = True
+        for h in range(H):
+            for g in sel[i, h]:
+                seen[i, h, S + G * g:S + G * (g + 1)] = True
+    scale = D ** -0.5 * flat
+    want, _ = attention(q, K, V, seen, scale)
+    got = groups.attend(lib, dev, v, B, N, N - 2, q, sel, sjk.F16, scale).get().reshape(q.shape)
+    plain = np.linalg.norm(want.astype(np.float16) - want)
+    assert np.linalg.norm(got - want) <= 1.1 * plain, np.linalg.norm(got - want) / plain
+    mask = np.eye(64, dtype=bool)
+    q = groups.queries(rng, 64, H * per, D)
+    seen = np.broadcast_to(np.concatenate([np.ones((64, N - 64), bool), mask], 1)[:, None], (64, H, N))[::9]
+    want, _ = attention(q[::9], K, V, seen, scale)
+    got = trees.run(lib, dev, v, B, N - 64, mask, q, sjk.F16, scale).get().reshape(q.shape)[::9]
+    plain = np.linalg.norm(want.astype(np.float16) - want)
+    assert np.linalg.norm(got - want) <= 1.1 * plain, np.linalg.norm(got - want) / plain
+
+
+class _Rows:
+    """what Ctx.rows asks of a context"""
+
+    def __init__(self, lib, dev, D, H):
+        self.lib, self.dev, self.D, self.H, self.view, self.B = lib, dev, D, H, None, 0
