@@ -329,6 +329,28 @@ def test_fp16_outputs_are_rounded_once(lib, dev, D, seed, flat):
     assert np.linalg.norm(got - want) <= 1.1 * plain, np.linalg.norm(got - want) / plain
 
 
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("bits", groups.BODIES, ids=groups.IDS)
+def test_fp32_outputs_of_every_body(lib, dev, D, bits):
+    """every body holds the same bound, the trellis bodies too: independent roundings, 2 D of a score's partial sums of U of about twice a
+    score's size each, make 2e-6 of a weight and of a result"""
+    rng = np.random.default_rng(D + bits[0])
+    H, per, n, n_q = 2, 4, 24, 3
+    ctx = Ctx(lib, dev, D, H, bits, n_groups=n, tail=300, seed=3)
+    K, V = ctx.rows(ctx.N)
+    q = groups.queries(rng, n_q, H * per, D)
+    for listed in (range(n), range(1, n, 3)):
+        sel = np.broadcast_to(np.array(listed, np.int32), (n_q, H, len(listed)))
+        want, _ = attention(q, K, V, groups.seen_of(ctx, [[listed] * H] * n_q, n_q, ctx.N - n_q), D ** -0.5)
+        got = groups.attend(lib, dev, ctx.view, ctx.B, ctx.N, ctx.N - n_q, q, sel).get().reshape(q.shape)
+        parts.check_norm(got, want, 1e-5, len(listed))
+    mask = trees.tree(rng, 20)
+    q = groups.queries(rng, 20, H * per, D)
+    want, _ = attention(q, K, V, trees.seen_of(mask, ctx.N - 20, H), D ** -0.5)
+    parts.check_norm(trees.run(lib, dev, ctx.view, ctx.B, ctx.N - 20, mask, q).get().reshape(q.shape), want, 1e-5, "tree")
+    ctx.close()
+
+
 class _Rows:
     """what Ctx.rows asks of a context"""
 
