@@ -95,6 +95,30 @@ def test_lists_longer_than_the_groups(lib, dev, D, H, per, bits):
         ctx.close()
 
 
+@pytest.mark.parametrize("bits", [(4, 4, 0), (3, 3, 0), (3, 3, 1)])
+@pytest.mark.parametrize("H,per,n_q", [(1, 17, 2), (2, 40, 1), (48, 1, 3), (1, 1, 1), (1, 128, 1)])
+def test_head_layouts(lib, dev, H, per, n_q, bits):
+    """more query heads per KV head than a tile has rows, many KV heads, and one; lists and trees of them"""
+    rng = np.random.default_rng(H + per)
+    D, n = 128, 5
+    ctx = Ctx(lib, dev, D, H, bits, n_groups=n, tail=33, seed=60)
+    K, V = ctx.rows(ctx.N)
+    q = groups.queries(rng, n_q, H * per, D)
+    pick = [[np.sort(rng.choice(n, 3, replace=False)).tolist() for _ in range(H)] for _ in range(n_q)]
+    want, tol = attention(q, K, V, groups.seen_of(ctx, pick, n_q, ctx.N - n_q), D ** -0.5)
+    mask = trees.tree(rng, n_q, 2)
+    tree_want, tree_tol = attention(q, K, V, trees.seen_of(mask, ctx.N - n_q, H), D ** -0.5)
+    for t in TYPES:
+        got = groups.attend(lib, dev, ctx.view, ctx.B, ctx.N, ctx.N - n_q, q, np.array(pick, np.int32), t).get().reshape(q.shape)
+        check(got, want, tol, t, t)
+        tree_got = trees.run(lib, dev, ctx.view, ctx.B, ctx.N - n_q, mask, q, t).get().reshape(q.shape)
+        check(tree_got, tree_want, tree_tol, t, t)
+        if t == sjk.F32:
+            parts.check_norm(got, want, 1e-5)
+            parts.check_norm(tree_got, tree_want, 1e-5)
+    ctx.close()
+
+
 # ---- descriptors ----
 
 @pytest.mark.parametrize("bits", [(4, 4, 0), (3, 3, 0), (2, 2, 1)])
