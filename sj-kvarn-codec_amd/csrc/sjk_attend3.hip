@@ -169,10 +169,10 @@ SJK_DEV uint32_t ext_seen(const A3Ext & a, int n, uint32_t p0) {
     if (s > 48u && i + 1u < (uint32_t) a.words) x |= m[i + 1] << (64u - s);
     return (uint32_t) x & 0xFFFFu;
 }
-// Two codes c (halves of x, c < 2^b) as the exact fp16 values c - 2^(b - 1): with 0x6400 above them they are 1024 + c. The products
-// of a record's sums then have both signs: with codes 0 .. 2^b - 1 the zero points take back nearly all of a sum over many
-// tokens, and with it the matrix unit's rounding of every product at the sum's own last place (1e-4 of the result at 1,024
-// positions, 5e-6 without).
+// Two codes c (halves of x, c < 2^b) as the exact fp16 values c - 2^(b - 1): with 0x6400 above them they are 1024 + c. A record's sums
+// are then of normal halves of both signs: of subnormal halves, codes at 2^-24 or so, the matrix unit drops the products' last bits
+// sooner (a4_records), and with codes 0 .. 2^b - 1 the zero points take back nearly all of a sum over many tokens (1e-4 of the
+// result at 1,024 positions, 5e-6 so).
 SJK_DEV uint32_t middle2(uint32_t x, int b) {
     typedef _Float16 hf2 __attribute__((ext_vector_type(2)));
     const _Float16 m = (_Float16) (-1024.0f - (float) (1 << (b - 1)));
@@ -2669,8 +2669,8 @@ __host__ __device__ static void a4_split(A3Args & a, int slots) {
 
 // The split of a job of listed groups: `share` workgroups of its KV head, a whole number of records for each record workgroup and
 // of chunks for each wavefront of the row workgroups; the split whose longer side is least, the fewest workgroups that reach it.
-// EXT_CHUNK: a wavefront's chunk in records of a workgroup. 0.5 / 0.7 / 0.9 / 1.05 / 1.2: 25.1 / 25.0 / 25.1 / 22.0 / 22.0 us for 64
-// groups and 5.7K staged positions of one sequence (D = 256), 42.1 / 34.1 / 33.7 / 33.7 / 37.8 for 32 groups and 517 of 8 (3/3, D = 128).
+// EXT_CHUNK: a wavefront's chunk in records of a workgroup. 0.5 / 0.7 / 0.9 / 1.05 / 1.2: 21.7 / 21.9 / 21.6 / 20.8 / 20.9 us for 64
+// groups and 5.7K staged positions of one sequence (D = 256), 26.9 / 27.0 / 26.8 / 27.1 / 27.3 for 32 groups and 517 of 8 (3/3, D = 128).
 constexpr double EXT_CHUNK = 1.05;
 __host__ __device__ static void ext_split(A3Args & a, int share) {
     int rec = 0, row = 0, per = 0;
@@ -3051,14 +3051,14 @@ extern "C" int sjk_hip_attend_dyn(const sjk_hip_view * v, const int32_t * d_desc
 // attention over listed groups, and of drafted nodes (A3Ext)
 // ------------------------------------------------------------------------------------------------
 //
-// The kernels are the bodies' own; they take the weights P' as hi and lo parts here, so that an output keeps the precision of 32 bits (but
-// for bf16 outputs of scalar records; ext_body: which kernel takes 4/4 records).
+// The kernels are the bodies' own; they take the weights P' as hi and lo parts here, so that an output keeps the precision of 32 bits
+// (but for bf16 outputs of scalar records; ext_body: which kernel takes 4/4 records).
 // A tile of a list's call is one query position (16 of its heads): each position has a list of its own per KV head.
 //
-// What bounds them: the streaming wavefronts HBM (384 of 3,100 groups for 3 positions, 8 KV heads of 128, fp16 out: 50.8 us for 173 MB, 3.4 TB/s); the
-// staged kernel of the scalar bodies latency where a workgroup has two records (64 of 736 groups, D = 256: 17.6 us, of them 6 to the
-// first record - arguments, list, record, one after the other - and 5 a record) and vector issue where it has more (32 groups of 8 sequences, 3/3: 24.4 us, 12 of them
-// vector instructions). The combine takes 3.9 to 4.7 us more.
+// What bounds them: the streaming wavefronts HBM and vector issue (384 of 3,100 groups for 3 positions, 8 KV heads of 128, fp16 out:
+// 51.2 us for 173 MB, 3.4 TB/s); the staged kernel of the scalar bodies latency where a workgroup has two records (64 of 736 groups,
+// D = 256: 17.3 us, of them 6 to the first record - arguments, list, record, one after the other - and 5 a record) and vector issue where
+// it has more (32 groups of 8 sequences, 3/3: 25.3 us, 12 of them vector instructions). The combine takes 3.8 to 4.7 us more.
 
 namespace sjk {
 

@@ -85,8 +85,8 @@ static uint64_t tiles(uint64_t words) { return (words + TILE_WORDS - 1) / TILE_W
 //
 // path ascends, so path[i] >= i: a row is never written before those that are copied from it at lower positions have been
 // read, if a workgroup reads ACC_ROWS rows of its columns, waits, writes them and goes on. A call moves little (5 rows of 16 layers
-// of 4 KV heads of 256: 125 KB, 3.4 us on the device; 90 of 64 layers of 8 of 128: 9 MB, 8.1) and is bound by its launch and two round trips; a
-// column is 16 bytes of one row of one layer.
+// of 4 KV heads of 256: 125 KB, 3.5 us on the device; 90 of 64 layers of 8 of 128: 9 MB, 7.7) and is bound by its launch and two
+// round trips; a column is 16 bytes of one row of one layer.
 constexpr int ACC_LAYERS = 160, ACC_COLS = 16, ACC_U = 8, ACC_ROWS = 256 / ACC_COLS * ACC_U, ACC_PATH = 512;
 struct AcceptBatch {
     struct { uint8_t * sink, * ring; } layer[ACC_LAYERS];

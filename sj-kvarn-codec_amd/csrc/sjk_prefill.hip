@@ -55,11 +55,12 @@ constexpr int PF_COST_CH = 3, PF_COST_REC = 4;
 // it takes 38.1 against 35.3 us at 600 positions, with 1 head 38.5 against 32.0 at 1,500. At 128 rows it takes up to twice as
 // long on short contexts. The line is on rows and heads alone: a captured call does not know its context.
 constexpr int PF_MIN_ROWS = 256, PF_MIN_ROWS_HEADS = 8;
-// Trees of drafted nodes, BF16 outputs (weights of records are rounded to fp16 once: beside a rounding to bf16 that is nothing, of
-// FP16 outputs it took the error from 2.0e-4 to 3.6e-4, so those stay with the 16-row kernel, which takes their low parts too): from 256 rows on at every length, and from 64 rows on where rows x heads x positions reach 24M (a captured call does not
+// Trees of drafted nodes, BF16 outputs (weights of records are rounded to fp16 once: 1.69e-3 of a result beside 1.67e-3 of the rounding
+// to bf16; of FP16 outputs it took the error from 2.0e-4 to 3.6e-4, so those stay with the 16-row kernel, which takes their low parts
+// too): from 256 rows on at every length, and from 64 rows on where rows x heads x positions reach 24M (a captured call does not
 // know its context: rows alone). Against the 16-row kernel: 256 rows of 4 heads, D = 256, 37 / 36 us at 300 positions, 55 / 59 at
 // 8.7K, 219 / 288 at 100K; 96 of 8 heads, D = 128, 35 / 26 at 8.7K, 61 / 79 at 42K; 64 of 4, D = 256, 44 / 21 at 8.7K, 85 / 79 at
-// 100K; 192 of 1, D = 128, 53 / 43 at 100K, of 2 72 / 83. 64 nodes x 16 heads of 256 at 100K: 226 us, 105 GFLOP of products at
+// 100K; 192 of 1, D = 128, 53 / 43 at 100K, of 2 72 / 83. 64 nodes x 16 heads of 256 at 100K: 224 us, 105 GFLOP of products at
 // 0.47 PFLOP/s, bound as the other calls are.
 constexpr int PF_TREE_ROWS = 256, PF_TREE_SOME = 64;
 constexpr uint64_t PF_TREE_WORK = 24u << 20;

@@ -10,8 +10,8 @@
 // Sums are 64-bit, on the fp64 matrix unit (v_mfma_f64_16x16x4: 16 groups x 16 query rows x 4 channels): a list is whole
 // numbers, and two scores next to its border must not change places with the order of a sum.
 //
-// What bounds it: few groups, its two launches (5.7 + 3.9 us); 8,000 groups of 8 KV heads of 128 for 4 positions, 21.9 us of scores (49 MB of
-// tables in pieces of 768 bytes, 9.5 us at a copy's rate, beside 6.9 us of fp64 products and as much of conversions) and 11.8 of lists (32
+// What bounds it: few groups, its two launches (5.7 + 3.9 us); 8,000 groups of 8 KV heads of 128 for 4 positions, 22.8 us of scores (49 MB of
+// tables in pieces of 768 bytes, 9.5 us at a copy's rate, beside 6.9 us of fp64 products and as much of conversions) and 11.9 of lists (32
 // workgroups, counts and barriers).
 #include "sjk_mfma.h"
 
