@@ -129,17 +129,18 @@ SJK_DEV int ext_group(const A3Ext & a, int h, int c) {
     const int g = s[c], before = c ? s[c - 1] : -1;
     return g > before && (uint32_t) g < a.n_grp ? g : -1;
 }
-// Records [r0, r1) of a job as entries of KV head h's list. A list of no more entries than there are groups is cut by its entries. A longer one is
-// cut by the groups that it names, so that a short context with lists of a fixed length is shared out by its groups: record r is
+// Records [r0, r1) of a job as entries of KV head h's list. A list of no more entries than there are groups is cut by its entries. A longer
+// one is cut by the groups that it names, so that a short context with lists of a fixed length is shared out by its groups: record r is
 // then the r-th entry that names one, wherever it stands, and the last range goes on to the last one that does. Every wavefront looks by
-// itself, 64 entries at a time (10 groups of 8 sequences, 3/3, lists of 64: 20.1 us; cut by entries 34).
+// itself, 64 entries at a time (10 groups of 8 sequences, 3/3, lists of 64: 20.1 us; cut by entries 34. 10 named of 64 groups, lists of
+// 1,000: 16.9 us; with ranges that went on to the list's end 329).
 SJK_DEV void ext_range(const A3Ext & a, int h, int & r0, int & r1) {
     if (!a.sel || a.n_rec >= a.top || r0 >= r1) return;
     const int lane = (int) (threadIdx.x & 63);
     const int32_t * s = a.sel + (size_t) h * a.top;
     const uint32_t top = (uint32_t) a.top;
     const bool last = r1 == a.n_rec;
-    uint32_t e0 = top, e1 = top;
+    uint32_t e0 = top, e1 = top, end = top;      // end: behind the last entry that names a group
     int seen = 0;                                // entries that name a group before these 64
     for (uint32_t i0 = 0; i0 < top && (e0 == top || e1 == top || last); i0 += 64) {
         const uint32_t i = i0 + (uint32_t) lane;
@@ -148,11 +149,12 @@ SJK_DEV void ext_range(const A3Ext & a, int h, int & r0, int & r1) {
         const int n = seen + __popcll(m), at = seen + (int) __builtin_amdgcn_mbcnt_hi((uint32_t) (m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) m, 0));
         const bool mine = (m >> lane) & 1u;
         if (r0 >= seen && r0 < n) e0 = i0 + (uint32_t) __builtin_ctzll(__ballot(mine && at == r0));
-        if (last && m) e1 = i0 + 64u - (uint32_t) __builtin_clzll(m);
+        if (m) end = i0 + 64u - (uint32_t) __builtin_clzll(m);
         if (!last && r1 >= seen && r1 < n) e1 = i0 + (uint32_t) __builtin_ctzll(__ballot(mine && at == r1));
         seen = n;
     }
-    r0 = __builtin_amdgcn_readfirstlane((int) e0);
+    if (e1 == top) e1 = end;
+    r0 = __builtin_amdgcn_readfirstlane((int) (e0 < e1 ? e0 : e1));
     r1 = __builtin_amdgcn_readfirstlane((int) e1);
 }
 // The 16 positions from p0 on that row n of the tile sees of the nodes and of what lies before them (a bit each)
