@@ -633,9 +633,10 @@ int sjk_hip_select_groups_dyn(const sjk_hip_view * v, const int32_t * d_desc, ui
 int sjk_hip_attend_groups_dyn(const sjk_hip_view * v, const int32_t * d_desc, uint32_t n_max, int n_q, int n_head, const float * d_q,
                               float scale, const int32_t * d_sel, int top, int out_type, void * d_out, void * stream);
 
-/* n_jobs independent calls with one n_q, n_head and top in as few launches as the kernels take (up to 16 jobs a selection, whose scores fit the
- * workspaces that they share - each alone at least, or nothing is launched: SJKVARN_ERR_CAPACITY; up to 13 tiles of
- * 16 query rows an attention, where a list's tile is one position). Views of a selection agree in layout and KV heads. d_out is not used by a selection. */
+/* n_jobs independent calls with one n_q, n_head and top in as few launches as the kernels take: up to 16 jobs a selection, as many as
+ * have room for their scores in the workspaces that they share (one that does not fit alone: SJKVARN_ERR_CAPACITY, nothing is
+ * launched); up to 13 tiles of 16 query rows an attention, where a list's tile is one position. Views of a selection agree in layout
+ * and KV heads. d_out is not used by a selection. */
 typedef struct sjk_hip_groups_job {
     sjk_hip_view  v;
     uint32_t      B, N, qpos0;

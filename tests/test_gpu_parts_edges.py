@@ -167,8 +167,8 @@ def test_descriptors_past_the_ring(lib, dev):
     g = Graph(dev, st, [lambda: lib.sjk_hip_select_groups_dyn(C.byref(v), desc, 1 << 20, 3, H * per, dq, top, sel, st),
                         lambda: lib.sjk_hip_attend_groups_dyn(C.byref(v), desc, 1 << 20, 3, H * per, dq, D ** -0.5, sel, top, sjk.F32, out.at, st)])
     lists = lambda: dev.get(sel, 3 * H * top * 4, np.int32).reshape(3, H, top)  # noqa: E731
-    for N, qpos0, ok in ((B + cap, B + cap - 3, 1), (B + cap + 1, B + cap - 2, 0), (1 << 20, B + 700, 0), (B + cap + 900, B + 5, 1), (B + 20, B + 700, 1),
-                         ((1 << 20) + 1, B + 5, 0), (B + 3, 2 ** 31 - 1, 1), (B + cap + 1, B + cap - 2, 0)):
+    for N, qpos0, ok in ((B + cap, B + cap - 3, 1), (B + cap + 1, B + cap - 2, 0), (1 << 20, B + 700, 0), (B + cap + 900, B + 5, 1),
+                         (B + 20, B + 700, 1), ((1 << 20) + 1, B + 5, 0), (B + 3, 2 ** 31 - 1, 1), (B + cap + 1, B + cap - 2, 0)):
         dev.upload(desc, descriptor(B, N, qpos0))
         dev.sync()
         g.replay()
@@ -286,7 +286,7 @@ def test_accept_of_long_paths(lib, dev, base, sink_type):
 
 
 def test_a_sequence_accepts_long_paths_of_many_nodes(lib, dev):
-    """paths past what one launch's arguments hold, of nodes past 65,535, from the sink on"""
+    """paths past what one launch's arguments hold, of nodes past 65,535"""
     rng = np.random.default_rng(6)
     D, H, n_pos = 128, 1, 66100
     cfg = lib.sj_kvarn_config_default(D, H, 70000, 256)
@@ -319,8 +319,8 @@ def test_a_sequence_accepts_long_paths_of_many_nodes(lib, dev):
 
 @pytest.mark.parametrize("D,seed,flat", [(128, 1, 1.0), (128, 2, 0.5), (128, 3, 0.25), (256, 4, 0.5), (256, 5, 0.25)])
 def test_fp16_outputs_are_rounded_once(lib, dev, D, seed, flat):
-    """4/4 records, 384 listed groups and a tree of 64 rows, weights from uneven to nearly equal: an error at most a tenth above that of the exact result rounded to fp16 (what
-    is computed before the rounding is then within 0.46 of the rounding's error)"""
+    """4/4 records, 384 listed groups and a tree of 64 rows, weights from uneven to nearly equal: an error at most a tenth above that of
+    the exact result rounded to fp16 (what is computed before the rounding is then within 0.46 of the rounding's error)"""
     rng = np.random.default_rng(seed)
     H, per, n = 2, 4, 400
     lay = sjk.layout(D, G, 4, 4, 0)
